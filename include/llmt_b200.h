@@ -401,6 +401,93 @@ LLMT_B200_API int llmt_b200_gemm_softmax_bwd(const llmt_b200_gemm_desc* desc, vo
 LLMT_B200_API int llmt_b200_rowdot(float* out, const void* x, const void* y, int64_t rows, int64_t cols, int64_t ldx,
                      int64_t ldy, int32_t dtype, void* stream);
 
+/* ---- what a transformer block runs between its products ----------------------------------------
+ *
+ * A view of per-head data [batch, tokens, heads, head_dim]: base and strides in elements, head_dim
+ * contiguous.  Strides are free, so the heads may lie in [B, H, T, hd] tensors or inside the token
+ * rows of a packed projection [B, T, (H + 2 Hkv) hd].  The stride of a dimension of extent 1 is not
+ * looked at. */
+typedef struct llmt_b200_head_view {
+    void* data;             /* inputs are not written */
+    int64_t stride_batch, stride_token, stride_head;
+} llmt_b200_head_view;
+
+/* Rotary positions (llmt include/llmt/kernels/rope.h: rotate-half in place on q and k; here also
+ * neighbouring pairs, part of a head, scaled frequencies, a position per token, and the inverse):
+ *   angle = position(b, t) * freqs[i],  i < rot_dim / 2
+ *   half layout:        u = x[i],      w = x[i + rot_dim / 2]
+ *   interleaved layout: u = x[2 i],    w = x[2 i + 1]
+ *   (u, w) -> scale * (u cos - w sin, u sin + w cos);   inverse: the angle's sign turned, which makes
+ *   the gradient with respect to x out of the gradient with respect to y.
+ * Values behind rot_dim are copied.  y may be x (same base and strides), else the two must not
+ * overlap; y's elements must be distinct.
+ *   freqs      device, fp64 [rot_dim / 2], radians per token; llmt_b200_rope_frequencies fills a host
+ *              array with them.  Angles are reduced in 64-bit fixed point, exact at any position.
+ *   positions  device, int32 [batch, tokens] contiguous, or NULL: offset + t.
+ *   dtype      fp32 or bf16; arithmetic in fp32.  head_dim <= 1024, rot_dim even.
+ * One call may do q and k of a packed projection together (heads = H + Hkv).  Nothing is done for
+ * batch, tokens or heads of 0. */
+typedef struct llmt_b200_rope_desc {
+    int64_t batch, tokens, heads, head_dim, rot_dim;
+    llmt_b200_head_view x, y;
+    const double* freqs;
+    const int32_t* positions;
+    int64_t offset;
+    int32_t dtype, interleaved, inverse;
+    float scale;
+} llmt_b200_rope_desc;
+LLMT_B200_API int llmt_b200_rope(const llmt_b200_rope_desc* desc, void* stream);
+
+/* freqs[i] = f_i ((1 - c_i) / factor + c_i),  f_i = base^(-2 i / rot_dim): a frequency that turns more
+ * than `high` times within `trained` tokens keeps its value (c = 1), one that turns fewer than `low`
+ * times is slowed by `factor` (c = 0), between them c is linear in the number of turns.  factor 1
+ * gives the plain frequencies, whatever the others are; low = high = infinity scales all positions. */
+LLMT_B200_API int llmt_b200_rope_frequencies(double* freqs, int64_t rot_dim, double base, double factor, double low, double high,
+                                             double trained);
+
+/* The norms after and before a block, its gate and the residual in one pass over the rows (llmt
+ * include/llmt/kernels/rmsnorm.h and residual.h are two kernels):
+ *   N(z; w) = z * rsqrt(mean(z^2) + eps) * w
+ *   out = x + scale * gate * N(y; w_post)      h = N(out; w_pre)
+ * x, out (dtype_res) is the residual stream; y (the block's output) and h (the next block's input) are
+ * dtype_act; weights, gate and statistics are fp32.  Types: (fp32, fp32), (fp32, bf16), (bf16, bf16).
+ *   y NULL       no block: out is not written, h = N(x; w_pre).
+ *   w_post NULL  no norm after the block: N(y; w_post) is y.
+ *   gate NULL    a gate of ones; else [groups, cols], row r uses gate row r / (rows / groups): groups = 1
+ *                is one gate for all, groups = sequences one for each; groups divides rows.
+ *   h NULL       no norm before the next block (w_pre is NULL too).
+ *   rstd_*       fp32 [rows], the rows' rsqrt(mean + eps), for the backward pass; may be NULL.
+ * out may be x.  h is made from out before out is rounded to dtype_res.  Row pitches ld_* in elements,
+ * any alignment of an element; cols <= 16384.
+ *
+ * llmt_b200_norm_residual_bwd: with g = dout + (gradient of h through N(.; w_pre)),
+ *   dx = g,  dy = the gradient of y,  dw_pre, dw_post [cols], dgate [groups, cols] summed over the rows they
+ *   serve, in fp32 and in a fixed order:  d = beta * d + sum.
+ * Reads out (as stored), y and the statistics of the forward call.  dout NULL: no gradient but the one
+ * through h.  dh NULL: h was not made.  dw_post, dgate, dw_pre NULL: not wanted.  dx may be dout.
+ * For y NULL `out` is the forward call's x, and dy is not written.  workspace: 16-byte aligned,
+ * llmt_b200_norm_residual_workspace_bytes(desc) bytes (0 where no weight gradient is wanted). */
+typedef struct llmt_b200_norm_residual_desc {
+    int64_t rows, cols, groups;
+    int32_t dtype_res, dtype_act;
+    float scale, eps;
+    const void *x, *y;                 /* forward: x, y; backward: y */
+    void *out, *h;                     /* forward: written; backward: out is read */
+    int64_t ld_x, ld_y, ld_out, ld_h;
+    const float *w_post, *gate, *w_pre;
+    float *rstd_post, *rstd_pre;       /* forward: written; backward: read */
+    const void *dout, *dh;
+    void *dx, *dy;
+    int64_t ld_dout, ld_dh, ld_dx, ld_dy;
+    float *dw_post, *dgate, *dw_pre;
+    float beta;
+    void* workspace;
+    uint64_t workspace_bytes;
+} llmt_b200_norm_residual_desc;
+LLMT_B200_API int llmt_b200_norm_residual_fwd(const llmt_b200_norm_residual_desc* desc, void* stream);
+LLMT_B200_API int llmt_b200_norm_residual_bwd(const llmt_b200_norm_residual_desc* desc, void* stream);
+LLMT_B200_API uint64_t llmt_b200_norm_residual_workspace_bytes(const llmt_b200_norm_residual_desc* desc);
+
 /* The same exchange with all `world` ranks living on ONE device (comms[r] is rank r's
  * descriptor, every pointer local): a single cooperative launch of world * ctas CTAs.
  * For tests of the algorithm where fewer GPUs than ranks are at hand. */

@@ -32,6 +32,8 @@ EXPORTS = [
     "llmt_b200_cross_entropy_fwd", "llmt_b200_lm_head_ce_workspace_bytes", "llmt_b200_lm_head_ce_fwd",
     "llmt_b200_gemm_softmax_workspace_bytes", "llmt_b200_gemm_softmax_fwd", "llmt_b200_gemm_softmax_bwd",
     "llmt_b200_rowdot", "llmt_b200_cross_entropy_bwd", "llmt_b200_lm_head_ce_bwd",
+    "llmt_b200_rope", "llmt_b200_rope_frequencies", "llmt_b200_norm_residual_fwd", "llmt_b200_norm_residual_bwd",
+    "llmt_b200_norm_residual_workspace_bytes",
 ]
 
 COMM_MAX_RANKS, COMM_MAX_CTAS = 8, 128
@@ -67,6 +69,30 @@ class GemmDesc(ctypes.Structure):
         ("stride_b_outer", ctypes.c_int64), ("stride_c_outer", ctypes.c_int64),
         ("aux", ctypes.c_void_p),
     ]
+
+
+class HeadView(ctypes.Structure):
+    """llmt_b200_head_view of include/llmt_b200.h."""
+    _fields_ = [("data", ctypes.c_void_p), ("stride_batch", ctypes.c_int64), ("stride_token", ctypes.c_int64), ("stride_head", ctypes.c_int64)]
+
+
+class RopeDesc(ctypes.Structure):
+    """llmt_b200_rope_desc of include/llmt_b200.h."""
+    _fields_ = [("batch", ctypes.c_int64), ("tokens", ctypes.c_int64), ("heads", ctypes.c_int64), ("head_dim", ctypes.c_int64),
+                ("rot_dim", ctypes.c_int64), ("x", HeadView), ("y", HeadView), ("freqs", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+                ("offset", ctypes.c_int64), ("dtype", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("inverse", ctypes.c_int32),
+                ("scale", ctypes.c_float)]
+
+
+class NormResidualDesc(ctypes.Structure):
+    """llmt_b200_norm_residual_desc of include/llmt_b200.h."""
+    _fields_ = ([("rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("groups", ctypes.c_int64), ("dtype_res", ctypes.c_int32),
+                 ("dtype_act", ctypes.c_int32), ("scale", ctypes.c_float), ("eps", ctypes.c_float)]
+                + [(n, ctypes.c_void_p) for n in ("x", "y", "out", "h")] + [(n, ctypes.c_int64) for n in ("ld_x", "ld_y", "ld_out", "ld_h")]
+                + [(n, ctypes.c_void_p) for n in ("w_post", "gate", "w_pre", "rstd_post", "rstd_pre", "dout", "dh", "dx", "dy")]
+                + [(n, ctypes.c_int64) for n in ("ld_dout", "ld_dh", "ld_dx", "ld_dy")]
+                + [(n, ctypes.c_void_p) for n in ("dw_post", "dgate", "dw_pre")]
+                + [("beta", ctypes.c_float), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)])
 
 
 class LlmtB200Error(RuntimeError):
@@ -159,6 +185,16 @@ def lib() -> ctypes.CDLL:
         L.llmt_b200_gemm_softmax_bwd.restype = ctypes.c_int
         L.llmt_b200_rowdot.argtypes = [ctypes.c_void_p] * 3 + [ctypes.c_int64] * 4 + [ctypes.c_int32, ctypes.c_void_p]
         L.llmt_b200_rowdot.restype = ctypes.c_int
+        L.llmt_b200_rope.argtypes = [ctypes.POINTER(RopeDesc), ctypes.c_void_p]
+        L.llmt_b200_rope.restype = ctypes.c_int
+        L.llmt_b200_rope_frequencies.argtypes = [ctypes.c_void_p, ctypes.c_int64] + [ctypes.c_double] * 5
+        L.llmt_b200_rope_frequencies.restype = ctypes.c_int
+        L.llmt_b200_norm_residual_fwd.argtypes = [ctypes.POINTER(NormResidualDesc), ctypes.c_void_p]
+        L.llmt_b200_norm_residual_fwd.restype = ctypes.c_int
+        L.llmt_b200_norm_residual_bwd.argtypes = L.llmt_b200_norm_residual_fwd.argtypes
+        L.llmt_b200_norm_residual_bwd.restype = ctypes.c_int
+        L.llmt_b200_norm_residual_workspace_bytes.argtypes = [ctypes.POINTER(NormResidualDesc)]
+        L.llmt_b200_norm_residual_workspace_bytes.restype = ctypes.c_uint64
         L.llmt_b200_exchange_begin_step.argtypes = [ctypes.POINTER(CommDesc), ctypes.c_void_p]
         L.llmt_b200_exchange_begin_step.restype = ctypes.c_int
         L.llmt_b200_zero_grads.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]
@@ -503,6 +539,170 @@ def rowdot(out, x, y, stream=None) -> None:
         raise LlmtB200Error(ERR_INVALID, "rowdot: contiguous tensors")
     _check(lib().llmt_b200_rowdot(out.data_ptr(), x.data_ptr(), y.data_ptr(), rows, cols, cols, cols,
                                   _dtype_code(x), _stream(stream)))
+
+
+# ---- what a transformer block runs between its products
+
+def _device_of(who: str, *tensors):
+    """The one CUDA device that the tensors (None ones apart) are on."""
+    device = None
+    for t in tensors:
+        if t is None:
+            continue
+        if t.device.type != "cuda" or (device is not None and t.device != device):
+            raise LlmtB200Error(ERR_INVALID, f"{who}: tensors of one CUDA device expected")
+        device = t.device
+    return device
+
+
+def _on(device, stream, call) -> None:
+    """Makes a call with `device` as the current one; None as stream is that device's current stream."""
+    import torch
+    if device.index == torch.cuda.current_device():
+        _check(call(_stream(stream)))
+    else:
+        with torch.cuda.device(device):
+            _check(call(_stream(stream)))
+
+
+def _need(ok: bool, message: str) -> None:
+    if not ok:
+        raise LlmtB200Error(ERR_INVALID, message)
+
+
+def _heads(t, who: str, name: str) -> HeadView:
+    """The view of a [batch, tokens, heads, head_dim] tensor."""
+    _need(t.dim() == 4 and (t.shape[3] == 1 or t.stride(3) == 1), f"{who}: {name} must be [batch, tokens, heads, head_dim] with contiguous head_dim")
+    return HeadView(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+
+
+def rope_frequencies(rot_dim: int, base: float = 10000.0, factor: float = 1.0, low: float = 1.0, high: float = 32.0, trained: float = 0.0,
+                     device="cuda"):
+    """Radians per token of each of the rot_dim / 2 pairs, fp64 on `device`: base^(-2i / rot_dim), those that turn fewer than
+    `low` times in `trained` tokens slowed by `factor`, those that turn more than `high` times kept, in between in
+    proportion (llmt_b200_rope_frequencies)."""
+    import torch
+    f = torch.empty(max(0, int(rot_dim)) // 2 or 1, dtype=torch.float64)
+    _check(lib().llmt_b200_rope_frequencies(f.data_ptr(), int(rot_dim), float(base), float(factor), float(low), float(high), float(trained)))
+    return f[:int(rot_dim) // 2].to(device)
+
+
+def rope(y, x, freqs, positions=None, offset: int = 0, interleaved: bool = False, inverse: bool = False, scale: float = 1.0,
+         stream=None) -> None:
+    """Turns the first 2 * len(freqs) values of every head of x [batch, tokens, heads, head_dim] (any strides) by
+    position * freqs, into y, which may be x.  positions: int32 [batch, tokens], or None for offset, offset + 1, ...
+    `inverse` turns back: the gradient of x from that of y.  interleaved: pairs (2i, 2i + 1), else (i, i + rot / 2)."""
+    import torch
+    d = RopeDesc()
+    d.x, d.y = _heads(x, "rope", "x"), _heads(y, "rope", "y")
+    _need(x.shape == y.shape and x.dtype == y.dtype, "rope: x and y of one shape and type")
+    _need(freqs.dim() == 1 and freqs.dtype == torch.float64 and freqs.is_contiguous(), "rope: freqs must be fp64 [rot / 2]")
+    d.batch, d.tokens, d.heads, d.head_dim = x.shape
+    d.rot_dim = 2 * freqs.shape[0]
+    d.freqs = freqs.data_ptr()
+    if positions is not None:
+        _need(positions.dtype == torch.int32 and tuple(positions.shape) == tuple(x.shape[:2]) and positions.is_contiguous(),
+              "rope: positions must be contiguous int32 [batch, tokens]")
+        d.positions = positions.data_ptr()
+    d.offset, d.dtype, d.interleaved, d.inverse, d.scale = int(offset), _dtype_code(x), int(interleaved), int(inverse), float(scale)
+    _on(_device_of("rope", x, y, freqs, positions), stream, lambda s: lib().llmt_b200_rope(ctypes.byref(d), s))
+
+
+def _rows(t, shape, who: str, name: str) -> int:
+    """The row pitch of a tensor [..., cols] whose rows are evenly spaced."""
+    _need(tuple(t.shape) == tuple(shape) and (t.shape[-1] == 1 or t.stride(-1) == 1), f"{who}: {name} must have the shape {tuple(shape)} and contiguous rows")
+    pitch, span = t.shape[-1], None
+    for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if n == 1:
+            continue
+        if span is None:
+            pitch = s
+        else:
+            _need(s == span, f"{who}: the rows of {name} must be evenly spaced")
+        span = s * n
+    return pitch
+
+
+def _norm_residual_desc(who: str, like, tensors: dict, w_post, gate, w_pre, rstd_post, rstd_pre, scale: float, eps: float) -> "NormResidualDesc":
+    """What both directions fill in; `tensors`: name -> (tensor or None, True for the block's type)."""
+    import torch
+    d = NormResidualDesc()
+    _need(like.dim() >= 1, f"{who}: tensors of rows expected")
+    d.cols = like.shape[-1]
+    d.rows = like.numel() // d.cols if d.cols else 0
+    kind = {True: None, False: None}
+    for name, (t, act) in tensors.items():
+        if t is None:
+            continue
+        setattr(d, "ld_" + name, _rows(t, like.shape, who, name))
+        setattr(d, name, t.data_ptr())
+        _need(kind[act] in (None, t.dtype), f"{who}: {name} has another type than the tensors of its kind")
+        kind[act] = t.dtype
+    code = {torch.float32: FP32, torch.bfloat16: BF16}
+    _need(all(k is None or k in code for k in kind.values()), f"{who}: fp32 or bf16 tensors")
+    d.dtype_res = code[kind[False] if kind[False] is not None else kind[True]]
+    d.dtype_act = code[kind[True] if kind[True] is not None else kind[False]]
+    for name, t, shape in (("w_post", w_post, (d.cols,)), ("w_pre", w_pre, (d.cols,)), ("rstd_post", rstd_post, (d.rows,)), ("rstd_pre", rstd_pre, (d.rows,))):
+        if t is not None:
+            _need(t.dtype == torch.float32 and t.numel() == shape[0] and t.is_contiguous(), f"{who}: {name} must be contiguous fp32 {list(shape)}")
+            setattr(d, name, t.data_ptr())
+    d.groups = 1
+    if gate is not None:
+        _need(gate.dtype == torch.float32 and gate.is_contiguous() and gate.dim() in (1, 2) and gate.shape[-1] == d.cols, f"{who}: gate must be contiguous fp32 [groups, {d.cols}]")
+        d.gate, d.groups = gate.data_ptr(), gate.numel() // d.cols
+    d.scale, d.eps = float(scale), float(eps)
+    return d
+
+
+def norm_residual_fwd(out, h, x, y=None, w_post=None, gate=None, w_pre=None, rstd_post=None, rstd_pre=None, scale: float = 1.0,
+                      eps: float = 1e-5, stream=None) -> None:
+    """out = x + scale * gate * N(y; w_post), h = N(out; w_pre) with N(z; w) = z * rsqrt(mean(z^2) + eps) * w over the last
+    dimension (llmt_b200_norm_residual_fwd).  y None: out is not written (may be None), h = N(x; w_pre).  h None: no norm
+    follows.  rstd_post, rstd_pre: fp32, one value per row, for the backward pass.  out may be x."""
+    who = "norm_residual_fwd"
+    d = _norm_residual_desc(who, x, dict(x=(x, False), y=(y, True), out=(out if y is not None else None, False), h=(h, True)), w_post, gate,
+                            w_pre, rstd_post, rstd_pre, scale, eps)
+    _on(_device_of(who, out, h, x, y, w_post, gate, w_pre, rstd_post, rstd_pre), stream,
+        lambda s: lib().llmt_b200_norm_residual_fwd(ctypes.byref(d), s))
+
+
+def norm_residual_bwd(dx, dy, dout, dh, out, y=None, w_post=None, gate=None, w_pre=None, rstd_post=None, rstd_pre=None, dw_post=None,
+                      dgate=None, dw_pre=None, scale: float = 1.0, beta: float = 0.0, workspace=None, stream=None) -> None:
+    """The gradients of norm_residual_fwd from what it read and left (llmt_b200_norm_residual_bwd): dx and dy, and the sums
+    over rows dw_post, dgate, dw_pre = beta * itself + sum (fp32; None: not wanted).  dout or dh may be None; dx may be
+    dout.  `workspace`: a uint8 tensor of norm_residual_workspace_bytes, or one is allocated for the call."""
+    import torch
+    who = "norm_residual_bwd"
+    d = _norm_residual_desc(who, dx, dict(out=(out if dh is not None else None, False), y=(y, True), dout=(dout, False), dh=(dh, True),
+                                          dx=(dx, False), dy=(dy if y is not None else None, True)),
+                            w_post, gate, w_pre, rstd_post, rstd_pre, scale, 0.0)
+    for name, t, n in (("dw_post", dw_post, d.cols), ("dgate", dgate, d.groups * d.cols), ("dw_pre", dw_pre, d.cols)):
+        if t is not None:
+            _need(t.dtype == torch.float32 and t.numel() == n and t.is_contiguous(), f"{who}: {name} must be contiguous fp32 of its weight's size")
+            setattr(d, name, t.data_ptr())
+    d.beta = float(beta)
+    device = _device_of(who, dx, dy, dout, dh, out, y, w_post, gate, w_pre, rstd_post, rstd_pre, dw_post, dgate, dw_pre, workspace)
+
+    def call(s):
+        ws = workspace
+        if ws is None:
+            need = lib().llmt_b200_norm_residual_workspace_bytes(ctypes.byref(d))
+            ws = _scratch(need, dx, stream) if need else None
+        if ws is not None:
+            d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
+        return lib().llmt_b200_norm_residual_bwd(ctypes.byref(d), s)
+    _on(device, stream, call)
+
+
+def norm_residual_workspace_bytes(rows: int, cols: int, groups: int = 1, weights: bool = True, gate: bool = True) -> int:
+    """Scratch of norm_residual_bwd on the current device; weights: dw_post or dw_pre is wanted, gate: dgate is."""
+    d = NormResidualDesc()
+    d.rows, d.cols, d.groups = int(rows), int(cols), int(groups)
+    if weights:
+        d.dw_pre = 4
+    if gate:
+        d.dgate = 4
+    return int(lib().llmt_b200_norm_residual_workspace_bytes(ctypes.byref(d)))
 
 
 def exchange_begin_step(desc: "CommDesc", stream=None) -> None:

@@ -3,6 +3,7 @@
 // cuBLASLt (llmt: src/kernels/matmul.cpp:175-214) but reports them as status
 // codes instead of aborting.
 #include <atomic>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -1733,6 +1734,268 @@ int llmt_b200_zero_grads(float* span, int64_t count, void* stream) {
     if (reinterpret_cast<uintptr_t>(span) % sizeof(float) != 0)
         return fail(LLMT_B200_ERR_INVALID, "zero_grads: span is not aligned to its element type");
     cudaError_t e = launch_zero_f32(span, count, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return fail(LLMT_B200_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
+    return LLMT_B200_OK;
+}
+
+namespace {
+
+// Extent in elements of a head view, from its base to one past its last element; -1: a negative stride, or extents whose
+// product leaves 62 bits.
+int64_t view_extent(const llmt_b200_head_view& v, int64_t batch, int64_t tokens, int64_t heads, int64_t hd) {
+    const int64_t n[3] = {batch, tokens, heads}, s[3] = {v.stride_batch, v.stride_token, v.stride_head};
+    __int128 e = hd;
+    for (int i = 0; i < 3; ++i) {
+        if (n[i] <= 1) continue;
+        if (s[i] < 0) return -1;
+        e += static_cast<__int128>(n[i] - 1) * s[i];
+    }
+    return e >> 60 ? -1 : static_cast<int64_t>(e);
+}
+
+// Whether the elements of a view to be written are distinct: each stride, in ascending order, is no shorter than what the
+// dimensions below it cover.
+bool view_distinct(const llmt_b200_head_view& v, int64_t batch, int64_t tokens, int64_t heads, int64_t hd) {
+    int64_t n[3] = {batch, tokens, heads}, s[3] = {v.stride_batch, v.stride_token, v.stride_head};
+    for (int i = 0; i < 3; ++i)
+        for (int j = i + 1; j < 3; ++j)
+            if (s[j] < s[i]) {
+                const int64_t a = s[i], b = n[i];
+                s[i] = s[j]; n[i] = n[j];
+                s[j] = a; n[j] = b;
+            }
+    int64_t covered = hd;
+    for (int i = 0; i < 3; ++i) {
+        if (n[i] <= 1) continue;
+        if (s[i] < covered) return false;
+        covered += (n[i] - 1) * s[i];
+    }
+    return true;
+}
+
+// Strides of dimensions of extent 1 are never used, but take part in alignment rules.
+llmt_b200_head_view without_idle_strides(llmt_b200_head_view v, int64_t batch, int64_t tokens, int64_t heads) {
+    if (batch <= 1) v.stride_batch = 0;
+    if (tokens <= 1) v.stride_token = 0;
+    if (heads <= 1) v.stride_head = 0;
+    return v;
+}
+
+bool misaligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
+
+}  // namespace
+
+int llmt_b200_rope_frequencies(double* freqs, int64_t rot_dim, double base, double factor, double low, double high, double trained) {
+    if (freqs == nullptr) return fail(LLMT_B200_ERR_INVALID, "rope_frequencies: null array");
+    if (rot_dim < 0 || rot_dim % 2 != 0) return fail(LLMT_B200_ERR_INVALID, "rope_frequencies: rot_dim must be even");
+    if (!(base > 0.0) || !(factor > 0.0)) return fail(LLMT_B200_ERR_INVALID, "rope_frequencies: base and factor must be positive");
+    if (factor != 1.0 && (!(high >= low) || !(trained >= 0.0)))
+        return fail(LLMT_B200_ERR_INVALID, "rope_frequencies: low <= high and trained >= 0 expected");
+    for (int64_t i = 0; i < rot_dim / 2; ++i) {
+        const double f = pow(base, -2.0 * static_cast<double>(i) / static_cast<double>(rot_dim));
+        double keep = 1.0;
+        if (factor != 1.0) {
+            const double turns = trained * f / 6.283185307179586477;
+            keep = turns >= high ? 1.0 : turns <= low ? 0.0 : (turns - low) / (high - low);
+        }
+        freqs[i] = keep == 1.0 ? f : f * ((1.0 - keep) / factor + keep);
+    }
+    return LLMT_B200_OK;
+}
+
+int llmt_b200_rope(const llmt_b200_rope_desc* d, void* stream) {
+    if (d == nullptr) return fail(LLMT_B200_ERR_INVALID, "rope: null descriptor");
+    if (d->batch < 0 || d->tokens < 0 || d->heads < 0 || d->head_dim < 1 || d->rot_dim < 0 || d->rot_dim > d->head_dim || d->rot_dim % 2 != 0)
+        return fail(LLMT_B200_ERR_INVALID, "rope: bad shape (batch %lld, tokens %lld, heads %lld, head_dim %lld, rot_dim %lld)", (long long)d->batch,
+                    (long long)d->tokens, (long long)d->heads, (long long)d->head_dim, (long long)d->rot_dim);
+    if (d->dtype != LLMT_B200_FP32 && d->dtype != LLMT_B200_BF16)
+        return fail(LLMT_B200_ERR_UNSUPPORTED, "rope: no kernel for dtype code %d", d->dtype);
+    if (d->head_dim > 1024 || d->heads > 65536 || d->batch > 0x7fffffff || d->tokens > 0x7fffffff || d->batch * d->tokens > 0x3fffffff8ll)
+        return fail(LLMT_B200_ERR_UNSUPPORTED, "rope: head_dim above 1024, heads above 65536 or tokens above 2^34 - 8");
+    if (d->batch == 0 || d->tokens == 0 || d->heads == 0) return LLMT_B200_OK;
+    if (d->x.data == nullptr || d->y.data == nullptr || (d->rot_dim > 0 && d->freqs == nullptr))
+        return fail(LLMT_B200_ERR_INVALID, "rope: invalid tensor (null data)");
+    const uintptr_t es = d->dtype == LLMT_B200_BF16 ? 2 : 4;
+    if (misaligned(d->x.data, es) || misaligned(d->y.data, es) || misaligned(d->freqs, 8) || misaligned(d->positions, 4))
+        return fail(LLMT_B200_ERR_INVALID, "rope: a tensor is not aligned to its element type");
+    const llmt_b200_head_view x = without_idle_strides(d->x, d->batch, d->tokens, d->heads), y = without_idle_strides(d->y, d->batch, d->tokens, d->heads);
+    const int64_t ex = view_extent(x, d->batch, d->tokens, d->heads, d->head_dim), ey = view_extent(y, d->batch, d->tokens, d->heads, d->head_dim);
+    if (ex < 0 || ey < 0) return fail(LLMT_B200_ERR_INVALID, "rope: negative or overlong strides");
+    if (!view_distinct(y, d->batch, d->tokens, d->heads, d->head_dim)) return fail(LLMT_B200_ERR_INVALID, "rope: y's elements overlap one another");
+    const bool same = x.data == y.data && x.stride_batch == y.stride_batch && x.stride_token == y.stride_token && x.stride_head == y.stride_head;
+    if (!same && overlaps(x.data, ex * es, y.data, ey * es)) return fail(LLMT_B200_ERR_INVALID, "rope: y must be x or not overlap it");
+    if (same && d->rot_dim == 0) return LLMT_B200_OK;
+    RopeParams p{};
+    p.x = x.data; p.y = y.data;
+    p.x_batch = x.stride_batch; p.x_token = x.stride_token; p.x_head = x.stride_head;
+    p.y_batch = y.stride_batch; p.y_token = y.stride_token; p.y_head = y.stride_head;
+    p.freqs = d->freqs; p.positions = d->positions; p.offset = d->offset;
+    p.tokens = d->tokens; p.total = d->batch * d->tokens;
+    p.heads = static_cast<int32_t>(d->heads); p.head_dim = static_cast<int32_t>(d->head_dim); p.rot = static_cast<int32_t>(d->rot_dim);
+    p.interleaved = d->interleaved != 0; p.inverse = d->inverse != 0; p.copy_rest = !same;
+    p.scale = d->scale;
+    const cudaError_t e = launch_rope(p, d->dtype == LLMT_B200_BF16, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return fail(LLMT_B200_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
+    return LLMT_B200_OK;
+}
+
+namespace {
+
+// The checks that both directions of norm_residual share; fills in everything but the gradients.
+int norm_residual_params(const llmt_b200_norm_residual_desc* d, const char* who, NormResidualParams* p) {
+    if (d == nullptr) return fail(LLMT_B200_ERR_INVALID, "%s: null descriptor", who);
+    if (d->rows < 0 || d->cols < 1 || d->groups < 1 || d->rows % d->groups != 0)
+        return fail(LLMT_B200_ERR_INVALID, "%s: bad shape (rows %lld, cols %lld, groups %lld)", who, (long long)d->rows, (long long)d->cols,
+                    (long long)d->groups);
+    if ((d->dtype_res != LLMT_B200_FP32 && d->dtype_res != LLMT_B200_BF16) || (d->dtype_act != LLMT_B200_FP32 && d->dtype_act != LLMT_B200_BF16) ||
+        (d->dtype_res == LLMT_B200_BF16 && d->dtype_act == LLMT_B200_FP32))
+        return fail(LLMT_B200_ERR_UNSUPPORTED, "%s: no kernel for dtype codes %d and %d", who, d->dtype_res, d->dtype_act);
+    if (d->cols > norm_residual_max_cols() || d->rows > 0x7fffffff)
+        return fail(LLMT_B200_ERR_UNSUPPORTED, "%s: more than %d columns or 2^31 - 1 rows", who, norm_residual_max_cols());
+    if (d->rows > 0 && d->y == nullptr && (d->w_post != nullptr || d->gate != nullptr))   // a tensor without rows may have no address
+        return fail(LLMT_B200_ERR_INVALID, "%s: w_post and gate belong to y, which is null", who);
+    for (const void* f : {static_cast<const void*>(d->w_post), static_cast<const void*>(d->gate), static_cast<const void*>(d->w_pre),
+                          static_cast<const void*>(d->rstd_post), static_cast<const void*>(d->rstd_pre)})
+        if (misaligned(f, 4)) return fail(LLMT_B200_ERR_INVALID, "%s: a weight or statistic is not aligned to its element type", who);
+    *p = NormResidualParams{};
+    p->rows = d->rows;
+    p->cols = static_cast<int32_t>(d->cols);
+    p->rows_per_gate = d->rows / d->groups;
+    p->x = d->x; p->y = d->y; p->out = d->out; p->h = d->h;
+    p->ld_x = d->ld_x; p->ld_y = d->ld_y; p->ld_out = d->ld_out; p->ld_h = d->ld_h;
+    p->w_post = d->w_post; p->gate = d->gate; p->w_pre = d->w_pre;
+    p->rstd_post = d->rstd_post; p->rstd_pre = d->rstd_pre;
+    p->scale = d->scale; p->eps = d->eps;
+    return LLMT_B200_OK;
+}
+
+// A [rows, cols] tensor of a norm_residual call.
+struct RowTensor {
+    const char* name;
+    const void* data;
+    int64_t ld;
+    bool act, written;
+};
+
+// Pitches and alignment of the tensors that are there (null ones are skipped), and that no written one overlaps another,
+// but for the pair that may be one tensor (`a` and `b`, same pitch).  `wide`: every row starts on a multiple of 8 elements.
+int norm_residual_tensors(const llmt_b200_norm_residual_desc* d, const char* who, const RowTensor* t, int n, const void* a, const void* b, bool* wide) {
+    auto size = [&](const RowTensor& r) { return static_cast<size_t>((r.act ? d->dtype_act : d->dtype_res) == LLMT_B200_BF16 ? 2 : 4); };
+    auto bytes = [&](const RowTensor& r) { return (static_cast<size_t>(d->rows - 1) * r.ld + d->cols) * size(r); };
+    for (int i = 0; i < n; ++i) {
+        if (t[i].data == nullptr) continue;
+        if (d->rows > 1 && (t[i].ld < 0 || t[i].ld > (int64_t{1} << 28) || (t[i].written && t[i].ld < d->cols)))
+            return fail(LLMT_B200_ERR_INVALID, "%s: bad row pitch of %s (%lld)", who, t[i].name, (long long)t[i].ld);
+        if (misaligned(t[i].data, size(t[i]))) return fail(LLMT_B200_ERR_INVALID, "%s: %s is not aligned to its element type", who, t[i].name);
+        *wide = *wide && !misaligned(t[i].data, 16) && (d->rows <= 1 || t[i].ld % 8 == 0);
+    }
+    for (int i = 0; i < n; ++i)
+        for (int j = 0; j < n; ++j) {
+            if (i == j || !t[i].written || t[i].data == nullptr || t[j].data == nullptr) continue;
+            if (((t[i].data == a && t[j].data == b) || (t[i].data == b && t[j].data == a)) && a == b && t[i].ld == t[j].ld && size(t[i]) == size(t[j])) continue;
+            if (overlaps(t[i].data, bytes(t[i]), t[j].data, bytes(t[j]))) return fail(LLMT_B200_ERR_INVALID, "%s: %s overlaps %s", who, t[i].name, t[j].name);
+        }
+    return LLMT_B200_OK;
+}
+
+}  // namespace
+
+int llmt_b200_norm_residual_fwd(const llmt_b200_norm_residual_desc* d, void* stream) {
+    const char* who = "norm_residual_fwd";
+    NormResidualParams p;
+    int st = norm_residual_params(d, who, &p);
+    if (st != LLMT_B200_OK || d->rows == 0) return st;
+    if (d->x == nullptr || (d->y != nullptr && d->out == nullptr)) return fail(LLMT_B200_ERR_INVALID, "%s: invalid tensor (null data)", who);
+    if ((d->h == nullptr) != (d->w_pre == nullptr)) return fail(LLMT_B200_ERR_INVALID, "%s: h and w_pre go together", who);
+    if (d->y == nullptr && d->h == nullptr) return fail(LLMT_B200_ERR_INVALID, "%s: neither y nor h: nothing to do", who);
+    const RowTensor t[4] = {{"x", d->x, d->ld_x, false, false}, {"y", d->y, d->ld_y, true, false},
+                            {"out", d->y != nullptr ? d->out : nullptr, d->ld_out, false, true}, {"h", d->h, d->ld_h, true, true}};
+    bool wide = d->cols % 8 == 0 && !misaligned(d->w_post, 16) && !misaligned(d->gate, 16) && !misaligned(d->w_pre, 16);
+    st = norm_residual_tensors(d, who, t, 4, d->x, d->out, &wide);
+    if (st != LLMT_B200_OK) return st;
+    const cudaError_t e = launch_norm_residual_fwd(p, d->dtype_res == LLMT_B200_BF16, d->dtype_act == LLMT_B200_BF16, wide, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return fail(LLMT_B200_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
+    return LLMT_B200_OK;
+}
+
+uint64_t llmt_b200_norm_residual_workspace_bytes(const llmt_b200_norm_residual_desc* d) {
+    NormResidualParams p;
+    if (norm_residual_params(d, "norm_residual_bwd", &p) != LLMT_B200_OK || d->rows == 0) return 0;
+    const NormResidualPlan pl = norm_residual_plan(d->rows, d->cols, d->groups, d->dw_post != nullptr || d->dw_pre != nullptr, d->dgate != nullptr, sm_count());
+    if (pl.floats_w + pl.floats_gate == 0) return 0;
+    return static_cast<uint64_t>(pl.floats_w + pl.floats_gate + 8) / 4 * 16;   // both parts start on 16 bytes
+}
+
+int llmt_b200_norm_residual_bwd(const llmt_b200_norm_residual_desc* d, void* stream) {
+    const char* who = "norm_residual_bwd";
+    NormResidualParams p;
+    int st = norm_residual_params(d, who, &p);
+    if (st != LLMT_B200_OK) return st;
+    if (d->rows > 0 && (d->dh == nullptr) != (d->w_pre == nullptr)) return fail(LLMT_B200_ERR_INVALID, "%s: dh and w_pre go together", who);
+    if ((d->dw_post != nullptr && d->w_post == nullptr) || (d->dgate != nullptr && d->gate == nullptr) || (d->dw_pre != nullptr && d->w_pre == nullptr))
+        return fail(LLMT_B200_ERR_INVALID, "%s: the gradient of a weight that is null", who);
+    if (d->rows > 0) {
+        if (d->dx == nullptr || (d->dout == nullptr && d->dh == nullptr) || (d->dh != nullptr && (d->out == nullptr || d->rstd_pre == nullptr)) ||
+            (d->y != nullptr && (d->dy == nullptr || (d->w_post != nullptr && d->rstd_post == nullptr))))
+            return fail(LLMT_B200_ERR_INVALID, "%s: invalid tensor (null data)", who);
+    }
+    for (const void* f : {static_cast<const void*>(d->dw_post), static_cast<const void*>(d->dgate), static_cast<const void*>(d->dw_pre)})
+        if (misaligned(f, 4)) return fail(LLMT_B200_ERR_INVALID, "%s: a weight gradient is not aligned to its element type", who);
+    const RowTensor t[6] = {{"out", d->dh != nullptr ? d->out : nullptr, d->ld_out, false, false}, {"y", d->y, d->ld_y, true, false},
+                            {"dout", d->dout, d->ld_dout, false, false}, {"dh", d->dh, d->ld_dh, true, false},
+                            {"dx", d->dx, d->ld_dx, false, true}, {"dy", d->y != nullptr ? d->dy : nullptr, d->ld_dy, true, true}};
+    bool wide = d->cols % 8 == 0 && !misaligned(d->w_post, 16) && !misaligned(d->gate, 16) && !misaligned(d->w_pre, 16);
+    if (d->rows > 0) {
+        st = norm_residual_tensors(d, who, t, 6, d->dx, d->dout, &wide);
+        if (st != LLMT_B200_OK) return st;
+    }
+    // what is summed over the rows: written apart from everything that is read, and from one another
+    struct { const char* name; const float* data; int64_t n; } sums[3] = {{"dw_post", d->dw_post, d->cols}, {"dgate", d->dgate, d->groups * d->cols}, {"dw_pre", d->dw_pre, d->cols}};
+    struct { const char* name; const float* data; int64_t n; } read[5] = {{"w_post", d->w_post, d->cols}, {"gate", d->gate, d->groups * d->cols}, {"w_pre", d->w_pre, d->cols},
+                                                                          {"rstd_post", d->rstd_post, d->rows}, {"rstd_pre", d->rstd_pre, d->rows}};
+    for (int i = 0; i < 3; ++i) {
+        if (sums[i].data == nullptr) continue;
+        for (int j = 0; j < 5; ++j)
+            if (read[j].data != nullptr && overlaps(sums[i].data, 4 * sums[i].n, read[j].data, 4 * read[j].n))
+                return fail(LLMT_B200_ERR_INVALID, "%s: %s overlaps %s", who, sums[i].name, read[j].name);
+        for (int j = 0; j < i; ++j)
+            if (sums[j].data != nullptr && overlaps(sums[i].data, 4 * sums[i].n, sums[j].data, 4 * sums[j].n))
+                return fail(LLMT_B200_ERR_INVALID, "%s: %s overlaps %s", who, sums[i].name, sums[j].name);
+    }
+    const NormResidualPlan pl = norm_residual_plan(d->rows, d->cols, d->groups, d->dw_post != nullptr || d->dw_pre != nullptr, d->dgate != nullptr, sm_count());
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (d->rows == 0) {   // sums of nothing
+        for (const auto& g : sums) {
+            if (g.data == nullptr || d->beta == 1.0f) continue;
+            if (d->beta != 0.0f) return fail(LLMT_B200_ERR_UNSUPPORTED, "%s: beta other than 0 and 1 with no rows", who);
+            const cudaError_t e = launch_zero_f32(const_cast<float*>(g.data), g.n, s);
+            if (e != cudaSuccess) return fail(LLMT_B200_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
+        }
+        return LLMT_B200_OK;
+    }
+    const uint64_t need = llmt_b200_norm_residual_workspace_bytes(d);
+    if (need > 0) {
+        if (d->workspace == nullptr || d->workspace_bytes < need)
+            return fail(LLMT_B200_ERR_WORKSPACE, "%s: workspace of %llu bytes needed, %llu given", who, (unsigned long long)need,
+                        (unsigned long long)(d->workspace == nullptr ? 0 : d->workspace_bytes));
+        if (misaligned(d->workspace, 16)) return fail(LLMT_B200_ERR_INVALID, "%s: workspace is not 16-byte aligned", who);
+        for (const RowTensor& x : t) {
+            const size_t es = (x.act ? d->dtype_act : d->dtype_res) == LLMT_B200_BF16 ? 2 : 4;
+            if (x.data != nullptr && overlaps(d->workspace, need, x.data, (static_cast<size_t>(d->rows - 1) * x.ld + d->cols) * es))
+                return fail(LLMT_B200_ERR_INVALID, "%s: workspace overlaps %s", who, x.name);
+        }
+        for (const auto& x : sums)
+            if (x.data != nullptr && overlaps(d->workspace, need, x.data, 4 * x.n)) return fail(LLMT_B200_ERR_INVALID, "%s: workspace overlaps %s", who, x.name);
+        for (const auto& x : read)
+            if (x.data != nullptr && overlaps(d->workspace, need, x.data, 4 * x.n)) return fail(LLMT_B200_ERR_INVALID, "%s: workspace overlaps %s", who, x.name);
+        p.part_w = pl.floats_w > 0 ? static_cast<float*>(d->workspace) : nullptr;
+        p.part_gate = pl.floats_gate > 0 ? static_cast<float*>(d->workspace) + (pl.floats_w + 3) / 4 * 4 : nullptr;
+    }
+    p.cluster = pl.cluster;
+    p.dout = d->dout; p.dh = d->dh; p.dx = d->dx; p.dy = d->dy;
+    p.ld_dout = d->ld_dout; p.ld_dh = d->ld_dh; p.ld_dx = d->ld_dx; p.ld_dy = d->ld_dy;
+    p.dw_post = d->dw_post; p.dgate = d->dgate; p.dw_pre = d->dw_pre;
+    const cudaError_t e = launch_norm_residual_bwd(p, pl, d->dtype_res == LLMT_B200_BF16, d->dtype_act == LLMT_B200_BF16, wide, d->beta, s);
     if (e != cudaSuccess) return fail(LLMT_B200_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
     return LLMT_B200_OK;
 }

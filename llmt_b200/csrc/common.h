@@ -223,6 +223,41 @@ struct RepackJobs {
     int32_t count;
 };
 
+// Rotary positions (rope.cu).  Strides in elements.
+struct RopeParams {
+    const void* x;
+    void* y;
+    int64_t x_batch, x_token, x_head, y_batch, y_token, y_head;
+    const double* freqs;       // radians per token, [rot / 2]
+    const int32_t* positions;  // [batch * tokens], or null: offset + the token's index
+    int64_t offset, tokens, total;   // tokens of a sequence, of all sequences
+    int32_t heads, head_dim, rot;
+    int32_t interleaved, inverse, copy_rest;   // copy_rest: y is not x, the values behind the rotated ones move too
+    int32_t per_block;
+    float scale;
+};
+
+// The norms around a block with its gate and residual (norm_residual.cu).
+struct NormResidualParams {
+    int64_t rows;
+    int64_t rows_per_gate;     // rows that share a gate row
+    int32_t cols, cluster;     // cluster: blocks that own a row together (backward)
+    const void *x, *y;
+    void *out, *h;
+    int64_t ld_x, ld_y, ld_out, ld_h, ld_dout, ld_dh, ld_dx, ld_dy;
+    const float *w_post, *gate, *w_pre;
+    float *rstd_post, *rstd_pre;
+    float scale, eps;
+    const void *dout, *dh;
+    void *dx, *dy;
+    float *dw_post, *dgate, *dw_pre;
+    float *part_w, *part_gate;   // workspace: [blocks][2][cols], [units][cols]
+};
+struct NormResidualPlan {
+    int cluster, warps, blocks, units, per_group;
+    int64_t floats_w, floats_gate;
+};
+
 // tanh-GELU in fp32, the expression of llmt's gelu kernel (src/kernels/gelu.cu:23-26).
 __device__ __forceinline__ float gelu_tanh_precise(float v) {
     const float k0 = 0.7978845608028654f, k1 = 0.044715f;
@@ -329,6 +364,12 @@ cudaError_t launch_ce_grad_rows(void* out, const float* lse, const float* mask, 
 cudaError_t launch_lse_from_stats(float* lse, const void* stats, int64_t rows, int parts, cudaStream_t stream);
 cudaError_t launch_rowdot(float* out, const void* x, const void* y, int64_t rows, int64_t cols, int64_t ldx,
                           int64_t ldy, int is_bf16, cudaStream_t stream);
+cudaError_t launch_rope(RopeParams p, int is_bf16, cudaStream_t stream);
+int norm_residual_max_cols(void);
+NormResidualPlan norm_residual_plan(int64_t rows, int64_t cols, int64_t groups, bool want_w, bool want_gate, int sms);
+cudaError_t launch_norm_residual_fwd(const NormResidualParams& p, int res_bf16, int act_bf16, bool wide, cudaStream_t stream);
+cudaError_t launch_norm_residual_bwd(const NormResidualParams& p, const NormResidualPlan& pl, int res_bf16, int act_bf16, bool wide, float beta,
+                                     cudaStream_t stream);
 DeviceStatus* device_status_ptr(void);
 
 void count_launch(int n);
