@@ -488,6 +488,47 @@ LLMT_B200_API int llmt_b200_norm_residual_fwd(const llmt_b200_norm_residual_desc
 LLMT_B200_API int llmt_b200_norm_residual_bwd(const llmt_b200_norm_residual_desc* desc, void* stream);
 LLMT_B200_API uint64_t llmt_b200_norm_residual_workspace_bytes(const llmt_b200_norm_residual_desc* desc);
 
+/* Causal attention with a sliding window and first tokens that stay visible (sinks), without the
+ * T x T probabilities of llmt's Naive composition (llmt include/llmt/kernels/attention.h:26-31 names
+ * a fused backend and has none).  bf16 tensors, fp32 arithmetic; the probabilities, and in the
+ * backward pass dS, are rounded to bf16 where they are operands of a product.
+ *   query i stands at p = i + tokens_k - tokens_q; it sees key j when j <= p and
+ *   (window <= 0 or j > p - window or j < sinks).
+ *   S = scale q k^T,  out = softmax over the visible keys of S, times v,  lse = log sum exp S
+ * A query that sees nothing (tokens_q > tokens_k) has a row of zeros and lse = -inf.  What hidden keys
+ * and queries hold, NaN and infinity among it, reaches no result.
+ *   q, out, dout, dq  [batch, tokens_q, heads, head_dim];  k, v, dk, dv  [batch, tokens_k, kv_heads, head_dim]
+ *   heads is a multiple of kv_heads: query head h reads key head h / (heads / kv_heads), and dk, dv are
+ *   summed over the heads that share them, in a fixed order.
+ *   head_dim is a multiple of 8, at most 128; bases are 16-byte aligned and strides multiples of 8
+ *   elements.  Results must not overlap one another or anything that is read.
+ *   lse  fp32 [batch, heads, tokens_q]: written by _fwd (NULL: not wanted), read by _bwd.
+ *
+ * _bwd: dV = P^T dO,  dS = P (dO v^T - rowsum(dO out)),  dQ = scale dS k,  dK = scale dS^T q, from out and lse as
+ * _fwd left them.  workspace: 16-byte aligned, llmt_b200_attention_window_workspace_bytes(desc) bytes.
+ *
+ * _decode: one new token per sequence (tokens_q = 1) over a cache of tokens_k places, of which
+ * sequence b holds lengths[b] (device, int32; NULL: all; values beyond tokens_k count as tokens_k,
+ * below 1 as none): the query stands at lengths[b] - 1, the newest key.  Places behind are not read.
+ *
+ * _fwd and _bwd occupy whole SMs, whatever llmt_b200_set_sm_budget says: their blocks are short. */
+typedef struct llmt_b200_attention_desc {
+    int64_t batch, heads, kv_heads, tokens_q, tokens_k, head_dim;
+    int64_t window, sinks;
+    float scale;
+    int32_t dtype;
+    llmt_b200_head_view q, k, v, out;
+    float* lse;
+    const int32_t* lengths;
+    llmt_b200_head_view dout, dq, dk, dv;
+    void* workspace;
+    uint64_t workspace_bytes;
+} llmt_b200_attention_desc;
+LLMT_B200_API int llmt_b200_attention_window_fwd(const llmt_b200_attention_desc* desc, void* stream);
+LLMT_B200_API int llmt_b200_attention_window_bwd(const llmt_b200_attention_desc* desc, void* stream);
+LLMT_B200_API int llmt_b200_attention_window_decode(const llmt_b200_attention_desc* desc, void* stream);
+LLMT_B200_API uint64_t llmt_b200_attention_window_workspace_bytes(const llmt_b200_attention_desc* desc);
+
 /* The same exchange with all `world` ranks living on ONE device (comms[r] is rank r's
  * descriptor, every pointer local): a single cooperative launch of world * ctas CTAs.
  * For tests of the algorithm where fewer GPUs than ranks are at hand. */

@@ -33,7 +33,8 @@ EXPORTS = [
     "llmt_b200_gemm_softmax_workspace_bytes", "llmt_b200_gemm_softmax_fwd", "llmt_b200_gemm_softmax_bwd",
     "llmt_b200_rowdot", "llmt_b200_cross_entropy_bwd", "llmt_b200_lm_head_ce_bwd",
     "llmt_b200_rope", "llmt_b200_rope_frequencies", "llmt_b200_norm_residual_fwd", "llmt_b200_norm_residual_bwd",
-    "llmt_b200_norm_residual_workspace_bytes",
+    "llmt_b200_norm_residual_workspace_bytes", "llmt_b200_attention_window_fwd", "llmt_b200_attention_window_bwd",
+    "llmt_b200_attention_window_decode", "llmt_b200_attention_window_workspace_bytes",
 ]
 
 COMM_MAX_RANKS, COMM_MAX_CTAS = 8, 128
@@ -93,6 +94,14 @@ class NormResidualDesc(ctypes.Structure):
                 + [(n, ctypes.c_int64) for n in ("ld_dout", "ld_dh", "ld_dx", "ld_dy")]
                 + [(n, ctypes.c_void_p) for n in ("dw_post", "dgate", "dw_pre")]
                 + [("beta", ctypes.c_float), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)])
+
+
+class AttentionDesc(ctypes.Structure):
+    """llmt_b200_attention_desc of include/llmt_b200.h."""
+    _fields_ = ([(n, ctypes.c_int64) for n in ("batch", "heads", "kv_heads", "tokens_q", "tokens_k", "head_dim", "window", "sinks")]
+                + [("scale", ctypes.c_float), ("dtype", ctypes.c_int32)] + [(n, HeadView) for n in ("q", "k", "v", "out")]
+                + [("lse", ctypes.c_void_p), ("lengths", ctypes.c_void_p)] + [(n, HeadView) for n in ("dout", "dq", "dk", "dv")]
+                + [("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)])
 
 
 class LlmtB200Error(RuntimeError):
@@ -195,6 +204,11 @@ def lib() -> ctypes.CDLL:
         L.llmt_b200_norm_residual_bwd.restype = ctypes.c_int
         L.llmt_b200_norm_residual_workspace_bytes.argtypes = [ctypes.POINTER(NormResidualDesc)]
         L.llmt_b200_norm_residual_workspace_bytes.restype = ctypes.c_uint64
+        for name in ("fwd", "bwd", "decode"):
+            f = getattr(L, "llmt_b200_attention_window_" + name)
+            f.argtypes, f.restype = [ctypes.POINTER(AttentionDesc), ctypes.c_void_p], ctypes.c_int
+        L.llmt_b200_attention_window_workspace_bytes.argtypes = [ctypes.POINTER(AttentionDesc)]
+        L.llmt_b200_attention_window_workspace_bytes.restype = ctypes.c_uint64
         L.llmt_b200_exchange_begin_step.argtypes = [ctypes.POINTER(CommDesc), ctypes.c_void_p]
         L.llmt_b200_exchange_begin_step.restype = ctypes.c_int
         L.llmt_b200_zero_grads.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]
@@ -703,6 +717,78 @@ def norm_residual_workspace_bytes(rows: int, cols: int, groups: int = 1, weights
     if gate:
         d.dgate = 4
     return int(lib().llmt_b200_norm_residual_workspace_bytes(ctypes.byref(d)))
+
+
+def _attention_desc(who: str, q, k, v, window: int, sinks: int, scale, results: dict) -> "AttentionDesc":
+    """q [B, Tq, H, hd], k and v [B, Tk, Hkv, hd]; `results`: name -> (tensor, what it is laid out like)."""
+    d = AttentionDesc()
+    for name, t in (("q", q), ("k", k), ("v", v), *((n, t) for n, (t, _) in results.items())):
+        setattr(d, name, _heads(t, who, name))
+        _need(t.dtype == q.dtype, f"{who}: {name} has another type than q")
+    _need(k.shape == v.shape and k.shape[0] == q.shape[0] and k.shape[3] == q.shape[3], f"{who}: k and v must be [batch, tokens, kv_heads, head_dim] for q's batch and head_dim")
+    for name, (t, like) in results.items():
+        _need(t.shape == like.shape, f"{who}: {name} must have the shape {tuple(like.shape)}")
+    d.batch, d.tokens_q, d.heads, d.head_dim = q.shape
+    d.tokens_k, d.kv_heads = k.shape[1], k.shape[2]
+    d.window, d.sinks, d.dtype = int(window), int(sinks), _dtype_code(q)
+    d.scale = float(scale) if scale is not None else d.head_dim ** -0.5 if d.head_dim else 1.0
+    return d
+
+
+def _put_lse(d: "AttentionDesc", who: str, lse, rows: int) -> None:
+    import torch
+    if lse is not None:
+        _need(lse.dtype == torch.float32 and lse.is_contiguous() and lse.numel() == rows, f"{who}: lse must be contiguous fp32 with one value per query and head")
+        d.lse = lse.data_ptr()
+
+
+def attention_window_fwd(out, lse, q, k, v, window: int = 0, sinks: int = 0, scale=None, stream=None) -> None:
+    """Causal attention of q [B, Tq, H, hd] over k, v [B, Tk, Hkv, hd] (any strides) into out, where a query at
+    p = i + Tk - Tq sees keys j <= p that are among the last `window` (0: all) or the first `sinks`
+    (llmt_b200_attention_window_fwd).  lse: fp32 [B, H, Tq] for the backward pass, or None.  scale: 1 / sqrt(hd) if None."""
+    who = "attention_window_fwd"
+    d = _attention_desc(who, q, k, v, window, sinks, scale, dict(out=(out, q)))
+    _put_lse(d, who, lse, d.batch * d.heads * d.tokens_q)
+    _on(_device_of(who, out, lse, q, k, v), stream, lambda s: lib().llmt_b200_attention_window_fwd(ctypes.byref(d), s))
+
+
+def attention_window_bwd(dq, dk, dv, dout, q, k, v, out, lse, window: int = 0, sinks: int = 0, scale=None, workspace=None, stream=None) -> None:
+    """The gradients of attention_window_fwd from its inputs and what it left (llmt_b200_attention_window_bwd); dk and dv
+    are summed over the heads that share a key head.  `workspace`: a uint8 tensor of attention_window_workspace_bytes,
+    or one is allocated for the call."""
+    who = "attention_window_bwd"
+    d = _attention_desc(who, q, k, v, window, sinks, scale, dict(out=(out, q), dout=(dout, q), dq=(dq, q), dk=(dk, k), dv=(dv, v)))
+    _put_lse(d, who, lse, d.batch * d.heads * d.tokens_q)
+
+    def call(s):
+        ws = workspace
+        if ws is None:
+            need = lib().llmt_b200_attention_window_workspace_bytes(ctypes.byref(d))
+            ws = _scratch(need, q, stream) if need else None
+        if ws is not None:
+            d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
+        return lib().llmt_b200_attention_window_bwd(ctypes.byref(d), s)
+    _on(_device_of(who, dq, dk, dv, dout, q, k, v, out, lse, workspace), stream, call)
+
+
+def attention_window_workspace_bytes(q, k, window: int = 0, sinks: int = 0) -> int:
+    """Scratch of attention_window_bwd for tensors of these shapes on the current device."""
+    d = _attention_desc("attention_window_workspace_bytes", q, k, k, window, sinks, None, {})
+    return int(lib().llmt_b200_attention_window_workspace_bytes(ctypes.byref(d)))
+
+
+def attention_window_decode(out, q, k, v, lengths=None, window: int = 0, sinks: int = 0, scale=None, lse=None, stream=None) -> None:
+    """attention_window_fwd for one new token per sequence: q, out [B, H, hd] over a cache k, v [B, places, Hkv, hd] of which
+    sequence b holds lengths[b] (int32 on the device; None: all), the new token's key the last of them."""
+    import torch
+    who = "attention_window_decode"
+    _need(q.dim() == 3 and out.dim() == 3, f"{who}: q and out must be [batch, heads, head_dim]")
+    d = _attention_desc(who, q.unsqueeze(1), k, v, window, sinks, scale, dict(out=(out.unsqueeze(1), q.unsqueeze(1))))
+    if lengths is not None:
+        _need(lengths.dtype == torch.int32 and lengths.is_contiguous() and lengths.numel() == q.shape[0], f"{who}: lengths must be contiguous int32 [batch]")
+        d.lengths = lengths.data_ptr()
+    _put_lse(d, who, lse, d.batch * d.heads)
+    _on(_device_of(who, out, q, k, v, lengths, lse), stream, lambda s: lib().llmt_b200_attention_window_decode(ctypes.byref(d), s))
 
 
 def exchange_begin_step(desc: "CommDesc", stream=None) -> None:

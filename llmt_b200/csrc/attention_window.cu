@@ -1,0 +1,68 @@
+// Causal attention with a sliding window and sinks, forward, backward and for one new token: a warp for each row.
+#include "attention_rows.cuh"
+#include "ptx_sm100.cuh"
+
+namespace llmt_b200 {
+namespace {
+
+constexpr int kRowThreads = 128;
+
+__global__ void __launch_bounds__(kRowThreads) attention_fwd_rows_kernel(AttentionParams p) {
+    ptx::grid_dependency_wait();
+    const int64_t row = (static_cast<int64_t>(blockIdx.x) * kRowThreads + threadIdx.x) >> 5;
+    if (row >= static_cast<int64_t>(p.batch) * p.heads * p.tq) return;
+    const int64_t i = row % p.tq, bh = row / p.tq;
+    attn::forward_row(p, bh / p.heads, bh % p.heads, i, i + p.tk - p.tq);
+}
+
+__global__ void __launch_bounds__(kRowThreads) attention_dq_rows_kernel(AttentionParams p) {
+    ptx::grid_dependency_wait();
+    const int64_t row = (static_cast<int64_t>(blockIdx.x) * kRowThreads + threadIdx.x) >> 5;
+    if (row >= static_cast<int64_t>(p.batch) * p.heads * p.tq) return;
+    const int64_t i = row % p.tq, bh = row / p.tq, b = bh / p.heads, h = bh % p.heads;
+    const float d = attn::dot_rows(attn::row_of(p.dout, b, i, h), attn::row_of(p.out, b, i, h), p.head_dim);
+    if ((threadIdx.x & 31) == 0) p.dvec[row] = d;
+    attn::dq_row(p, b, h, i, d);
+}
+
+__global__ void __launch_bounds__(kRowThreads) attention_dkdv_rows_kernel(AttentionParams p) {
+    ptx::grid_dependency_wait();
+    const int64_t row = (static_cast<int64_t>(blockIdx.x) * kRowThreads + threadIdx.x) >> 5;
+    const int64_t hkv = p.heads / p.group;
+    if (row >= static_cast<int64_t>(p.batch) * hkv * p.tk) return;
+    const int64_t j = row % p.tk, bh = row / p.tk;
+    attn::dkdv_row(p, bh / hkv, bh % hkv, j);
+}
+
+__global__ void __launch_bounds__(kRowThreads) attention_decode_rows_kernel(AttentionParams p) {
+    ptx::grid_dependency_wait();
+    const int64_t row = (static_cast<int64_t>(blockIdx.x) * kRowThreads + threadIdx.x) >> 5;
+    if (row >= static_cast<int64_t>(p.batch) * p.heads) return;
+    const int64_t b = row / p.heads;
+    int64_t n = p.lengths != nullptr ? p.lengths[b] : p.tk;
+    n = n < p.tk ? n : p.tk;   // never past the cache
+    attn::forward_row(p, b, row % p.heads, 0, n - 1);
+}
+
+unsigned row_blocks(int64_t rows) { return static_cast<unsigned>((rows * 32 + kRowThreads - 1) / kRowThreads); }
+
+}  // namespace
+
+size_t attention_window_bwd_workspace(const AttentionParams& p) { return static_cast<size_t>(p.batch) * p.heads * p.tq * sizeof(float); }
+
+cudaError_t launch_attention_window_fwd(const AttentionParams& p, cudaStream_t stream) {
+    return launch_dependent(attention_fwd_rows_kernel, row_blocks(static_cast<int64_t>(p.batch) * p.heads * p.tq), kRowThreads, stream, p);
+}
+cudaError_t launch_attention_window_bwd(AttentionParams p, void* workspace, cudaStream_t stream) {
+    p.dvec = static_cast<float*>(workspace);
+    if (p.tq > 0) {
+        const cudaError_t e = launch_dependent(attention_dq_rows_kernel, row_blocks(static_cast<int64_t>(p.batch) * p.heads * p.tq), kRowThreads, stream, p);
+        if (e != cudaSuccess || p.tk == 0) return e;
+    }
+    return launch_dependent(attention_dkdv_rows_kernel, row_blocks(static_cast<int64_t>(p.batch) * (p.heads / p.group) * p.tk), kRowThreads, stream, p);
+}
+cudaError_t launch_attention_window_decode(const AttentionParams& p, cudaStream_t stream) {
+    return launch_dependent(attention_decode_rows_kernel, row_blocks(static_cast<int64_t>(p.batch) * p.heads), kRowThreads, stream, p);
+}
+
+}  // namespace llmt_b200

@@ -2000,6 +2000,182 @@ int llmt_b200_norm_residual_bwd(const llmt_b200_norm_residual_desc* d, void* str
     return LLMT_B200_OK;
 }
 
+namespace {
+
+struct NamedView {
+    const char* name;
+    const llmt_b200_head_view* v;
+    bool keys, written;   // tokens_k and kv_heads; a result
+};
+
+// The checks that the attention calls share; fills in everything but the gradients.
+int attention_params(const llmt_b200_attention_desc* d, const char* who, AttentionParams* p) {
+    if (d == nullptr) return fail(LLMT_B200_ERR_INVALID, "%s: null descriptor", who);
+    if (d->batch < 0 || d->heads < 0 || d->tokens_q < 0 || d->tokens_k < 0 || d->kv_heads < 0 || d->head_dim < 1 || d->sinks < 0)
+        return fail(LLMT_B200_ERR_INVALID, "%s: negative dimension", who);
+    if (d->heads > 0 && (d->kv_heads == 0 || d->heads % d->kv_heads != 0))
+        return fail(LLMT_B200_ERR_INVALID, "%s: heads (%lld) must be a multiple of kv_heads (%lld)", who, (long long)d->heads, (long long)d->kv_heads);
+    if (d->dtype != LLMT_B200_BF16) return fail(LLMT_B200_ERR_UNSUPPORTED, "%s: no kernel for dtype code %d (bf16 only)", who, d->dtype);
+    if (d->head_dim > 128 || d->head_dim % 8 != 0)
+        return fail(LLMT_B200_ERR_UNSUPPORTED, "%s: head_dim %lld is not a multiple of 8 up to 128", who, (long long)d->head_dim);
+    constexpr int64_t kMaxDim = 0x7fffffff - 1024;
+    if (d->tokens_q > kMaxDim || d->tokens_k > kMaxDim || d->batch > kMaxDim || d->heads > 65536)
+        return fail(LLMT_B200_ERR_UNSUPPORTED, "%s: dimension above 2^31 - 1025, or more than 65536 heads", who);
+    // a warp or more for each row of each head, counted in 32 bits
+    const int64_t rows = d->tokens_q > d->tokens_k ? d->tokens_q : d->tokens_k;
+    if (static_cast<__int128>(rows) * d->heads * d->batch > (int64_t{1} << 32))
+        return fail(LLMT_B200_ERR_UNSUPPORTED, "%s: more than 2^32 rows over all heads", who);
+    if (misaligned(d->lse, 4) || misaligned(d->lengths, 4)) return fail(LLMT_B200_ERR_INVALID, "%s: lse or lengths is not aligned to its element type", who);
+    *p = AttentionParams{};
+    auto view = [&](const llmt_b200_head_view& v, int64_t tokens, int64_t heads) {
+        const llmt_b200_head_view x = without_idle_strides(v, d->batch, tokens, heads);
+        return HeadView{x.data, x.stride_batch, x.stride_token, x.stride_head};
+    };
+    p->q = view(d->q, d->tokens_q, d->heads);
+    p->k = view(d->k, d->tokens_k, d->kv_heads);
+    p->v = view(d->v, d->tokens_k, d->kv_heads);
+    p->out = view(d->out, d->tokens_q, d->heads);
+    p->dout = view(d->dout, d->tokens_q, d->heads);
+    p->dq = view(d->dq, d->tokens_q, d->heads);
+    p->dk = view(d->dk, d->tokens_k, d->kv_heads);
+    p->dv = view(d->dv, d->tokens_k, d->kv_heads);
+    p->lse = d->lse;
+    p->lengths = d->lengths;
+    p->batch = static_cast<int32_t>(d->batch);
+    p->heads = static_cast<int32_t>(d->heads);
+    p->group = d->heads > 0 ? static_cast<int32_t>(d->heads / d->kv_heads) : 1;
+    p->tq = static_cast<int32_t>(d->tokens_q);
+    p->tk = static_cast<int32_t>(d->tokens_k);
+    p->head_dim = static_cast<int32_t>(d->head_dim);
+    const int64_t most = d->tokens_k > 0 ? d->tokens_k : 1;
+    p->window = static_cast<int32_t>(d->window <= 0 || d->window > most ? most : d->window);
+    p->sinks = static_cast<int32_t>(d->sinks > d->tokens_k ? d->tokens_k : d->sinks);
+    p->scale = d->scale;
+    return LLMT_B200_OK;
+}
+
+// The views of a call: there, aligned, with strides that are multiples of 8 elements; results distinct in themselves and
+// apart from everything else.
+int attention_views(const llmt_b200_attention_desc* d, const char* who, const NamedView* t, int n) {
+    int64_t bytes[8];
+    llmt_b200_head_view view[8];
+    for (int i = 0; i < n; ++i) {
+        const int64_t tokens = t[i].keys ? d->tokens_k : d->tokens_q, heads = t[i].keys ? d->kv_heads : d->heads;
+        bytes[i] = 0;
+        view[i] = without_idle_strides(*t[i].v, d->batch, tokens, heads);
+        if (tokens == 0 || heads == 0 || d->batch == 0) continue;   // an empty tensor may have no address
+        if (view[i].data == nullptr) return fail(LLMT_B200_ERR_INVALID, "%s: invalid tensor %s (null data)", who, t[i].name);
+        const int64_t extent = view_extent(view[i], d->batch, tokens, heads, d->head_dim);
+        if (extent < 0) return fail(LLMT_B200_ERR_INVALID, "%s: negative or overlong strides of %s", who, t[i].name);
+        if (misaligned(view[i].data, 16) || (view[i].stride_batch | view[i].stride_token | view[i].stride_head) % 8 != 0)
+            return fail(LLMT_B200_ERR_INVALID, "%s: %s needs a 16-byte aligned base and strides that are multiples of 8 elements", who, t[i].name);
+        if (t[i].written && !view_distinct(view[i], d->batch, tokens, heads, d->head_dim))
+            return fail(LLMT_B200_ERR_INVALID, "%s: the elements of %s overlap one another", who, t[i].name);
+        bytes[i] = 2 * extent;
+    }
+    // Two views may lie in each other's rows (dq, dk and dv of a packed projection): they are apart if one base is behind the
+    // other by less than the smallest common stride leaves room for.
+    auto apart = [&](int a, int b) {
+        if (bytes[a] == 0 || bytes[b] == 0 || !overlaps(view[a].data, bytes[a], view[b].data, bytes[b])) return true;
+        if (reinterpret_cast<uintptr_t>(view[a].data) > reinterpret_cast<uintptr_t>(view[b].data)) { const int c = a; a = b; b = c; }
+        const int64_t gap = static_cast<int64_t>(reinterpret_cast<uintptr_t>(view[b].data) - reinterpret_cast<uintptr_t>(view[a].data)) / 2;
+        auto heads = [&](int i) { return t[i].keys ? d->kv_heads : d->heads; };
+        auto tokens = [&](int i) { return t[i].keys ? d->tokens_k : d->tokens_q; };
+        // token rows of one pitch, both within the first view's row
+        const int64_t wa = (heads(a) - 1) * view[a].stride_head + d->head_dim, wb = (heads(b) - 1) * view[b].stride_head + d->head_dim;
+        const int64_t pitch = tokens(a) > 1 ? view[a].stride_token : tokens(b) > 1 ? view[b].stride_token : d->batch > 1 ? view[a].stride_batch : 0;
+        if ((tokens(a) > 1 && view[a].stride_token != pitch) || (tokens(b) > 1 && view[b].stride_token != pitch)) return false;
+        if (d->batch > 1 && (view[a].stride_batch != view[b].stride_batch || pitch <= 0 || view[a].stride_batch % pitch != 0 ||
+                             (tokens(a) - 1) * pitch + pitch > view[a].stride_batch || (tokens(b) - 1) * pitch + pitch > view[a].stride_batch))
+            return false;
+        return pitch > 0 && wa <= gap && gap + wb <= pitch;
+    };
+    for (int i = 0; i < n; ++i)
+        for (int j = 0; j < n; ++j)
+            if (i != j && t[i].written && !apart(i, j)) return fail(LLMT_B200_ERR_INVALID, "%s: %s overlaps %s", who, t[i].name, t[j].name);
+    return LLMT_B200_OK;
+}
+
+// Whether `bytes` at `at` (lse, workspace) touch any of the views.
+int attention_apart(const llmt_b200_attention_desc* d, const char* who, const char* what, const void* at, size_t bytes, const NamedView* t, int n) {
+    for (int i = 0; i < n && at != nullptr && bytes > 0; ++i) {
+        const int64_t tokens = t[i].keys ? d->tokens_k : d->tokens_q, heads = t[i].keys ? d->kv_heads : d->heads;
+        if (tokens == 0 || heads == 0 || d->batch == 0) continue;
+        const llmt_b200_head_view v = without_idle_strides(*t[i].v, d->batch, tokens, heads);
+        if (overlaps(at, bytes, v.data, 2 * view_extent(v, d->batch, tokens, heads, d->head_dim)))
+            return fail(LLMT_B200_ERR_INVALID, "%s: %s overlaps %s", who, what, t[i].name);
+    }
+    return LLMT_B200_OK;
+}
+
+}  // namespace
+
+int llmt_b200_attention_window_fwd(const llmt_b200_attention_desc* d, void* stream) {
+    const char* who = "attention_window_fwd";
+    AttentionParams p;
+    int st = attention_params(d, who, &p);
+    if (st != LLMT_B200_OK) return st;
+    if (d->lengths != nullptr) return fail(LLMT_B200_ERR_INVALID, "%s: lengths belong to attention_window_decode", who);
+    const NamedView t[4] = {{"q", &d->q, false, false}, {"k", &d->k, true, false}, {"v", &d->v, true, false}, {"out", &d->out, false, true}};
+    st = attention_views(d, who, t, 4);
+    if (st == LLMT_B200_OK) st = attention_apart(d, who, "lse", d->lse, 4 * static_cast<size_t>(d->batch * d->heads * d->tokens_q), t, 4);
+    if (st != LLMT_B200_OK) return st;
+    if (p.batch == 0 || p.heads == 0 || p.tq == 0) return LLMT_B200_OK;
+    const cudaError_t e = launch_attention_window_fwd(p, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return fail(LLMT_B200_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
+    return LLMT_B200_OK;
+}
+
+uint64_t llmt_b200_attention_window_workspace_bytes(const llmt_b200_attention_desc* d) {
+    AttentionParams p;
+    if (attention_params(d, "attention_window_bwd", &p) != LLMT_B200_OK) return 0;
+    return (attention_window_bwd_workspace(p) + 255) / 256 * 256;
+}
+
+int llmt_b200_attention_window_bwd(const llmt_b200_attention_desc* d, void* stream) {
+    const char* who = "attention_window_bwd";
+    AttentionParams p;
+    int st = attention_params(d, who, &p);
+    if (st != LLMT_B200_OK) return st;
+    if (d->lengths != nullptr) return fail(LLMT_B200_ERR_INVALID, "%s: lengths belong to attention_window_decode", who);
+    const NamedView t[8] = {{"q", &d->q, false, false}, {"k", &d->k, true, false}, {"v", &d->v, true, false}, {"out", &d->out, false, false},
+                            {"dout", &d->dout, false, false}, {"dq", &d->dq, false, true}, {"dk", &d->dk, true, true}, {"dv", &d->dv, true, true}};
+    st = attention_views(d, who, t, 8);
+    if (st != LLMT_B200_OK) return st;
+    if (p.batch == 0 || p.heads == 0 || (p.tq == 0 && p.tk == 0)) return LLMT_B200_OK;
+    if (p.tq > 0 && d->lse == nullptr) return fail(LLMT_B200_ERR_INVALID, "%s: invalid tensor lse (null data)", who);
+    st = attention_apart(d, who, "lse", d->lse, 4 * static_cast<size_t>(d->batch * d->heads * d->tokens_q), t + 5, 3);
+    if (st != LLMT_B200_OK) return st;
+    const uint64_t need = llmt_b200_attention_window_workspace_bytes(d);
+    if (need > 0 && (d->workspace == nullptr || d->workspace_bytes < need))
+        return fail(LLMT_B200_ERR_WORKSPACE, "%s: workspace of %llu bytes needed, %llu given", who, (unsigned long long)need,
+                    (unsigned long long)(d->workspace == nullptr ? 0 : d->workspace_bytes));
+    if (misaligned(d->workspace, 16)) return fail(LLMT_B200_ERR_INVALID, "%s: workspace is not 16-byte aligned", who);
+    st = attention_apart(d, who, "workspace", d->workspace, need, t, 8);
+    if (st != LLMT_B200_OK) return st;
+    if (overlaps(d->workspace, need, d->lse, 4 * static_cast<size_t>(d->batch * d->heads * d->tokens_q)))
+        return fail(LLMT_B200_ERR_INVALID, "%s: workspace overlaps lse", who);
+    const cudaError_t e = launch_attention_window_bwd(p, d->workspace, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return fail(LLMT_B200_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
+    return LLMT_B200_OK;
+}
+
+int llmt_b200_attention_window_decode(const llmt_b200_attention_desc* d, void* stream) {
+    const char* who = "attention_window_decode";
+    AttentionParams p;
+    int st = attention_params(d, who, &p);
+    if (st != LLMT_B200_OK) return st;
+    if (d->tokens_q != 1) return fail(LLMT_B200_ERR_INVALID, "%s: tokens_q must be 1 (%lld)", who, (long long)d->tokens_q);
+    const NamedView t[4] = {{"q", &d->q, false, false}, {"k", &d->k, true, false}, {"v", &d->v, true, false}, {"out", &d->out, false, true}};
+    st = attention_views(d, who, t, 4);
+    if (st == LLMT_B200_OK) st = attention_apart(d, who, "lse", d->lse, 4 * static_cast<size_t>(d->batch * d->heads), t, 4);
+    if (st != LLMT_B200_OK) return st;
+    if (p.batch == 0 || p.heads == 0) return LLMT_B200_OK;
+    const cudaError_t e = launch_attention_window_decode(p, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return fail(LLMT_B200_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
+    return LLMT_B200_OK;
+}
+
 int llmt_b200_set_sm_budget(int32_t sms) {
     if (sms < 0) {
         fail(LLMT_B200_ERR_INVALID, "sm budget: must be >= 0 (0 = every SM)");

@@ -258,6 +258,21 @@ struct NormResidualPlan {
     int64_t floats_w, floats_gate;
 };
 
+// Attention with a sliding window and sinks (attention_rows.cuh, attention_window.cu).  bf16; strides in elements.
+struct HeadView {
+    void* data;
+    int64_t stride_batch, stride_token, stride_head;
+};
+struct AttentionParams {
+    HeadView q, k, v, out, dout, dq, dk, dv;
+    float* lse;                // [batch][heads][tq]
+    float* dvec;               // workspace: rowsum(dout * out), [batch][heads][tq]
+    const int32_t* lengths;    // one new token: keys of each sequence, or null (all)
+    int32_t batch, heads, group, tq, tk, head_dim;   // group: query heads that share a key head
+    int32_t window, sinks;     // 1 <= window <= max(tk, 1), 0 <= sinks <= tk
+    float scale;
+};
+
 // tanh-GELU in fp32, the expression of llmt's gelu kernel (src/kernels/gelu.cu:23-26).
 __device__ __forceinline__ float gelu_tanh_precise(float v) {
     const float k0 = 0.7978845608028654f, k1 = 0.044715f;
@@ -370,6 +385,10 @@ NormResidualPlan norm_residual_plan(int64_t rows, int64_t cols, int64_t groups, 
 cudaError_t launch_norm_residual_fwd(const NormResidualParams& p, int res_bf16, int act_bf16, bool wide, cudaStream_t stream);
 cudaError_t launch_norm_residual_bwd(const NormResidualParams& p, const NormResidualPlan& pl, int res_bf16, int act_bf16, bool wide, float beta,
                                      cudaStream_t stream);
+size_t attention_window_bwd_workspace(const AttentionParams& p);
+cudaError_t launch_attention_window_fwd(const AttentionParams& p, cudaStream_t stream);
+cudaError_t launch_attention_window_bwd(AttentionParams p, void* workspace, cudaStream_t stream);
+cudaError_t launch_attention_window_decode(const AttentionParams& p, cudaStream_t stream);
 DeviceStatus* device_status_ptr(void);
 
 void count_launch(int n);
