@@ -501,7 +501,8 @@ LLMT_B200_API uint64_t llmt_b200_norm_residual_workspace_bytes(const llmt_b200_n
  *   heads is a multiple of kv_heads: query head h reads key head h / (heads / kv_heads), and dk, dv are
  *   summed over the heads that share them, in a fixed order.
  *   head_dim is a multiple of 8, at most 128; bases are 16-byte aligned and strides multiples of 8
- *   elements.  Results must not overlap one another or anything that is read.
+ *   elements, not 0 (an operand cannot be broadcast).  Results must not overlap one another or
+ *   anything that is read.  scale is positive.
  *   lse  fp32 [batch, heads, tokens_q]: written by _fwd (NULL: not wanted), read by _bwd.
  *
  * _bwd: dV = P^T dO,  dS = P (dO v^T - rowsum(dO out)),  dQ = scale dS k,  dK = scale dS^T q, from out and lse as

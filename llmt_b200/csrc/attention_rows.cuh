@@ -76,7 +76,7 @@ struct Keys {
 };
 
 // One row of the output and its log-sum-exp, for the query at position `pos`.
-__device__ __noinline__ void forward_row(const AttentionParams& p, int64_t b, int64_t h, int64_t i, int64_t pos) {
+static __device__ __noinline__ void forward_row(const AttentionParams& p, int64_t b, int64_t h, int64_t i, int64_t pos) {
     const int lane = threadIdx.x & 31, hd = p.head_dim;
     const int64_t hk = h / p.group;
     const __nv_bfloat16* q = row_of(p.q, b, i, h);
@@ -100,7 +100,7 @@ __device__ __noinline__ void forward_row(const AttentionParams& p, int64_t b, in
 }
 
 // One row of dQ.
-__device__ __noinline__ void dq_row(const AttentionParams& p, int64_t b, int64_t h, int64_t i, float d) {
+static __device__ __noinline__ void dq_row(const AttentionParams& p, int64_t b, int64_t h, int64_t i, float d) {
     const int lane = threadIdx.x & 31, hd = p.head_dim;
     const int64_t hk = h / p.group;
     const __nv_bfloat16 *q = row_of(p.q, b, i, h), *dout = row_of(p.dout, b, i, h);
@@ -122,7 +122,7 @@ __device__ __noinline__ void dq_row(const AttentionParams& p, int64_t b, int64_t
 }
 
 // One row of dK and dV: the sums over the group's heads and the queries that see key j.
-__device__ __noinline__ void dkdv_row(const AttentionParams& p, int64_t b, int64_t hk, int64_t j) {
+static __device__ __noinline__ void dkdv_row(const AttentionParams& p, int64_t b, int64_t hk, int64_t j) {
     const int lane = threadIdx.x & 31, hd = p.head_dim;
     const __nv_bfloat16 *k = row_of(p.k, b, j, hk), *v = row_of(p.v, b, j, hk);
     const int64_t off = static_cast<int64_t>(p.tk) - p.tq;

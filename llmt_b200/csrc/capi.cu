@@ -2025,6 +2025,7 @@ int attention_params(const llmt_b200_attention_desc* d, const char* who, Attenti
     const int64_t rows = d->tokens_q > d->tokens_k ? d->tokens_q : d->tokens_k;
     if (static_cast<__int128>(rows) * d->heads * d->batch > (int64_t{1} << 32))
         return fail(LLMT_B200_ERR_UNSUPPORTED, "%s: more than 2^32 rows over all heads", who);
+    if (!(d->scale > 0.0f) || !std::isfinite(d->scale)) return fail(LLMT_B200_ERR_INVALID, "%s: scale must be positive and finite", who);
     if (misaligned(d->lse, 4) || misaligned(d->lengths, 4)) return fail(LLMT_B200_ERR_INVALID, "%s: lse or lengths is not aligned to its element type", who);
     *p = AttentionParams{};
     auto view = [&](const llmt_b200_head_view& v, int64_t tokens, int64_t heads) {
@@ -2067,6 +2068,8 @@ int attention_views(const llmt_b200_attention_desc* d, const char* who, const Na
         if (view[i].data == nullptr) return fail(LLMT_B200_ERR_INVALID, "%s: invalid tensor %s (null data)", who, t[i].name);
         const int64_t extent = view_extent(view[i], d->batch, tokens, heads, d->head_dim);
         if (extent < 0) return fail(LLMT_B200_ERR_INVALID, "%s: negative or overlong strides of %s", who, t[i].name);
+        if ((d->batch > 1 && view[i].stride_batch == 0) || (tokens > 1 && view[i].stride_token == 0) || (heads > 1 && view[i].stride_head == 0))
+            return fail(LLMT_B200_ERR_INVALID, "%s: %s is broadcast (a stride of 0)", who, t[i].name);
         if (misaligned(view[i].data, 16) || (view[i].stride_batch | view[i].stride_token | view[i].stride_head) % 8 != 0)
             return fail(LLMT_B200_ERR_INVALID, "%s: %s needs a 16-byte aligned base and strides that are multiples of 8 elements", who, t[i].name);
         if (t[i].written && !view_distinct(view[i], d->batch, tokens, heads, d->head_dim))
@@ -2108,6 +2111,14 @@ int attention_apart(const llmt_b200_attention_desc* d, const char* who, const ch
     return LLMT_B200_OK;
 }
 
+// Tensor map of a head view: boxes of 64 values x box_rows tokens of one head, 128-byte swizzle.
+int head_map(CUtensorMap* map, const HeadView& v, const AttentionParams& p, bool keys, int box_rows) {
+    const int64_t tokens = keys ? p.tk : p.tq, heads = keys ? p.heads / p.group : p.heads;
+    BatchLayout bl;
+    bl.inner = heads; bl.stride = v.stride_head; bl.outer = p.batch; bl.stride_outer = v.stride_batch;
+    return cached_map(map, v.data, 2, tokens, p.head_dim, tokens > 1 ? v.stride_token : p.head_dim, bl, 64, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 }  // namespace
 
 int llmt_b200_attention_window_fwd(const llmt_b200_attention_desc* d, void* stream) {
@@ -2121,7 +2132,21 @@ int llmt_b200_attention_window_fwd(const llmt_b200_attention_desc* d, void* stre
     if (st == LLMT_B200_OK) st = attention_apart(d, who, "lse", d->lse, 4 * static_cast<size_t>(d->batch * d->heads * d->tokens_q), t, 4);
     if (st != LLMT_B200_OK) return st;
     if (p.batch == 0 || p.heads == 0 || p.tq == 0) return LLMT_B200_OK;
-    const cudaError_t e = launch_attention_window_fwd(p, static_cast<cudaStream_t>(stream));
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    cudaError_t e;
+    if (p.tk == 0) {
+        e = launch_attention_window_fwd(p, s);
+    } else {
+        CUtensorMap maps[4];
+        st = head_map(&maps[0], p.q, p, false, 128);
+        if (st == LLMT_B200_OK) st = head_map(&maps[1], p.k, p, true, 128);
+        if (st == LLMT_B200_OK) st = head_map(&maps[2], p.v, p, true, 128);
+        if (st == LLMT_B200_OK) st = head_map(&maps[3], p.out, p, false, 128);
+        if (st != LLMT_B200_OK) return st;
+        DeviceStatus* status = device_status_ptr();
+        if (status == nullptr) return fail(LLMT_B200_ERR_CUDA, "cannot resolve the device status word");
+        e = launch_attention_fwd_sm100(p, maps, status, g_wait_limit_ns, s);
+    }
     if (e != cudaSuccess) return fail(LLMT_B200_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
     return LLMT_B200_OK;
 }

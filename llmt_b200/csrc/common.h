@@ -387,6 +387,8 @@ cudaError_t launch_norm_residual_bwd(const NormResidualParams& p, const NormResi
                                      cudaStream_t stream);
 size_t attention_window_bwd_workspace(const AttentionParams& p);
 cudaError_t launch_attention_window_fwd(const AttentionParams& p, cudaStream_t stream);
+// The tensor-core form; maps of q, k, v, out: boxes of 128 rows x 64 values, 128-byte swizzle.
+cudaError_t launch_attention_fwd_sm100(const AttentionParams& p, const CUtensorMap* maps, DeviceStatus* status, uint64_t wait_ns, cudaStream_t stream);
 cudaError_t launch_attention_window_bwd(AttentionParams p, void* workspace, cudaStream_t stream);
 cudaError_t launch_attention_window_decode(const AttentionParams& p, cudaStream_t stream);
 DeviceStatus* device_status_ptr(void);
