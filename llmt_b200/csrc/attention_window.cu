@@ -48,8 +48,6 @@ unsigned row_blocks(int64_t rows) { return static_cast<unsigned>((rows * 32 + kR
 
 }  // namespace
 
-size_t attention_window_bwd_workspace(const AttentionParams& p) { return static_cast<size_t>(p.batch) * p.heads * p.tq * sizeof(float); }
-
 cudaError_t launch_attention_window_fwd(const AttentionParams& p, cudaStream_t stream) {
     return launch_dependent(attention_fwd_rows_kernel, row_blocks(static_cast<int64_t>(p.batch) * p.heads * p.tq), kRowThreads, stream, p);
 }

@@ -371,6 +371,513 @@ attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_co
     }
 }
 
+// ----------------------------------------------------------------------------------------------------------- backward
+
+// The tiles of 64 queries that see a key of [j0, j0 + 128).
+struct QueryTiles {
+    int first, count;
+    __host__ __device__ QueryTiles(const AttentionParams& p, int j0) {
+        const int64_t off = static_cast<int64_t>(p.tk) - p.tq, j1 = j0 + kRows - 1;
+        const int64_t begin = j0 - off > 0 ? j0 - off : 0;
+        int64_t end = j0 < p.sinks ? p.tq : j1 + p.window - off;   // one past the last
+        if (end > p.tq) end = p.tq;
+        first = static_cast<int>(begin / 64);
+        count = end > begin ? static_cast<int>((end - 1) / 64) - first + 1 : 0;
+    }
+};
+
+// How the key tiles are shared out: those with keys that stay visible in `sink_parts` parts, the others in `parts`.
+struct DkdvPlan {
+    int tiles, sink_tiles, sink_parts, parts;
+    __host__ __device__ int64_t items() const { return static_cast<int64_t>(sink_tiles) * sink_parts + static_cast<int64_t>(tiles - sink_tiles) * parts; }
+    // Places in the workspace: [unit][item] of either class, where it is done in more than one part.
+    __host__ __device__ int64_t kept_slots(int64_t units) const { return sink_parts > 1 ? units * sink_tiles * sink_parts : 0; }
+    __host__ __device__ int64_t slots(int64_t units) const { return kept_slots(units) + (parts > 1 ? units * (tiles - sink_tiles) * parts : 0); }
+    __device__ int64_t slot(bool kept, int unit, int item, int units) const {
+        return kept ? static_cast<int64_t>(unit) * sink_tiles * sink_parts + item
+                    : kept_slots(units) + static_cast<int64_t>(unit) * (tiles - sink_tiles) * parts + item;
+    }
+};
+
+// dQ and dK, dV are two kernels, each of which forms P and dS again for itself: neither has to add to memory that another
+// block adds to, so the order of every sum is fixed.  Both walk tiles of 64 columns, which two warpgroups take in turn: one
+// takes its exponentials while the tensor core works for the other.
+constexpr int kCols = 64;
+constexpr uint32_t kHalfCols = kCols * 128;    // 64 rows of 64 bf16 values
+constexpr int kBwdThreads = 320;
+constexpr int kBwdSlots = 4;
+
+struct BwdControl {
+    uint64_t fixed, full[kBwdSlots], empty[kBwdSlots], scores[2], ready[2], done;
+    uint32_t tmem;
+    int abort;
+    uint32_t bad[4];
+    alignas(16) float2 stats[8][kCols];   // of each warp, read two at a time: (lse log2 e, D) of a tile's queries
+};
+static_assert(sizeof(BwdControl) <= 5 * 1024, "the control block sits below the tiles");
+constexpr uint32_t kBwdControl = 5 * 1024;
+template <int HALVES> constexpr size_t bwd_smem() { return 1024 + kBwdControl + 2 * HALVES * kHalfTile + static_cast<size_t>(kBwdSlots) * 2 * HALVES * kHalfCols; }
+
+// What both kernels have around their loops: barriers, tensor memory, and the two-deep pipeline
+//   scores(0), scores(1), then for each tile: its second products when its P / dS are there, scores two tiles on.
+struct BwdRoles {
+    BwdControl* ctl;
+    volatile int* abort_flag;
+    DeviceStatus* status;
+    uint64_t wait_ns;
+    int n;
+
+    __device__ __forceinline__ void set_up(int warp) {
+        if (threadIdx.x == 0) {
+            mbar_init(smem_u32(&ctl->fixed), 1);
+            mbar_init(smem_u32(&ctl->done), 1);
+            for (int w = 0; w < 2; ++w) {
+                mbar_init(smem_u32(&ctl->scores[w]), 1);
+                mbar_init(smem_u32(&ctl->ready[w]), 4);
+            }
+            for (int s = 0; s < kBwdSlots; ++s) {
+                mbar_init(smem_u32(&ctl->full[s]), 1);
+                mbar_init(smem_u32(&ctl->empty[s]), 1);
+            }
+            ctl->abort = 0;
+            for (uint32_t& x : ctl->bad) x = 0;
+            fence_barrier_init();
+        }
+        if (warp == 9) {
+            tmem_alloc(smem_u32(&ctl->tmem), 512);
+            tmem_relinquish_alloc_permit();
+        }
+        tc_fence_before_thread_sync();
+        __syncthreads();
+        tc_fence_after_thread_sync();
+    }
+    // load(tile, slot, barrier): the tile's copies, issued by one lane.
+    template <typename Load> __device__ __forceinline__ void loads(uint32_t bytes, Load load) const {
+        int slot = 0;
+        uint32_t phase = 0;
+        for (int it = 0; it < n; ++it) {
+            if (!bounded_wait_warp(smem_u32(&ctl->empty[slot]), phase ^ 1u, abort_flag, status, kDevWaitSmemEmpty, slot, wait_ns)) break;
+            if (elect_one()) {
+                mbar_arrive_expect_tx(smem_u32(&ctl->full[slot]), bytes);
+                load(it, slot, smem_u32(&ctl->full[slot]));
+            }
+            __syncwarp();
+            if (++slot == kBwdSlots) { slot = 0; phase ^= 1u; }
+        }
+    }
+    // first(slot, buffer), second(slot, buffer, tile): the products, issued by one lane.
+    template <typename First, typename Second> __device__ __forceinline__ void products(First first, Second second) const {
+        bool ok = n == 0 || bounded_wait_warp(smem_u32(&ctl->fixed), 0, abort_flag, status, kDevWaitSmemFull, 100, wait_ns);
+        for (int it = -2; it < n && ok; ++it) {
+            if (it >= 0) {
+                ok = bounded_wait_warp(smem_u32(&ctl->ready[it & 1]), static_cast<uint32_t>(it >> 1) & 1u, abort_flag, status, kDevWaitTmemEmpty, it & 1, wait_ns);
+                if (!ok) break;
+                tc_fence_after_thread_sync();
+                if (elect_one()) {
+                    second(it % kBwdSlots, it & 1, it);
+                    umma_commit(smem_u32(&ctl->empty[it % kBwdSlots]));
+                    if (it + 1 == n) umma_commit(smem_u32(&ctl->done));
+                }
+                __syncwarp();
+            }
+            if (it + 2 < n) {
+                const int slot = (it + 2) % kBwdSlots;
+                ok = bounded_wait_warp(smem_u32(&ctl->full[slot]), static_cast<uint32_t>((it + 2) / kBwdSlots) & 1u, abort_flag, status, kDevWaitSmemFull, slot, wait_ns);
+                if (!ok) break;
+                tc_fence_after_thread_sync();
+                if (elect_one()) {
+                    first(slot, (it + 2) & 1);
+                    umma_commit(smem_u32(&ctl->scores[(it + 2) & 1]));
+                }
+                __syncwarp();
+            }
+        }
+    }
+    __device__ __forceinline__ bool wait_scores(int it) const {
+        const bool ok = bounded_wait_warp(smem_u32(&ctl->scores[it & 1]), static_cast<uint32_t>(it >> 1) & 1u, abort_flag, status, kDevWaitTmemFull, it & 1, wait_ns);
+        tc_fence_after_thread_sync();
+        return ok;
+    }
+    __device__ __forceinline__ void post_ready(int it) const {
+        tmem_st_wait();
+        tc_fence_before_thread_sync();
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&ctl->ready[it & 1]));
+    }
+    __device__ __forceinline__ bool wait_done() const {
+        const bool ok = bounded_wait_warp(smem_u32(&ctl->done), 0, abort_flag, status, kDevWaitTmemFull, 2, wait_ns);
+        tc_fence_after_thread_sync();
+        return ok;
+    }
+    __device__ __forceinline__ void tear_down(int warp, uint32_t tmem) {
+        if (*abort_flag) __nanosleep(200000);
+        tc_fence_before_thread_sync();
+        __syncthreads();
+        if (warp == 9) {
+            tc_fence_after_thread_sync();
+            tmem_dealloc(tmem, 512);
+        }
+    }
+};
+
+// 16 fp32 values of a row as bf16 into a 128-row swizzled tile: columns 16 x .. of the row.
+__device__ __forceinline__ void put_row16(uint8_t* tile, int row, int x, const uint32_t* o) {
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+        uint4 v;
+        v.x = pack_bf16(__uint_as_float(o[8 * y]), __uint_as_float(o[8 * y + 1]));
+        v.y = pack_bf16(__uint_as_float(o[8 * y + 2]), __uint_as_float(o[8 * y + 3]));
+        v.z = pack_bf16(__uint_as_float(o[8 * y + 4]), __uint_as_float(o[8 * y + 5]));
+        v.w = pack_bf16(__uint_as_float(o[8 * y + 6]), __uint_as_float(o[8 * y + 7]));
+        *reinterpret_cast<uint4*>(tile + (x >> 2) * kHalfTile + row * 128 + ((((x & 3) * 2 + y) ^ (row & 7)) * 16)) = v;
+    }
+}
+
+// dQ of 128 queries: S = Q K^T and dP = dO V^T of 64 keys, dS = P (dP - D), dQ += dS K.
+template <int HALVES>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_constant__ AttentionParams p, int blocks_q, DeviceStatus* status, uint64_t wait_ns) {
+    extern __shared__ uint8_t raw[];
+    uint8_t* const base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    uint8_t* const tiles_ptr = base + kBwdControl;
+    const uint32_t tiles = smem_u32(tiles_ptr);
+    constexpr uint32_t kFixed = HALVES * kHalfTile, kStream = HALVES * kHalfCols;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int units = p.batch * p.heads, unit = blockIdx.x % units;
+    const int b = unit / p.heads, h = unit % p.heads, hk = h / p.group;
+    const int r0 = (blocks_q - 1 - static_cast<int>(blockIdx.x / units)) * kRows;
+    const int p0 = r0 + p.tk - p.tq, p1 = min(r0 + kRows, p.tq) - 1 + p.tk - p.tq;
+    const int first = max(0, p0 - p.window + 1);
+    const int low = first / kCols, sink_tiles = min((min(p.sinks, first) + kCols - 1) / kCols, low);
+    BwdRoles roles{reinterpret_cast<BwdControl*>(base), nullptr, status, wait_ns, p1 >= 0 ? sink_tiles + p1 / kCols - low + 1 : 0};
+    roles.abort_flag = &roles.ctl->abort;
+    auto tile_of = [&](int it) { return it < sink_tiles ? it : low + it - sink_tiles; };
+    roles.set_up(warp);
+    const uint32_t tmem = roles.ctl->tmem;
+    grid_dependency_wait();
+    const int steps_d = (p.head_dim + 15) / 16;
+    const uint32_t ring = tiles + 2 * kFixed;
+    const uint32_t tmem_dq = tmem + 4u * kCols;   // behind two buffers of S and dP
+
+    if (warp == 8) {
+        if (roles.n > 0 && elect_one()) {
+            mbar_arrive_expect_tx(smem_u32(&roles.ctl->fixed), 2 * kFixed);
+            for (int x = 0; x < HALVES; ++x) {
+                tma_load_4d(tiles + x * kHalfTile, &maps.q, smem_u32(&roles.ctl->fixed), x * 64, r0, h, b);
+                tma_load_4d(tiles + kFixed + x * kHalfTile, &maps.dout, smem_u32(&roles.ctl->fixed), x * 64, r0, h, b);
+            }
+        }
+        __syncwarp();
+        roles.loads(2 * kStream, [&](int it, int slot, uint32_t bar) {
+            const uint32_t at = ring + slot * 2 * kStream;
+            for (int x = 0; x < HALVES; ++x) {
+                tma_load_4d(at + x * kHalfCols, &maps.k, bar, x * 64, tile_of(it) * kCols, hk, b);
+                tma_load_4d(at + kStream + x * kHalfCols, &maps.v, bar, x * 64, tile_of(it) * kCols, hk, b);
+            }
+        });
+    } else if (warp == 9) {
+        const uint32_t idesc_s = make_idesc_bf16(kRows, kCols, 0, 0), idesc_d = make_idesc_bf16(kRows, steps_d * 16, 0, 1);
+        roles.products(
+            [&](int slot, int buffer) {
+                const uint32_t at = ring + slot * 2 * kStream, to = tmem + buffer * 2 * kCols;
+                for (int k = 0; k < steps_d; ++k) {
+                    const uint32_t off = (k >> 2) * kHalfTile + (k & 3) * 32, offc = (k >> 2) * kHalfCols + (k & 3) * 32;
+                    umma_bf16_cg<1>(to, smem_desc(tiles + off, 16), smem_desc(at + offc, 16), idesc_s, k > 0 ? 1u : 0u);
+                }
+                for (int k = 0; k < steps_d; ++k) {
+                    const uint32_t off = (k >> 2) * kHalfTile + (k & 3) * 32, offc = (k >> 2) * kHalfCols + (k & 3) * 32;
+                    umma_bf16_cg<1>(to + kCols, smem_desc(tiles + kFixed + off, 16), smem_desc(at + kStream + offc, 16), idesc_s, k > 0 ? 1u : 0u);
+                }
+            },
+            [&](int slot, int buffer, int it) {
+                const uint32_t at = ring + slot * 2 * kStream;
+#pragma unroll
+                for (int k = 0; k < kCols / 16; ++k)
+                    umma_bf16_ts(tmem_dq, tmem + buffer * 2 * kCols + k * 8, smem_desc(at + k * 2048, kHalfCols), idesc_d, it > 0 || k > 0 ? 1u : 0u);
+            });
+    } else {
+        const int w = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane, i = r0 + row, pos = i + p.tk - p.tq;
+        const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+        const float c = p.scale * kLog2e;
+        const int64_t at = (static_cast<int64_t>(b) * p.heads + h) * p.tq + i;
+        float d = 0.0f, lse2 = INFINITY;   // P = 0 for a query that is not there or sees nothing
+        if (i < p.tq) {
+            d = attn::dot_rows(attn::row_of(p.dout, b, i, h), attn::row_of(p.out, b, i, h), p.head_dim);
+            if (w == 0) p.dvec[at] = d;
+            const float lse = p.lse[at];
+            if (lse != -INFINITY) lse2 = lse * kLog2e;
+        }
+        bool ok = true;
+        for (int it = w; it < roles.n && ok; it += 2) {
+            ok = roles.wait_scores(it);
+            if (!ok) break;
+            const uint32_t ts = tmem + w * 2 * kCols + lanes;
+            const int j0 = tile_of(it) * kCols;
+            uint32_t s[kCols], dp[kCols];
+            tmem_ld_32x32(ts, s);
+            tmem_ld_32x32(ts + 32, s + 32);
+            tmem_ld_32x32(ts + kCols, dp);
+            tmem_ld_32x32(ts + kCols + 32, dp + 32);
+            tmem_ld_wait();
+            uint32_t seen[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
+            const bool part = !(j0 + kCols - 1 <= p0 && (j0 > p1 - p.window || j0 + kCols <= p.sinks));
+            if (part) {
+                const int from = pos - p.window + 1 - j0, to_ = pos + 1 - j0, sink = min(p.sinks, pos + 1) - j0;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) seen[x] = bits_between(from, to_, x * 32) | bits_between(0, sink, x * 32);
+            }
+#pragma unroll
+            for (int y = 0; y < kCols; ++y) {
+                const float e = ex2_approx(fmaf(__uint_as_float(s[y]), c, -lse2));
+                s[y] = __float_as_uint(e * (__uint_as_float(dp[y]) - d));
+            }
+            if (part) {
+#pragma unroll
+                for (int y = 0; y < kCols; ++y)
+                    if (!(seen[y >> 5] >> (y & 31) & 1u)) s[y] = 0;
+            }
+#pragma unroll
+            for (int y = 0; y < kCols / 2; ++y) s[y] = pack_bf16(__uint_as_float(s[2 * y]), __uint_as_float(s[2 * y + 1]));
+            tmem_st_32x32(ts, s);
+            roles.post_ready(it);
+        }
+        if (ok && roles.n > 0) ok = roles.wait_done();
+        bool bad = false;
+        for (int x = w; x < 4 * HALVES; x += 2) {   // the warpgroups share the columns
+            uint32_t o[16];
+#pragma unroll
+            for (int y = 0; y < 16; ++y) o[y] = 0;
+            if (ok && roles.n > 0 && x < steps_d) {
+                tmem_ld_32x16(tmem_dq + lanes + x * 16, o);
+                tmem_ld_wait();
+            }
+#pragma unroll
+            for (int y = 0; y < 16; ++y) {
+                const float f = __uint_as_float(o[y]) * p.scale;
+                bad = bad || !(fabsf(f) < INFINITY);
+                o[y] = __float_as_uint(f);
+            }
+            put_row16(tiles_ptr, row, x, o);
+        }
+        const uint32_t again = __ballot_sync(0xffffffffu, bad && ok && i < p.tq);
+        if (lane == 0 && again != 0) atomicOr(&roles.ctl->bad[quarter], again);
+        fence_proxy_async_smem();
+        named_barrier_sync(1, 256);
+        if (threadIdx.x == 0) {
+            for (int x = 0; x < HALVES; ++x) tma_store_4d(&maps.dq, tiles + x * kHalfTile, x * 64, r0, h, b);
+            bulk_commit_group();
+            bulk_wait_group0();
+        }
+        named_barrier_sync(1, 256);
+        // as in the forward kernel: a hidden key that is not finite has spoilt the row
+        for (uint32_t m = w == 0 ? roles.ctl->bad[quarter] : 0; m != 0; m &= m - 1) {
+            const int r = __ffs(m) - 1;
+            attn::dq_row(p, b, h, r0 + quarter * 32 + r, __shfl_sync(0xffffffffu, d, r));
+        }
+    }
+    roles.tear_down(warp, tmem);
+}
+
+// dK and dV of 128 keys: S^T = K Q^T and dP^T = V dO^T of 64 queries, dV += P^T dO, dK += dS^T Q.  The queries are those of all
+// heads of the group, one head after the other.  A block may do a part of them only: its sums then go to the workspace in
+// fp32, and attention_dkdv_sum_kernel adds the parts in order.
+template <int HALVES>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+attention_dkdv_kernel(const __grid_constant__ AttentionMaps maps, const __grid_constant__ AttentionParams p, const DkdvPlan plan, DeviceStatus* status,
+                      uint64_t wait_ns) {
+    extern __shared__ uint8_t raw[];
+    uint8_t* const base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    uint8_t* const tiles_ptr = base + kBwdControl;
+    const uint32_t tiles = smem_u32(tiles_ptr);
+    constexpr uint32_t kFixed = HALVES * kHalfTile, kStream = HALVES * kHalfCols;
+    constexpr int kHd = 64 * HALVES;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int heads_k = p.heads / p.group, units = p.batch * heads_k, unit = blockIdx.x % units;
+    const int b = unit / heads_k, hk = unit % heads_k;
+    // tiles whose keys stay visible come first, in their parts, then the others in theirs
+    const int item = static_cast<int>(blockIdx.x / units);
+    const bool keep = item < plan.sink_tiles * plan.sink_parts;
+    const int parts = keep ? plan.sink_parts : plan.parts;
+    const int at_item = keep ? item : item - plan.sink_tiles * plan.sink_parts;
+    const int tile = (keep ? 0 : plan.sink_tiles) + at_item / parts, part = at_item % parts;
+    const int j0 = tile * kRows, off = p.tk - p.tq;
+    const QueryTiles q(p, j0);
+    const int all = q.count * p.group, it0 = static_cast<int>(static_cast<int64_t>(all) * part / parts);
+    BwdRoles roles{reinterpret_cast<BwdControl*>(base), nullptr, status, wait_ns, static_cast<int>(static_cast<int64_t>(all) * (part + 1) / parts) - it0};
+    roles.abort_flag = &roles.ctl->abort;
+    auto head_of = [&](int it) { return hk * p.group + (it0 + it) / q.count; };
+    auto query_of = [&](int it) { return (q.first + (it0 + it) % q.count) * kCols; };
+    roles.set_up(warp);
+    const uint32_t tmem = roles.ctl->tmem;
+    grid_dependency_wait();
+    const int steps_d = (p.head_dim + 15) / 16;
+    const uint32_t ring = tiles + 2 * kFixed;
+    auto tmem_acc = [&](int w) { return tmem + 4u * kCols + static_cast<uint32_t>(w) * kHd; };   // dV, dK
+
+    if (warp == 8) {
+        if (roles.n > 0 && elect_one()) {
+            mbar_arrive_expect_tx(smem_u32(&roles.ctl->fixed), 2 * kFixed);
+            for (int x = 0; x < HALVES; ++x) {
+                tma_load_4d(tiles + x * kHalfTile, &maps.k, smem_u32(&roles.ctl->fixed), x * 64, j0, hk, b);
+                tma_load_4d(tiles + kFixed + x * kHalfTile, &maps.v, smem_u32(&roles.ctl->fixed), x * 64, j0, hk, b);
+            }
+        }
+        __syncwarp();
+        roles.loads(2 * kStream, [&](int it, int slot, uint32_t bar) {
+            const uint32_t at = ring + slot * 2 * kStream;
+            for (int x = 0; x < HALVES; ++x) {
+                tma_load_4d(at + x * kHalfCols, &maps.q, bar, x * 64, query_of(it), head_of(it), b);
+                tma_load_4d(at + kStream + x * kHalfCols, &maps.dout, bar, x * 64, query_of(it), head_of(it), b);
+            }
+        });
+    } else if (warp == 9) {
+        const uint32_t idesc_s = make_idesc_bf16(kRows, kCols, 0, 0), idesc_d = make_idesc_bf16(kRows, steps_d * 16, 0, 1);
+        roles.products(
+            [&](int slot, int buffer) {
+                const uint32_t at = ring + slot * 2 * kStream, to = tmem + buffer * 2 * kCols;
+                for (int k = 0; k < steps_d; ++k) {
+                    const uint32_t o = (k >> 2) * kHalfTile + (k & 3) * 32, oc = (k >> 2) * kHalfCols + (k & 3) * 32;
+                    umma_bf16_cg<1>(to, smem_desc(tiles + o, 16), smem_desc(at + oc, 16), idesc_s, k > 0 ? 1u : 0u);
+                }
+                for (int k = 0; k < steps_d; ++k) {
+                    const uint32_t o = (k >> 2) * kHalfTile + (k & 3) * 32, oc = (k >> 2) * kHalfCols + (k & 3) * 32;
+                    umma_bf16_cg<1>(to + kCols, smem_desc(tiles + kFixed + o, 16), smem_desc(at + kStream + oc, 16), idesc_s, k > 0 ? 1u : 0u);
+                }
+            },
+            [&](int slot, int buffer, int it) {
+                const uint32_t at = ring + slot * 2 * kStream, from = tmem + buffer * 2 * kCols;
+#pragma unroll
+                for (int k = 0; k < kCols / 16; ++k)   // dV += P^T dO
+                    umma_bf16_ts(tmem_acc(0), from + k * 8, smem_desc(at + kStream + k * 2048, kHalfCols), idesc_d, it > 0 || k > 0 ? 1u : 0u);
+#pragma unroll
+                for (int k = 0; k < kCols / 16; ++k)   // dK += dS^T Q
+                    umma_bf16_ts(tmem_acc(1), from + kCols + k * 8, smem_desc(at + k * 2048, kHalfCols), idesc_d, it > 0 || k > 0 ? 1u : 0u);
+            });
+    } else {
+        const int w = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane, j = j0 + row;
+        const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+        const float c = p.scale * kLog2e;
+        float2* const stats = roles.ctl->stats[warp];
+        bool ok = true;
+        for (int it = w; it < roles.n && ok; it += 2) {
+            const int i0 = query_of(it);
+            const int64_t at = (static_cast<int64_t>(b) * p.heads + head_of(it)) * p.tq + i0;
+            float2 mine[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {   // P = 0 for a query that is not there or sees nothing
+                const bool there = i0 + x * 32 + lane < p.tq;
+                const float lse = there ? p.lse[at + x * 32 + lane] : -INFINITY;
+                mine[x] = make_float2(lse == -INFINITY ? INFINITY : lse * kLog2e, there ? p.dvec[at + x * 32 + lane] : 0.0f);
+            }
+            __syncwarp();
+            stats[lane] = mine[0];
+            stats[32 + lane] = mine[1];
+            __syncwarp();
+            ok = roles.wait_scores(it);
+            if (!ok) break;
+            const uint32_t ts = tmem + w * 2 * kCols + lanes;
+            uint32_t s[kCols], dp[kCols];
+            tmem_ld_32x32(ts, s);
+            tmem_ld_32x32(ts + 32, s + 32);
+            tmem_ld_32x32(ts + kCols, dp);
+            tmem_ld_32x32(ts + kCols + 32, dp + 32);
+            tmem_ld_wait();
+            uint32_t seen[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
+            const bool some = !(i0 + off >= j0 + kRows - 1 && (i0 + kCols - 1 + off - j0 < p.window || j0 + kRows <= p.sinks));
+            if (some) {
+                const int from = j - off - i0, to_ = j < p.sinks ? kCols : static_cast<int>(min(static_cast<int64_t>(kCols), static_cast<int64_t>(from) + p.window));
+#pragma unroll
+                for (int x = 0; x < 2; ++x) seen[x] = bits_between(from, to_, x * 32);
+            }
+            uint32_t pk[kCols / 2];
+#pragma unroll
+            for (int y = 0; y < kCols; y += 2) {
+                const float4 st = *reinterpret_cast<const float4*>(&stats[y]);
+                float e0 = ex2_approx(fmaf(__uint_as_float(s[y]), c, -st.x)), e1 = ex2_approx(fmaf(__uint_as_float(s[y + 1]), c, -st.z));
+                float f0 = e0 * (__uint_as_float(dp[y]) - st.y), f1 = e1 * (__uint_as_float(dp[y + 1]) - st.w);
+                if (some) {
+                    if (!(seen[y >> 5] >> (y & 31) & 1u)) e0 = f0 = 0.0f;
+                    if (!(seen[y >> 5] >> (y & 31) & 2u)) e1 = f1 = 0.0f;
+                }
+                pk[y / 2] = pack_bf16(e0, e1);
+                dp[y / 2] = pack_bf16(f0, f1);
+            }
+            tmem_st_32x32(ts, pk);
+            tmem_st_32x32(ts + kCols, dp);
+            roles.post_ready(it);
+        }
+        if (ok && roles.n > 0) ok = roles.wait_done();
+        // warpgroup 0 has dV to write, warpgroup 1 dK
+        const float factor = w == 0 ? 1.0f : p.scale;
+        float* const sums = parts > 1 ? p.partial + ((plan.slot(keep, unit, at_item, units) * 2 + w) * kRows + row) * kHd : nullptr;
+        bool bad = false;
+        for (int x = 0; x < 4 * HALVES; ++x) {
+            uint32_t o[16];
+#pragma unroll
+            for (int y = 0; y < 16; ++y) o[y] = 0;
+            if (ok && roles.n > 0 && x < steps_d) {
+                tmem_ld_32x16(tmem_acc(w) + lanes + x * 16, o);
+                tmem_ld_wait();
+            }
+#pragma unroll
+            for (int y = 0; y < 16; ++y) {
+                const float f = __uint_as_float(o[y]) * factor;
+                bad = bad || !(fabsf(f) < INFINITY);
+                o[y] = __float_as_uint(f);
+            }
+            if (sums != nullptr) {
+#pragma unroll
+                for (int y = 0; y < 16; y += 4) *reinterpret_cast<uint4*>(sums + x * 16 + y) = make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]);
+            } else {
+                put_row16(tiles_ptr + w * kFixed, row, x, o);
+            }
+        }
+        if (parts == 1) {
+            const uint32_t again = __ballot_sync(0xffffffffu, bad && ok && j < p.tk);
+            if (lane == 0 && again != 0) atomicOr(&roles.ctl->bad[quarter], again);
+            fence_proxy_async_smem();
+            named_barrier_sync(1, 256);
+            if (row == 0) {
+                for (int x = 0; x < HALVES; ++x) tma_store_4d(w == 0 ? &maps.dv : &maps.dk, tiles + w * kFixed + x * kHalfTile, x * 64, j0, hk, b);
+                bulk_commit_group();
+                bulk_wait_group0();
+            }
+            named_barrier_sync(1, 256);
+            for (uint32_t m = w == 0 ? roles.ctl->bad[quarter] : 0; m != 0; m &= m - 1)
+                attn::dkdv_row(p, b, hk, j0 + quarter * 32 + __ffs(m) - 1);
+        }
+    }
+    roles.tear_down(warp, tmem);
+}
+
+// Adds the parts of the tiles that were done in parts, a row of dV and dK per warp.
+constexpr int kSumThreads = 256;
+__global__ void __launch_bounds__(kSumThreads) attention_dkdv_sum_kernel(AttentionParams p, DkdvPlan plan, int kept, int pitch) {
+    grid_dependency_wait();
+    const int64_t at = (static_cast<int64_t>(blockIdx.x) * kSumThreads + threadIdx.x) >> 5;
+    const int units = p.batch * (p.heads / p.group), n_tiles = kept ? plan.sink_tiles : plan.tiles - plan.sink_tiles, parts = kept ? plan.sink_parts : plan.parts;
+    if (at >= static_cast<int64_t>(units) * n_tiles * kRows) return;
+    const int row = static_cast<int>(at % kRows), tile = static_cast<int>(at / kRows % n_tiles), unit = static_cast<int>(at / kRows / n_tiles);
+    const int64_t j = static_cast<int64_t>(tile + (kept ? 0 : plan.sink_tiles)) * kRows + row;
+    if (j >= p.tk) return;
+    const int b = unit / (p.heads / p.group), hk = unit % (p.heads / p.group), c = 4 * (threadIdx.x & 31);
+    bool bad = false;
+    for (int what = 0; what < 2; ++what) {
+        attn::Four s;
+        if (c < p.head_dim)
+            for (int part = 0; part < parts; ++part) {
+                const float4 v = *reinterpret_cast<const float4*>(p.partial + ((plan.slot(kept != 0, unit, tile * parts + part, units) * 2 + what) * kRows + row) * pitch + c);
+                s.v[0] += v.x; s.v[1] += v.y; s.v[2] += v.z; s.v[3] += v.w;
+            }
+        for (const float x : s.v) bad = bad || !(fabsf(x) < INFINITY);
+        s.store(attn::row_to(what == 0 ? p.dv : p.dk, b, j, hk), 1.0f, p.head_dim);
+    }
+    if (__any_sync(0xffffffffu, bad)) {
+        __syncwarp();
+        attn::dkdv_row(p, b, hk, j);
+    }
+}
+
 // ------------------------------------------------------------------------------------------------------------- launches
 
 template <typename K, typename... A>
@@ -392,7 +899,72 @@ cudaError_t launch_sm(K kernel, int64_t blocks, int threads, size_t smem, cudaSt
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 
+DkdvPlan dkdv_plan(const AttentionParams& p, int sms) {
+    DkdvPlan pl{};
+    pl.tiles = (p.tk + kRows - 1) / kRows;
+    // keys that queries far behind their window see: only worth a class of their own where such queries are
+    const int last_far = (p.sinks < p.tk - p.window ? p.sinks : p.tk - p.window) - 1;   // the last sink that is one beyond its window
+    pl.sink_tiles = last_far < 0 ? 0 : last_far / kRows + 1;
+    pl.sink_parts = pl.parts = 1;
+    if (p.tq == 0) return pl;
+    // Query tiles over all blocks; what one SM does if they are shared evenly bounds a part from below.
+    const int64_t units = static_cast<int64_t>(p.batch) * (p.heads / p.group);
+    const int step = pl.tiles / 512 + 1;
+    int64_t total = 0, most = 0, most_kept = 0;
+    for (int t = 0; t < pl.tiles; t += step) {
+        const int64_t n = static_cast<int64_t>(QueryTiles(p, t * kRows).count) * p.group;
+        total += n * step;
+        int64_t& m = t < pl.sink_tiles ? most_kept : most;
+        m = n > m ? n : m;
+    }
+    int64_t share = total * units / sms;
+    share = share > 16 ? share : 16;
+    if (most_kept > share) pl.sink_parts = static_cast<int>((most_kept + share - 1) / share < 64 ? (most_kept + share - 1) / share : 64);
+    if (most > share && units * (pl.tiles - pl.sink_tiles) < 2 * sms) pl.parts = static_cast<int>((most + share - 1) / share < 16 ? (most + share - 1) / share : 16);
+    return pl;
+}
+
+size_t dkdv_partial_floats(const AttentionParams& p, const DkdvPlan& pl) {
+    const int64_t units = static_cast<int64_t>(p.batch) * (p.heads / p.group);
+    return static_cast<size_t>(pl.slots(units)) * 2 * kRows * (p.head_dim <= 64 ? 64 : 128);
+}
+
+size_t dvec_bytes(const AttentionParams& p) { return (static_cast<size_t>(p.batch) * p.heads * p.tq * sizeof(float) + 255) / 256 * 256; }
+
 }  // namespace
+
+size_t attention_bwd_sm100_workspace(const AttentionParams& p, int sms) {
+    return dvec_bytes(p) + dkdv_partial_floats(p, dkdv_plan(p, sms)) * sizeof(float);
+}
+
+cudaError_t launch_attention_bwd_sm100(AttentionParams p, const CUtensorMap* m, void* workspace, int sms, DeviceStatus* status, uint64_t wait_ns,
+                                       cudaStream_t stream) {
+    p.dvec = static_cast<float*>(workspace);
+    p.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + dvec_bytes(p));
+    AttentionMaps maps{};
+    // dQ: blocks of 128 queries, tiles of 64 keys; dK, dV: blocks of 128 keys, tiles of 64 queries
+    maps.q = m[0]; maps.dout = m[1]; maps.k = m[2]; maps.v = m[3]; maps.dq = m[4];
+    const int blocks_q = (p.tq + kRows - 1) / kRows;
+    const bool narrow = p.head_dim <= 64;
+    int64_t blocks = static_cast<int64_t>(p.batch) * p.heads * blocks_q;
+    cudaError_t e = narrow ? launch_sm(attention_dq_kernel<1>, blocks, kBwdThreads, bwd_smem<1>(), stream, maps, p, blocks_q, status, wait_ns)
+                           : launch_sm(attention_dq_kernel<2>, blocks, kBwdThreads, bwd_smem<2>(), stream, maps, p, blocks_q, status, wait_ns);
+    if (e != cudaSuccess) return e;
+    maps.q = m[5]; maps.dout = m[6]; maps.k = m[7]; maps.v = m[8]; maps.dk = m[9]; maps.dv = m[10];
+    const DkdvPlan pl = dkdv_plan(p, sms);
+    const int64_t units = static_cast<int64_t>(p.batch) * (p.heads / p.group);
+    blocks = units * pl.items();
+    e = narrow ? launch_sm(attention_dkdv_kernel<1>, blocks, kBwdThreads, bwd_smem<1>(), stream, maps, p, pl, status, wait_ns)
+               : launch_sm(attention_dkdv_kernel<2>, blocks, kBwdThreads, bwd_smem<2>(), stream, maps, p, pl, status, wait_ns);
+    for (int kept = 1; kept >= 0 && e == cudaSuccess; --kept) {
+        const int n_tiles = kept ? pl.sink_tiles : pl.tiles - pl.sink_tiles;
+        if (n_tiles == 0 || (kept ? pl.sink_parts : pl.parts) == 1) continue;
+        const int64_t rows = units * n_tiles * kRows;
+        e = launch_dependent(attention_dkdv_sum_kernel, static_cast<unsigned>((rows * 32 + kSumThreads - 1) / kSumThreads), kSumThreads, stream, p, pl, kept,
+                             narrow ? 64 : 128);
+    }
+    return e;
+}
 
 cudaError_t launch_attention_fwd_sm100(const AttentionParams& p, const CUtensorMap* m, DeviceStatus* status, uint64_t wait_ns, cudaStream_t stream) {
     AttentionMaps maps{};

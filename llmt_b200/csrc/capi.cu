@@ -2154,7 +2154,7 @@ int llmt_b200_attention_window_fwd(const llmt_b200_attention_desc* d, void* stre
 uint64_t llmt_b200_attention_window_workspace_bytes(const llmt_b200_attention_desc* d) {
     AttentionParams p;
     if (attention_params(d, "attention_window_bwd", &p) != LLMT_B200_OK) return 0;
-    return (attention_window_bwd_workspace(p) + 255) / 256 * 256;
+    return attention_bwd_sm100_workspace(p, sm_count());
 }
 
 int llmt_b200_attention_window_bwd(const llmt_b200_attention_desc* d, void* stream) {
@@ -2180,7 +2180,21 @@ int llmt_b200_attention_window_bwd(const llmt_b200_attention_desc* d, void* stre
     if (st != LLMT_B200_OK) return st;
     if (overlaps(d->workspace, need, d->lse, 4 * static_cast<size_t>(d->batch * d->heads * d->tokens_q)))
         return fail(LLMT_B200_ERR_INVALID, "%s: workspace overlaps lse", who);
-    const cudaError_t e = launch_attention_window_bwd(p, d->workspace, static_cast<cudaStream_t>(stream));
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    cudaError_t e;
+    if (p.tq == 0 || p.tk == 0) {
+        e = launch_attention_window_bwd(p, d->workspace, s);
+    } else {
+        const struct { const HeadView* v; bool keys; int rows; } views[11] = {{&p.q, false, 128}, {&p.dout, false, 128}, {&p.k, true, 64}, {&p.v, true, 64},
+                                                                              {&p.dq, false, 128}, {&p.q, false, 64}, {&p.dout, false, 64}, {&p.k, true, 128},
+                                                                              {&p.v, true, 128}, {&p.dk, true, 128}, {&p.dv, true, 128}};
+        CUtensorMap maps[11];
+        for (int i = 0; i < 11 && st == LLMT_B200_OK; ++i) st = head_map(&maps[i], *views[i].v, p, views[i].keys, views[i].rows);
+        if (st != LLMT_B200_OK) return st;
+        DeviceStatus* status = device_status_ptr();
+        if (status == nullptr) return fail(LLMT_B200_ERR_CUDA, "cannot resolve the device status word");
+        e = launch_attention_bwd_sm100(p, maps, d->workspace, sm_count(), status, g_wait_limit_ns, s);
+    }
     if (e != cudaSuccess) return fail(LLMT_B200_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
     return LLMT_B200_OK;
 }

@@ -267,6 +267,7 @@ struct AttentionParams {
     HeadView q, k, v, out, dout, dq, dk, dv;
     float* lse;                // [batch][heads][tq]
     float* dvec;               // workspace: rowsum(dout * out), [batch][heads][tq]
+    float* partial;            // workspace: sums of dV and dK of key tiles that are done in parts
     const int32_t* lengths;    // one new token: keys of each sequence, or null (all)
     int32_t batch, heads, group, tq, tk, head_dim;   // group: query heads that share a key head
     int32_t window, sinks;     // 1 <= window <= max(tk, 1), 0 <= sinks <= tk
@@ -385,10 +386,14 @@ NormResidualPlan norm_residual_plan(int64_t rows, int64_t cols, int64_t groups, 
 cudaError_t launch_norm_residual_fwd(const NormResidualParams& p, int res_bf16, int act_bf16, bool wide, cudaStream_t stream);
 cudaError_t launch_norm_residual_bwd(const NormResidualParams& p, const NormResidualPlan& pl, int res_bf16, int act_bf16, bool wide, float beta,
                                      cudaStream_t stream);
-size_t attention_window_bwd_workspace(const AttentionParams& p);
 cudaError_t launch_attention_window_fwd(const AttentionParams& p, cudaStream_t stream);
 // The tensor-core form; maps of q, k, v, out: boxes of 128 rows x 64 values, 128-byte swizzle.
 cudaError_t launch_attention_fwd_sm100(const AttentionParams& p, const CUtensorMap* maps, DeviceStatus* status, uint64_t wait_ns, cudaStream_t stream);
+// The backward kernels; maps of q, dout, k, v, dq with boxes of 128, 128, 64, 64, 128 rows, then of q, dout, k, v, dk, dv with boxes
+// of 64, 64, 128, 128, 128, 128 rows.
+cudaError_t launch_attention_bwd_sm100(AttentionParams p, const CUtensorMap* maps, void* workspace, int sms, DeviceStatus* status, uint64_t wait_ns,
+                                       cudaStream_t stream);
+size_t attention_bwd_sm100_workspace(const AttentionParams& p, int sms);
 cudaError_t launch_attention_window_bwd(AttentionParams p, void* workspace, cudaStream_t stream);
 cudaError_t launch_attention_window_decode(const AttentionParams& p, cudaStream_t stream);
 DeviceStatus* device_status_ptr(void);
