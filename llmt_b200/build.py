@@ -22,7 +22,8 @@ LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libllmt_b200.so")
 
 SOURCES = ["capi.cu", "gemm_grouped_sm100.cu", "gemm_fp32_simt.cu", "gemm_fp32_sm100.cu", "grad_allreduce_sm100.cu", "cross_entropy.cu",
-           "rope.cu", "norm_residual.cu", "attention_window.cu", "attention_window_sm100.cu"]
+           "rope.cu", "norm_residual.cu", "attention_window.cu", "attention_window_sm100.cu",
+           "attention_decode.cu"]
 HEADERS = ["common.h", "ptx_sm100.cuh", "waits_sm100.cuh", "gemm_fp32.cuh", "attention_rows.cuh", os.path.join("..", "..", "include", "llmt_b200.h")]
 
 NVCC_FLAGS = [

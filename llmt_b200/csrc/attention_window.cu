@@ -34,16 +34,6 @@ __global__ void __launch_bounds__(kRowThreads) attention_dkdv_rows_kernel(Attent
     attn::dkdv_row(p, bh / hkv, bh % hkv, j);
 }
 
-__global__ void __launch_bounds__(kRowThreads) attention_decode_rows_kernel(AttentionParams p) {
-    ptx::grid_dependency_wait();
-    const int64_t row = (static_cast<int64_t>(blockIdx.x) * kRowThreads + threadIdx.x) >> 5;
-    if (row >= static_cast<int64_t>(p.batch) * p.heads) return;
-    const int64_t b = row / p.heads;
-    int64_t n = p.lengths != nullptr ? p.lengths[b] : p.tk;
-    n = n < p.tk ? n : p.tk;   // never past the cache
-    attn::forward_row(p, b, row % p.heads, 0, n - 1);
-}
-
 unsigned row_blocks(int64_t rows) { return static_cast<unsigned>((rows * 32 + kRowThreads - 1) / kRowThreads); }
 
 }  // namespace
@@ -58,9 +48,6 @@ cudaError_t launch_attention_window_bwd(AttentionParams p, void* workspace, cuda
         if (e != cudaSuccess || p.tk == 0) return e;
     }
     return launch_dependent(attention_dkdv_rows_kernel, row_blocks(static_cast<int64_t>(p.batch) * (p.heads / p.group) * p.tk), kRowThreads, stream, p);
-}
-cudaError_t launch_attention_window_decode(const AttentionParams& p, cudaStream_t stream) {
-    return launch_dependent(attention_decode_rows_kernel, row_blocks(static_cast<int64_t>(p.batch) * p.heads), kRowThreads, stream, p);
 }
 
 }  // namespace llmt_b200

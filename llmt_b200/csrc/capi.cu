@@ -2210,7 +2210,7 @@ int llmt_b200_attention_window_decode(const llmt_b200_attention_desc* d, void* s
     if (st == LLMT_B200_OK) st = attention_apart(d, who, "lse", d->lse, 4 * static_cast<size_t>(d->batch * d->heads), t, 4);
     if (st != LLMT_B200_OK) return st;
     if (p.batch == 0 || p.heads == 0) return LLMT_B200_OK;
-    const cudaError_t e = launch_attention_window_decode(p, static_cast<cudaStream_t>(stream));
+    const cudaError_t e = launch_attention_window_decode(p, sm_count(), static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return fail(LLMT_B200_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
     return LLMT_B200_OK;
 }
