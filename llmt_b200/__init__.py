@@ -828,13 +828,14 @@ def _bind_native() -> None:
     import torch
     entries = lib()
     _native.bind(tuple(ctypes.cast(getattr(entries, "llmt_b200_" + n), ctypes.c_void_p).value for n in _native.NAMES),
-                 torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice, torch.float32, torch.bfloat16, torch.int32, GemmDesc)
+                 torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice, torch.float32, torch.bfloat16, torch.int32, torch.float64, GemmDesc)
 
 
 if os.path.exists(os.path.join(_HERE, "_native" + importlib.machinery.EXTENSION_SUFFIXES[0])):   # built for this interpreter
     from . import _native
     _native.setup(_bind_native, _check, _scratch)
     for _f in (_group_run, gemm, gemm_desc, zero_grads, softmax_fwd, softmax_bwd, gemm_softmax_fwd, gemm_softmax_bwd, rowdot,
-               head_split, head_merge, cross_entropy_fwd, cross_entropy_bwd, lm_head_ce_fwd, lm_head_ce_bwd):
+               head_split, head_merge, cross_entropy_fwd, cross_entropy_bwd, lm_head_ce_fwd, lm_head_ce_bwd, rope, norm_residual_fwd,
+               norm_residual_bwd, attention_window_fwd, attention_window_bwd, attention_window_decode):
         globals()[_f.__name__] = _native.fast(_f)
     del _f

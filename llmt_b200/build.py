@@ -97,7 +97,7 @@ def build_native(force: bool = False) -> str:
         cc = shutil.which("cc") or shutil.which("gcc")
         if cc is None:
             raise RuntimeError("a C compiler is required to build llmt_b200._native")
-        cmd = [cc, "-std=c11", "-O2", "-Wall", "-fPIC", "-shared", "-I" + sysconfig.get_paths()["include"], NATIVE_SRC, "-o", NATIVE_PATH]
+        cmd = [cc, "-std=c11", "-O2", "-Wall", "-fPIC", "-shared", "-I" + sysconfig.get_paths()["include"], NATIVE_SRC, "-o", NATIVE_PATH, "-lm"]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             sys.stderr.write(r.stdout + r.stderr)

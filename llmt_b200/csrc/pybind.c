@@ -9,6 +9,7 @@
 // messages.  Both fill in the same descriptor and call the same C entry point.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
+#include <math.h>
 #include <stddef.h>
 #include <stdint.h>
 #include <string.h>
@@ -32,10 +33,20 @@ typedef struct {
     int (*cross_entropy_bwd)(float*, const float*, const int32_t*, const float*, float, int64_t, int64_t, int64_t, int64_t, void*);
     int (*lm_head_ce_fwd)(const llmt_b200_gemm_desc*, void*, const void*, const void*, const int32_t*, const float*, float*, float*, void*);
     int (*lm_head_ce_bwd)(const llmt_b200_gemm_desc*, void*, const void*, const void*, const int32_t*, const float*, float, int32_t, void*);
+    int (*rope)(const llmt_b200_rope_desc*, void*);
+    int (*norm_residual_fwd)(const llmt_b200_norm_residual_desc*, void*);
+    int (*norm_residual_bwd)(const llmt_b200_norm_residual_desc*, void*);
+    uint64_t (*norm_residual_workspace_bytes)(const llmt_b200_norm_residual_desc*);
+    int (*attention_window_fwd)(const llmt_b200_attention_desc*, void*);
+    int (*attention_window_bwd)(const llmt_b200_attention_desc*, void*);
+    int (*attention_window_decode)(const llmt_b200_attention_desc*, void*);
+    uint64_t (*attention_window_workspace_bytes)(const llmt_b200_attention_desc*);
 } Entry;
 static const char* const kNames[] = {"gemm", "gemm_workspace_bytes_for", "gemm_grouped", "zero_grads", "softmax_fwd", "softmax_bwd",
                                      "gemm_softmax_fwd", "gemm_softmax_bwd", "rowdot", "head_split", "head_merge",
-                                     "cross_entropy_fwd", "cross_entropy_bwd", "lm_head_ce_fwd", "lm_head_ce_bwd"};
+                                     "cross_entropy_fwd", "cross_entropy_bwd", "lm_head_ce_fwd", "lm_head_ce_bwd",
+                                     "rope", "norm_residual_fwd", "norm_residual_bwd", "norm_residual_workspace_bytes", "attention_window_fwd",
+                                     "attention_window_bwd", "attention_window_decode", "attention_window_workspace_bytes"};
 #define N_ENTRIES ((Py_ssize_t)(sizeof(kNames) / sizeof(kNames[0])))
 _Static_assert(sizeof(Entry) == sizeof(kNames), "one pointer per name");
 
@@ -43,9 +54,9 @@ static Entry E;
 static int g_bound = 0;
 static PyObject *g_binder, *g_raise, *g_scratch;            // Python: loads the library; raises for a status; allocates scratch
 static PyObject *g_raw_stream, *g_get_device;               // torch's current stream handle of a device, and its current device
-static PyObject *g_float32, *g_bfloat16, *g_int32;
+static PyObject *g_float32, *g_bfloat16, *g_int32, *g_float64;
 static PyObject* g_desc_type;                               // the ctypes structure GemmDesc
-static PyObject *s_data_ptr, *s_shape, *s_stride, *s_dtype, *s_cuda_stream, *s_nbytes;
+static PyObject *s_data_ptr, *s_shape, *s_stride, *s_dtype, *s_cuda_stream, *s_nbytes, *s_get_device;
 
 static int ensure_bound(void) {
     if (g_bound) return 0;
@@ -61,7 +72,7 @@ typedef struct {
     void* ptr;
     int nd;
     int64_t shape[4], stride[4];
-    int dtype;   // LLMT_B200_FP32 / _BF16, 2 = int32
+    int dtype;   // LLMT_B200_FP32 / _BF16, 2 = int32, 3 = fp64
 } Tensor;
 
 static int as_ptr(PyObject* o, void** out) {
@@ -95,7 +106,7 @@ static int as_tensor(PyObject* o, Tensor* t) {
     if (t->nd < 0 || read_tuple(PyObject_CallMethodNoArgs(o, s_stride), t->stride, 4) != t->nd) return -1;
     PyObject* d = PyObject_GetAttr(o, s_dtype);
     if (d == NULL) { PyErr_Clear(); return -1; }
-    t->dtype = d == g_float32 ? LLMT_B200_FP32 : d == g_bfloat16 ? LLMT_B200_BF16 : d == g_int32 ? 2 : -1;
+    t->dtype = d == g_float32 ? LLMT_B200_FP32 : d == g_bfloat16 ? LLMT_B200_BF16 : d == g_int32 ? 2 : d == g_float64 ? 3 : -1;
     Py_DECREF(d);
     return t->dtype < 0 ? -1 : 0;
 }
@@ -417,6 +428,286 @@ FAST(lm_head_ce_bwd) {
     RUN(E.lm_head_ce_bwd(&d, l, a, b, (const int32_t*)t, (const float*)m, g, valid, s));
 }
 
+// ---- what a transformer block runs between its products
+
+// A tensor on the device that the others are on (*device, -1 before the first).
+static int on_device(PyObject* o, int* device) {
+    PyObject* v = PyObject_CallMethodNoArgs(o, s_get_device);
+    if (v == NULL) { PyErr_Clear(); return -1; }
+    const long d = PyLong_AsLong(v);
+    Py_DECREF(v);
+    if (d < 0) { PyErr_Clear(); return -1; }
+    if (*device >= 0 && *device != (int)d) return -1;
+    *device = (int)d;
+    return 0;
+}
+// The current device, which the tensors have to be on, and the stream.
+static int stream_of(PyObject* o, int device, void** out) {
+    PyObject* dev = PyObject_CallNoArgs(g_get_device);
+    if (dev == NULL) { PyErr_Clear(); return -1; }
+    const long at = PyLong_AsLong(dev);
+    PyObject* v = NULL;
+    if (at == device) v = o == NULL || o == Py_None ? PyObject_CallOneArg(g_raw_stream, dev) : PyObject_GetAttr(o, s_cuda_stream);
+    Py_DECREF(dev);
+    if (v == NULL) { PyErr_Clear(); return -1; }
+    *out = PyLong_AsVoidPtr(v);
+    Py_DECREF(v);
+    if (*out == NULL && PyErr_Occurred()) { PyErr_Clear(); return -1; }
+    return 0;
+}
+static int is_there(PyObject* o) { return o != NULL && o != Py_None; }
+static int as_long(PyObject* o, int64_t dflt, int64_t* out) {
+    if (o == NULL) { *out = dflt; return 0; }
+    *out = PyLong_AsLongLong(o);
+    if (*out == -1 && PyErr_Occurred()) { PyErr_Clear(); return -1; }
+    return 0;
+}
+static int same_shape(const Tensor* a, const Tensor* b) { return a->nd == b->nd && memcmp(a->shape, b->shape, sizeof(int64_t) * (size_t)a->nd) == 0; }
+// A contiguous tensor of n values of one type; NULL for one that is not there.
+static int as_vector(PyObject* o, int dtype, int64_t n, int* device, void** out) {
+    *out = NULL;
+    if (!is_there(o)) return 0;
+    Tensor t;
+    if (as_tensor(o, &t) < 0 || t.dtype != dtype || numel(&t) != n || !is_contiguous(&t) || on_device(o, device) < 0) return -1;
+    *out = t.ptr;
+    return 0;
+}
+static int as_workspace(PyObject* o, int* device, void** at, uint64_t* bytes) {
+    PyObject* nb = PyObject_GetAttr(o, s_nbytes);
+    if (nb == NULL) { PyErr_Clear(); return -1; }
+    *bytes = PyLong_AsUnsignedLongLong(nb);
+    Py_DECREF(nb);
+    if (PyErr_Occurred()) { PyErr_Clear(); return -1; }
+    return as_ptr(o, at) < 0 || on_device(o, device) < 0 ? -1 : 0;
+}
+// Scratch for one call; NULL with an exception set if torch has none.
+static PyObject* scratch_for(uint64_t need, PyObject* like, PyObject* stream) {
+    PyObject* n = PyLong_FromUnsignedLongLong(need);
+    if (n == NULL) return NULL;
+    PyObject* r = PyObject_CallFunctionObjArgs(g_scratch, n, like, stream != NULL ? stream : Py_None, NULL);
+    Py_DECREF(n);
+    return r;
+}
+
+// [batch, tokens, heads, head_dim] with contiguous head_dim.
+static int as_heads(PyObject* o, Tensor* t, llmt_b200_head_view* v, int* device) {
+    if (as_tensor(o, t) < 0 || t->nd != 4 || !pitch_ok(t) || on_device(o, device) < 0) return -1;
+    v->data = t->ptr;
+    v->stride_batch = t->stride[0];
+    v->stride_token = t->stride[1];
+    v->stride_head = t->stride[2];
+    return 0;
+}
+
+FAST(rope) {
+    BEGIN(3, "y", "x", "freqs", "positions", "offset", "interleaved", "inverse", "scale", "stream");
+    llmt_b200_rope_desc d;
+    Tensor x, y, f, pos;
+    int dev = -1;
+    void* s;
+    memset(&d, 0, sizeof d);
+    NEED(as_heads(v[0], &y, &d.y, &dev) == 0 && as_heads(v[1], &x, &d.x, &dev) == 0 && as_tensor(v[2], &f) == 0 && on_device(v[2], &dev) == 0);
+    NEED(x.dtype < 2 && x.dtype == y.dtype && same_shape(&x, &y) && f.nd == 1 && f.dtype == 3 && is_contiguous(&f));
+    if (is_there(v[3])) {
+        NEED(as_tensor(v[3], &pos) == 0 && on_device(v[3], &dev) == 0 && pos.nd == 2 && pos.dtype == 2 && is_contiguous(&pos) &&
+             pos.shape[0] == x.shape[0] && pos.shape[1] == x.shape[1]);
+        d.positions = (const int32_t*)pos.ptr;
+    }
+    NEED(as_long(v[4], 0, &d.offset) == 0 && as_bool(v[5], &d.interleaved) == 0 && as_bool(v[6], &d.inverse) == 0 && as_float(v[7], 1.0f, &d.scale) == 0 &&
+         stream_of(v[8], dev, &s) == 0);
+    d.batch = x.shape[0]; d.tokens = x.shape[1]; d.heads = x.shape[2]; d.head_dim = x.shape[3];
+    d.rot_dim = 2 * f.shape[0];
+    d.freqs = (const double*)f.ptr;
+    d.dtype = x.dtype;
+    RUN(E.rope(&d, s));
+}
+
+// A tensor [..., cols] of the shape of `like` whose rows are evenly spaced, of the type that its kind has (-1: not known yet).
+static int as_rows(PyObject* o, const Tensor* like, int* kind, int* device, void** at, int64_t* pitch) {
+    Tensor t;
+    if (!is_there(o)) return 0;
+    if (as_tensor(o, &t) < 0 || t.dtype > 1 || (*kind >= 0 && *kind != t.dtype) || !same_shape(&t, like) || !pitch_ok(&t) || on_device(o, device) < 0) return -1;
+    int64_t span = -1;
+    *pitch = t.shape[t.nd - 1];
+    for (int i = t.nd - 2; i >= 0; --i) {
+        if (t.shape[i] == 1) continue;
+        if (span < 0) *pitch = t.stride[i];
+        else if (t.stride[i] != span) return -1;
+        span = t.stride[i] * t.shape[i];
+    }
+    *at = t.ptr;
+    *kind = t.dtype;
+    return 0;
+}
+static int as_gate(PyObject* o, llmt_b200_norm_residual_desc* d, int* device) {
+    Tensor t;
+    d->groups = 1;
+    if (!is_there(o)) return 0;
+    if (as_tensor(o, &t) < 0 || t.dtype != LLMT_B200_FP32 || t.nd < 1 || t.nd > 2 || t.shape[t.nd - 1] != d->cols || !is_contiguous(&t) || on_device(o, device) < 0) return -1;
+    d->gate = (const float*)t.ptr;
+    d->groups = t.nd == 2 ? t.shape[0] : 1;
+    return 0;
+}
+
+FAST(norm_residual_fwd) {
+    BEGIN(3, "out", "h", "x", "y", "w_post", "gate", "w_pre", "rstd_post", "rstd_pre", "scale", "eps", "stream");
+    llmt_b200_norm_residual_desc d;
+    Tensor like;
+    int dev = -1, res = -1, act = -1;
+    void *s, *x = NULL, *y = NULL, *wp, *wq, *rp, *rq;
+    memset(&d, 0, sizeof d);
+    NEED(as_tensor(v[2], &like) == 0 && like.nd >= 1 && like.shape[like.nd - 1] > 0);
+    d.cols = like.shape[like.nd - 1];
+    d.rows = numel(&like) / d.cols;
+    NEED(as_rows(v[2], &like, &res, &dev, &x, &d.ld_x) == 0 && as_rows(v[3], &like, &act, &dev, &y, &d.ld_y) == 0);
+    NEED(!is_there(v[3]) || as_rows(v[0], &like, &res, &dev, &d.out, &d.ld_out) == 0);
+    NEED(is_there(v[3]) || !is_there(v[0]) || on_device(v[0], &dev) == 0);
+    NEED(as_rows(v[1], &like, &act, &dev, &d.h, &d.ld_h) == 0 && as_vector(v[4], LLMT_B200_FP32, d.cols, &dev, &wp) == 0 && as_gate(v[5], &d, &dev) == 0 &&
+         as_vector(v[6], LLMT_B200_FP32, d.cols, &dev, &wq) == 0 && as_vector(v[7], LLMT_B200_FP32, d.rows, &dev, &rp) == 0 &&
+         as_vector(v[8], LLMT_B200_FP32, d.rows, &dev, &rq) == 0);
+    NEED(as_float(v[9], 1.0f, &d.scale) == 0 && as_float(v[10], 1e-5f, &d.eps) == 0 && stream_of(v[11], dev, &s) == 0);
+    d.x = x; d.y = y;
+    d.dtype_res = res; d.dtype_act = act >= 0 ? act : res;
+    d.w_post = (const float*)wp; d.w_pre = (const float*)wq;
+    d.rstd_post = (float*)rp; d.rstd_pre = (float*)rq;
+    RUN(E.norm_residual_fwd(&d, s));
+}
+
+FAST(norm_residual_bwd) {
+    BEGIN(5, "dx", "dy", "dout", "dh", "out", "y", "w_post", "gate", "w_pre", "rstd_post", "rstd_pre", "dw_post", "dgate", "dw_pre", "scale", "beta",
+          "workspace", "stream");
+    llmt_b200_norm_residual_desc d;
+    Tensor like;
+    int dev = -1, res = -1, act = -1;
+    void *s, *y = NULL, *dout = NULL, *dh = NULL, *wp, *wq, *rp, *rq, *gp, *gg, *gq;
+    memset(&d, 0, sizeof d);
+    NEED(as_tensor(v[0], &like) == 0 && like.nd >= 1 && like.shape[like.nd - 1] > 0);
+    d.cols = like.shape[like.nd - 1];
+    d.rows = numel(&like) / d.cols;
+    NEED(as_rows(v[0], &like, &res, &dev, &d.dx, &d.ld_dx) == 0 && as_rows(v[2], &like, &res, &dev, &dout, &d.ld_dout) == 0 &&
+         as_rows(v[3], &like, &act, &dev, &dh, &d.ld_dh) == 0 && as_rows(v[5], &like, &act, &dev, &y, &d.ld_y) == 0);
+    if (is_there(v[5])) NEED(as_rows(v[1], &like, &act, &dev, &d.dy, &d.ld_dy) == 0);
+    else NEED(!is_there(v[1]));
+    if (is_there(v[3])) NEED(as_rows(v[4], &like, &res, &dev, &d.out, &d.ld_out) == 0);
+    else NEED(!is_there(v[4]));
+    NEED(as_vector(v[6], LLMT_B200_FP32, d.cols, &dev, &wp) == 0 && as_gate(v[7], &d, &dev) == 0 && as_vector(v[8], LLMT_B200_FP32, d.cols, &dev, &wq) == 0 &&
+         as_vector(v[9], LLMT_B200_FP32, d.rows, &dev, &rp) == 0 && as_vector(v[10], LLMT_B200_FP32, d.rows, &dev, &rq) == 0 &&
+         as_vector(v[11], LLMT_B200_FP32, d.cols, &dev, &gp) == 0 && as_vector(v[12], LLMT_B200_FP32, d.groups * d.cols, &dev, &gg) == 0 &&
+         as_vector(v[13], LLMT_B200_FP32, d.cols, &dev, &gq) == 0);
+    NEED(as_float(v[14], 1.0f, &d.scale) == 0 && as_float(v[15], 0.0f, &d.beta) == 0);
+    d.y = y; d.dout = dout; d.dh = dh;
+    d.dtype_res = res; d.dtype_act = act >= 0 ? act : res;
+    d.w_post = (const float*)wp; d.w_pre = (const float*)wq;
+    d.rstd_post = (float*)rp; d.rstd_pre = (float*)rq;
+    d.dw_post = (float*)gp; d.dgate = (float*)gg; d.dw_pre = (float*)gq;
+    PyObject* scratch = NULL;
+    if (is_there(v[16])) NEED(as_workspace(v[16], &dev, &d.workspace, &d.workspace_bytes) == 0);
+    NEED(stream_of(v[17], dev, &s) == 0);
+    if (!is_there(v[16])) {
+        d.workspace_bytes = E.norm_residual_workspace_bytes(&d);
+        if (d.workspace_bytes > 0) {
+            scratch = scratch_for(d.workspace_bytes, v[0], v[17]);
+            if (scratch == NULL) return NULL;   // out of memory: torch's own error
+            if (as_ptr(scratch, &d.workspace) < 0) { Py_DECREF(scratch); SLOW(); }
+        }
+    }
+    int st;
+    Py_BEGIN_ALLOW_THREADS
+    st = E.norm_residual_bwd(&d, s);
+    Py_END_ALLOW_THREADS
+    Py_XDECREF(scratch);
+    return finish(st);
+}
+
+// q, k, v and the scalars of the three attention calls.
+static int attention_of(llmt_b200_attention_desc* d, const Tensor* q, const Tensor* k, const Tensor* vv, PyObject* window, PyObject* sinks, PyObject* scale) {
+    if (q->dtype > 1 || k->dtype != q->dtype || vv->dtype != q->dtype || !same_shape(k, vv) || k->shape[0] != q->shape[0] || k->shape[3] != q->shape[3] ||
+        q->shape[3] < 1)
+        return -1;
+    d->batch = q->shape[0]; d->tokens_q = q->shape[1]; d->heads = q->shape[2]; d->head_dim = q->shape[3];
+    d->tokens_k = k->shape[1]; d->kv_heads = k->shape[2];
+    d->dtype = q->dtype;
+    if (as_long(window, 0, &d->window) < 0 || as_long(sinks, 0, &d->sinks) < 0) return -1;
+    return as_float(is_there(scale) ? scale : NULL, (float)pow((double)d->head_dim, -0.5), &d->scale);
+}
+
+FAST(attention_window_fwd) {
+    BEGIN(5, "out", "lse", "q", "k", "v", "window", "sinks", "scale", "stream");
+    llmt_b200_attention_desc d;
+    Tensor out, q, k, vv;
+    int dev = -1;
+    void *s, *lse;
+    memset(&d, 0, sizeof d);
+    NEED(as_heads(v[0], &out, &d.out, &dev) == 0 && as_heads(v[2], &q, &d.q, &dev) == 0 && as_heads(v[3], &k, &d.k, &dev) == 0 &&
+         as_heads(v[4], &vv, &d.v, &dev) == 0);
+    NEED(attention_of(&d, &q, &k, &vv, v[5], v[6], v[7]) == 0 && out.dtype == q.dtype && same_shape(&out, &q) &&
+         as_vector(v[1], LLMT_B200_FP32, d.batch * d.heads * d.tokens_q, &dev, &lse) == 0 && stream_of(v[8], dev, &s) == 0);
+    d.lse = (float*)lse;
+    RUN(E.attention_window_fwd(&d, s));
+}
+
+FAST(attention_window_bwd) {
+    BEGIN(9, "dq", "dk", "dv", "dout", "q", "k", "v", "out", "lse", "window", "sinks", "scale", "workspace", "stream");
+    llmt_b200_attention_desc d;
+    Tensor dq, dk, dv, dout, q, k, vv, out;
+    int dev = -1;
+    void *s, *lse;
+    memset(&d, 0, sizeof d);
+    NEED(as_heads(v[0], &dq, &d.dq, &dev) == 0 && as_heads(v[1], &dk, &d.dk, &dev) == 0 && as_heads(v[2], &dv, &d.dv, &dev) == 0 &&
+         as_heads(v[3], &dout, &d.dout, &dev) == 0 && as_heads(v[4], &q, &d.q, &dev) == 0 && as_heads(v[5], &k, &d.k, &dev) == 0 &&
+         as_heads(v[6], &vv, &d.v, &dev) == 0 && as_heads(v[7], &out, &d.out, &dev) == 0);
+    NEED(attention_of(&d, &q, &k, &vv, v[9], v[10], v[11]) == 0 && same_shape(&dq, &q) && same_shape(&dout, &q) && same_shape(&out, &q) &&
+         same_shape(&dk, &k) && same_shape(&dv, &k) && dq.dtype == q.dtype && dk.dtype == q.dtype && dv.dtype == q.dtype && dout.dtype == q.dtype &&
+         out.dtype == q.dtype && as_vector(v[8], LLMT_B200_FP32, d.batch * d.heads * d.tokens_q, &dev, &lse) == 0);
+    d.lse = (float*)lse;
+    PyObject* scratch = NULL;
+    if (is_there(v[12])) NEED(as_workspace(v[12], &dev, &d.workspace, &d.workspace_bytes) == 0);
+    NEED(stream_of(v[13], dev, &s) == 0);
+    if (!is_there(v[12])) {
+        d.workspace_bytes = E.attention_window_workspace_bytes(&d);
+        if (d.workspace_bytes > 0) {
+            scratch = scratch_for(d.workspace_bytes, v[4], v[13]);
+            if (scratch == NULL) return NULL;
+            if (as_ptr(scratch, &d.workspace) < 0) { Py_DECREF(scratch); SLOW(); }
+        }
+    }
+    int st;
+    Py_BEGIN_ALLOW_THREADS
+    st = E.attention_window_bwd(&d, s);
+    Py_END_ALLOW_THREADS
+    Py_XDECREF(scratch);
+    return finish(st);
+}
+
+// [batch, heads, head_dim] as one token of each sequence.
+static int as_token(PyObject* o, Tensor* t, llmt_b200_head_view* v, int* device) {
+    if (as_tensor(o, t) < 0 || t->nd != 3 || !pitch_ok(t) || on_device(o, device) < 0) return -1;
+    v->data = t->ptr;
+    v->stride_batch = t->stride[0];
+    v->stride_token = 0;
+    v->stride_head = t->stride[1];
+    t->nd = 4;
+    t->shape[3] = t->shape[2]; t->shape[2] = t->shape[1]; t->shape[1] = 1;
+    return 0;
+}
+
+FAST(attention_window_decode) {
+    BEGIN(4, "out", "q", "k", "v", "lengths", "window", "sinks", "scale", "lse", "stream");
+    llmt_b200_attention_desc d;
+    Tensor out, q, k, vv;
+    int dev = -1;
+    void *s, *lse, *lengths;
+    memset(&d, 0, sizeof d);
+    NEED(as_token(v[0], &out, &d.out, &dev) == 0 && as_token(v[1], &q, &d.q, &dev) == 0 && as_heads(v[2], &k, &d.k, &dev) == 0 &&
+         as_heads(v[3], &vv, &d.v, &dev) == 0);
+    NEED(attention_of(&d, &q, &k, &vv, v[5], v[6], v[7]) == 0 && out.dtype == q.dtype && same_shape(&out, &q) &&
+         as_vector(v[4], 2, d.batch, &dev, &lengths) == 0 && as_vector(v[8], LLMT_B200_FP32, d.batch * d.heads, &dev, &lse) == 0 &&
+         stream_of(v[9], dev, &s) == 0);
+    d.lse = (float*)lse;
+    d.lengths = (const int32_t*)lengths;
+    RUN(E.attention_window_decode(&d, s));
+}
+
 // ---------------------------------------------------------------------------------- module
 
 typedef PyObject* (*FastFn)(PyObject*, PyObject* const*, Py_ssize_t, PyObject*);
@@ -424,7 +715,8 @@ static const struct { const char* name; FastFn fn; } kFast[] = {
 #define ROW(name) {#name, fast_##name}
     {"_group_run", fast_group_run}, ROW(gemm), ROW(gemm_desc), ROW(zero_grads), ROW(softmax_fwd), ROW(softmax_bwd), ROW(gemm_softmax_fwd),
     ROW(gemm_softmax_bwd), ROW(rowdot), ROW(head_split), ROW(head_merge), ROW(cross_entropy_fwd), ROW(cross_entropy_bwd),
-    ROW(lm_head_ce_fwd), ROW(lm_head_ce_bwd)};
+    ROW(lm_head_ce_fwd), ROW(lm_head_ce_bwd), ROW(rope), ROW(norm_residual_fwd), ROW(norm_residual_bwd), ROW(attention_window_fwd),
+    ROW(attention_window_bwd), ROW(attention_window_decode)};
 
 // What stands in the Python function's place: calls go to the native function, every attribute that it does not have itself
 // is the Python function's, and it is pickled by name as a function is.
@@ -519,11 +811,11 @@ static PyObject* py_setup(PyObject* self, PyObject* args) {
     Py_RETURN_NONE;
 }
 
-// bind(addresses in the order of NAMES, torch's raw-stream and device getters, float32, bfloat16, int32, GemmDesc)
+// bind(addresses in the order of NAMES, torch's raw-stream and device getters, float32, bfloat16, int32, float64, GemmDesc)
 static PyObject* py_bind(PyObject* self, PyObject* args) {
     (void)self;
-    PyObject *list, *rs, *gd, *f, *h, *i32, *desc;
-    if (!PyArg_ParseTuple(args, "O!OOOOOO!", &PyTuple_Type, &list, &rs, &gd, &f, &h, &i32, &PyType_Type, &desc)) return NULL;
+    PyObject *list, *rs, *gd, *f, *h, *i32, *f64, *desc;
+    if (!PyArg_ParseTuple(args, "O!OOOOOOO!", &PyTuple_Type, &list, &rs, &gd, &f, &h, &i32, &f64, &PyType_Type, &desc)) return NULL;
     if (PyTuple_GET_SIZE(list) != N_ENTRIES) return PyErr_Format(PyExc_ValueError, "bind: %zd addresses expected", N_ENTRIES);
     void* p[sizeof(kNames) / sizeof(kNames[0])];
     for (Py_ssize_t i = 0; i < N_ENTRIES; ++i) {
@@ -531,8 +823,8 @@ static PyObject* py_bind(PyObject* self, PyObject* args) {
         if (p[i] == NULL) return PyErr_Occurred() ? NULL : PyErr_Format(PyExc_ValueError, "bind: null address for %s", kNames[i]);
     }
     memcpy(&E, p, sizeof E);
-    Py_INCREF(rs); Py_INCREF(gd); Py_INCREF(f); Py_INCREF(h); Py_INCREF(i32); Py_INCREF(desc);
-    g_raw_stream = rs; g_get_device = gd; g_float32 = f; g_bfloat16 = h; g_int32 = i32; g_desc_type = desc;
+    Py_INCREF(rs); Py_INCREF(gd); Py_INCREF(f); Py_INCREF(h); Py_INCREF(i32); Py_INCREF(f64); Py_INCREF(desc);
+    g_raw_stream = rs; g_get_device = gd; g_float32 = f; g_bfloat16 = h; g_int32 = i32; g_float64 = f64; g_desc_type = desc;
     g_bound = 1;
     Py_RETURN_NONE;
 }
@@ -553,8 +845,9 @@ PyMODINIT_FUNC PyInit__native(void) {
     s_dtype = PyUnicode_InternFromString("dtype");
     s_cuda_stream = PyUnicode_InternFromString("cuda_stream");
     s_nbytes = PyUnicode_InternFromString("nbytes");
+    s_get_device = PyUnicode_InternFromString("get_device");
     PyObject* names = PyTuple_New(N_ENTRIES);
-    if (names == NULL || s_data_ptr == NULL || s_shape == NULL || s_stride == NULL || s_dtype == NULL || s_cuda_stream == NULL || s_nbytes == NULL) {
+    if (names == NULL || s_data_ptr == NULL || s_shape == NULL || s_stride == NULL || s_dtype == NULL || s_cuda_stream == NULL || s_nbytes == NULL || s_get_device == NULL) {
         Py_DECREF(m);
         return NULL;
     }
