@@ -26,8 +26,26 @@ struct alignas(64) AttentionMaps {
 
 // The high word of a shared-memory descriptor: 8-row groups of 1024 bytes, version 1, 128-byte swizzle.
 constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
-__device__ __forceinline__ uint64_t smem_desc(uint32_t at, uint32_t lbo) {
-    return (static_cast<uint64_t>(kDescHi) << 32) | ((lbo >> 4) << 16) | (at >> 4);
+// Its low word for a tile at `at`; further steps of the product add to it in units of 16 bytes.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t at, uint32_t lbo) { return ((lbo >> 4) << 16) | (at >> 4); }
+__device__ __forceinline__ uint64_t desc(uint32_t lo) { return (static_cast<uint64_t>(kDescHi) << 32) | static_cast<uint64_t>(lo); }
+
+// Products of a tile, issued by one lane of a converged warp from warp-uniform operands and in unrolled loops: with
+// descriptors in ordinary registers and loops that are not, an instruction takes 80 cycles to issue, longer than the tensor
+// core takes for it.
+//   D[128 x N] = A B^T over HALVES * 64 values: A 128 rows, B N rows of a tile of `half_a`, `half_b` bytes a half
+template <int HALVES> __device__ __forceinline__ void product_ss(uint32_t d, uint32_t a_lo, uint32_t half_a, uint32_t b_lo, uint32_t half_b, uint32_t idesc, int steps) {
+#pragma unroll
+    for (int k = 0; k < 4 * HALVES; ++k)
+        if (k < steps)
+            umma_bf16_cg<1>(d, desc(a_lo + ((k >> 2) * half_a + (k & 3) * 32) / 16), desc(b_lo + ((k >> 2) * half_b + (k & 3) * 32) / 16), idesc, k > 0 ? 1u : 0u);
+}
+//   D[128 x N] (+)= A[tmem, 128 x 16 STEPS] B: B 16 STEPS rows, its columns the result's
+//   (PART: the columns of A from each PART-th step on sit 2 * 8 * PART columns behind the last ones)
+template <int STEPS, int PART = STEPS> __device__ __forceinline__ void product_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, bool accumulate) {
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k)
+        umma_bf16_ts(d, a + (k / PART) * 16 * PART + (k % PART) * 8, desc(b_lo + k * (2048 / 16)), idesc, accumulate || k > 0 ? 1u : 0u);
 }
 
 // Bits [lo, hi) of a word that stands for places [base, base + 32).
@@ -133,7 +151,7 @@ attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_co
     tc_fence_before_thread_sync();
     __syncthreads();
     tc_fence_after_thread_sync();
-    const uint32_t tmem = ctl->tmem;
+    const uint32_t tmem = uniform(ctl->tmem);
     grid_dependency_wait();
 
     const uint32_t q_at = tiles, ring = tiles + 2 * kTile;
@@ -171,6 +189,7 @@ attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_co
     } else if (warp == 9) {
         // ---------------------------------------------------------------- products
         const uint32_t idesc_s = make_idesc_bf16(kRows, kRows, 0, 0), idesc_o = make_idesc_bf16(kRows, steps_d * 16, 0, 1);
+        const uint32_t q_lo = uniform(desc_lo(q_at, 16)), ring_k = uniform(desc_lo(ring, 16)), ring_v = uniform(desc_lo(ring, kHalfTile));
         int slot = 0;
         uint32_t phase = 0, p_phase[2] = {0, 0};
         int last[2] = {-1, -1};
@@ -203,10 +222,7 @@ attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_co
                     p_phase[w] ^= 1u;
                     tc_fence_after_thread_sync();
                     if (elect_one()) {
-                        const uint32_t v_at = ring + v_slot * kTile;
-#pragma unroll
-                        for (int k = 0; k < kRows / 16; ++k)
-                            umma_bf16_ts(tmem_o(w), tmem_s(w) + k * 8, smem_desc(v_at + k * 2048, kHalfTile), idesc_o, begun[w] || k > 0 ? 1u : 0u);
+                        product_ts<kRows / 16>(tmem_o(w), tmem_s(w), ring_v + v_slot * (kTile / 16), idesc_o, begun[w]);
                         if (it == last[w]) umma_commit(smem_u32(&ctl->o_full[w]));
                     }
                     __syncwarp();
@@ -215,11 +231,7 @@ attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_co
                 if (it + 1 < n_tiles && blk.sees(tile_of(it + 1))) {
                     tc_fence_after_thread_sync();
                     if (elect_one()) {
-                        const uint32_t k_at = ring + k_slot * kTile;
-                        for (int k = 0; k < steps_d; ++k) {
-                            const uint32_t off = (k >> 2) * kHalfTile + (k & 3) * 32;
-                            umma_bf16_cg<1>(tmem_s(w), smem_desc(q_at + w * kTile + off, 16), smem_desc(k_at + off, 16), idesc_s, k > 0 ? 1u : 0u);
-                        }
+                        product_ss<HALVES>(tmem_s(w), q_lo + w * (kTile / 16), kHalfTile, ring_k + k_slot * (kTile / 16), kHalfTile, idesc_s, steps_d);
                         umma_commit(smem_u32(&ctl->s_full[w]));
                     }
                     __syncwarp();
@@ -400,27 +412,32 @@ struct DkdvPlan {
 };
 
 // dQ and dK, dV are two kernels, each of which forms P and dS again for itself: neither has to add to memory that another
-// block adds to, so the order of every sum is fixed.  Both walk tiles of 64 columns, which two warpgroups take in turn: one
-// takes its exponentials while the tensor core works for the other.
+// block adds to, so the order of every sum is fixed.  Both walk tiles of 64 columns; two warpgroups take half of a tile's
+// columns each.  Scores of two or three tiles (what tensor memory holds) are in flight: from the moment that P and dS of a
+// tile are there it takes 1100 cycles to the scores of the next tile in the same place, and with two tiles taken in turn by
+// the warpgroups, 64 columns at a time, both the tensor core and the exponentials stood still for half of the time.
 constexpr int kCols = 64;
 constexpr uint32_t kHalfCols = kCols * 128;    // 64 rows of 64 bf16 values
 constexpr int kBwdThreads = 320;
 constexpr int kBwdSlots = 4;
 
+constexpr int kMaxBuffers = 3;
+
 struct BwdControl {
-    uint64_t fixed, full[kBwdSlots], empty[kBwdSlots], scores[2], ready[2], done;
+    uint64_t fixed, full[kBwdSlots], empty[kBwdSlots], scores[kMaxBuffers], ready[kMaxBuffers], done;
     uint32_t tmem;
     int abort;
     uint32_t bad[4];
-    alignas(16) float2 stats[8][kCols];   // of each warp, read two at a time: (lse log2 e, D) of a tile's queries
+    float sums[kRows];
+    alignas(16) float2 stats[8][kCols / 2];   // of each warp, read two at a time: (lse log2 e, D) of its half of a tile's queries
 };
-static_assert(sizeof(BwdControl) <= 5 * 1024, "the control block sits below the tiles");
-constexpr uint32_t kBwdControl = 5 * 1024;
+static_assert(sizeof(BwdControl) <= 3 * 1024, "the control block sits below the tiles");
+constexpr uint32_t kBwdControl = 3 * 1024;
 template <int HALVES> constexpr size_t bwd_smem() { return 1024 + kBwdControl + 2 * HALVES * kHalfTile + static_cast<size_t>(kBwdSlots) * 2 * HALVES * kHalfCols; }
 
-// What both kernels have around their loops: barriers, tensor memory, and the two-deep pipeline
-//   scores(0), scores(1), then for each tile: its second products when its P / dS are there, scores two tiles on.
-struct BwdRoles {
+// What both kernels have around their loops: barriers, tensor memory, and the pipeline over BUFFERS places for scores
+//   scores(0), .., scores(BUFFERS - 1), then for each tile: its second products when its P / dS are there, scores BUFFERS on.
+template <int BUFFERS> struct BwdRoles {
     BwdControl* ctl;
     volatile int* abort_flag;
     DeviceStatus* status;
@@ -431,9 +448,9 @@ struct BwdRoles {
         if (threadIdx.x == 0) {
             mbar_init(smem_u32(&ctl->fixed), 1);
             mbar_init(smem_u32(&ctl->done), 1);
-            for (int w = 0; w < 2; ++w) {
+            for (int w = 0; w < BUFFERS; ++w) {
                 mbar_init(smem_u32(&ctl->scores[w]), 1);
-                mbar_init(smem_u32(&ctl->ready[w]), 4);
+                mbar_init(smem_u32(&ctl->ready[w]), 8);
             }
             for (int s = 0; s < kBwdSlots; ++s) {
                 mbar_init(smem_u32(&ctl->full[s]), 1);
@@ -465,47 +482,56 @@ struct BwdRoles {
             if (++slot == kBwdSlots) { slot = 0; phase ^= 1u; }
         }
     }
-    // first(slot, buffer), second(slot, buffer, tile): the products, issued by one lane.
+    // first(slot, buffer), second(slot, buffer, accumulate): the products, issued by one lane.
     template <typename First, typename Second> __device__ __forceinline__ void products(First first, Second second) const {
         bool ok = n == 0 || bounded_wait_warp(smem_u32(&ctl->fixed), 0, abort_flag, status, kDevWaitSmemFull, 100, wait_ns);
-        for (int it = -2; it < n && ok; ++it) {
+        int slot = 0, buffer = 0, slot_2 = 0, buffer_2 = 0;   // of the next first products, and of the next second ones
+        uint32_t phase = 0, phase_2 = 0;
+        for (int it = -BUFFERS; it < n && ok; ++it) {
             if (it >= 0) {
-                ok = bounded_wait_warp(smem_u32(&ctl->ready[it & 1]), static_cast<uint32_t>(it >> 1) & 1u, abort_flag, status, kDevWaitTmemEmpty, it & 1, wait_ns);
+                ok = bounded_wait_warp(smem_u32(&ctl->ready[buffer_2]), phase_2, abort_flag, status, kDevWaitTmemEmpty, buffer_2, wait_ns);
                 if (!ok) break;
                 tc_fence_after_thread_sync();
                 if (elect_one()) {
-                    second(it % kBwdSlots, it & 1, it);
-                    umma_commit(smem_u32(&ctl->empty[it % kBwdSlots]));
+                    second(slot_2, buffer_2, it > 0);
+                    umma_commit(smem_u32(&ctl->empty[slot_2]));
                     if (it + 1 == n) umma_commit(smem_u32(&ctl->done));
                 }
                 __syncwarp();
+                if (++slot_2 == kBwdSlots) slot_2 = 0;
+                if (++buffer_2 == BUFFERS) { buffer_2 = 0; phase_2 ^= 1u; }
             }
-            if (it + 2 < n) {
-                const int slot = (it + 2) % kBwdSlots;
-                ok = bounded_wait_warp(smem_u32(&ctl->full[slot]), static_cast<uint32_t>((it + 2) / kBwdSlots) & 1u, abort_flag, status, kDevWaitSmemFull, slot, wait_ns);
+            if (it + BUFFERS < n) {
+                ok = bounded_wait_warp(smem_u32(&ctl->full[slot]), phase, abort_flag, status, kDevWaitSmemFull, slot, wait_ns);
                 if (!ok) break;
                 tc_fence_after_thread_sync();
                 if (elect_one()) {
-                    first(slot, (it + 2) & 1);
-                    umma_commit(smem_u32(&ctl->scores[(it + 2) & 1]));
+                    first(slot, buffer);
+                    umma_commit(smem_u32(&ctl->scores[buffer]));
                 }
                 __syncwarp();
+                if (++slot == kBwdSlots) { slot = 0; phase ^= 1u; }
+                if (++buffer == BUFFERS) buffer = 0;
             }
         }
     }
-    __device__ __forceinline__ bool wait_scores(int it) const {
-        const bool ok = bounded_wait_warp(smem_u32(&ctl->scores[it & 1]), static_cast<uint32_t>(it >> 1) & 1u, abort_flag, status, kDevWaitTmemFull, it & 1, wait_ns);
-        tc_fence_after_thread_sync();
-        return ok;
-    }
-    __device__ __forceinline__ void post_ready(int it) const {
-        tmem_st_wait();
-        tc_fence_before_thread_sync();
-        __syncwarp();
-        if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&ctl->ready[it & 1]));
-    }
-    __device__ __forceinline__ bool wait_done() const {
-        const bool ok = bounded_wait_warp(smem_u32(&ctl->done), 0, abort_flag, status, kDevWaitTmemFull, 2, wait_ns);
+    // work(it, buffer): what a warp does with a tile's scores once they are there; before(it) ahead of the wait.
+    template <typename Before, typename Work> __device__ __forceinline__ bool tiles(Before before, Work work) const {
+        int buffer = 0;
+        uint32_t phase = 0;
+        for (int it = 0; it < n; ++it) {
+            before(it);
+            if (!bounded_wait_warp(smem_u32(&ctl->scores[buffer]), phase, abort_flag, status, kDevWaitTmemFull, buffer, wait_ns)) return false;
+            tc_fence_after_thread_sync();
+            work(it, buffer);
+            tmem_st_wait();
+            tc_fence_before_thread_sync();
+            __syncwarp();
+            if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&ctl->ready[buffer]));
+            if (++buffer == BUFFERS) { buffer = 0; phase ^= 1u; }
+        }
+        if (n == 0) return true;
+        const bool ok = bounded_wait_warp(smem_u32(&ctl->done), 0, abort_flag, status, kDevWaitTmemFull, 100, wait_ns);
         tc_fence_after_thread_sync();
         return ok;
     }
@@ -541,6 +567,7 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
     uint8_t* const base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint8_t* const tiles_ptr = base + kBwdControl;
     const uint32_t tiles = smem_u32(tiles_ptr);
+    constexpr int kBuffers = 3;
     constexpr uint32_t kFixed = HALVES * kHalfTile, kStream = HALVES * kHalfCols;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int units = p.batch * p.heads, unit = blockIdx.x % units;
@@ -549,15 +576,15 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
     const int p0 = r0 + p.tk - p.tq, p1 = min(r0 + kRows, p.tq) - 1 + p.tk - p.tq;
     const int first = max(0, p0 - p.window + 1);
     const int low = first / kCols, sink_tiles = min((min(p.sinks, first) + kCols - 1) / kCols, low);
-    BwdRoles roles{reinterpret_cast<BwdControl*>(base), nullptr, status, wait_ns, p1 >= 0 ? sink_tiles + p1 / kCols - low + 1 : 0};
+    BwdRoles<kBuffers> roles{reinterpret_cast<BwdControl*>(base), nullptr, status, wait_ns, p1 >= 0 ? sink_tiles + p1 / kCols - low + 1 : 0};
     roles.abort_flag = &roles.ctl->abort;
     auto tile_of = [&](int it) { return it < sink_tiles ? it : low + it - sink_tiles; };
     roles.set_up(warp);
-    const uint32_t tmem = roles.ctl->tmem;
+    const uint32_t tmem = uniform(roles.ctl->tmem);
     grid_dependency_wait();
     const int steps_d = (p.head_dim + 15) / 16;
     const uint32_t ring = tiles + 2 * kFixed;
-    const uint32_t tmem_dq = tmem + 4u * kCols;   // behind two buffers of S and dP
+    const uint32_t tmem_dq = tmem + kBuffers * 2u * kCols;   // behind the places of S and dP
 
     if (warp == 8) {
         if (roles.n > 0 && elect_one()) {
@@ -577,23 +604,15 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
         });
     } else if (warp == 9) {
         const uint32_t idesc_s = make_idesc_bf16(kRows, kCols, 0, 0), idesc_d = make_idesc_bf16(kRows, steps_d * 16, 0, 1);
+        const uint32_t fixed_lo = uniform(desc_lo(tiles, 16)), ring_lo = uniform(desc_lo(ring, 16)), ring_mn = uniform(desc_lo(ring, kHalfCols));
         roles.products(
             [&](int slot, int buffer) {
-                const uint32_t at = ring + slot * 2 * kStream, to = tmem + buffer * 2 * kCols;
-                for (int k = 0; k < steps_d; ++k) {
-                    const uint32_t off = (k >> 2) * kHalfTile + (k & 3) * 32, offc = (k >> 2) * kHalfCols + (k & 3) * 32;
-                    umma_bf16_cg<1>(to, smem_desc(tiles + off, 16), smem_desc(at + offc, 16), idesc_s, k > 0 ? 1u : 0u);
-                }
-                for (int k = 0; k < steps_d; ++k) {
-                    const uint32_t off = (k >> 2) * kHalfTile + (k & 3) * 32, offc = (k >> 2) * kHalfCols + (k & 3) * 32;
-                    umma_bf16_cg<1>(to + kCols, smem_desc(tiles + kFixed + off, 16), smem_desc(at + kStream + offc, 16), idesc_s, k > 0 ? 1u : 0u);
-                }
+                const uint32_t at = ring_lo + slot * (2 * kStream / 16), to = tmem + buffer * 2 * kCols;
+                product_ss<HALVES>(to, fixed_lo, kHalfTile, at, kHalfCols, idesc_s, steps_d);
+                product_ss<HALVES>(to + kCols, fixed_lo + kFixed / 16, kHalfTile, at + kStream / 16, kHalfCols, idesc_s, steps_d);
             },
-            [&](int slot, int buffer, int it) {
-                const uint32_t at = ring + slot * 2 * kStream;
-#pragma unroll
-                for (int k = 0; k < kCols / 16; ++k)
-                    umma_bf16_ts(tmem_dq, tmem + buffer * 2 * kCols + k * 8, smem_desc(at + k * 2048, kHalfCols), idesc_d, it > 0 || k > 0 ? 1u : 0u);
+            [&](int slot, int buffer, bool more) {
+                product_ts<kCols / 16, 2>(tmem_dq, tmem + buffer * 2 * kCols, ring_mn + slot * (2 * kStream / 16), idesc_d, more);
             });
     } else {
         const int w = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane, i = r0 + row, pos = i + p.tk - p.tq;
@@ -603,45 +622,49 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
         float d = 0.0f, lse2 = INFINITY;   // P = 0 for a query that is not there or sees nothing
         if (i < p.tq) {
             d = attn::dot_rows(attn::row_of(p.dout, b, i, h), attn::row_of(p.out, b, i, h), p.head_dim);
-            if (w == 0) p.dvec[at] = d;
             const float lse = p.lse[at];
             if (lse != -INFINITY) lse2 = lse * kLog2e;
         }
-        bool ok = true;
-        for (int it = w; it < roles.n && ok; it += 2) {
-            ok = roles.wait_scores(it);
-            if (!ok) break;
-            const uint32_t ts = tmem + w * 2 * kCols + lanes;
-            const int j0 = tile_of(it) * kCols;
-            uint32_t s[kCols], dp[kCols];
-            tmem_ld_32x32(ts, s);
-            tmem_ld_32x32(ts + 32, s + 32);
-            tmem_ld_32x32(ts + kCols, dp);
-            tmem_ld_32x32(ts + kCols + 32, dp + 32);
-            tmem_ld_wait();
-            uint32_t seen[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
-            const bool part = !(j0 + kCols - 1 <= p0 && (j0 > p1 - p.window || j0 + kCols <= p.sinks));
-            if (part) {
-                const int from = pos - p.window + 1 - j0, to_ = pos + 1 - j0, sink = min(p.sinks, pos + 1) - j0;
+        // A warp's share of a tile: 32 queries, 32 keys.
+        const int pw = r0 + quarter * 32 + p.tk - p.tq;
+        float sum = 0.0f;
+        const bool ok = roles.tiles([](int) {}, [&](int it, int buffer) {
+            const uint32_t ts = tmem + buffer * 2 * kCols + w * 32 + lanes;
+            const int j0 = tile_of(it) * kCols + w * 32;
+            uint32_t s[32];
+            if (j0 > pw + 31 || (j0 + 31 <= pw - p.window && j0 >= p.sinks)) {   // nothing is seen
 #pragma unroll
-                for (int x = 0; x < 2; ++x) seen[x] = bits_between(from, to_, x * 32) | bits_between(0, sink, x * 32);
+                for (int y = 0; y < 16; ++y) s[y] = 0;
+            } else {
+                uint32_t dp[32];
+                tmem_ld_32x32(ts, s);
+                tmem_ld_32x32(ts + kCols, dp);
+                tmem_ld_wait();
+#pragma unroll
+                for (int y = 0; y < 32; ++y) {
+                    const float e = ex2_approx(fmaf(__uint_as_float(s[y]), c, -lse2));
+                    s[y] = __float_as_uint(e * (__uint_as_float(dp[y]) - d));
+                }
+                if (!(j0 + 31 <= pw && (j0 > pw + 31 - p.window || j0 + 32 <= p.sinks))) {
+                    const uint32_t seen = bits_between(pos - p.window + 1 - j0, pos + 1 - j0, 0) | bits_between(0, min(p.sinks, pos + 1) - j0, 0);
+#pragma unroll
+                    for (int y = 0; y < 32; ++y)
+                        if (!(seen >> y & 1u)) s[y] = 0;
+                }
+#pragma unroll
+                for (int y = 0; y < 32; ++y) sum += __uint_as_float(s[y]);
+#pragma unroll
+                for (int y = 0; y < 16; ++y) s[y] = pack_bf16(__uint_as_float(s[2 * y]), __uint_as_float(s[2 * y + 1]));
             }
-#pragma unroll
-            for (int y = 0; y < kCols; ++y) {
-                const float e = ex2_approx(fmaf(__uint_as_float(s[y]), c, -lse2));
-                s[y] = __float_as_uint(e * (__uint_as_float(dp[y]) - d));
-            }
-            if (part) {
-#pragma unroll
-                for (int y = 0; y < kCols; ++y)
-                    if (!(seen[y >> 5] >> (y & 31) & 1u)) s[y] = 0;
-            }
-#pragma unroll
-            for (int y = 0; y < kCols / 2; ++y) s[y] = pack_bf16(__uint_as_float(s[2 * y]), __uint_as_float(s[2 * y + 1]));
-            tmem_st_32x32(ts, s);
-            roles.post_ready(it);
+            tmem_st_32x16(ts, s);
+        });
+        // A row of dS adds up to nothing but for what the rounding of `out` has put into D: dK's kernel gets D without it.
+        if (w == 1) roles.ctl->sums[row] = sum;
+        named_barrier_sync(1, 256);
+        if (w == 0 && i < p.tq) {
+            const float more = d + sum + roles.ctl->sums[row];
+            p.dvec[at] = fabsf(more) < INFINITY ? more : d;
         }
-        if (ok && roles.n > 0) ok = roles.wait_done();
         bool bad = false;
         for (int x = w; x < 4 * HALVES; x += 2) {   // the warpgroups share the columns
             uint32_t o[16];
@@ -691,6 +714,7 @@ attention_dkdv_kernel(const __grid_constant__ AttentionMaps maps, const __grid_c
     const uint32_t tiles = smem_u32(tiles_ptr);
     constexpr uint32_t kFixed = HALVES * kHalfTile, kStream = HALVES * kHalfCols;
     constexpr int kHd = 64 * HALVES;
+    constexpr int kBuffers = HALVES == 1 ? 3 : 2;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int heads_k = p.heads / p.group, units = p.batch * heads_k, unit = blockIdx.x % units;
     const int b = unit / heads_k, hk = unit % heads_k;
@@ -703,16 +727,16 @@ attention_dkdv_kernel(const __grid_constant__ AttentionMaps maps, const __grid_c
     const int j0 = tile * kRows, off = p.tk - p.tq;
     const QueryTiles q(p, j0);
     const int all = q.count * p.group, it0 = static_cast<int>(static_cast<int64_t>(all) * part / parts);
-    BwdRoles roles{reinterpret_cast<BwdControl*>(base), nullptr, status, wait_ns, static_cast<int>(static_cast<int64_t>(all) * (part + 1) / parts) - it0};
+    BwdRoles<kBuffers> roles{reinterpret_cast<BwdControl*>(base), nullptr, status, wait_ns, static_cast<int>(static_cast<int64_t>(all) * (part + 1) / parts) - it0};
     roles.abort_flag = &roles.ctl->abort;
     auto head_of = [&](int it) { return hk * p.group + (it0 + it) / q.count; };
     auto query_of = [&](int it) { return (q.first + (it0 + it) % q.count) * kCols; };
     roles.set_up(warp);
-    const uint32_t tmem = roles.ctl->tmem;
+    const uint32_t tmem = uniform(roles.ctl->tmem);
     grid_dependency_wait();
     const int steps_d = (p.head_dim + 15) / 16;
     const uint32_t ring = tiles + 2 * kFixed;
-    auto tmem_acc = [&](int w) { return tmem + 4u * kCols + static_cast<uint32_t>(w) * kHd; };   // dV, dK
+    auto tmem_acc = [&](int w) { return tmem + kBuffers * 2u * kCols + static_cast<uint32_t>(w) * kHd; };   // dV, dK
 
     if (warp == 8) {
         if (roles.n > 0 && elect_one()) {
@@ -732,81 +756,67 @@ attention_dkdv_kernel(const __grid_constant__ AttentionMaps maps, const __grid_c
         });
     } else if (warp == 9) {
         const uint32_t idesc_s = make_idesc_bf16(kRows, kCols, 0, 0), idesc_d = make_idesc_bf16(kRows, steps_d * 16, 0, 1);
+        const uint32_t fixed_lo = uniform(desc_lo(tiles, 16)), ring_lo = uniform(desc_lo(ring, 16)), ring_mn = uniform(desc_lo(ring, kHalfCols));
         roles.products(
             [&](int slot, int buffer) {
-                const uint32_t at = ring + slot * 2 * kStream, to = tmem + buffer * 2 * kCols;
-                for (int k = 0; k < steps_d; ++k) {
-                    const uint32_t o = (k >> 2) * kHalfTile + (k & 3) * 32, oc = (k >> 2) * kHalfCols + (k & 3) * 32;
-                    umma_bf16_cg<1>(to, smem_desc(tiles + o, 16), smem_desc(at + oc, 16), idesc_s, k > 0 ? 1u : 0u);
-                }
-                for (int k = 0; k < steps_d; ++k) {
-                    const uint32_t o = (k >> 2) * kHalfTile + (k & 3) * 32, oc = (k >> 2) * kHalfCols + (k & 3) * 32;
-                    umma_bf16_cg<1>(to + kCols, smem_desc(tiles + kFixed + o, 16), smem_desc(at + kStream + oc, 16), idesc_s, k > 0 ? 1u : 0u);
-                }
+                const uint32_t at = ring_lo + slot * (2 * kStream / 16), to = tmem + buffer * 2 * kCols;
+                product_ss<HALVES>(to, fixed_lo, kHalfTile, at, kHalfCols, idesc_s, steps_d);
+                product_ss<HALVES>(to + kCols, fixed_lo + kFixed / 16, kHalfTile, at + kStream / 16, kHalfCols, idesc_s, steps_d);
             },
-            [&](int slot, int buffer, int it) {
-                const uint32_t at = ring + slot * 2 * kStream, from = tmem + buffer * 2 * kCols;
-#pragma unroll
-                for (int k = 0; k < kCols / 16; ++k)   // dV += P^T dO
-                    umma_bf16_ts(tmem_acc(0), from + k * 8, smem_desc(at + kStream + k * 2048, kHalfCols), idesc_d, it > 0 || k > 0 ? 1u : 0u);
-#pragma unroll
-                for (int k = 0; k < kCols / 16; ++k)   // dK += dS^T Q
-                    umma_bf16_ts(tmem_acc(1), from + kCols + k * 8, smem_desc(at + k * 2048, kHalfCols), idesc_d, it > 0 || k > 0 ? 1u : 0u);
+            [&](int slot, int buffer, bool more) {
+                const uint32_t at = ring_mn + slot * (2 * kStream / 16), from = tmem + buffer * 2 * kCols;
+                product_ts<kCols / 16, 2>(tmem_acc(0), from, at + kStream / 16, idesc_d, more);        // dV += P^T dO
+                product_ts<kCols / 16, 2>(tmem_acc(1), from + kCols, at, idesc_d, more);               // dK += dS^T Q
             });
     } else {
         const int w = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane, j = j0 + row;
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
         const float c = p.scale * kLog2e;
         float2* const stats = roles.ctl->stats[warp];
-        bool ok = true;
-        for (int it = w; it < roles.n && ok; it += 2) {
-            const int i0 = query_of(it);
-            const int64_t at = (static_cast<int64_t>(b) * p.heads + head_of(it)) * p.tq + i0;
-            float2 mine[2];
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {   // P = 0 for a query that is not there or sees nothing
-                const bool there = i0 + x * 32 + lane < p.tq;
-                const float lse = there ? p.lse[at + x * 32 + lane] : -INFINITY;
-                mine[x] = make_float2(lse == -INFINITY ? INFINITY : lse * kLog2e, there ? p.dvec[at + x * 32 + lane] : 0.0f);
-            }
+        // A warp's share of a tile: 32 keys, 32 queries.
+        const int jw = j0 + quarter * 32;
+        const bool ok = roles.tiles([&](int it) {
+            const int i0 = query_of(it) + w * 32;
+            const int64_t at = (static_cast<int64_t>(b) * p.heads + head_of(it)) * p.tq + i0 + lane;
+            const bool there = i0 + lane < p.tq;   // P = 0 for a query that is not there or sees nothing
+            const float lse = there ? p.lse[at] : -INFINITY;
+            const float2 mine = make_float2(lse == -INFINITY ? INFINITY : lse * kLog2e, there ? p.dvec[at] : 0.0f);
             __syncwarp();
-            stats[lane] = mine[0];
-            stats[32 + lane] = mine[1];
+            stats[lane] = mine;
             __syncwarp();
-            ok = roles.wait_scores(it);
-            if (!ok) break;
-            const uint32_t ts = tmem + w * 2 * kCols + lanes;
-            uint32_t s[kCols], dp[kCols];
-            tmem_ld_32x32(ts, s);
-            tmem_ld_32x32(ts + 32, s + 32);
-            tmem_ld_32x32(ts + kCols, dp);
-            tmem_ld_32x32(ts + kCols + 32, dp + 32);
-            tmem_ld_wait();
-            uint32_t seen[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
-            const bool some = !(i0 + off >= j0 + kRows - 1 && (i0 + kCols - 1 + off - j0 < p.window || j0 + kRows <= p.sinks));
-            if (some) {
-                const int from = j - off - i0, to_ = j < p.sinks ? kCols : static_cast<int>(min(static_cast<int64_t>(kCols), static_cast<int64_t>(from) + p.window));
+        }, [&](int it, int buffer) {
+            const uint32_t ts = tmem + buffer * 2 * kCols + w * 32 + lanes;
+            const int p0 = query_of(it) + w * 32 + off;   // position of the first of the 32 queries
+            uint32_t s[32], dp[32];
+            if (p0 + 31 < jw || (p0 - p.window >= jw + 31 && jw >= p.sinks)) {   // nothing is seen
 #pragma unroll
-                for (int x = 0; x < 2; ++x) seen[x] = bits_between(from, to_, x * 32);
-            }
-            uint32_t pk[kCols / 2];
-#pragma unroll
-            for (int y = 0; y < kCols; y += 2) {
-                const float4 st = *reinterpret_cast<const float4*>(&stats[y]);
-                float e0 = ex2_approx(fmaf(__uint_as_float(s[y]), c, -st.x)), e1 = ex2_approx(fmaf(__uint_as_float(s[y + 1]), c, -st.z));
-                float f0 = e0 * (__uint_as_float(dp[y]) - st.y), f1 = e1 * (__uint_as_float(dp[y + 1]) - st.w);
+                for (int y = 0; y < 16; ++y) s[y] = dp[y] = 0;
+            } else {
+                tmem_ld_32x32(ts, s);
+                tmem_ld_32x32(ts + kCols, dp);
+                tmem_ld_wait();
+                const bool some = !(p0 >= jw + 31 && (p0 + 31 - p.window < jw || jw + 32 <= p.sinks));
+                uint32_t seen = 0xFFFFFFFFu;
                 if (some) {
-                    if (!(seen[y >> 5] >> (y & 31) & 1u)) e0 = f0 = 0.0f;
-                    if (!(seen[y >> 5] >> (y & 31) & 2u)) e1 = f1 = 0.0f;
+                    const int from = j - p0;
+                    seen = bits_between(from, j < p.sinks || from > 32 - p.window ? 32 : from + p.window, 0);
                 }
-                pk[y / 2] = pack_bf16(e0, e1);
-                dp[y / 2] = pack_bf16(f0, f1);
+#pragma unroll
+                for (int y = 0; y < 32; y += 2) {
+                    const float4 st = *reinterpret_cast<const float4*>(&stats[y]);
+                    float e0 = ex2_approx(fmaf(__uint_as_float(s[y]), c, -st.x)), e1 = ex2_approx(fmaf(__uint_as_float(s[y + 1]), c, -st.z));
+                    float f0 = e0 * (__uint_as_float(dp[y]) - st.y), f1 = e1 * (__uint_as_float(dp[y + 1]) - st.w);
+                    if (some) {
+                        if (!(seen >> y & 1u)) e0 = f0 = 0.0f;
+                        if (!(seen >> y & 2u)) e1 = f1 = 0.0f;
+                    }
+                    s[y / 2] = pack_bf16(e0, e1);
+                    dp[y / 2] = pack_bf16(f0, f1);
+                }
             }
-            tmem_st_32x32(ts, pk);
-            tmem_st_32x32(ts + kCols, dp);
-            roles.post_ready(it);
-        }
-        if (ok && roles.n > 0) ok = roles.wait_done();
+            tmem_st_32x16(ts, s);
+            tmem_st_32x16(ts + kCols, dp);
+        });
         // warpgroup 0 has dV to write, warpgroup 1 dK
         const float factor = w == 0 ? 1.0f : p.scale;
         float* const sums = parts > 1 ? p.partial + ((plan.slot(keep, unit, at_item, units) * 2 + w) * kRows + row) * kHd : nullptr;

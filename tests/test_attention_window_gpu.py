@@ -65,13 +65,15 @@ def _check_backward(dq, dk, dv, dout, q, k, v, out, lse, window, sinks, scale=No
     p = torch.where(seen, (qd @ kd.transpose(-1, -2) * c - lse.double()[..., None]).exp(), 0)
     dp, d = dod @ vd.transpose(-1, -2), (dod * od).sum(-1, keepdim=True)
     ds = torch.where(seen, p * (dp - d), 0)
+    # dK is formed with the row sums of P dP, which are D but for the rounding of out
+    ds_k = torch.where(seen, p * (dp - (p * dp).sum(-1, keepdim=True)), 0)
     # dS: its rounding as an operand and P's relative error, fp32 products of hd terms in dP and D
-    off = P * ds.abs() + p * hd * 2.0 ** -23 * (dod.abs() @ vd.abs().transpose(-1, -2) + (dod * od).abs().sum(-1, keepdim=True))
+    off = P * torch.maximum(ds.abs(), ds_k.abs()) + p * hd * 2.0 ** -23 * (dod.abs() @ vd.abs().transpose(-1, -2) + (dod * od).abs().sum(-1, keepdim=True))
 
     def group(x):
         return x.reshape(b, hkv, h // hkv, x.shape[-2], hd).sum(2).transpose(1, 2)
     for name, got, want, bound in (("dq", dq, (c * ds @ kd).transpose(1, 2), (c * off @ kd.abs()).transpose(1, 2)),
-                                   ("dk", dk, group(c * ds.transpose(-1, -2) @ qd), group(c * off.transpose(-1, -2) @ qd.abs())),
+                                   ("dk", dk, group(c * ds_k.transpose(-1, -2) @ qd), group(c * off.transpose(-1, -2) @ qd.abs())),
                                    ("dv", dv, group(p.transpose(-1, -2) @ dod), group(P * p.transpose(-1, -2) @ dod.abs()))):
         # accumulation in fp32, truncated by the tensor cores, of at most 4096 terms: 2^-11 of the terms' sizes
         bound = want.abs() * 2.0 ** -8 + bound * (1 + 2.0 ** -3) + 1e-30
