@@ -412,13 +412,12 @@ struct DkdvPlan {
 };
 
 // dQ and dK, dV are two kernels, each of which forms P and dS again for itself: neither has to add to memory that another
-// block adds to, so the order of every sum is fixed.  Both walk tiles of 64 columns; two warpgroups take half of a tile's
-// columns each.  Scores of two or three tiles (what tensor memory holds) are in flight: from the moment that P and dS of a
-// tile are there it takes 1100 cycles to the scores of the next tile in the same place, and with two tiles taken in turn by
-// the warpgroups, 64 columns at a time, both the tensor core and the exponentials stood still for half of the time.
+// block adds to, so the order of every sum is fixed.  Both walk tiles of 64 columns, which as many warpgroups take in turn as
+// tensor memory has places for scores: two or three.  A warpgroup's turn is a chain of 900 cycles of its own work and 900 of
+// waiting for its products; with two of them both the tensor core and the exponentials stood still for a third of the time
+// (two warpgroups on the halves of one tile, three places: no better, they want the special-function unit at the same time).
 constexpr int kCols = 64;
 constexpr uint32_t kHalfCols = kCols * 128;    // 64 rows of 64 bf16 values
-constexpr int kBwdThreads = 320;
 constexpr int kBwdSlots = 4;
 
 constexpr int kMaxBuffers = 3;
@@ -428,16 +427,19 @@ struct BwdControl {
     uint32_t tmem;
     int abort;
     uint32_t bad[4];
-    float sums[kRows];
-    alignas(16) float2 stats[8][kCols / 2];   // of each warp, read two at a time: (lse log2 e, D) of its half of a tile's queries
+    float d[kRows];               // dQ: D of the block's queries
+    float sums[kMaxBuffers][kRows];   // dQ: row sums of dS by each warpgroup
+    alignas(16) float2 stats[4 * kMaxBuffers][kCols];   // dK, dV: of each warp, read two at a time: (lse log2 e, D) of a tile's queries
 };
-static_assert(sizeof(BwdControl) <= 3 * 1024, "the control block sits below the tiles");
-constexpr uint32_t kBwdControl = 3 * 1024;
+static_assert(sizeof(BwdControl) <= 9 * 1024, "the control block sits below the tiles");
+constexpr uint32_t kBwdControl = 9 * 1024;
 template <int HALVES> constexpr size_t bwd_smem() { return 1024 + kBwdControl + 2 * HALVES * kHalfTile + static_cast<size_t>(kBwdSlots) * 2 * HALVES * kHalfCols; }
 
-// What both kernels have around their loops: barriers, tensor memory, and the pipeline over BUFFERS places for scores
+// What both kernels have around their loops: barriers, tensor memory, and the pipeline over BUFFERS places for scores, each
+// with a warpgroup of its own (warps 0 .. 4 BUFFERS - 1; then a warp for the loads and one for the products)
 //   scores(0), .., scores(BUFFERS - 1), then for each tile: its second products when its P / dS are there, scores BUFFERS on.
 template <int BUFFERS> struct BwdRoles {
+    static constexpr int kSoftmax = 128 * BUFFERS, kThreads = kSoftmax + 64, kLoadWarp = 4 * BUFFERS, kProductWarp = 4 * BUFFERS + 1;
     BwdControl* ctl;
     volatile int* abort_flag;
     DeviceStatus* status;
@@ -450,7 +452,7 @@ template <int BUFFERS> struct BwdRoles {
             mbar_init(smem_u32(&ctl->done), 1);
             for (int w = 0; w < BUFFERS; ++w) {
                 mbar_init(smem_u32(&ctl->scores[w]), 1);
-                mbar_init(smem_u32(&ctl->ready[w]), 8);
+                mbar_init(smem_u32(&ctl->ready[w]), 4);
             }
             for (int s = 0; s < kBwdSlots; ++s) {
                 mbar_init(smem_u32(&ctl->full[s]), 1);
@@ -460,7 +462,7 @@ template <int BUFFERS> struct BwdRoles {
             for (uint32_t& x : ctl->bad) x = 0;
             fence_barrier_init();
         }
-        if (warp == 9) {
+        if (warp == kProductWarp) {
             tmem_alloc(smem_u32(&ctl->tmem), 512);
             tmem_relinquish_alloc_permit();
         }
@@ -515,31 +517,47 @@ template <int BUFFERS> struct BwdRoles {
             }
         }
     }
-    // work(it, buffer): what a warp does with a tile's scores once they are there; before(it) ahead of the wait.
-    template <typename Before, typename Work> __device__ __forceinline__ bool tiles(Before before, Work work) const {
-        int buffer = 0;
+    // work(it): what warpgroup `w` does with a tile's scores once they are there; before(it) ahead of the wait.
+    template <typename Before, typename Work> __device__ __forceinline__ bool tiles(int w, Before before, Work work) const {
         uint32_t phase = 0;
-        for (int it = 0; it < n; ++it) {
+        for (int it = w; it < n; it += BUFFERS) {
             before(it);
-            if (!bounded_wait_warp(smem_u32(&ctl->scores[buffer]), phase, abort_flag, status, kDevWaitTmemFull, buffer, wait_ns)) return false;
+            if (!bounded_wait_warp(smem_u32(&ctl->scores[w]), phase, abort_flag, status, kDevWaitTmemFull, w, wait_ns)) return false;
             tc_fence_after_thread_sync();
-            work(it, buffer);
+            work(it);
             tmem_st_wait();
             tc_fence_before_thread_sync();
             __syncwarp();
-            if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&ctl->ready[buffer]));
-            if (++buffer == BUFFERS) { buffer = 0; phase ^= 1u; }
+            if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&ctl->ready[w]));
+            phase ^= 1u;
         }
         if (n == 0) return true;
         const bool ok = bounded_wait_warp(smem_u32(&ctl->done), 0, abort_flag, status, kDevWaitTmemFull, 100, wait_ns);
         tc_fence_after_thread_sync();
         return ok;
     }
+    // The end of a block's copy-out, for all softmax threads: `mine` rows of this warp's 32 hold values that are not finite.
+    // store() issues the copies; the rows are formed again by again(row in the quarter) once the copies are complete.
+    template <typename Store, typename Again> __device__ __forceinline__ void copy_out(int w, int quarter, uint32_t mine, Store store, Again again) const {
+        if ((threadIdx.x & 31) == 0 && mine != 0) atomicOr(&ctl->bad[quarter], mine);
+        fence_proxy_async_smem();
+        named_barrier_sync(1, kSoftmax);
+        const bool any = (ctl->bad[0] | ctl->bad[1] | ctl->bad[2] | ctl->bad[3]) != 0;
+        if (threadIdx.x == 0) {
+            store();
+            bulk_commit_group();
+            if (any) bulk_wait_group0();
+            else bulk_wait_group_read0();   // the tiles are given back, the copies end by themselves
+        }
+        if (!any) return;
+        named_barrier_sync(1, kSoftmax);
+        for (uint32_t m = w == 0 ? ctl->bad[quarter] : 0; m != 0; m &= m - 1) again(__ffs(m) - 1);
+    }
     __device__ __forceinline__ void tear_down(int warp, uint32_t tmem) {
         if (*abort_flag) __nanosleep(200000);
         tc_fence_before_thread_sync();
         __syncthreads();
-        if (warp == 9) {
+        if (warp == kProductWarp) {
             tc_fence_after_thread_sync();
             tmem_dealloc(tmem, 512);
         }
@@ -559,9 +577,38 @@ __device__ __forceinline__ void put_row16(uint8_t* tile, int row, int x, const u
     }
 }
 
+// D of 128 queries into shared memory by the first eight warps, 16 queries each: 8 HALVES lanes for a row, a row's 16 bytes
+// each, so that the loads of all of a warp's rows are in flight at once (a thread a row took 6000 to 12000 cycles).
+template <int HALVES>
+__device__ __forceinline__ void row_products(const AttentionParams& p, int b, int h, int r0, float* d, int warp) {
+    constexpr int kLanes = 8 * HALVES, kAtOnce = 32 / kLanes, kTurns = 16 / kAtOnce;
+    if (warp >= 8) return;
+    const int lane = threadIdx.x & 31, col = lane % kLanes * 8, first = warp * 16 + lane / kLanes;
+    uint4 x[kTurns], y[kTurns];
+#pragma unroll
+    for (int n = 0; n < kTurns; ++n) {
+        const int i = r0 + first + n * kAtOnce;
+        x[n] = y[n] = make_uint4(0, 0, 0, 0);
+        if (i < p.tq && col < p.head_dim) {
+            x[n] = *reinterpret_cast<const uint4*>(attn::row_of(p.dout, b, i, h) + col);
+            y[n] = *reinterpret_cast<const uint4*>(attn::row_of(p.out, b, i, h) + col);
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < kTurns; ++n) {
+        const uint32_t xs[4] = {x[n].x, x[n].y, x[n].z, x[n].w}, ys[4] = {y[n].x, y[n].y, y[n].z, y[n].w};
+        float s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s = fmaf(attn::hi_f(xs[k]), attn::hi_f(ys[k]), fmaf(attn::lo_f(xs[k]), attn::lo_f(ys[k]), s));
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (lane % kLanes == 0) d[first + n * kAtOnce] = s;
+    }
+}
+
 // dQ of 128 queries: S = Q K^T and dP = dO V^T of 64 keys, dS = P (dP - D), dQ += dS K.
 template <int HALVES>
-__global__ void __launch_bounds__(kBwdThreads, 1)
+__global__ void __launch_bounds__(BwdRoles<3>::kThreads, 1)
 attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_constant__ AttentionParams p, int blocks_q, DeviceStatus* status, uint64_t wait_ns) {
     extern __shared__ uint8_t raw[];
     uint8_t* const base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -586,7 +633,7 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
     const uint32_t ring = tiles + 2 * kFixed;
     const uint32_t tmem_dq = tmem + kBuffers * 2u * kCols;   // behind the places of S and dP
 
-    if (warp == 8) {
+    if (warp == roles.kLoadWarp) {
         if (roles.n > 0 && elect_one()) {
             mbar_arrive_expect_tx(smem_u32(&roles.ctl->fixed), 2 * kFixed);
             for (int x = 0; x < HALVES; ++x) {
@@ -602,7 +649,7 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
                 tma_load_4d(at + kStream + x * kHalfCols, &maps.v, bar, x * 64, tile_of(it) * kCols, hk, b);
             }
         });
-    } else if (warp == 9) {
+    } else if (warp == roles.kProductWarp) {
         const uint32_t idesc_s = make_idesc_bf16(kRows, kCols, 0, 0), idesc_d = make_idesc_bf16(kRows, steps_d * 16, 0, 1);
         const uint32_t fixed_lo = uniform(desc_lo(tiles, 16)), ring_lo = uniform(desc_lo(ring, 16)), ring_mn = uniform(desc_lo(ring, kHalfCols));
         roles.products(
@@ -619,54 +666,60 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
         const float c = p.scale * kLog2e;
         const int64_t at = (static_cast<int64_t>(b) * p.heads + h) * p.tq + i;
-        float d = 0.0f, lse2 = INFINITY;   // P = 0 for a query that is not there or sees nothing
+        row_products<HALVES>(p, b, h, r0, roles.ctl->d, warp);
+        named_barrier_sync(1, roles.kSoftmax);
+        const float d = roles.ctl->d[row];
+        float lse2 = INFINITY;   // P = 0 for a query that is not there or sees nothing
         if (i < p.tq) {
-            d = attn::dot_rows(attn::row_of(p.dout, b, i, h), attn::row_of(p.out, b, i, h), p.head_dim);
             const float lse = p.lse[at];
             if (lse != -INFINITY) lse2 = lse * kLog2e;
         }
-        // A warp's share of a tile: 32 queries, 32 keys.
-        const int pw = r0 + quarter * 32 + p.tk - p.tq;
+        const int pw = r0 + quarter * 32 + p.tk - p.tq;   // position of the warp's first query
         float sum = 0.0f;
-        const bool ok = roles.tiles([](int) {}, [&](int it, int buffer) {
-            const uint32_t ts = tmem + buffer * 2 * kCols + w * 32 + lanes;
-            const int j0 = tile_of(it) * kCols + w * 32;
-            uint32_t s[32];
-            if (j0 > pw + 31 || (j0 + 31 <= pw - p.window && j0 >= p.sinks)) {   // nothing is seen
+        const bool ok = roles.tiles(w, [](int) {}, [&](int it) {
 #pragma unroll
-                for (int y = 0; y < 16; ++y) s[y] = 0;
-            } else {
-                uint32_t dp[32];
-                tmem_ld_32x32(ts, s);
-                tmem_ld_32x32(ts + kCols, dp);
-                tmem_ld_wait();
+            for (int x = 0; x < 2; ++x) {   // 32 keys at a time
+                const uint32_t ts = tmem + w * 2 * kCols + x * 32 + lanes;
+                const int j0 = tile_of(it) * kCols + x * 32;
+                uint32_t s[32];
+                if (j0 > pw + 31 || (j0 + 31 <= pw - p.window && j0 >= p.sinks)) {   // nothing is seen
 #pragma unroll
-                for (int y = 0; y < 32; ++y) {
-                    const float e = ex2_approx(fmaf(__uint_as_float(s[y]), c, -lse2));
-                    s[y] = __float_as_uint(e * (__uint_as_float(dp[y]) - d));
+                    for (int y = 0; y < 16; ++y) s[y] = 0;
+                } else {
+                    uint32_t dp[32];
+                    tmem_ld_32x32(ts, s);
+                    tmem_ld_32x32(ts + kCols, dp);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int y = 0; y < 32; ++y) {
+                        const float e = ex2_approx(fmaf(__uint_as_float(s[y]), c, -lse2));
+                        s[y] = __float_as_uint(e * (__uint_as_float(dp[y]) - d));
+                    }
+                    if (!(j0 + 31 <= pw && (j0 > pw + 31 - p.window || j0 + 32 <= p.sinks))) {
+                        const uint32_t seen = bits_between(pos - p.window + 1 - j0, pos + 1 - j0, 0) | bits_between(0, min(p.sinks, pos + 1) - j0, 0);
+#pragma unroll
+                        for (int y = 0; y < 32; ++y)
+                            if (!(seen >> y & 1u)) s[y] = 0;
+                    }
+#pragma unroll
+                    for (int y = 0; y < 32; ++y) sum += __uint_as_float(s[y]);
+#pragma unroll
+                    for (int y = 0; y < 16; ++y) s[y] = pack_bf16(__uint_as_float(s[2 * y]), __uint_as_float(s[2 * y + 1]));
                 }
-                if (!(j0 + 31 <= pw && (j0 > pw + 31 - p.window || j0 + 32 <= p.sinks))) {
-                    const uint32_t seen = bits_between(pos - p.window + 1 - j0, pos + 1 - j0, 0) | bits_between(0, min(p.sinks, pos + 1) - j0, 0);
-#pragma unroll
-                    for (int y = 0; y < 32; ++y)
-                        if (!(seen >> y & 1u)) s[y] = 0;
-                }
-#pragma unroll
-                for (int y = 0; y < 32; ++y) sum += __uint_as_float(s[y]);
-#pragma unroll
-                for (int y = 0; y < 16; ++y) s[y] = pack_bf16(__uint_as_float(s[2 * y]), __uint_as_float(s[2 * y + 1]));
+                tmem_st_32x16(ts, s);
             }
-            tmem_st_32x16(ts, s);
         });
         // A row of dS adds up to nothing but for what the rounding of `out` has put into D: dK's kernel gets D without it.
-        if (w == 1) roles.ctl->sums[row] = sum;
-        named_barrier_sync(1, 256);
+        roles.ctl->sums[w][row] = sum;
+        named_barrier_sync(1, roles.kSoftmax);
         if (w == 0 && i < p.tq) {
-            const float more = d + sum + roles.ctl->sums[row];
+            float more = d;
+#pragma unroll
+            for (int x = 0; x < kBuffers; ++x) more += roles.ctl->sums[x][row];
             p.dvec[at] = fabsf(more) < INFINITY ? more : d;
         }
         bool bad = false;
-        for (int x = w; x < 4 * HALVES; x += 2) {   // the warpgroups share the columns
+        for (int x = w; x < 4 * HALVES; x += kBuffers) {   // the warpgroups share the columns
             uint32_t o[16];
 #pragma unroll
             for (int y = 0; y < 16; ++y) o[y] = 0;
@@ -682,21 +735,10 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
             }
             put_row16(tiles_ptr, row, x, o);
         }
-        const uint32_t again = __ballot_sync(0xffffffffu, bad && ok && i < p.tq);
-        if (lane == 0 && again != 0) atomicOr(&roles.ctl->bad[quarter], again);
-        fence_proxy_async_smem();
-        named_barrier_sync(1, 256);
-        if (threadIdx.x == 0) {
-            for (int x = 0; x < HALVES; ++x) tma_store_4d(&maps.dq, tiles + x * kHalfTile, x * 64, r0, h, b);
-            bulk_commit_group();
-            bulk_wait_group0();
-        }
-        named_barrier_sync(1, 256);
         // as in the forward kernel: a hidden key that is not finite has spoilt the row
-        for (uint32_t m = w == 0 ? roles.ctl->bad[quarter] : 0; m != 0; m &= m - 1) {
-            const int r = __ffs(m) - 1;
-            attn::dq_row(p, b, h, r0 + quarter * 32 + r, __shfl_sync(0xffffffffu, d, r));
-        }
+        roles.copy_out(w, quarter, __ballot_sync(0xffffffffu, bad && ok && i < p.tq), [&] {
+            for (int x = 0; x < HALVES; ++x) tma_store_4d(&maps.dq, tiles + x * kHalfTile, x * 64, r0, h, b);
+        }, [&](int r) { attn::dq_row(p, b, h, r0 + quarter * 32 + r, __shfl_sync(0xffffffffu, d, r)); });
     }
     roles.tear_down(warp, tmem);
 }
@@ -705,7 +747,7 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
 // heads of the group, one head after the other.  A block may do a part of them only: its sums then go to the workspace in
 // fp32, and attention_dkdv_sum_kernel adds the parts in order.
 template <int HALVES>
-__global__ void __launch_bounds__(kBwdThreads, 1)
+__global__ void __launch_bounds__(BwdRoles<HALVES == 1 ? 3 : 2>::kThreads, 1)
 attention_dkdv_kernel(const __grid_constant__ AttentionMaps maps, const __grid_constant__ AttentionParams p, const DkdvPlan plan, DeviceStatus* status,
                       uint64_t wait_ns) {
     extern __shared__ uint8_t raw[];
@@ -738,7 +780,7 @@ attention_dkdv_kernel(const __grid_constant__ AttentionMaps maps, const __grid_c
     const uint32_t ring = tiles + 2 * kFixed;
     auto tmem_acc = [&](int w) { return tmem + kBuffers * 2u * kCols + static_cast<uint32_t>(w) * kHd; };   // dV, dK
 
-    if (warp == 8) {
+    if (warp == roles.kLoadWarp) {
         if (roles.n > 0 && elect_one()) {
             mbar_arrive_expect_tx(smem_u32(&roles.ctl->fixed), 2 * kFixed);
             for (int x = 0; x < HALVES; ++x) {
@@ -754,7 +796,7 @@ attention_dkdv_kernel(const __grid_constant__ AttentionMaps maps, const __grid_c
                 tma_load_4d(at + kStream + x * kHalfCols, &maps.dout, bar, x * 64, query_of(it), head_of(it), b);
             }
         });
-    } else if (warp == 9) {
+    } else if (warp == roles.kProductWarp) {
         const uint32_t idesc_s = make_idesc_bf16(kRows, kCols, 0, 0), idesc_d = make_idesc_bf16(kRows, steps_d * 16, 0, 1);
         const uint32_t fixed_lo = uniform(desc_lo(tiles, 16)), ring_lo = uniform(desc_lo(ring, 16)), ring_mn = uniform(desc_lo(ring, kHalfCols));
         roles.products(
@@ -773,60 +815,67 @@ attention_dkdv_kernel(const __grid_constant__ AttentionMaps maps, const __grid_c
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
         const float c = p.scale * kLog2e;
         float2* const stats = roles.ctl->stats[warp];
-        // A warp's share of a tile: 32 keys, 32 queries.
-        const int jw = j0 + quarter * 32;
-        const bool ok = roles.tiles([&](int it) {
-            const int i0 = query_of(it) + w * 32;
-            const int64_t at = (static_cast<int64_t>(b) * p.heads + head_of(it)) * p.tq + i0 + lane;
-            const bool there = i0 + lane < p.tq;   // P = 0 for a query that is not there or sees nothing
-            const float lse = there ? p.lse[at] : -INFINITY;
-            const float2 mine = make_float2(lse == -INFINITY ? INFINITY : lse * kLog2e, there ? p.dvec[at] : 0.0f);
-            __syncwarp();
-            stats[lane] = mine;
-            __syncwarp();
-        }, [&](int it, int buffer) {
-            const uint32_t ts = tmem + buffer * 2 * kCols + w * 32 + lanes;
-            const int p0 = query_of(it) + w * 32 + off;   // position of the first of the 32 queries
-            uint32_t s[32], dp[32];
-            if (p0 + 31 < jw || (p0 - p.window >= jw + 31 && jw >= p.sinks)) {   // nothing is seen
+        const int jw = j0 + quarter * 32;   // the warp's first key
+        const bool ok = roles.tiles(w, [&](int it) {
+            const int i0 = query_of(it);
+            const int64_t at = (static_cast<int64_t>(b) * p.heads + head_of(it)) * p.tq + i0;
+            float2 mine[2];
 #pragma unroll
-                for (int y = 0; y < 16; ++y) s[y] = dp[y] = 0;
-            } else {
-                tmem_ld_32x32(ts, s);
-                tmem_ld_32x32(ts + kCols, dp);
-                tmem_ld_wait();
-                const bool some = !(p0 >= jw + 31 && (p0 + 31 - p.window < jw || jw + 32 <= p.sinks));
-                uint32_t seen = 0xFFFFFFFFu;
-                if (some) {
-                    const int from = j - p0;
-                    seen = bits_between(from, j < p.sinks || from > 32 - p.window ? 32 : from + p.window, 0);
-                }
-#pragma unroll
-                for (int y = 0; y < 32; y += 2) {
-                    const float4 st = *reinterpret_cast<const float4*>(&stats[y]);
-                    float e0 = ex2_approx(fmaf(__uint_as_float(s[y]), c, -st.x)), e1 = ex2_approx(fmaf(__uint_as_float(s[y + 1]), c, -st.z));
-                    float f0 = e0 * (__uint_as_float(dp[y]) - st.y), f1 = e1 * (__uint_as_float(dp[y + 1]) - st.w);
-                    if (some) {
-                        if (!(seen >> y & 1u)) e0 = f0 = 0.0f;
-                        if (!(seen >> y & 2u)) e1 = f1 = 0.0f;
-                    }
-                    s[y / 2] = pack_bf16(e0, e1);
-                    dp[y / 2] = pack_bf16(f0, f1);
-                }
+            for (int x = 0; x < 2; ++x) {   // P = 0 for a query that is not there or sees nothing
+                const bool there = i0 + x * 32 + lane < p.tq;
+                const float lse = there ? p.lse[at + x * 32 + lane] : -INFINITY;
+                mine[x] = make_float2(lse == -INFINITY ? INFINITY : lse * kLog2e, there ? p.dvec[at + x * 32 + lane] : 0.0f);
             }
-            tmem_st_32x16(ts, s);
-            tmem_st_32x16(ts + kCols, dp);
+            __syncwarp();
+            stats[lane] = mine[0];
+            stats[32 + lane] = mine[1];
+            __syncwarp();
+        }, [&](int it) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {   // 32 queries at a time
+                const uint32_t ts = tmem + w * 2 * kCols + x * 32 + lanes;
+                const int p0 = query_of(it) + x * 32 + off;   // position of the first of them
+                uint32_t s[32], dp[32];
+                if (p0 + 31 < jw || (p0 - p.window >= jw + 31 && jw >= p.sinks)) {   // nothing is seen
+#pragma unroll
+                    for (int y = 0; y < 16; ++y) s[y] = dp[y] = 0;
+                } else {
+                    tmem_ld_32x32(ts, s);
+                    tmem_ld_32x32(ts + kCols, dp);
+                    tmem_ld_wait();
+                    const bool some = !(p0 >= jw + 31 && (p0 + 31 - p.window < jw || jw + 32 <= p.sinks));
+                    uint32_t seen = 0xFFFFFFFFu;
+                    if (some) {
+                        const int from = j - p0;
+                        seen = bits_between(from, j < p.sinks || from > 32 - p.window ? 32 : from + p.window, 0);
+                    }
+#pragma unroll
+                    for (int y = 0; y < 32; y += 2) {
+                        const float4 st = *reinterpret_cast<const float4*>(&stats[x * 32 + y]);
+                        float e0 = ex2_approx(fmaf(__uint_as_float(s[y]), c, -st.x)), e1 = ex2_approx(fmaf(__uint_as_float(s[y + 1]), c, -st.z));
+                        float f0 = e0 * (__uint_as_float(dp[y]) - st.y), f1 = e1 * (__uint_as_float(dp[y + 1]) - st.w);
+                        if (some) {
+                            if (!(seen >> y & 1u)) e0 = f0 = 0.0f;
+                            if (!(seen >> y & 2u)) e1 = f1 = 0.0f;
+                        }
+                        s[y / 2] = pack_bf16(e0, e1);
+                        dp[y / 2] = pack_bf16(f0, f1);
+                    }
+                }
+                tmem_st_32x16(ts, s);
+                tmem_st_32x16(ts + kCols, dp);
+            }
         });
-        // warpgroup 0 has dV to write, warpgroup 1 dK
-        const float factor = w == 0 ? 1.0f : p.scale;
-        float* const sums = parts > 1 ? p.partial + ((plan.slot(keep, unit, at_item, units) * 2 + w) * kRows + row) * kHd : nullptr;
+        // the warpgroups share the 16-column pieces of dV and dK
         bool bad = false;
-        for (int x = 0; x < 4 * HALVES; ++x) {
+        for (int x = w; x < 8 * HALVES; x += kBuffers) {
+            const int which = x / (4 * HALVES), piece = x % (4 * HALVES);
+            const float factor = which == 0 ? 1.0f : p.scale;
             uint32_t o[16];
 #pragma unroll
             for (int y = 0; y < 16; ++y) o[y] = 0;
-            if (ok && roles.n > 0 && x < steps_d) {
-                tmem_ld_32x16(tmem_acc(w) + lanes + x * 16, o);
+            if (ok && roles.n > 0 && piece < steps_d) {
+                tmem_ld_32x16(tmem_acc(which) + lanes + piece * 16, o);
                 tmem_ld_wait();
             }
 #pragma unroll
@@ -835,27 +884,21 @@ attention_dkdv_kernel(const __grid_constant__ AttentionMaps maps, const __grid_c
                 bad = bad || !(fabsf(f) < INFINITY);
                 o[y] = __float_as_uint(f);
             }
-            if (sums != nullptr) {
+            if (parts > 1) {
+                float* const sums = p.partial + ((plan.slot(keep, unit, at_item, units) * 2 + which) * kRows + row) * kHd + piece * 16;
 #pragma unroll
-                for (int y = 0; y < 16; y += 4) *reinterpret_cast<uint4*>(sums + x * 16 + y) = make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]);
+                for (int y = 0; y < 16; y += 4) *reinterpret_cast<uint4*>(sums + y) = make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]);
             } else {
-                put_row16(tiles_ptr + w * kFixed, row, x, o);
+                put_row16(tiles_ptr + which * kFixed, row, piece, o);
             }
         }
-        if (parts == 1) {
-            const uint32_t again = __ballot_sync(0xffffffffu, bad && ok && j < p.tk);
-            if (lane == 0 && again != 0) atomicOr(&roles.ctl->bad[quarter], again);
-            fence_proxy_async_smem();
-            named_barrier_sync(1, 256);
-            if (row == 0) {
-                for (int x = 0; x < HALVES; ++x) tma_store_4d(w == 0 ? &maps.dv : &maps.dk, tiles + w * kFixed + x * kHalfTile, x * 64, j0, hk, b);
-                bulk_commit_group();
-                bulk_wait_group0();
-            }
-            named_barrier_sync(1, 256);
-            for (uint32_t m = w == 0 ? roles.ctl->bad[quarter] : 0; m != 0; m &= m - 1)
-                attn::dkdv_row(p, b, hk, j0 + quarter * 32 + __ffs(m) - 1);
-        }
+        if (parts == 1)
+            roles.copy_out(w, quarter, __ballot_sync(0xffffffffu, bad && ok && j < p.tk), [&] {
+                for (int x = 0; x < HALVES; ++x) {
+                    tma_store_4d(&maps.dv, tiles + x * kHalfTile, x * 64, j0, hk, b);
+                    tma_store_4d(&maps.dk, tiles + kFixed + x * kHalfTile, x * 64, j0, hk, b);
+                }
+            }, [&](int r) { attn::dkdv_row(p, b, hk, j0 + quarter * 32 + r); });
     }
     roles.tear_down(warp, tmem);
 }
@@ -957,15 +1000,15 @@ cudaError_t launch_attention_bwd_sm100(AttentionParams p, const CUtensorMap* m, 
     const int blocks_q = (p.tq + kRows - 1) / kRows;
     const bool narrow = p.head_dim <= 64;
     int64_t blocks = static_cast<int64_t>(p.batch) * p.heads * blocks_q;
-    cudaError_t e = narrow ? launch_sm(attention_dq_kernel<1>, blocks, kBwdThreads, bwd_smem<1>(), stream, maps, p, blocks_q, status, wait_ns)
-                           : launch_sm(attention_dq_kernel<2>, blocks, kBwdThreads, bwd_smem<2>(), stream, maps, p, blocks_q, status, wait_ns);
+    cudaError_t e = narrow ? launch_sm(attention_dq_kernel<1>, blocks, BwdRoles<3>::kThreads, bwd_smem<1>(), stream, maps, p, blocks_q, status, wait_ns)
+                           : launch_sm(attention_dq_kernel<2>, blocks, BwdRoles<3>::kThreads, bwd_smem<2>(), stream, maps, p, blocks_q, status, wait_ns);
     if (e != cudaSuccess) return e;
     maps.q = m[5]; maps.dout = m[6]; maps.k = m[7]; maps.v = m[8]; maps.dk = m[9]; maps.dv = m[10];
     const DkdvPlan pl = dkdv_plan(p, sms);
     const int64_t units = static_cast<int64_t>(p.batch) * (p.heads / p.group);
     blocks = units * pl.items();
-    e = narrow ? launch_sm(attention_dkdv_kernel<1>, blocks, kBwdThreads, bwd_smem<1>(), stream, maps, p, pl, status, wait_ns)
-               : launch_sm(attention_dkdv_kernel<2>, blocks, kBwdThreads, bwd_smem<2>(), stream, maps, p, pl, status, wait_ns);
+    e = narrow ? launch_sm(attention_dkdv_kernel<1>, blocks, BwdRoles<3>::kThreads, bwd_smem<1>(), stream, maps, p, pl, status, wait_ns)
+               : launch_sm(attention_dkdv_kernel<2>, blocks, BwdRoles<2>::kThreads, bwd_smem<2>(), stream, maps, p, pl, status, wait_ns);
     for (int kept = 1; kept >= 0 && e == cudaSuccess; --kept) {
         const int n_tiles = kept ? pl.sink_tiles : pl.tiles - pl.sink_tiles;
         if (n_tiles == 0 || (kept ? pl.sink_parts : pl.parts) == 1) continue;
