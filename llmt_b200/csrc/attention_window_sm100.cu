@@ -62,6 +62,34 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return r;
 }
 
+// Two fp32 values as the packed instructions take them.
+__device__ __forceinline__ uint64_t two(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 both(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t two(uint32_t lo, uint32_t hi) { return two(__uint_as_float(lo), __uint_as_float(hi)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 // What a block of queries [r0, r0 + 128) of one head sees, in tiles of keys.
 struct QueryBlock {
     int head, r0;
@@ -429,7 +457,7 @@ struct BwdControl {
     uint32_t bad[4];
     float d[kRows];               // dQ: D of the block's queries
     float sums[kMaxBuffers][kRows];   // dQ: row sums of dS by each warpgroup
-    alignas(16) float2 stats[4 * kMaxBuffers][kCols];   // dK, dV: of each warp, read two at a time: (lse log2 e, D) of a tile's queries
+    alignas(16) float4 stats[4 * kMaxBuffers][kCols / 2];   // dK, dV: of each warp, for two queries of a tile each: - lse log2 e of both, - D of both
 };
 static_assert(sizeof(BwdControl) <= 9 * 1024, "the control block sits below the tiles");
 constexpr uint32_t kBwdControl = 9 * 1024;
@@ -675,7 +703,8 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
             if (lse != -INFINITY) lse2 = lse * kLog2e;
         }
         const int pw = r0 + quarter * 32 + p.tk - p.tq;   // position of the warp's first query
-        float sum = 0.0f;
+        uint64_t sum = 0;
+        const uint64_t c2 = two(c, c), less2 = two(-lse2, -lse2), lessd = two(-d, -d);
         const bool ok = roles.tiles(w, [](int) {}, [&](int it) {
 #pragma unroll
             for (int x = 0; x < 2; ++x) {   // 32 keys at a time
@@ -690,27 +719,31 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
                     tmem_ld_32x32(ts, s);
                     tmem_ld_32x32(ts + kCols, dp);
                     tmem_ld_wait();
+                    uint64_t f[16];
 #pragma unroll
-                    for (int y = 0; y < 32; ++y) {
-                        const float e = ex2_approx(fmaf(__uint_as_float(s[y]), c, -lse2));
-                        s[y] = __float_as_uint(e * (__uint_as_float(dp[y]) - d));
+                    for (int y = 0; y < 16; ++y) {
+                        const float2 a = both(fma2(two(s[2 * y], s[2 * y + 1]), c2, less2));
+                        f[y] = mul2(two(ex2_approx(a.x), ex2_approx(a.y)), add2(two(dp[2 * y], dp[2 * y + 1]), lessd));
                     }
                     if (!(j0 + 31 <= pw && (j0 > pw + 31 - p.window || j0 + 32 <= p.sinks))) {
                         const uint32_t seen = bits_between(pos - p.window + 1 - j0, pos + 1 - j0, 0) | bits_between(0, min(p.sinks, pos + 1) - j0, 0);
 #pragma unroll
-                        for (int y = 0; y < 32; ++y)
-                            if (!(seen >> y & 1u)) s[y] = 0;
+                        for (int y = 0; y < 16; ++y) {
+                            const float2 a = both(f[y]);
+                            f[y] = two(seen >> 2 * y & 1u ? a.x : 0.0f, seen >> 2 * y & 2u ? a.y : 0.0f);
+                        }
                     }
 #pragma unroll
-                    for (int y = 0; y < 32; ++y) sum += __uint_as_float(s[y]);
-#pragma unroll
-                    for (int y = 0; y < 16; ++y) s[y] = pack_bf16(__uint_as_float(s[2 * y]), __uint_as_float(s[2 * y + 1]));
+                    for (int y = 0; y < 16; ++y) {
+                        sum = add2(sum, f[y]);
+                        s[y] = pack_bf16(both(f[y]).x, both(f[y]).y);
+                    }
                 }
                 tmem_st_32x16(ts, s);
             }
         });
         // A row of dS adds up to nothing but for what the rounding of `out` has put into D: dK's kernel gets D without it.
-        roles.ctl->sums[w][row] = sum;
+        roles.ctl->sums[w][row] = both(sum).x + both(sum).y;
         named_barrier_sync(1, roles.kSoftmax);
         if (w == 0 && i < p.tq) {
             float more = d;
@@ -814,21 +847,23 @@ attention_dkdv_kernel(const __grid_constant__ AttentionMaps maps, const __grid_c
         const int w = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane, j = j0 + row;
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
         const float c = p.scale * kLog2e;
-        float2* const stats = roles.ctl->stats[warp];
+        float4* const stats = roles.ctl->stats[warp];
+        const uint64_t c2 = two(c, c);
         const int jw = j0 + quarter * 32;   // the warp's first key
         const bool ok = roles.tiles(w, [&](int it) {
             const int i0 = query_of(it);
             const int64_t at = (static_cast<int64_t>(b) * p.heads + head_of(it)) * p.tq + i0;
-            float2 mine[2];
+            // lane l has queries 2 l and 2 l + 1; P = 0 for a query that is not there or sees nothing
+            float lse[2], d[2];
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {   // P = 0 for a query that is not there or sees nothing
-                const bool there = i0 + x * 32 + lane < p.tq;
-                const float lse = there ? p.lse[at + x * 32 + lane] : -INFINITY;
-                mine[x] = make_float2(lse == -INFINITY ? INFINITY : lse * kLog2e, there ? p.dvec[at + x * 32 + lane] : 0.0f);
+            for (int x = 0; x < 2; ++x) {
+                const bool there = i0 + 2 * lane + x < p.tq;
+                lse[x] = there ? p.lse[at + 2 * lane + x] : -INFINITY;
+                d[x] = there ? p.dvec[at + 2 * lane + x] : 0.0f;
+                lse[x] = lse[x] == -INFINITY ? INFINITY : lse[x] * kLog2e;
             }
             __syncwarp();
-            stats[lane] = mine[0];
-            stats[32 + lane] = mine[1];
+            stats[lane] = make_float4(-lse[0], -lse[1], -d[0], -d[1]);
             __syncwarp();
         }, [&](int it) {
 #pragma unroll
@@ -844,22 +879,30 @@ attention_dkdv_kernel(const __grid_constant__ AttentionMaps maps, const __grid_c
                     tmem_ld_32x32(ts + kCols, dp);
                     tmem_ld_wait();
                     const bool some = !(p0 >= jw + 31 && (p0 + 31 - p.window < jw || jw + 32 <= p.sinks));
-                    uint32_t seen = 0xFFFFFFFFu;
-                    if (some) {
-                        const int from = j - p0;
-                        seen = bits_between(from, j < p.sinks || from > 32 - p.window ? 32 : from + p.window, 0);
-                    }
+                    if (!some) {
 #pragma unroll
-                    for (int y = 0; y < 32; y += 2) {
-                        const float4 st = *reinterpret_cast<const float4*>(&stats[x * 32 + y]);
-                        float e0 = ex2_approx(fmaf(__uint_as_float(s[y]), c, -st.x)), e1 = ex2_approx(fmaf(__uint_as_float(s[y + 1]), c, -st.z));
-                        float f0 = e0 * (__uint_as_float(dp[y]) - st.y), f1 = e1 * (__uint_as_float(dp[y + 1]) - st.w);
-                        if (some) {
-                            if (!(seen >> y & 1u)) e0 = f0 = 0.0f;
-                            if (!(seen >> y & 2u)) e1 = f1 = 0.0f;
+                        for (int y = 0; y < 16; ++y) {
+                            const ulonglong2 st = *reinterpret_cast<const ulonglong2*>(&stats[x * 16 + y]);
+                            const float2 a = both(fma2(two(s[2 * y], s[2 * y + 1]), c2, st.x));
+                            const float e0 = ex2_approx(a.x), e1 = ex2_approx(a.y);
+                            const float2 f = both(mul2(two(e0, e1), add2(two(dp[2 * y], dp[2 * y + 1]), st.y)));
+                            s[y] = pack_bf16(e0, e1);
+                            dp[y] = pack_bf16(f.x, f.y);
                         }
-                        s[y / 2] = pack_bf16(e0, e1);
-                        dp[y / 2] = pack_bf16(f0, f1);
+                    } else {
+                        const int from = j - p0;
+                        const uint32_t seen = bits_between(from, j < p.sinks || from > 32 - p.window ? 32 : from + p.window, 0);
+#pragma unroll
+                        for (int y = 0; y < 16; ++y) {
+                            const ulonglong2 st = *reinterpret_cast<const ulonglong2*>(&stats[x * 16 + y]);
+                            const float2 a = both(fma2(two(s[2 * y], s[2 * y + 1]), c2, st.x));
+                            float e0 = ex2_approx(a.x), e1 = ex2_approx(a.y);
+                            float2 f = both(mul2(two(e0, e1), add2(two(dp[2 * y], dp[2 * y + 1]), st.y)));
+                            if (!(seen >> 2 * y & 1u)) e0 = f.x = 0.0f;
+                            if (!(seen >> 2 * y & 2u)) e1 = f.y = 0.0f;
+                            s[y] = pack_bf16(e0, e1);
+                            dp[y] = pack_bf16(f.x, f.y);
+                        }
                     }
                 }
                 tmem_st_32x16(ts, s);
