@@ -6,6 +6,8 @@
 // same factor in l takes out again, and bf16 keeps its relative precision.
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "attention_rows.cuh"
 #include "common.h"
 #include "ptx_sm100.cuh"
@@ -16,8 +18,9 @@ namespace {
 
 using namespace ptx;
 
-constexpr int kRows = 128;                      // queries of a softmax warpgroup, keys of a tile
+constexpr int kRows = 128, kCols = 64;          // of a tile of scores (forward: 128 columns)
 constexpr uint32_t kHalfTile = kRows * 128;     // 128 rows of 64 bf16 values, 128-byte swizzle
+constexpr uint32_t kHalfCols = kCols * 128;     // 64 of them
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct alignas(64) AttentionMaps {
@@ -90,56 +93,110 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
     return r;
 }
 
-// What a block of queries [r0, r0 + 128) of one head sees, in tiles of keys.
+// The larger of three.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// What a block of queries [r0, r0 + 128) of one head sees, in tiles of 128 keys.
 struct QueryBlock {
     int head, r0;
-    int p0, p1;                // positions of the first and the last query
     int low, high, sinks;      // tiles [0, sinks) and [low, high]
     bool any;
     __device__ __forceinline__ QueryBlock(const AttentionParams& p, int head_, int r0_) {
         head = head_;
         r0 = r0_;
-        p0 = r0 + p.tk - p.tq;
-        p1 = min(r0 + kRows, p.tq) - 1 + p.tk - p.tq;
+        const int p0 = r0 + p.tk - p.tq, p1 = min(r0 + kRows, p.tq) - 1 + p.tk - p.tq;   // positions of the first and the last
         any = r0 < p.tq && p1 >= 0;
         const int first = max(0, p0 - p.window + 1);
         low = first / kRows;
         high = p1 / kRows;
         sinks = min((min(p.sinks, first) + kRows - 1) / kRows, low);
     }
+    __device__ __forceinline__ int tiles() const { return any ? sinks + high - low + 1 : 0; }
     __device__ __forceinline__ bool sees(int tile) const { return any && tile <= high && (tile >= low || tile < sinks); }
-    // Every query sees every key of [j0, j0 + n).
-    __device__ __forceinline__ bool sees_all(const AttentionParams& p, int j0, int n) const {
-        return j0 + n - 1 <= p0 && (j0 > p1 - p.window || j0 + n <= p.sinks);
-    }
 };
+
+// What the 32 queries from position p0 on see of the 32 keys from j0 on: nothing, everything, or a part.
+__device__ __forceinline__ bool sees_none(const AttentionParams& p, int p0, int j0) {
+    return j0 > p0 + 31 || (j0 + 31 <= p0 - p.window && j0 >= p.sinks);
+}
+__device__ __forceinline__ bool sees_all(const AttentionParams& p, int p0, int j0) {
+    return j0 + 31 <= p0 && (j0 > p0 + 31 - p.window || j0 + 32 <= p.sinks);
+}
+// The keys of [j0, j0 + 32) that the query at position pos sees.
+__device__ __forceinline__ uint32_t seen_keys(const AttentionParams& p, int pos, int j0) {
+    return bits_between(pos - p.window + 1 - j0, pos + 1 - j0, 0) | bits_between(0, min(p.sinks, pos + 1) - j0, 0);
+}
+
+// 16 fp32 values of a row as bf16 into a 128-row swizzled tile: columns 16 x .. of the row.
+__device__ __forceinline__ void put_row16(uint8_t* tile, int row, int x, const uint32_t* o) {
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+        uint4 v;
+        v.x = pack_bf16(__uint_as_float(o[8 * y]), __uint_as_float(o[8 * y + 1]));
+        v.y = pack_bf16(__uint_as_float(o[8 * y + 2]), __uint_as_float(o[8 * y + 3]));
+        v.z = pack_bf16(__uint_as_float(o[8 * y + 4]), __uint_as_float(o[8 * y + 5]));
+        v.w = pack_bf16(__uint_as_float(o[8 * y + 6]), __uint_as_float(o[8 * y + 7]));
+        *reinterpret_cast<uint4*>(tile + (x >> 2) * kHalfTile + row * 128 + ((((x & 3) * 2 + y) ^ (row & 7)) * 16)) = v;
+    }
+}
+
+// The end of a copy-out by `threads` threads that meet at barrier `id`: `mine` rows of this warp's 32 hold values that are
+// not finite.  store() issues the copies (by the thread that `first` names); the rows are formed again by again(row in the
+// quarter) once the copies are complete, by the warps that `mend` names.
+template <typename Store, typename Again>
+__device__ __forceinline__ void copy_out(uint32_t* bad, int id, int threads, bool first, int quarter, bool mend, uint32_t mine, Store store, Again again) {
+    if ((threadIdx.x & 31) == 0 && mine != 0) atomicOr(&bad[quarter], mine);
+    fence_proxy_async_smem();
+    named_barrier_sync(id, threads);
+    const bool any = (bad[0] | bad[1] | bad[2] | bad[3]) != 0;
+    if (first) {
+        store();
+        bulk_commit_group();
+        if (any) bulk_wait_group0();
+        else bulk_wait_group_read0();   // the tiles are given back, the copies end by themselves
+    }
+    if (!any) return;
+    named_barrier_sync(id, threads);
+    for (uint32_t m = mend ? bad[quarter] : 0; m != 0; m &= m - 1) again(__ffs(m) - 1);
+}
 
 // ------------------------------------------------------------------------------------------------------------ forward
 
-// A block of threads does two query blocks, each with a warpgroup of its own (a query per thread), against the same keys:
-// two heads that share a key head, or two neighbouring blocks of one head.  While one warpgroup takes its exponentials the
-// tensor core works for the other.
-constexpr int kFwdThreads = 320;   // two warpgroups, a TMA warp, an MMA warp
-constexpr int kFwdSlots = 4;       // tiles of K and V in flight
-
-struct FwdControl {
-    uint64_t q_full[2], full[kFwdSlots], empty[kFwdSlots], s_full[2], p_ready[2], o_full[2];
+// A warpgroup has a query block, a query per thread, and a tile of 128 keys at a time: with 64 the products of scores are
+// bound by their reads of Q from shared memory (8192 tokens, window 2048, head_dim 128: 158 us against 133).
+// head_dim <= 64: a block of threads has one warpgroup and 256 columns of tensor memory, and two blocks share an SM, so that
+// one works while the other begins or ends.  The probabilities have a place beside the scores: as soon as a warpgroup has
+// taken its scores out, the tensor core makes the next.
+// head_dim <= 128: two warpgroups against the same keys: two heads that share a key head, or two neighbouring query blocks of
+// one head.  Scores and outputs fill tensor memory, the probabilities take their scores' place, and while one warpgroup takes
+// its exponentials the tensor core works for the other.
+template <int WGS> struct FwdControl {
+    static constexpr int kSlots = 4;   // tiles of K and V in flight
+    uint64_t q_full[WGS], full[kSlots], empty[kSlots], s_full[WGS], s_taken[WGS], p_ready[WGS], o_done[WGS], o_full[WGS];
     uint32_t tmem;
     int abort;
+    uint32_t bad[WGS][4];
 };
 
-template <int HALVES> constexpr size_t fwd_smem() { return 2048 + static_cast<size_t>(2 + kFwdSlots) * HALVES * kHalfTile; }
+template <int HALVES, int WGS> constexpr size_t fwd_smem() { return 2048 + static_cast<size_t>(WGS + FwdControl<WGS>::kSlots) * HALVES * kHalfTile; }
 
-template <int HALVES>
-__global__ void __launch_bounds__(kFwdThreads, 1)
+template <int HALVES, int WGS>
+__global__ void __launch_bounds__(128 * WGS + 64, 3 - WGS)
 attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_constant__ AttentionParams p, int pair_heads, int blocks_q, DeviceStatus* status,
                      uint64_t wait_ns) {
+    using Control = FwdControl<WGS>;
+    constexpr int kSlots = Control::kSlots, kLoadWarp = 4 * WGS, kProductWarp = 4 * WGS + 1, kHd = 64 * HALVES;
+    constexpr bool kApart = HALVES == 1;   // the probabilities have a place of their own
+    constexpr uint32_t kTile = HALVES * kHalfTile, kScores = kRows + (kApart ? kRows / 2 : 0), kTmem = WGS * (kScores + kHd);
+    static_assert(kTmem == 256 || kTmem == 512, "allocations are powers of two");
     extern __shared__ uint8_t raw[];
     uint8_t* const base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    FwdControl* const ctl = reinterpret_cast<FwdControl*>(base);
+    Control* const ctl = reinterpret_cast<Control*>(base);
     const uint32_t tiles = smem_u32(base + 1024);
-    constexpr uint32_t kTile = HALVES * kHalfTile;
-    constexpr int kHd = 64 * HALVES;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int* const abort_flag = &ctl->abort;
 
@@ -147,8 +204,9 @@ attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_co
     const int units = p.batch * p.heads / (pair_heads ? 2 : 1);
     const int unit = blockIdx.x % units, tile_q = blocks_q - 1 - static_cast<int>(blockIdx.x / units);
     const int per_batch = units / p.batch, b = unit / per_batch, h0 = unit % per_batch * (pair_heads ? 2 : 1);
-    const QueryBlock blk0(p, h0, tile_q * (pair_heads ? kRows : 2 * kRows));
-    const QueryBlock blk1(p, pair_heads ? h0 + 1 : h0, pair_heads ? blk0.r0 : blk0.r0 + kRows);
+    const QueryBlock blk0(p, h0, tile_q * (pair_heads ? kRows : WGS * kRows));
+    const QueryBlock blk1(p, pair_heads ? h0 + 1 : h0, WGS == 1 ? p.tq : pair_heads ? blk0.r0 : blk0.r0 + kRows);
+    auto block = [&](int w) -> const QueryBlock& { return WGS == 1 || w == 0 ? blk0 : blk1; };
     const int head_k = h0 / p.group;
     // the tiles that either sees: sinks, then a range
     const int low = blk0.any ? blk0.low : blk1.low;
@@ -158,208 +216,240 @@ attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_co
     auto tile_of = [&](int it) { return it < sink_tiles ? it : low + it - sink_tiles; };
 
     if (threadIdx.x == 0) {
-        for (int w = 0; w < 2; ++w) {
+        for (int w = 0; w < WGS; ++w) {
             mbar_init(smem_u32(&ctl->q_full[w]), 1);
-            mbar_init(smem_u32(&ctl->s_full[w]), 1);
-            mbar_init(smem_u32(&ctl->p_ready[w]), 4);
+            mbar_init(smem_u32(&ctl->o_done[w]), 1);
             mbar_init(smem_u32(&ctl->o_full[w]), 1);
+            mbar_init(smem_u32(&ctl->s_full[w]), 1);
+            mbar_init(smem_u32(&ctl->s_taken[w]), 4);
+            mbar_init(smem_u32(&ctl->p_ready[w]), 4);
+            for (uint32_t& x : ctl->bad[w]) x = 0;
         }
-        for (int s = 0; s < kFwdSlots; ++s) {
+        for (int s = 0; s < kSlots; ++s) {
             mbar_init(smem_u32(&ctl->full[s]), 1);
             mbar_init(smem_u32(&ctl->empty[s]), 1);
         }
         ctl->abort = 0;
         fence_barrier_init();
     }
-    if (warp == 9) {
-        tmem_alloc(smem_u32(&ctl->tmem), 512);
+    if (warp == kProductWarp) {
+        tmem_alloc(smem_u32(&ctl->tmem), kTmem);
         tmem_relinquish_alloc_permit();
     }
-    if (warp == 8 && lane < 4) prefetch_tensormap(lane == 0 ? &maps.q : lane == 1 ? &maps.k : lane == 2 ? &maps.v : &maps.out);
+    if (warp == kLoadWarp && lane < 4) prefetch_tensormap(lane == 0 ? &maps.q : lane == 1 ? &maps.k : lane == 2 ? &maps.v : &maps.out);
     tc_fence_before_thread_sync();
     __syncthreads();
     tc_fence_after_thread_sync();
     const uint32_t tmem = uniform(ctl->tmem);
     grid_dependency_wait();
 
-    const uint32_t q_at = tiles, ring = tiles + 2 * kTile;
-    // TMEM: scores (and in their place the probabilities) of either block, then the outputs
-    auto tmem_s = [&](int w) { return tmem + static_cast<uint32_t>(w) * kRows; };
-    auto tmem_o = [&](int w) { return tmem + 2u * kRows + static_cast<uint32_t>(w) * kHd; };
+    const uint32_t q_at = tiles, ring = tiles + WGS * kTile;
+    // TMEM of a block: scores (in their place or behind them the probabilities), then the output
+    auto tmem_s = [&](int w) { return tmem + static_cast<uint32_t>(w) * kScores; };
+    auto tmem_p = [&](int w) { return tmem_s(w) + (kApart ? kRows : 0); };
+    auto tmem_o = [&](int w) { return tmem + WGS * kScores + static_cast<uint32_t>(w) * kHd; };
     const int steps_d = (p.head_dim + 15) / 16;   // 16-deep steps of S, and 16-wide columns of O
 
-    if (warp == 8) {
+    // Round `it` takes K(it + 1) and V(it): the ring holds K(0), then K(1), V(0), K(2), V(1), ...
+    if (warp == kLoadWarp) {
         // ---------------------------------------------------------------- loads
-        const bool lead = elect_one();
-        if (lead) {
-            for (int w = 0; w < 2; ++w) {
-                const QueryBlock& blk = w == 0 ? blk0 : blk1;
-                if (!blk.any) continue;
+        if (elect_one()) {
+            for (int w = 0; w < WGS; ++w) {
+                if (!block(w).any) continue;
                 mbar_arrive_expect_tx(smem_u32(&ctl->q_full[w]), kTile);
                 for (int x = 0; x < HALVES; ++x)
-                    tma_load_4d(q_at + w * kTile + x * kHalfTile, &maps.q, smem_u32(&ctl->q_full[w]), x * 64, blk.r0, blk.head, b);
+                    tma_load_4d(q_at + w * kTile + x * kHalfTile, &maps.q, smem_u32(&ctl->q_full[w]), x * 64, block(w).r0, block(w).head, b);
             }
         }
         __syncwarp();
         int slot = 0;
         uint32_t phase = 0;
-        for (int i = 0; i < 2 * n_tiles; ++i) {
-            if (!bounded_wait_warp(smem_u32(&ctl->empty[slot]), phase ^ 1u, abort_flag, status, kDevWaitSmemEmpty, slot, wait_ns)) break;
+        bool ok = true;
+        auto load = [&](const CUtensorMap* map, int tile) {
+            ok = bounded_wait_warp(smem_u32(&ctl->empty[slot]), phase ^ 1u, abort_flag, status, kDevWaitSmemEmpty, slot, wait_ns);
+            if (!ok) return;
             if (elect_one()) {
                 const uint32_t bar = smem_u32(&ctl->full[slot]), at = ring + slot * kTile;
                 mbar_arrive_expect_tx(bar, kTile);
-                for (int x = 0; x < HALVES; ++x)
-                    tma_load_4d(at + x * kHalfTile, i & 1 ? &maps.v : &maps.k, bar, x * 64, tile_of(i >> 1) * kRows, head_k, b);
+                for (int x = 0; x < HALVES; ++x) tma_load_4d(at + x * kHalfTile, map, bar, x * 64, tile * kRows, head_k, b);
             }
             __syncwarp();
-            if (++slot == kFwdSlots) { slot = 0; phase ^= 1u; }
+            if (++slot == kSlots) { slot = 0; phase ^= 1u; }
+        };
+        for (int it = -1; it < n_tiles && ok; ++it) {
+            if (it + 1 < n_tiles) load(&maps.k, tile_of(it + 1));
+            if (ok && it >= 0) load(&maps.v, tile_of(it));
         }
-    } else if (warp == 9) {
+    } else if (warp == kProductWarp) {
         // ---------------------------------------------------------------- products
         const uint32_t idesc_s = make_idesc_bf16(kRows, kRows, 0, 0), idesc_o = make_idesc_bf16(kRows, steps_d * 16, 0, 1);
         const uint32_t q_lo = uniform(desc_lo(q_at, 16)), ring_k = uniform(desc_lo(ring, 16)), ring_v = uniform(desc_lo(ring, kHalfTile));
         int slot = 0;
-        uint32_t phase = 0, p_phase[2] = {0, 0};
-        int last[2] = {-1, -1};
-        for (int it = 0; it < n_tiles; ++it) {
-            if (blk0.sees(tile_of(it))) last[0] = it;
-            if (blk1.sees(tile_of(it))) last[1] = it;
-        }
-        bool begun[2] = {false, false}, ok = true;
-        for (int w = 0; w < 2 && ok; ++w)
-            if ((w == 0 ? blk0 : blk1).any) ok = bounded_wait_warp(smem_u32(&ctl->q_full[w]), 0, abort_flag, status, kDevWaitSmemFull, 100 + w, wait_ns);
-        // the ring holds K(0), V(0), K(1), ...; round `it` takes V(it) and K(it + 1)
-        for (int it = -1; it < n_tiles && ok; ++it) {
-            int v_slot = -1, k_slot = -1;
-            if (it >= 0) {
-                v_slot = slot;
-                ok = bounded_wait_warp(smem_u32(&ctl->full[slot]), phase, abort_flag, status, kDevWaitSmemFull, slot, wait_ns);
-                if (++slot == kFwdSlots) { slot = 0; phase ^= 1u; }
+        uint32_t phase = 0;
+        int scores[2] = {0, 0}, values[2] = {0, 0};   // products made for either block
+        bool ok = true;
+        for (int w = 0; w < WGS && ok; ++w)
+            if (block(w).any) ok = bounded_wait_warp(smem_u32(&ctl->q_full[w]), 0, abort_flag, status, kDevWaitSmemFull, 100 + w, wait_ns);
+        auto next = [&]() {
+            const int s = slot;
+            ok = bounded_wait_warp(smem_u32(&ctl->full[slot]), phase, abort_flag, status, kDevWaitSmemFull, slot, wait_ns);
+            if (++slot == kSlots) { slot = 0; phase ^= 1u; }
+            return s;
+        };
+        auto make_scores = [&](int w, int k_slot) {
+            // their place is free: the last ones are taken out (or, as probabilities, the operand of a product made before)
+            if (kApart && scores[w] > 0) {
+                ok = bounded_wait_warp(smem_u32(&ctl->s_taken[w]), static_cast<uint32_t>(scores[w] - 1) & 1u, abort_flag, status, kDevWaitTmemEmpty, 10 + w, wait_ns);
+                if (!ok) return;
             }
-            if (ok && it + 1 < n_tiles) {
-                k_slot = slot;
-                ok = bounded_wait_warp(smem_u32(&ctl->full[slot]), phase, abort_flag, status, kDevWaitSmemFull, slot, wait_ns);
-                if (++slot == kFwdSlots) { slot = 0; phase ^= 1u; }
-            }
-            if (!ok) break;
-            for (int w = 0; w < 2; ++w) {
-                const QueryBlock& blk = w == 0 ? blk0 : blk1;
-                if (it >= 0 && blk.sees(tile_of(it))) {
-                    ok = bounded_wait_warp(smem_u32(&ctl->p_ready[w]), p_phase[w], abort_flag, status, kDevWaitTmemEmpty, w, wait_ns);
-                    if (!ok) break;
-                    p_phase[w] ^= 1u;
-                    tc_fence_after_thread_sync();
-                    if (elect_one()) {
-                        product_ts<kRows / 16>(tmem_o(w), tmem_s(w), ring_v + v_slot * (kTile / 16), idesc_o, begun[w]);
-                        if (it == last[w]) umma_commit(smem_u32(&ctl->o_full[w]));
-                    }
-                    __syncwarp();
-                    begun[w] = true;
-                }
-                if (it + 1 < n_tiles && blk.sees(tile_of(it + 1))) {
-                    tc_fence_after_thread_sync();
-                    if (elect_one()) {
-                        product_ss<HALVES>(tmem_s(w), q_lo + w * (kTile / 16), kHalfTile, ring_k + k_slot * (kTile / 16), kHalfTile, idesc_s, steps_d);
-                        umma_commit(smem_u32(&ctl->s_full[w]));
-                    }
-                    __syncwarp();
-                }
-            }
+            tc_fence_after_thread_sync();
             if (elect_one()) {
-                if (v_slot >= 0) umma_commit(smem_u32(&ctl->empty[v_slot]));
-                if (k_slot >= 0) umma_commit(smem_u32(&ctl->empty[k_slot]));
+                product_ss<HALVES>(tmem_s(w), q_lo + w * (kTile / 16), kHalfTile, ring_k + k_slot * (kTile / 16), kHalfTile, idesc_s, steps_d);
+                umma_commit(smem_u32(&ctl->s_full[w]));
             }
             __syncwarp();
+            ++scores[w];
+        };
+        auto make_values = [&](int w, int v_slot) {
+            ok = bounded_wait_warp(smem_u32(&ctl->p_ready[w]), static_cast<uint32_t>(values[w]) & 1u, abort_flag, status, kDevWaitTmemEmpty, w, wait_ns);
+            if (!ok) return;
+            tc_fence_after_thread_sync();
+            if (elect_one()) {
+                product_ts<kRows / 16>(tmem_o(w), tmem_p(w), ring_v + v_slot * (kTile / 16), idesc_o, values[w] > 0);
+                umma_commit(smem_u32(values[w] + 1 < block(w).tiles() ? &ctl->o_done[w] : &ctl->o_full[w]));
+            }
+            __syncwarp();
+            ++values[w];
+        };
+        for (int it = -1; it < n_tiles && ok; ++it) {
+            int v_slot = -1, k_slot = -1;
+            if (it + 1 < n_tiles) k_slot = next();
+            if (kApart) {   // scores first: their operands are there long before the probabilities
+                if (ok && k_slot >= 0) {
+#pragma unroll
+                    for (int w = 0; w < WGS; ++w)
+                        if (ok && block(w).sees(tile_of(it + 1))) make_scores(w, k_slot);
+                    if (elect_one()) umma_commit(smem_u32(&ctl->empty[k_slot]));
+                    __syncwarp();
+                }
+                if (ok && it >= 0) v_slot = next();
+                if (ok && v_slot >= 0) {
+#pragma unroll
+                    for (int w = 0; w < WGS; ++w)
+                        if (ok && block(w).sees(tile_of(it))) make_values(w, v_slot);
+                    if (elect_one()) umma_commit(smem_u32(&ctl->empty[v_slot]));
+                    __syncwarp();
+                }
+            } else {
+                if (ok && it >= 0) v_slot = next();
+#pragma unroll
+                for (int w = 0; w < WGS; ++w) {
+                    if (ok && v_slot >= 0 && block(w).sees(tile_of(it))) make_values(w, v_slot);
+                    if (ok && k_slot >= 0 && block(w).sees(tile_of(it + 1))) make_scores(w, k_slot);
+                }
+                if (elect_one()) {
+                    if (v_slot >= 0) umma_commit(smem_u32(&ctl->empty[v_slot]));
+                    if (k_slot >= 0) umma_commit(smem_u32(&ctl->empty[k_slot]));
+                }
+                __syncwarp();
+            }
         }
     } else {
         // ---------------------------------------------------------------- softmax: a query per thread
-        const int w = warp >> 2, quarter = warp & 3;
-        const QueryBlock& blk = w == 0 ? blk0 : blk1;
+        const int w = WGS == 1 ? 0 : warp >> 2, quarter = warp & 3;
+        const QueryBlock& blk = block(w);
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-        const uint32_t ts = tmem_s(w) + lanes, to = tmem_o(w) + lanes;
-        const int row = quarter * 32 + lane, i = blk.r0 + row, pos = i + p.tk - p.tq;
+        const uint32_t ts = tmem_s(w) + lanes, tp = tmem_p(w) + lanes, to = tmem_o(w) + lanes;
+        const int row = quarter * 32 + lane, i = blk.r0 + row, pos = i + p.tk - p.tq, pw = blk.r0 + quarter * 32 + p.tk - p.tq;
         const float c = p.scale * kLog2e;
-        float m = -INFINITY, l = 0.0f;
-        uint32_t phase = 0;
-        bool ok = true, begun = false;
+        float m = -INFINITY;
+        uint64_t l2 = 0;
+        int done = 0;   // tiles of this block
+        bool ok = true;
+        // The product of the tile before `done` has written O and read its probabilities; the one before that is known to have, so
+        // the barrier is in one of two phases.
+        auto wait_o = [&]() {
+            ok = bounded_wait_warp(smem_u32(&ctl->o_done[w]), static_cast<uint32_t>(done - 1) & 1u, abort_flag, status, kDevWaitTmemFull, 2 + w, wait_ns);
+            tc_fence_after_thread_sync();
+        };
         for (int it = 0; it < n_tiles && ok; ++it) {
-            const int tile = tile_of(it), j0 = tile * kRows;
-            if (!blk.sees(tile)) continue;
-            ok = bounded_wait_warp(smem_u32(&ctl->s_full[w]), phase, abort_flag, status, kDevWaitTmemFull, w, wait_ns);
+            const int j0 = tile_of(it) * kRows;
+            if (!blk.sees(tile_of(it))) continue;
+            ok = bounded_wait_warp(smem_u32(&ctl->s_full[w]), static_cast<uint32_t>(done) & 1u, abort_flag, status, kDevWaitTmemFull, w, wait_ns);
             if (!ok) break;
-            phase ^= 1u;
             tc_fence_after_thread_sync();
             uint32_t s[kRows];
 #pragma unroll
             for (int x = 0; x < 4; ++x) tmem_ld_32x32(ts + x * 32, s + x * 32);
             tmem_ld_wait();
-            if (!blk.sees_all(p, j0, kRows)) {
-                const int from = pos - p.window + 1 - j0, to_ = pos + 1 - j0, first = min(p.sinks, pos + 1) - j0;
+            if (kApart) {
+                tc_fence_before_thread_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&ctl->s_taken[w]));
+            }
+            if (!(j0 + kRows - 1 <= pw && (j0 > pw + 31 - p.window || j0 + kRows <= p.sinks))) {   // hidden places for one of the warp's queries
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
-                    const uint32_t seen = bits_between(from, to_, x * 32) | bits_between(0, first, x * 32);
+                    const uint32_t seen = seen_keys(p, pos, j0 + x * 32);
 #pragma unroll
                     for (int y = 0; y < 32; ++y)
                         if (!(seen >> y & 1u)) s[x * 32 + y] = 0xFF800000u;   // -inf
                 }
             }
-            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            float top[4] = {m, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int y = 0; y < kRows; ++y) top[y & 3] = fmaxf(top[y & 3], __uint_as_float(s[y]));
-            const float m_new = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), m);
+            for (int y = 0; y < kRows; y += 2) top[y / 2 & 3] = max3(top[y / 2 & 3], __uint_as_float(s[y]), __uint_as_float(s[y + 1]));
+            const float m_new = fmaxf(max3(top[0], top[1], top[2]), top[3]);
             const bool grow = (m_new - m) * c > 8.0f;
+            if (kApart && done > 0) {   // the last tile's probabilities have been read, and O holds its product
+                wait_o();
+                if (!ok) break;
+            }
             if (__any_sync(0xffffffffu, grow)) {
-                // The product that wrote O last is complete: the scores of this tile were made after it.
                 const float shrink = grow ? ex2_approx((m - m_new) * c) : 1.0f;
                 if (grow) m = m_new;
-                l *= shrink;
-                if (begun) {
-                    for (int x = 0; x < steps_d; ++x) {
-                        uint32_t o[16];
-                        tmem_ld_32x16(to + x * 16, o);
-                        tmem_ld_wait();
+                l2 = mul2(l2, two(shrink, shrink));
+                for (int x = 0; x < (done > 0 ? steps_d : 0); ++x) {
+                    uint32_t o[16];
+                    tmem_ld_32x16(to + x * 16, o);
+                    tmem_ld_wait();
 #pragma unroll
-                        for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * shrink);
-                        tmem_st_32x16(to + x * 16, o);
-                    }
+                    for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * shrink);
+                    tmem_st_32x16(to + x * 16, o);
                 }
             }
-            begun = true;
             const float off = m == -INFINITY ? 0.0f : -m * c;
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            uint64_t sum[2] = {0, 0};
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                uint32_t e[32];
 #pragma unroll
                 for (int y = 0; y < 32; ++y) {
-                    const float a = ex2_approx(fmaf(__uint_as_float(s[x * 64 + 2 * y]), c, off));
-                    const float d = ex2_approx(fmaf(__uint_as_float(s[x * 64 + 2 * y + 1]), c, off));
-                    sum[(2 * y) & 3] += a;
-                    sum[(2 * y + 1) & 3] += d;
-                    e[y] = pack_bf16(a, d);
+                    const float2 a = make_float2(fmaf(__uint_as_float(s[x * 64 + 2 * y]), c, off), fmaf(__uint_as_float(s[x * 64 + 2 * y + 1]), c, off));
+                    const float e0 = ex2_approx(a.x), e1 = ex2_approx(a.y);
+                    sum[y & 1] = add2(sum[y & 1], two(e0, e1));
+                    s[x * 64 + y] = pack_bf16(e0, e1);
                 }
-                tmem_st_32x32(ts + x * 32, e);
+                tmem_st_32x32(tp + x * 32, s + x * 64);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            l2 = add2(l2, add2(sum[0], sum[1]));
             tmem_st_wait();
             tc_fence_before_thread_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&ctl->p_ready[w]));
+            ++done;
         }
         // ---------------------------------------------------------------- out, through the block's place in the Q tiles
-        if (ok && begun) {
-            ok = bounded_wait_warp(smem_u32(&ctl->o_full[w]), 0, abort_flag, status, kDevWaitTmemFull, 2 + w, wait_ns);
-            tc_fence_after_thread_sync();
-        }
-        bool bad = false;
+        if (ok && done > 0) ok = bounded_wait_warp(smem_u32(&ctl->o_full[w]), 0, abort_flag, status, kDevWaitTmemFull, 4 + w, wait_ns);
+        tc_fence_after_thread_sync();
         if (blk.r0 < p.tq) {
-            uint8_t* const mine = base + 1024 + w * kTile + row * 128;
-            const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;   // l NaN: so is the row
+            const float l = both(l2).x + both(l2).y;
+            const float inv = l > 0.0f ? 1.0f / l : l;   // l NaN: so is the row
+            bool bad = false;
             for (int x = 0; x < 4 * HALVES; ++x) {
                 uint32_t o[16];
 #pragma unroll
                 for (int y = 0; y < 16; ++y) o[y] = 0;
-                if (ok && begun && x < steps_d) {
+                if (ok && done > 0 && x < steps_d) {
                     tmem_ld_32x16(to + x * 16, o);
                     tmem_ld_wait();
                 }
@@ -369,45 +459,27 @@ attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_co
                     bad = bad || !(fabsf(f) < INFINITY);
                     o[y] = __float_as_uint(f);
                 }
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    uint4 v;
-                    v.x = pack_bf16(__uint_as_float(o[8 * y]), __uint_as_float(o[8 * y + 1]));
-                    v.y = pack_bf16(__uint_as_float(o[8 * y + 2]), __uint_as_float(o[8 * y + 3]));
-                    v.z = pack_bf16(__uint_as_float(o[8 * y + 4]), __uint_as_float(o[8 * y + 5]));
-                    v.w = pack_bf16(__uint_as_float(o[8 * y + 6]), __uint_as_float(o[8 * y + 7]));
-                    const int chunk = ((x & 3) * 2 + y) ^ (row & 7);
-                    *reinterpret_cast<uint4*>(mine + (x >> 2) * kHalfTile + chunk * 16) = v;
-                }
+                put_row16(base + 1024 + w * kTile, row, x, o);
             }
             if (i < p.tq && p.lse != nullptr)
                 p.lse[(static_cast<int64_t>(b) * p.heads + blk.head) * p.tq + i] = l == 0.0f ? -INFINITY : fmaf(m, p.scale, log2f(l) * (1.0f / kLog2e));
-            fence_proxy_async_smem();
-            named_barrier_sync(1 + w, 128);
-            if (row == 0) {
-                for (int x = 0; x < HALVES; ++x) tma_store_4d(&maps.out, q_at + w * kTile + x * kHalfTile, x * 64, blk.r0, blk.head, b);
-                bulk_commit_group();
-                bulk_wait_group0();
-            }
-            named_barrier_sync(1 + w, 128);
             // A product with a hidden value that is not finite (0 * inf) has spoilt the row, or it sees such a value: it is
             // formed again from the keys it sees.
-            uint32_t again = __ballot_sync(0xffffffffu, bad && ok && i < p.tq);
-            while (again != 0) {
-                const int r = __ffs(again) - 1;
-                again &= again - 1;
+            copy_out(ctl->bad[w], 1 + w, 128, row == 0, quarter, true, __ballot_sync(0xffffffffu, bad && ok && i < p.tq), [&] {
+                for (int x = 0; x < HALVES; ++x) tma_store_4d(&maps.out, q_at + w * kTile + x * kHalfTile, x * 64, blk.r0, blk.head, b);
+            }, [&](int r) {
                 const int64_t at = blk.r0 + quarter * 32 + r;
                 attn::forward_row(p, b, blk.head, at, at + p.tk - p.tq);
-            }
+            });
         }
     }
     // -------------------------------------------------------------------- teardown
     if (*abort_flag) __nanosleep(200000);   // copies in flight land before the shared memory is given back
     tc_fence_before_thread_sync();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == kProductWarp) {
         tc_fence_after_thread_sync();
-        tmem_dealloc(tmem, 512);
+        tmem_dealloc(tmem, kTmem);
     }
 }
 
@@ -444,8 +516,6 @@ struct DkdvPlan {
 // tensor memory has places for scores: two or three.  A warpgroup's turn is a chain of 900 cycles of its own work and 900 of
 // waiting for its products; with two of them both the tensor core and the exponentials stood still for a third of the time
 // (two warpgroups on the halves of one tile, three places: no better, they want the special-function unit at the same time).
-constexpr int kCols = 64;
-constexpr uint32_t kHalfCols = kCols * 128;    // 64 rows of 64 bf16 values
 constexpr int kBwdSlots = 4;
 
 constexpr int kMaxBuffers = 3;
@@ -564,23 +634,6 @@ template <int BUFFERS> struct BwdRoles {
         tc_fence_after_thread_sync();
         return ok;
     }
-    // The end of a block's copy-out, for all softmax threads: `mine` rows of this warp's 32 hold values that are not finite.
-    // store() issues the copies; the rows are formed again by again(row in the quarter) once the copies are complete.
-    template <typename Store, typename Again> __device__ __forceinline__ void copy_out(int w, int quarter, uint32_t mine, Store store, Again again) const {
-        if ((threadIdx.x & 31) == 0 && mine != 0) atomicOr(&ctl->bad[quarter], mine);
-        fence_proxy_async_smem();
-        named_barrier_sync(1, kSoftmax);
-        const bool any = (ctl->bad[0] | ctl->bad[1] | ctl->bad[2] | ctl->bad[3]) != 0;
-        if (threadIdx.x == 0) {
-            store();
-            bulk_commit_group();
-            if (any) bulk_wait_group0();
-            else bulk_wait_group_read0();   // the tiles are given back, the copies end by themselves
-        }
-        if (!any) return;
-        named_barrier_sync(1, kSoftmax);
-        for (uint32_t m = w == 0 ? ctl->bad[quarter] : 0; m != 0; m &= m - 1) again(__ffs(m) - 1);
-    }
     __device__ __forceinline__ void tear_down(int warp, uint32_t tmem) {
         if (*abort_flag) __nanosleep(200000);
         tc_fence_before_thread_sync();
@@ -591,19 +644,6 @@ template <int BUFFERS> struct BwdRoles {
         }
     }
 };
-
-// 16 fp32 values of a row as bf16 into a 128-row swizzled tile: columns 16 x .. of the row.
-__device__ __forceinline__ void put_row16(uint8_t* tile, int row, int x, const uint32_t* o) {
-#pragma unroll
-    for (int y = 0; y < 2; ++y) {
-        uint4 v;
-        v.x = pack_bf16(__uint_as_float(o[8 * y]), __uint_as_float(o[8 * y + 1]));
-        v.y = pack_bf16(__uint_as_float(o[8 * y + 2]), __uint_as_float(o[8 * y + 3]));
-        v.z = pack_bf16(__uint_as_float(o[8 * y + 4]), __uint_as_float(o[8 * y + 5]));
-        v.w = pack_bf16(__uint_as_float(o[8 * y + 6]), __uint_as_float(o[8 * y + 7]));
-        *reinterpret_cast<uint4*>(tile + (x >> 2) * kHalfTile + row * 128 + ((((x & 3) * 2 + y) ^ (row & 7)) * 16)) = v;
-    }
-}
 
 // D of 128 queries into shared memory by the first eight warps, 16 queries each: 8 HALVES lanes for a row, a row's 16 bytes
 // each, so that the loads of all of a warp's rows are in flight at once (a thread a row took 6000 to 12000 cycles).
@@ -711,7 +751,7 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
                 const uint32_t ts = tmem + w * 2 * kCols + x * 32 + lanes;
                 const int j0 = tile_of(it) * kCols + x * 32;
                 uint32_t s[32];
-                if (j0 > pw + 31 || (j0 + 31 <= pw - p.window && j0 >= p.sinks)) {   // nothing is seen
+                if (sees_none(p, pw, j0)) {
 #pragma unroll
                     for (int y = 0; y < 16; ++y) s[y] = 0;
                 } else {
@@ -725,8 +765,8 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
                         const float2 a = both(fma2(two(s[2 * y], s[2 * y + 1]), c2, less2));
                         f[y] = mul2(two(ex2_approx(a.x), ex2_approx(a.y)), add2(two(dp[2 * y], dp[2 * y + 1]), lessd));
                     }
-                    if (!(j0 + 31 <= pw && (j0 > pw + 31 - p.window || j0 + 32 <= p.sinks))) {
-                        const uint32_t seen = bits_between(pos - p.window + 1 - j0, pos + 1 - j0, 0) | bits_between(0, min(p.sinks, pos + 1) - j0, 0);
+                    if (!sees_all(p, pw, j0)) {
+                        const uint32_t seen = seen_keys(p, pos, j0);
 #pragma unroll
                         for (int y = 0; y < 16; ++y) {
                             const float2 a = both(f[y]);
@@ -769,7 +809,7 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
             put_row16(tiles_ptr, row, x, o);
         }
         // as in the forward kernel: a hidden key that is not finite has spoilt the row
-        roles.copy_out(w, quarter, __ballot_sync(0xffffffffu, bad && ok && i < p.tq), [&] {
+        copy_out(roles.ctl->bad, 1, roles.kSoftmax, threadIdx.x == 0, quarter, w == 0, __ballot_sync(0xffffffffu, bad && ok && i < p.tq), [&] {
             for (int x = 0; x < HALVES; ++x) tma_store_4d(&maps.dq, tiles + x * kHalfTile, x * 64, r0, h, b);
         }, [&](int r) { attn::dq_row(p, b, h, r0 + quarter * 32 + r, __shfl_sync(0xffffffffu, d, r)); });
     }
@@ -871,15 +911,14 @@ attention_dkdv_kernel(const __grid_constant__ AttentionMaps maps, const __grid_c
                 const uint32_t ts = tmem + w * 2 * kCols + x * 32 + lanes;
                 const int p0 = query_of(it) + x * 32 + off;   // position of the first of them
                 uint32_t s[32], dp[32];
-                if (p0 + 31 < jw || (p0 - p.window >= jw + 31 && jw >= p.sinks)) {   // nothing is seen
+                if (sees_none(p, p0, jw)) {
 #pragma unroll
                     for (int y = 0; y < 16; ++y) s[y] = dp[y] = 0;
                 } else {
                     tmem_ld_32x32(ts, s);
                     tmem_ld_32x32(ts + kCols, dp);
                     tmem_ld_wait();
-                    const bool some = !(p0 >= jw + 31 && (p0 + 31 - p.window < jw || jw + 32 <= p.sinks));
-                    if (!some) {
+                    if (sees_all(p, p0, jw)) {
 #pragma unroll
                         for (int y = 0; y < 16; ++y) {
                             const ulonglong2 st = *reinterpret_cast<const ulonglong2*>(&stats[x * 16 + y]);
@@ -936,7 +975,7 @@ attention_dkdv_kernel(const __grid_constant__ AttentionMaps maps, const __grid_c
             }
         }
         if (parts == 1)
-            roles.copy_out(w, quarter, __ballot_sync(0xffffffffu, bad && ok && j < p.tk), [&] {
+            copy_out(roles.ctl->bad, 1, roles.kSoftmax, threadIdx.x == 0, quarter, w == 0, __ballot_sync(0xffffffffu, bad && ok && j < p.tk), [&] {
                 for (int x = 0; x < HALVES; ++x) {
                     tma_store_4d(&maps.dv, tiles + x * kHalfTile, x * 64, j0, hk, b);
                     tma_store_4d(&maps.dk, tiles + kFixed + x * kHalfTile, x * 64, j0, hk, b);
@@ -1065,11 +1104,14 @@ cudaError_t launch_attention_bwd_sm100(AttentionParams p, const CUtensorMap* m, 
 cudaError_t launch_attention_fwd_sm100(const AttentionParams& p, const CUtensorMap* m, DeviceStatus* status, uint64_t wait_ns, cudaStream_t stream) {
     AttentionMaps maps{};
     maps.q = m[0]; maps.k = m[1]; maps.v = m[2]; maps.out = m[3];
-    const int pair_heads = p.group % 2 == 0;
-    const int per = pair_heads ? kRows : 2 * kRows, blocks_q = (p.tq + per - 1) / per;
-    const int64_t blocks = static_cast<int64_t>(p.batch) * p.heads / (pair_heads ? 2 : 1) * blocks_q;
-    return p.head_dim <= 64 ? launch_sm(attention_fwd_kernel<1>, blocks, kFwdThreads, fwd_smem<1>(), stream, maps, p, pair_heads, blocks_q, status, wait_ns)
-                            : launch_sm(attention_fwd_kernel<2>, blocks, kFwdThreads, fwd_smem<2>(), stream, maps, p, pair_heads, blocks_q, status, wait_ns);
+    const int64_t heads = static_cast<int64_t>(p.batch) * p.heads;
+    if (p.head_dim <= 64) {
+        const int blocks_q = (p.tq + kRows - 1) / kRows;
+        return launch_sm(attention_fwd_kernel<1, 1>, heads * blocks_q, 192, fwd_smem<1, 1>(), stream, maps, p, 0, blocks_q, status, wait_ns);
+    }
+    const int pair_heads = p.group % 2 == 0, per = pair_heads ? kRows : 2 * kRows, blocks_q = (p.tq + per - 1) / per;
+    return launch_sm(attention_fwd_kernel<2, 2>, heads / (pair_heads ? 2 : 1) * blocks_q, 320, fwd_smem<2, 2>(), stream, maps, p, pair_heads, blocks_q, status,
+                     wait_ns);
 }
 
 }  // namespace llmt_b200
