@@ -521,7 +521,7 @@ constexpr int kBwdSlots = 4;
 constexpr int kMaxBuffers = 3;
 
 struct BwdControl {
-    uint64_t fixed, full[kBwdSlots], empty[kBwdSlots], scores[kMaxBuffers], ready[kMaxBuffers], done;
+    uint64_t fixed, full[kBwdSlots], empty[kBwdSlots], scores[kMaxBuffers], ready[kMaxBuffers], taken, done;
     uint32_t tmem;
     int abort;
     uint32_t bad[4];
@@ -536,7 +536,9 @@ template <int HALVES> constexpr size_t bwd_smem() { return 1024 + kBwdControl + 
 // What both kernels have around their loops: barriers, tensor memory, and the pipeline over BUFFERS places for scores, each
 // with a warpgroup of its own (warps 0 .. 4 BUFFERS - 1; then a warp for the loads and one for the products)
 //   scores(0), .., scores(BUFFERS - 1), then for each tile: its second products when its P / dS are there, scores BUFFERS on.
-template <int BUFFERS> struct BwdRoles {
+template <int BUFFERS, int TMEM> struct BwdRoles {
+    static constexpr int kTmem = TMEM <= 256 ? 256 : 512;
+    static_assert(TMEM <= 512, "tensor memory has 512 columns");
     static constexpr int kSoftmax = 128 * BUFFERS, kThreads = kSoftmax + 64, kLoadWarp = 4 * BUFFERS, kProductWarp = 4 * BUFFERS + 1;
     BwdControl* ctl;
     volatile int* abort_flag;
@@ -548,6 +550,7 @@ template <int BUFFERS> struct BwdRoles {
         if (threadIdx.x == 0) {
             mbar_init(smem_u32(&ctl->fixed), 1);
             mbar_init(smem_u32(&ctl->done), 1);
+            mbar_init(smem_u32(&ctl->taken), 4);
             for (int w = 0; w < BUFFERS; ++w) {
                 mbar_init(smem_u32(&ctl->scores[w]), 1);
                 mbar_init(smem_u32(&ctl->ready[w]), 4);
@@ -561,7 +564,7 @@ template <int BUFFERS> struct BwdRoles {
             fence_barrier_init();
         }
         if (warp == kProductWarp) {
-            tmem_alloc(smem_u32(&ctl->tmem), 512);
+            tmem_alloc(smem_u32(&ctl->tmem), kTmem);
             tmem_relinquish_alloc_permit();
         }
         tc_fence_before_thread_sync();
@@ -582,27 +585,32 @@ template <int BUFFERS> struct BwdRoles {
             if (++slot == kBwdSlots) { slot = 0; phase ^= 1u; }
         }
     }
-    // first(slot, buffer), second(slot, buffer, accumulate): the products, issued by one lane.
-    template <typename First, typename Second> __device__ __forceinline__ void products(First first, Second second) const {
+    // first(slot, buffer), second(slot, buffer, accumulate): the products, issued by one lane.  EARLY (one buffer): dS has a
+    // place of its own, and the next scores are made as soon as the warpgroup has taken the last ones out.
+    template <bool EARLY, typename First, typename Second> __device__ __forceinline__ void products(First first, Second second) const {
+        static_assert(!EARLY || BUFFERS == 1, "one place for scores");
         bool ok = n == 0 || bounded_wait_warp(smem_u32(&ctl->fixed), 0, abort_flag, status, kDevWaitSmemFull, 100, wait_ns);
         int slot = 0, buffer = 0, slot_2 = 0, buffer_2 = 0;   // of the next first products, and of the next second ones
         uint32_t phase = 0, phase_2 = 0;
-        for (int it = -BUFFERS; it < n && ok; ++it) {
-            if (it >= 0) {
-                ok = bounded_wait_warp(smem_u32(&ctl->ready[buffer_2]), phase_2, abort_flag, status, kDevWaitTmemEmpty, buffer_2, wait_ns);
-                if (!ok) break;
-                tc_fence_after_thread_sync();
-                if (elect_one()) {
-                    second(slot_2, buffer_2, it > 0);
-                    umma_commit(smem_u32(&ctl->empty[slot_2]));
-                    if (it + 1 == n) umma_commit(smem_u32(&ctl->done));
-                }
-                __syncwarp();
-                if (++slot_2 == kBwdSlots) slot_2 = 0;
-                if (++buffer_2 == BUFFERS) { buffer_2 = 0; phase_2 ^= 1u; }
+        auto make_second = [&](int it) {
+            ok = bounded_wait_warp(smem_u32(&ctl->ready[buffer_2]), phase_2, abort_flag, status, kDevWaitTmemEmpty, buffer_2, wait_ns);
+            if (!ok) return;
+            tc_fence_after_thread_sync();
+            if (elect_one()) {
+                second(slot_2, buffer_2, it > 0);
+                umma_commit(smem_u32(&ctl->empty[slot_2]));
+                if (it + 1 == n) umma_commit(smem_u32(&ctl->done));
             }
-            if (it + BUFFERS < n) {
+            __syncwarp();
+            if (++slot_2 == kBwdSlots) slot_2 = 0;
+            if (++buffer_2 == BUFFERS) { buffer_2 = 0; phase_2 ^= 1u; }
+        };
+        for (int it = -BUFFERS; it < n && ok; ++it) {
+            if (!EARLY && it >= 0) make_second(it);
+            if (ok && it + BUFFERS < n) {
                 ok = bounded_wait_warp(smem_u32(&ctl->full[slot]), phase, abort_flag, status, kDevWaitSmemFull, slot, wait_ns);
+                if (ok && EARLY && it >= 0)
+                    ok = bounded_wait_warp(smem_u32(&ctl->taken), static_cast<uint32_t>(it) & 1u, abort_flag, status, kDevWaitTmemEmpty, 50, wait_ns);
                 if (!ok) break;
                 tc_fence_after_thread_sync();
                 if (elect_one()) {
@@ -613,7 +621,19 @@ template <int BUFFERS> struct BwdRoles {
                 if (++slot == kBwdSlots) { slot = 0; phase ^= 1u; }
                 if (++buffer == BUFFERS) buffer = 0;
             }
+            if (EARLY && ok && it >= 0) make_second(it);
         }
+    }
+    // The second products of a tile are complete.
+    __device__ __forceinline__ bool wait_second(int it) const {
+        const bool ok = bounded_wait_warp(smem_u32(&ctl->empty[it % kBwdSlots]), static_cast<uint32_t>(it / kBwdSlots) & 1u, abort_flag, status, kDevWaitTmemFull, 60, wait_ns);
+        tc_fence_after_thread_sync();
+        return ok;
+    }
+    __device__ __forceinline__ void post_taken() const {
+        tc_fence_before_thread_sync();
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&ctl->taken));
     }
     // work(it): what warpgroup `w` does with a tile's scores once they are there; before(it) ahead of the wait.
     template <typename Before, typename Work> __device__ __forceinline__ bool tiles(int w, Before before, Work work) const {
@@ -640,18 +660,18 @@ template <int BUFFERS> struct BwdRoles {
         __syncthreads();
         if (warp == kProductWarp) {
             tc_fence_after_thread_sync();
-            tmem_dealloc(tmem, 512);
+            tmem_dealloc(tmem, kTmem);
         }
     }
 };
 
-// D of 128 queries into shared memory by the first eight warps, 16 queries each: 8 HALVES lanes for a row, a row's 16 bytes
+// D of 128 queries into shared memory by the first WARPS warps: 8 HALVES lanes for a row, a row's 16 bytes
 // each, so that the loads of all of a warp's rows are in flight at once (a thread a row took 6000 to 12000 cycles).
-template <int HALVES>
+template <int HALVES, int WARPS>
 __device__ __forceinline__ void row_products(const AttentionParams& p, int b, int h, int r0, float* d, int warp) {
-    constexpr int kLanes = 8 * HALVES, kAtOnce = 32 / kLanes, kTurns = 16 / kAtOnce;
-    if (warp >= 8) return;
-    const int lane = threadIdx.x & 31, col = lane % kLanes * 8, first = warp * 16 + lane / kLanes;
+    constexpr int kLanes = 8 * HALVES, kAtOnce = 32 / kLanes, kEach = kRows / WARPS, kTurns = kEach / kAtOnce;
+    if (warp >= WARPS) return;
+    const int lane = threadIdx.x & 31, col = lane % kLanes * 8, first = warp * kEach + lane / kLanes;
     uint4 x[kTurns], y[kTurns];
 #pragma unroll
     for (int n = 0; n < kTurns; ++n) {
@@ -675,14 +695,19 @@ __device__ __forceinline__ void row_products(const AttentionParams& p, int b, in
 }
 
 // dQ of 128 queries: S = Q K^T and dP = dO V^T of 64 keys, dS = P (dP - D), dQ += dS K.
-template <int HALVES>
-__global__ void __launch_bounds__(BwdRoles<3>::kThreads, 1)
+// head_dim <= 64: one warpgroup a block and two blocks an SM, so that one works while the other begins or ends; dS has a place
+// of its own, and the next scores are made while the warpgroup works on the last ones.  (BUFFERS = 3 there: 8 x 12 x 1024,
+// window 256: dQ, dK, dV 100 us against 90; 2 x 16 x 4096: 368 against 344.)
+template <int HALVES, int BUFFERS> using DqRoles = BwdRoles<BUFFERS, BUFFERS * 2 * kCols + (BUFFERS == 1 ? kCols / 2 : 0) + 64 * HALVES>;
+template <int HALVES, int BUFFERS>
+__global__ void __launch_bounds__(128 * BUFFERS + 64, BUFFERS == 1 ? 2 : 1)
 attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_constant__ AttentionParams p, int blocks_q, DeviceStatus* status, uint64_t wait_ns) {
     extern __shared__ uint8_t raw[];
     uint8_t* const base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint8_t* const tiles_ptr = base + kBwdControl;
     const uint32_t tiles = smem_u32(tiles_ptr);
-    constexpr int kBuffers = 3;
+    constexpr int kBuffers = BUFFERS;
+    constexpr bool kEarly = BUFFERS == 1;
     constexpr uint32_t kFixed = HALVES * kHalfTile, kStream = HALVES * kHalfCols;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int units = p.batch * p.heads, unit = blockIdx.x % units;
@@ -691,7 +716,7 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
     const int p0 = r0 + p.tk - p.tq, p1 = min(r0 + kRows, p.tq) - 1 + p.tk - p.tq;
     const int first = max(0, p0 - p.window + 1);
     const int low = first / kCols, sink_tiles = min((min(p.sinks, first) + kCols - 1) / kCols, low);
-    BwdRoles<kBuffers> roles{reinterpret_cast<BwdControl*>(base), nullptr, status, wait_ns, p1 >= 0 ? sink_tiles + p1 / kCols - low + 1 : 0};
+    DqRoles<HALVES, BUFFERS> roles{reinterpret_cast<BwdControl*>(base), nullptr, status, wait_ns, p1 >= 0 ? sink_tiles + p1 / kCols - low + 1 : 0};
     roles.abort_flag = &roles.ctl->abort;
     auto tile_of = [&](int it) { return it < sink_tiles ? it : low + it - sink_tiles; };
     roles.set_up(warp);
@@ -699,7 +724,7 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
     grid_dependency_wait();
     const int steps_d = (p.head_dim + 15) / 16;
     const uint32_t ring = tiles + 2 * kFixed;
-    const uint32_t tmem_dq = tmem + kBuffers * 2u * kCols;   // behind the places of S and dP
+    const uint32_t tmem_ds = tmem + 2u * kCols, tmem_dq = tmem + kBuffers * 2u * kCols + (kEarly ? kCols / 2 : 0);   // behind the places of S and dP
 
     if (warp == roles.kLoadWarp) {
         if (roles.n > 0 && elect_one()) {
@@ -720,21 +745,22 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
     } else if (warp == roles.kProductWarp) {
         const uint32_t idesc_s = make_idesc_bf16(kRows, kCols, 0, 0), idesc_d = make_idesc_bf16(kRows, steps_d * 16, 0, 1);
         const uint32_t fixed_lo = uniform(desc_lo(tiles, 16)), ring_lo = uniform(desc_lo(ring, 16)), ring_mn = uniform(desc_lo(ring, kHalfCols));
-        roles.products(
+        roles.template products<kEarly>(
             [&](int slot, int buffer) {
                 const uint32_t at = ring_lo + slot * (2 * kStream / 16), to = tmem + buffer * 2 * kCols;
                 product_ss<HALVES>(to, fixed_lo, kHalfTile, at, kHalfCols, idesc_s, steps_d);
                 product_ss<HALVES>(to + kCols, fixed_lo + kFixed / 16, kHalfTile, at + kStream / 16, kHalfCols, idesc_s, steps_d);
             },
             [&](int slot, int buffer, bool more) {
-                product_ts<kCols / 16, 2>(tmem_dq, tmem + buffer * 2 * kCols, ring_mn + slot * (2 * kStream / 16), idesc_d, more);
+                if (kEarly) product_ts<kCols / 16>(tmem_dq, tmem_ds, ring_mn + slot * (2 * kStream / 16), idesc_d, more);
+                else product_ts<kCols / 16, 2>(tmem_dq, tmem + buffer * 2 * kCols, ring_mn + slot * (2 * kStream / 16), idesc_d, more);
             });
     } else {
         const int w = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane, i = r0 + row, pos = i + p.tk - p.tq;
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
         const float c = p.scale * kLog2e;
         const int64_t at = (static_cast<int64_t>(b) * p.heads + h) * p.tq + i;
-        row_products<HALVES>(p, b, h, r0, roles.ctl->d, warp);
+        row_products<HALVES, BUFFERS == 1 ? 4 : 8>(p, b, h, r0, roles.ctl->d, warp);
         named_barrier_sync(1, roles.kSoftmax);
         const float d = roles.ctl->d[row];
         float lse2 = INFINITY;   // P = 0 for a query that is not there or sees nothing
@@ -750,15 +776,18 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
             for (int x = 0; x < 2; ++x) {   // 32 keys at a time
                 const uint32_t ts = tmem + w * 2 * kCols + x * 32 + lanes;
                 const int j0 = tile_of(it) * kCols + x * 32;
-                uint32_t s[32];
-                if (sees_none(p, pw, j0)) {
-#pragma unroll
-                    for (int y = 0; y < 16; ++y) s[y] = 0;
-                } else {
-                    uint32_t dp[32];
+                const bool none = sees_none(p, pw, j0);
+                uint32_t s[32], dp[32];
+                if (!none) {
                     tmem_ld_32x32(ts, s);
                     tmem_ld_32x32(ts + kCols, dp);
                     tmem_ld_wait();
+                }
+                if (kEarly && x == 1) roles.post_taken();
+                if (none) {
+#pragma unroll
+                    for (int y = 0; y < 16; ++y) s[y] = 0;
+                } else {
                     uint64_t f[16];
 #pragma unroll
                     for (int y = 0; y < 16; ++y) {
@@ -779,7 +808,8 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
                         s[y] = pack_bf16(both(f[y]).x, both(f[y]).y);
                     }
                 }
-                tmem_st_32x16(ts, s);
+                if (kEarly && x == 0 && it > 0) roles.wait_second(it - 1);   // they have read the last dS (a wait that runs out ends the next one too)
+                tmem_st_32x16(kEarly ? tmem_ds + x * 16 + lanes : ts, s);
             }
         });
         // A row of dS adds up to nothing but for what the rounding of `out` has put into D: dK's kernel gets D without it.
@@ -819,8 +849,9 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
 // dK and dV of 128 keys: S^T = K Q^T and dP^T = V dO^T of 64 queries, dV += P^T dO, dK += dS^T Q.  The queries are those of all
 // heads of the group, one head after the other.  A block may do a part of them only: its sums then go to the workspace in
 // fp32, and attention_dkdv_sum_kernel adds the parts in order.
-template <int HALVES>
-__global__ void __launch_bounds__(BwdRoles<HALVES == 1 ? 3 : 2>::kThreads, 1)
+template <int HALVES, int BUFFERS> using DkdvRoles = BwdRoles<BUFFERS, BUFFERS * 2 * kCols + 128 * HALVES>;
+template <int HALVES, int BUFFERS>
+__global__ void __launch_bounds__(128 * BUFFERS + 64, 1)
 attention_dkdv_kernel(const __grid_constant__ AttentionMaps maps, const __grid_constant__ AttentionParams p, const DkdvPlan plan, DeviceStatus* status,
                       uint64_t wait_ns) {
     extern __shared__ uint8_t raw[];
@@ -829,7 +860,7 @@ attention_dkdv_kernel(const __grid_constant__ AttentionMaps maps, const __grid_c
     const uint32_t tiles = smem_u32(tiles_ptr);
     constexpr uint32_t kFixed = HALVES * kHalfTile, kStream = HALVES * kHalfCols;
     constexpr int kHd = 64 * HALVES;
-    constexpr int kBuffers = HALVES == 1 ? 3 : 2;
+    constexpr int kBuffers = BUFFERS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int heads_k = p.heads / p.group, units = p.batch * heads_k, unit = blockIdx.x % units;
     const int b = unit / heads_k, hk = unit % heads_k;
@@ -842,7 +873,7 @@ attention_dkdv_kernel(const __grid_constant__ AttentionMaps maps, const __grid_c
     const int j0 = tile * kRows, off = p.tk - p.tq;
     const QueryTiles q(p, j0);
     const int all = q.count * p.group, it0 = static_cast<int>(static_cast<int64_t>(all) * part / parts);
-    BwdRoles<kBuffers> roles{reinterpret_cast<BwdControl*>(base), nullptr, status, wait_ns, static_cast<int>(static_cast<int64_t>(all) * (part + 1) / parts) - it0};
+    DkdvRoles<HALVES, BUFFERS> roles{reinterpret_cast<BwdControl*>(base), nullptr, status, wait_ns, static_cast<int>(static_cast<int64_t>(all) * (part + 1) / parts) - it0};
     roles.abort_flag = &roles.ctl->abort;
     auto head_of = [&](int it) { return hk * p.group + (it0 + it) / q.count; };
     auto query_of = [&](int it) { return (q.first + (it0 + it) % q.count) * kCols; };
@@ -872,7 +903,7 @@ attention_dkdv_kernel(const __grid_constant__ AttentionMaps maps, const __grid_c
     } else if (warp == roles.kProductWarp) {
         const uint32_t idesc_s = make_idesc_bf16(kRows, kCols, 0, 0), idesc_d = make_idesc_bf16(kRows, steps_d * 16, 0, 1);
         const uint32_t fixed_lo = uniform(desc_lo(tiles, 16)), ring_lo = uniform(desc_lo(ring, 16)), ring_mn = uniform(desc_lo(ring, kHalfCols));
-        roles.products(
+        roles.template products<false>(
             [&](int slot, int buffer) {
                 const uint32_t at = ring_lo + slot * (2 * kStream / 16), to = tmem + buffer * 2 * kCols;
                 product_ss<HALVES>(to, fixed_lo, kHalfTile, at, kHalfCols, idesc_s, steps_d);
@@ -1042,20 +1073,35 @@ DkdvPlan dkdv_plan(const AttentionParams& p, int sms) {
     pl.sink_tiles = last_far < 0 ? 0 : last_far / kRows + 1;
     pl.sink_parts = pl.parts = 1;
     if (p.tq == 0) return pl;
-    // Query tiles over all blocks; what one SM does if they are shared evenly bounds a part from below.
-    const int64_t units = static_cast<int64_t>(p.batch) * (p.heads / p.group);
+    // Microseconds of a tile and of a block's beginning and end, measured (8192 tokens, 16 heads on 4 of 128; 4096 tokens of 64).
+    const float per_tile = p.head_dim <= 64 ? 0.75f : 1.05f, per_block = 5.0f;
+    const int64_t units = static_cast<int64_t>(p.batch) * (p.heads / p.group), others = units * (pl.tiles - pl.sink_tiles);
     const int step = pl.tiles / 512 + 1;
     int64_t total = 0, most = 0, most_kept = 0;
     for (int t = 0; t < pl.tiles; t += step) {
         const int64_t n = static_cast<int64_t>(QueryTiles(p, t * kRows).count) * p.group;
-        total += n * step;
+        total += n * step * units;
         int64_t& m = t < pl.sink_tiles ? most_kept : most;
         m = n > m ? n : m;
     }
-    int64_t share = total * units / sms;
-    share = share > 16 ? share : 16;
-    if (most_kept > share) pl.sink_parts = static_cast<int>((most_kept + share - 1) / share < 64 ? (most_kept + share - 1) / share : 64);
-    if (most > share && units * (pl.tiles - pl.sink_tiles) < 2 * sms) pl.parts = static_cast<int>((most + share - 1) / share < 16 ? (most + share - 1) / share : 16);
+    // Time of a list of blocks, longest first: an even share of all, and a part of the longest that comes last.  Parts cost
+    // their sums' way through memory and the launch that adds them.
+    float best = 0.0f;
+    for (int parts : {1, 2, 3, 4, 6, 8, 12, 16}) {
+        if (parts > 1 && parts * 4 > most) break;
+        const float all = static_cast<float>(total) * per_tile + static_cast<float>(others * parts) * per_block;
+        const float longest = per_block + static_cast<float>((most + parts - 1) / parts) * per_tile;
+        const float share = all / static_cast<float>(sms);
+        const float cost = (share > longest ? share : longest) + 0.5f * longest +
+                           (parts > 1 ? 4.0f + static_cast<float>(others * parts) * (p.head_dim <= 64 ? 0.044f : 0.087f) : 0.0f);
+        if (parts == 1 || cost < best) {
+            best = cost;
+            pl.parts = parts;
+        }
+    }
+    // Tiles that all later queries see: parts no longer than the other tiles' blocks.
+    const int64_t longest = (most + pl.parts - 1) / pl.parts > 16 ? (most + pl.parts - 1) / pl.parts : 16;
+    if (most_kept > longest) pl.sink_parts = static_cast<int>((most_kept + longest - 1) / longest < 64 ? (most_kept + longest - 1) / longest : 64);
     return pl;
 }
 
@@ -1082,15 +1128,15 @@ cudaError_t launch_attention_bwd_sm100(AttentionParams p, const CUtensorMap* m, 
     const int blocks_q = (p.tq + kRows - 1) / kRows;
     const bool narrow = p.head_dim <= 64;
     int64_t blocks = static_cast<int64_t>(p.batch) * p.heads * blocks_q;
-    cudaError_t e = narrow ? launch_sm(attention_dq_kernel<1>, blocks, BwdRoles<3>::kThreads, bwd_smem<1>(), stream, maps, p, blocks_q, status, wait_ns)
-                           : launch_sm(attention_dq_kernel<2>, blocks, BwdRoles<3>::kThreads, bwd_smem<2>(), stream, maps, p, blocks_q, status, wait_ns);
+    cudaError_t e = narrow ? launch_sm(attention_dq_kernel<1, 1>, blocks, DqRoles<1, 1>::kThreads, bwd_smem<1>(), stream, maps, p, blocks_q, status, wait_ns)
+                           : launch_sm(attention_dq_kernel<2, 3>, blocks, DqRoles<2, 3>::kThreads, bwd_smem<2>(), stream, maps, p, blocks_q, status, wait_ns);
     if (e != cudaSuccess) return e;
     maps.q = m[5]; maps.dout = m[6]; maps.k = m[7]; maps.v = m[8]; maps.dk = m[9]; maps.dv = m[10];
     const DkdvPlan pl = dkdv_plan(p, sms);
     const int64_t units = static_cast<int64_t>(p.batch) * (p.heads / p.group);
     blocks = units * pl.items();
-    e = narrow ? launch_sm(attention_dkdv_kernel<1>, blocks, BwdRoles<3>::kThreads, bwd_smem<1>(), stream, maps, p, pl, status, wait_ns)
-               : launch_sm(attention_dkdv_kernel<2>, blocks, BwdRoles<2>::kThreads, bwd_smem<2>(), stream, maps, p, pl, status, wait_ns);
+    e = narrow ? launch_sm(attention_dkdv_kernel<1, 3>, blocks, DkdvRoles<1, 3>::kThreads, bwd_smem<1>(), stream, maps, p, pl, status, wait_ns)
+               : launch_sm(attention_dkdv_kernel<2, 2>, blocks, DkdvRoles<2, 2>::kThreads, bwd_smem<2>(), stream, maps, p, pl, status, wait_ns);
     for (int kept = 1; kept >= 0 && e == cudaSuccess; --kept) {
         const int n_tiles = kept ? pl.sink_tiles : pl.tiles - pl.sink_tiles;
         if (n_tiles == 0 || (kept ? pl.sink_parts : pl.parts) == 1) continue;
