@@ -512,6 +512,8 @@ LLMT_B200_API uint64_t llmt_b200_norm_residual_workspace_bytes(const llmt_b200_n
  * _decode: one new token per sequence (tokens_q = 1) over a cache of tokens_k places, of which
  * sequence b holds lengths[b] (device, int32; NULL: all; values beyond tokens_k count as tokens_k,
  * below 1 as none): the query stands at lengths[b] - 1, the newest key.  Places behind are not read.
+ * workspace: 16-byte aligned, llmt_b200_attention_window_decode_workspace_bytes(desc) bytes (0 for many
+ * calls): results of the chunks that long sequences are split into.
  *
  * _fwd and _bwd occupy whole SMs, whatever llmt_b200_set_sm_budget says: their blocks are short. */
 typedef struct llmt_b200_attention_desc {
@@ -530,6 +532,7 @@ LLMT_B200_API int llmt_b200_attention_window_fwd(const llmt_b200_attention_desc*
 LLMT_B200_API int llmt_b200_attention_window_bwd(const llmt_b200_attention_desc* desc, void* stream);
 LLMT_B200_API int llmt_b200_attention_window_decode(const llmt_b200_attention_desc* desc, void* stream);
 LLMT_B200_API uint64_t llmt_b200_attention_window_workspace_bytes(const llmt_b200_attention_desc* desc);
+LLMT_B200_API uint64_t llmt_b200_attention_window_decode_workspace_bytes(const llmt_b200_attention_desc* desc);
 
 /* The same exchange with all `world` ranks living on ONE device (comms[r] is rank r's
  * descriptor, every pointer local): a single cooperative launch of world * ctas CTAs.

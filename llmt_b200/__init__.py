@@ -35,6 +35,7 @@ EXPORTS = [
     "llmt_b200_rope", "llmt_b200_rope_frequencies", "llmt_b200_norm_residual_fwd", "llmt_b200_norm_residual_bwd",
     "llmt_b200_norm_residual_workspace_bytes", "llmt_b200_attention_window_fwd", "llmt_b200_attention_window_bwd",
     "llmt_b200_attention_window_decode", "llmt_b200_attention_window_workspace_bytes",
+    "llmt_b200_attention_window_decode_workspace_bytes",
 ]
 
 COMM_MAX_RANKS, COMM_MAX_CTAS = 8, 128
@@ -207,8 +208,9 @@ def lib() -> ctypes.CDLL:
         for name in ("fwd", "bwd", "decode"):
             f = getattr(L, "llmt_b200_attention_window_" + name)
             f.argtypes, f.restype = [ctypes.POINTER(AttentionDesc), ctypes.c_void_p], ctypes.c_int
-        L.llmt_b200_attention_window_workspace_bytes.argtypes = [ctypes.POINTER(AttentionDesc)]
-        L.llmt_b200_attention_window_workspace_bytes.restype = ctypes.c_uint64
+        for name in ("workspace_bytes", "decode_workspace_bytes"):
+            f = getattr(L, "llmt_b200_attention_window_" + name)
+            f.argtypes, f.restype = [ctypes.POINTER(AttentionDesc)], ctypes.c_uint64
         L.llmt_b200_exchange_begin_step.argtypes = [ctypes.POINTER(CommDesc), ctypes.c_void_p]
         L.llmt_b200_exchange_begin_step.restype = ctypes.c_int
         L.llmt_b200_zero_grads.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]
@@ -777,9 +779,10 @@ def attention_window_workspace_bytes(q, k, window: int = 0, sinks: int = 0) -> i
     return int(lib().llmt_b200_attention_window_workspace_bytes(ctypes.byref(d)))
 
 
-def attention_window_decode(out, q, k, v, lengths=None, window: int = 0, sinks: int = 0, scale=None, lse=None, stream=None) -> None:
+def attention_window_decode(out, q, k, v, lengths=None, window: int = 0, sinks: int = 0, scale=None, lse=None, workspace=None, stream=None) -> None:
     """attention_window_fwd for one new token per sequence: q, out [B, H, hd] over a cache k, v [B, places, Hkv, hd] of which
-    sequence b holds lengths[b] (int32 on the device; None: all), the new token's key the last of them."""
+    sequence b holds lengths[b] (int32 on the device; None: all), the new token's key the last of them.  `workspace`: a
+    uint8 tensor of attention_window_decode_workspace_bytes, or one is allocated for the call where it needs one."""
     import torch
     who = "attention_window_decode"
     _need(q.dim() == 3 and out.dim() == 3, f"{who}: q and out must be [batch, heads, head_dim]")
@@ -788,7 +791,22 @@ def attention_window_decode(out, q, k, v, lengths=None, window: int = 0, sinks: 
         _need(lengths.dtype == torch.int32 and lengths.is_contiguous() and lengths.numel() == q.shape[0], f"{who}: lengths must be contiguous int32 [batch]")
         d.lengths = lengths.data_ptr()
     _put_lse(d, who, lse, d.batch * d.heads)
-    _on(_device_of(who, out, q, k, v, lengths, lse), stream, lambda s: lib().llmt_b200_attention_window_decode(ctypes.byref(d), s))
+
+    def call(s):
+        ws = workspace
+        if ws is None:
+            need = lib().llmt_b200_attention_window_decode_workspace_bytes(ctypes.byref(d))
+            ws = _scratch(need, q, stream) if need else None
+        if ws is not None:
+            d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
+        return lib().llmt_b200_attention_window_decode(ctypes.byref(d), s)
+    _on(_device_of(who, out, q, k, v, lengths, lse, workspace), stream, call)
+
+
+def attention_window_decode_workspace_bytes(q, k, window: int = 0, sinks: int = 0) -> int:
+    """Scratch of attention_window_decode for tensors of these shapes (q [B, H, hd]) on the current device."""
+    d = _attention_desc("attention_window_decode_workspace_bytes", q.unsqueeze(1), k, k, window, sinks, None, {})
+    return int(lib().llmt_b200_attention_window_decode_workspace_bytes(ctypes.byref(d)))
 
 
 def exchange_begin_step(desc: "CommDesc", stream=None) -> None:

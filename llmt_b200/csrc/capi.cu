@@ -2199,6 +2199,12 @@ int llmt_b200_attention_window_bwd(const llmt_b200_attention_desc* d, void* stre
     return LLMT_B200_OK;
 }
 
+uint64_t llmt_b200_attention_window_decode_workspace_bytes(const llmt_b200_attention_desc* d) {
+    AttentionParams p;
+    if (attention_params(d, "attention_window_decode", &p) != LLMT_B200_OK) return 0;
+    return (attention_decode_workspace(p, sm_count()) + 15) / 16 * 16;
+}
+
 int llmt_b200_attention_window_decode(const llmt_b200_attention_desc* d, void* stream) {
     const char* who = "attention_window_decode";
     AttentionParams p;
@@ -2210,7 +2216,19 @@ int llmt_b200_attention_window_decode(const llmt_b200_attention_desc* d, void* s
     if (st == LLMT_B200_OK) st = attention_apart(d, who, "lse", d->lse, 4 * static_cast<size_t>(d->batch * d->heads), t, 4);
     if (st != LLMT_B200_OK) return st;
     if (p.batch == 0 || p.heads == 0) return LLMT_B200_OK;
-    const cudaError_t e = launch_attention_window_decode(p, sm_count(), static_cast<cudaStream_t>(stream));
+    const uint64_t need = llmt_b200_attention_window_decode_workspace_bytes(d);
+    if (need > 0) {
+        if (d->workspace == nullptr || d->workspace_bytes < need)
+            return fail(LLMT_B200_ERR_WORKSPACE, "%s: workspace of %llu bytes needed, %llu given", who, (unsigned long long)need,
+                        (unsigned long long)(d->workspace == nullptr ? 0 : d->workspace_bytes));
+        if (misaligned(d->workspace, 16)) return fail(LLMT_B200_ERR_INVALID, "%s: workspace is not 16-byte aligned", who);
+        st = attention_apart(d, who, "workspace", d->workspace, need, t, 4);
+        if (st != LLMT_B200_OK) return st;
+        if (overlaps(d->workspace, need, d->lse, d->lse != nullptr ? 4 * static_cast<size_t>(d->batch * d->heads) : 0) ||
+            (d->lengths != nullptr && overlaps(d->workspace, need, d->lengths, 4 * static_cast<size_t>(d->batch))))
+            return fail(LLMT_B200_ERR_INVALID, "%s: workspace overlaps lse or lengths", who);
+    }
+    const cudaError_t e = launch_attention_window_decode(p, sm_count(), d->workspace, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return fail(LLMT_B200_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
     return LLMT_B200_OK;
 }

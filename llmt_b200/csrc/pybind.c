@@ -41,12 +41,14 @@ typedef struct {
     int (*attention_window_bwd)(const llmt_b200_attention_desc*, void*);
     int (*attention_window_decode)(const llmt_b200_attention_desc*, void*);
     uint64_t (*attention_window_workspace_bytes)(const llmt_b200_attention_desc*);
+    uint64_t (*attention_window_decode_workspace_bytes)(const llmt_b200_attention_desc*);
 } Entry;
 static const char* const kNames[] = {"gemm", "gemm_workspace_bytes_for", "gemm_grouped", "zero_grads", "softmax_fwd", "softmax_bwd",
                                      "gemm_softmax_fwd", "gemm_softmax_bwd", "rowdot", "head_split", "head_merge",
                                      "cross_entropy_fwd", "cross_entropy_bwd", "lm_head_ce_fwd", "lm_head_ce_bwd",
                                      "rope", "norm_residual_fwd", "norm_residual_bwd", "norm_residual_workspace_bytes", "attention_window_fwd",
-                                     "attention_window_bwd", "attention_window_decode", "attention_window_workspace_bytes"};
+                                     "attention_window_bwd", "attention_window_decode", "attention_window_workspace_bytes",
+                                     "attention_window_decode_workspace_bytes"};
 #define N_ENTRIES ((Py_ssize_t)(sizeof(kNames) / sizeof(kNames[0])))
 _Static_assert(sizeof(Entry) == sizeof(kNames), "one pointer per name");
 
@@ -692,7 +694,7 @@ static int as_token(PyObject* o, Tensor* t, llmt_b200_head_view* v, int* device)
 }
 
 FAST(attention_window_decode) {
-    BEGIN(4, "out", "q", "k", "v", "lengths", "window", "sinks", "scale", "lse", "stream");
+    BEGIN(4, "out", "q", "k", "v", "lengths", "window", "sinks", "scale", "lse", "workspace", "stream");
     llmt_b200_attention_desc d;
     Tensor out, q, k, vv;
     int dev = -1;
@@ -701,11 +703,26 @@ FAST(attention_window_decode) {
     NEED(as_token(v[0], &out, &d.out, &dev) == 0 && as_token(v[1], &q, &d.q, &dev) == 0 && as_heads(v[2], &k, &d.k, &dev) == 0 &&
          as_heads(v[3], &vv, &d.v, &dev) == 0);
     NEED(attention_of(&d, &q, &k, &vv, v[5], v[6], v[7]) == 0 && out.dtype == q.dtype && same_shape(&out, &q) &&
-         as_vector(v[4], 2, d.batch, &dev, &lengths) == 0 && as_vector(v[8], LLMT_B200_FP32, d.batch * d.heads, &dev, &lse) == 0 &&
-         stream_of(v[9], dev, &s) == 0);
+         as_vector(v[4], 2, d.batch, &dev, &lengths) == 0 && as_vector(v[8], LLMT_B200_FP32, d.batch * d.heads, &dev, &lse) == 0);
     d.lse = (float*)lse;
     d.lengths = (const int32_t*)lengths;
-    RUN(E.attention_window_decode(&d, s));
+    PyObject* scratch = NULL;
+    if (is_there(v[9])) NEED(as_workspace(v[9], &dev, &d.workspace, &d.workspace_bytes) == 0);
+    NEED(stream_of(v[10], dev, &s) == 0);
+    if (!is_there(v[9])) {
+        d.workspace_bytes = E.attention_window_decode_workspace_bytes(&d);
+        if (d.workspace_bytes > 0) {
+            scratch = scratch_for(d.workspace_bytes, v[1], v[10]);
+            if (scratch == NULL) return NULL;
+            if (as_ptr(scratch, &d.workspace) < 0) { Py_DECREF(scratch); SLOW(); }
+        }
+    }
+    int st;
+    Py_BEGIN_ALLOW_THREADS
+    st = E.attention_window_decode(&d, s);
+    Py_END_ALLOW_THREADS
+    Py_XDECREF(scratch);
+    return finish(st);
 }
 
 // ---------------------------------------------------------------------------------- module
