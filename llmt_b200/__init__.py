@@ -710,12 +710,18 @@ def norm_residual_bwd(dx, dy, dout, dh, out, y=None, w_post=None, gate=None, w_p
     _on(device, stream, call)
 
 
-def norm_residual_workspace_bytes(rows: int, cols: int, groups: int = 1, weights: bool = True, gate: bool = True) -> int:
-    """Scratch of norm_residual_bwd on the current device; weights: dw_post or dw_pre is wanted, gate: dgate is."""
+def norm_residual_workspace_bytes(rows: int, cols: int, groups: int = 1, weights: bool = True, gate: bool = True, res=None, act=None) -> int:
+    """Scratch of norm_residual_bwd on the current device; weights: dw_post or dw_pre is wanted, gate: dgate is; res, act: the
+    types of the residual stream and of the block, or None for enough whatever they are."""
+    import torch
+    if res is None or act is None:
+        kinds = ((torch.float32, torch.float32), (torch.float32, torch.bfloat16), (torch.bfloat16, torch.bfloat16))
+        return max(norm_residual_workspace_bytes(rows, cols, groups, weights, gate, r, a) for r, a in kinds)
     d = NormResidualDesc()
     d.rows, d.cols, d.groups = int(rows), int(cols), int(groups)
+    d.dtype_res, d.dtype_act = (BF16 if t == torch.bfloat16 else FP32 for t in (res, act))
     if weights:
-        d.dw_pre = 4
+        d.dw_pre = d.dw_post = 4
     if gate:
         d.dgate = 4
     return int(lib().llmt_b200_norm_residual_workspace_bytes(ctypes.byref(d)))

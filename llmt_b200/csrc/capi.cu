@@ -1869,6 +1869,10 @@ int norm_residual_params(const llmt_b200_norm_residual_desc* d, const char* who,
     return LLMT_B200_OK;
 }
 
+int norm_residual_row_bytes(const llmt_b200_norm_residual_desc* d) {
+    return 2 * ((d->dtype_res == LLMT_B200_BF16 ? 2 : 4) + (d->dtype_act == LLMT_B200_BF16 ? 2 : 4));
+}
+
 // A [rows, cols] tensor of a norm_residual call.
 struct RowTensor {
     const char* name;
@@ -1913,7 +1917,7 @@ int llmt_b200_norm_residual_fwd(const llmt_b200_norm_residual_desc* d, void* str
     bool wide = d->cols % 8 == 0 && !misaligned(d->w_post, 16) && !misaligned(d->gate, 16) && !misaligned(d->w_pre, 16);
     st = norm_residual_tensors(d, who, t, 4, d->x, d->out, &wide);
     if (st != LLMT_B200_OK) return st;
-    const cudaError_t e = launch_norm_residual_fwd(p, d->dtype_res == LLMT_B200_BF16, d->dtype_act == LLMT_B200_BF16, wide, static_cast<cudaStream_t>(stream));
+    const cudaError_t e = launch_norm_residual_fwd(p, d->dtype_res == LLMT_B200_BF16, d->dtype_act == LLMT_B200_BF16, wide, sm_count(), static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return fail(LLMT_B200_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
     return LLMT_B200_OK;
 }
@@ -1921,9 +1925,9 @@ int llmt_b200_norm_residual_fwd(const llmt_b200_norm_residual_desc* d, void* str
 uint64_t llmt_b200_norm_residual_workspace_bytes(const llmt_b200_norm_residual_desc* d) {
     NormResidualParams p;
     if (norm_residual_params(d, "norm_residual_bwd", &p) != LLMT_B200_OK || d->rows == 0) return 0;
-    const NormResidualPlan pl = norm_residual_plan(d->rows, d->cols, d->groups, d->dw_post != nullptr || d->dw_pre != nullptr, d->dgate != nullptr, sm_count());
-    if (pl.floats_w + pl.floats_gate == 0) return 0;
-    return static_cast<uint64_t>(pl.floats_w + pl.floats_gate + 8) / 4 * 16;   // both parts start on 16 bytes
+    const NormResidualPlan pl = norm_residual_plan(d->rows, d->cols, d->groups, norm_residual_row_bytes(d), d->dw_pre != nullptr, d->dw_post != nullptr || d->dgate != nullptr, sm_count());
+    if (pl.floats_w + pl.floats_gc == 0) return 0;
+    return static_cast<uint64_t>(pl.floats_w + pl.floats_gc + 8) / 4 * 16;   // both parts start on 16 bytes
 }
 
 int llmt_b200_norm_residual_bwd(const llmt_b200_norm_residual_desc* d, void* stream) {
@@ -1962,7 +1966,7 @@ int llmt_b200_norm_residual_bwd(const llmt_b200_norm_residual_desc* d, void* str
             if (sums[j].data != nullptr && overlaps(sums[i].data, 4 * sums[i].n, sums[j].data, 4 * sums[j].n))
                 return fail(LLMT_B200_ERR_INVALID, "%s: %s overlaps %s", who, sums[i].name, sums[j].name);
     }
-    const NormResidualPlan pl = norm_residual_plan(d->rows, d->cols, d->groups, d->dw_post != nullptr || d->dw_pre != nullptr, d->dgate != nullptr, sm_count());
+    const NormResidualPlan pl = norm_residual_plan(d->rows, d->cols, d->groups, norm_residual_row_bytes(d), d->dw_pre != nullptr, d->dw_post != nullptr || d->dgate != nullptr, sm_count());
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (d->rows == 0) {   // sums of nothing
         for (const auto& g : sums) {
@@ -1989,7 +1993,7 @@ int llmt_b200_norm_residual_bwd(const llmt_b200_norm_residual_desc* d, void* str
         for (const auto& x : read)
             if (x.data != nullptr && overlaps(d->workspace, need, x.data, 4 * x.n)) return fail(LLMT_B200_ERR_INVALID, "%s: workspace overlaps %s", who, x.name);
         p.part_w = pl.floats_w > 0 ? static_cast<float*>(d->workspace) : nullptr;
-        p.part_gate = pl.floats_gate > 0 ? static_cast<float*>(d->workspace) + (pl.floats_w + 3) / 4 * 4 : nullptr;
+        p.part_gc = pl.floats_gc > 0 ? static_cast<float*>(d->workspace) + (pl.floats_w + 3) / 4 * 4 : nullptr;
     }
     p.cluster = pl.cluster;
     p.dout = d->dout; p.dh = d->dh; p.dx = d->dx; p.dy = d->dy;

@@ -251,11 +251,11 @@ struct NormResidualParams {
     const void *dout, *dh;
     void *dx, *dy;
     float *dw_post, *dgate, *dw_pre;
-    float *part_w, *part_gate;   // workspace: [blocks][2][cols], [units][cols]
+    float *part_w, *part_gc;     // workspace: sums for dw_pre [blocks][cols], for dw_post and dgate [units][cols]
 };
 struct NormResidualPlan {
     int cluster, warps, blocks, units, per_group;
-    int64_t floats_w, floats_gate;
+    int64_t floats_w, floats_gc;
 };
 
 // Attention with a sliding window and sinks (attention_rows.cuh, attention_window.cu).  bf16; strides in elements.
@@ -382,8 +382,9 @@ cudaError_t launch_rowdot(float* out, const void* x, const void* y, int64_t rows
                           int64_t ldy, int is_bf16, cudaStream_t stream);
 cudaError_t launch_rope(RopeParams p, int is_bf16, cudaStream_t stream);
 int norm_residual_max_cols(void);
-NormResidualPlan norm_residual_plan(int64_t rows, int64_t cols, int64_t groups, bool want_w, bool want_gate, int sms);
-cudaError_t launch_norm_residual_fwd(const NormResidualParams& p, int res_bf16, int act_bf16, bool wide, cudaStream_t stream);
+// row_bytes: of one column in the four tensors that the backward pass reads
+NormResidualPlan norm_residual_plan(int64_t rows, int64_t cols, int64_t groups, int row_bytes, bool want_pre, bool want_gc, int sms);
+cudaError_t launch_norm_residual_fwd(const NormResidualParams& p, int res_bf16, int act_bf16, bool wide, int sms, cudaStream_t stream);
 cudaError_t launch_norm_residual_bwd(const NormResidualParams& p, const NormResidualPlan& pl, int res_bf16, int act_bf16, bool wide, float beta,
                                      cudaStream_t stream);
 cudaError_t launch_attention_window_fwd(const AttentionParams& p, cudaStream_t stream);

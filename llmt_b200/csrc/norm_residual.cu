@@ -8,11 +8,15 @@
 //   dy = rstd_post (e g - c mean(e g c))
 //   dw_pre += dh b,  dw_post += k g c,  dgate += scale g c w_post
 // mean(e g c) is linear in mean(a b), so the three row sums  a b,  e c (dout + rstd_pre a)  and  e c b  are formed in one round.
+// While the gate stays the same, dw_post and dgate are the same sum of g c, times scale gate and times scale w_post: one sum per
+// block and piece of a gate's rows serves both.
 //
-// Bound: memory; every tensor is read and written once, all sums are fp32.  Forward: a row's values stay in the registers of
-// the warps that own the row.  Backward: a block owns all columns (a cluster of blocks those of a wide row), takes rows one after
-// the other with the next row's loads in flight, and keeps the three weight gradients of its columns in registers; each
-// block leaves one row of sums, and a second launch adds those in a fixed order.
+// Bound: memory; every tensor is read and written once, all sums are fp32.  A block owns all columns, takes rows one after the
+// other and keeps the weights of its columns in registers (read for every row they are more than the row).  A thread copies
+// its own pieces of the rows to come into shared memory (cp.async, two or three rows ahead): what is under way takes no
+// registers, and nobody else reads it, so nothing has to be waited for but the row sums.
+// Backward: a cluster of blocks owns a row of more than 4096 columns; the three weight gradients of a block's columns are in
+// registers too, each block leaves one row of sums, and a second launch adds those in a fixed order.
 #include <cuda_bf16.h>
 
 #include "common.h"
@@ -30,124 +34,31 @@ template <> __device__ __forceinline__ __nv_bfloat16 rounded<__nv_bfloat16>(floa
 // V values of a row that start on a multiple of V: one or two 16-byte accesses (V = 8) or one value (V = 1).
 template <typename T, int V> struct alignas(V * sizeof(T) < 16 ? V * sizeof(T) : 16) Vec { T v[V]; };
 
-template <int V> __device__ __forceinline__ void load_weights(float* w, const float* at, bool there, float otherwise) {
-    if (there) {
-        const Vec<float, V> x = *reinterpret_cast<const Vec<float, V>*>(at);
-#pragma unroll
-        for (int i = 0; i < V; ++i) w[i] = x.v[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) w[i] = otherwise;
-    }
-}
-
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
 
-// ------------------------------------------------------------------------------------------------------------ forward
-
-constexpr int kFwdRows = 4;   // rows of a block whose rows are one warp's each
-
-// The sum over the warps of a row (all of the block's, or one).
-__device__ __forceinline__ float row_sum(float v, float* part, int warps) {
-    v = warp_sum(v);
-    if (warps == 1) return v;
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float s = 0.0f;
-    for (int i = 0; i < warps; ++i) s += part[i];
-    return s;
-}
-
-template <typename TR, typename TA, int V, int NV>
-__global__ void __launch_bounds__(512) norm_residual_fwd_kernel(NormResidualParams p, int warps) {
-    __shared__ float part[2][16];
-    ptx::grid_dependency_wait();
-    const int64_t row = warps == 1 ? static_cast<int64_t>(blockIdx.x) * kFwdRows + (threadIdx.x >> 5) : static_cast<int64_t>(blockIdx.x);
-    if (row >= p.rows) return;
-    const int across = warps * 32, me = warps == 1 ? threadIdx.x & 31 : threadIdx.x;
-    const TR* x = static_cast<const TR*>(p.x) + row * p.ld_x;
-    const TA* y = static_cast<const TA*>(p.y) + row * p.ld_y;
-    const float* gate = p.gate != nullptr ? p.gate + row / p.rows_per_gate * p.cols : nullptr;
-    const bool block = p.y != nullptr;
-    Vec<TR, V> xs[NV];
-    Vec<TA, V> ys[NV];
-#pragma unroll
-    for (int n = 0; n < NV; ++n) {
-        const int col = (me + n * across) * V;
-        xs[n] = {};
-        ys[n] = {};
-        if (col < p.cols) {
-            xs[n] = *reinterpret_cast<const Vec<TR, V>*>(x + col);
-            if (block) ys[n] = *reinterpret_cast<const Vec<TA, V>*>(y + col);
-        }
-    }
-    const float of = 1.0f / static_cast<float>(p.cols);
-    float k = p.scale;
-    if (block && p.w_post != nullptr) {
-        float s = 0.0f;
-#pragma unroll
-        for (int n = 0; n < NV; ++n)
-#pragma unroll
-            for (int i = 0; i < V; ++i) s = fmaf(to_float(ys[n].v[i]), to_float(ys[n].v[i]), s);
-        const float r = 1.0f / sqrtf(row_sum(s, part[0], warps) * of + p.eps);
-        if (me == 0 && p.rstd_post != nullptr) p.rstd_post[row] = r;
-        k *= r;
-    }
-    float z[NV * V], s = 0.0f;
-#pragma unroll
-    for (int n = 0; n < NV; ++n) {
-        const int col = (me + n * across) * V;
-        if (col < p.cols) {
-            if (block) {
-                float w[V], g[V];
-                load_weights<V>(w, p.w_post + col, p.w_post != nullptr, 1.0f);
-                load_weights<V>(g, gate + col, gate != nullptr, 1.0f);
-                Vec<TR, V> o;
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    z[n * V + i] = fmaf(k * to_float(ys[n].v[i]), w[i] * g[i], to_float(xs[n].v[i]));
-                    o.v[i] = rounded<TR>(z[n * V + i]);
-                }
-                *reinterpret_cast<Vec<TR, V>*>(static_cast<TR*>(p.out) + row * p.ld_out + col) = o;
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i) z[n * V + i] = to_float(xs[n].v[i]);
-            }
-#pragma unroll
-            for (int i = 0; i < V; ++i) s = fmaf(z[n * V + i], z[n * V + i], s);
-        }
-    }
-    if (p.h == nullptr) return;
-    const float r = 1.0f / sqrtf(row_sum(s, part[1], warps) * of + p.eps);
-    if (me == 0 && p.rstd_pre != nullptr) p.rstd_pre[row] = r;
-#pragma unroll
-    for (int n = 0; n < NV; ++n) {
-        const int col = (me + n * across) * V;
-        if (col < p.cols) {
-            float w[V];
-            load_weights<V>(w, p.w_pre + col, true, 1.0f);
-            Vec<TA, V> o;
-#pragma unroll
-            for (int i = 0; i < V; ++i) o.v[i] = rounded<TA>(z[n * V + i] * r * w[i]);
-            *reinterpret_cast<Vec<TA, V>*>(static_cast<TA*>(p.h) + row * p.ld_h + col) = o;
-        }
-    }
-}
-
-// ----------------------------------------------------------------------------------------------------------- backward
-
-constexpr int kBwdWarps = 16;                  // of a block at most
-constexpr int kBwdCols = kBwdWarps * 32 * 8;   // columns that one block owns at most
-
 // Eight columns of a thread: V = 8 neighbours, or (V = 1) eight that are the block's width apart.
 template <typename T, int V> struct Eight {
     Vec<T, V> g[8 / V];
     __device__ __forceinline__ float at(int i) const { return to_float(g[i / V].v[i % V]); }
     __device__ __forceinline__ void put(int i, float x) { g[i / V].v[i % V] = rounded<T>(x); }
+    // All eight; bf16 in pairs (a conversion of one value takes four times as long as that of two).
+    __device__ __forceinline__ void put(const float (&x)[8]) {
+        if (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) put(i, x[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                const __nv_bfloat162 two = __floats2bfloat162_rn(x[i], x[i + 1]);
+                g[i / V].v[i % V] = reinterpret_cast<const T&>(two.x);
+                g[(i + 1) / V].v[(i + 1) % V] = reinterpret_cast<const T&>(two.y);
+            }
+        }
+    }
     __device__ __forceinline__ void load(const T* row, int first, int step, int cols, bool there) {
 #pragma unroll
         for (int n = 0; n < 8 / V; ++n) {
@@ -161,16 +72,201 @@ template <typename T, int V> struct Eight {
             if (first + n * step < cols) *reinterpret_cast<Vec<T, V>*>(row + first + n * step) = g[n];
     }
 };
-template <typename TR, typename TA, int V> struct BwdRow {
-    Eight<TR, V> out, dout;
-    Eight<TA, V> dh, y;
-    float r_pre, r_post;
+
+// A thread's eight columns of one tensor's row on their way through shared memory: `place` is where the thread's share begins in the
+// tensor's part of a stage, [16-byte piece or value][thread].  Places whose columns are not there are never copied to: the
+// kernels put zeros into all of them once.
+template <typename T, int V> struct Staged {
+    static constexpr int kUnit = V == 8 ? 16 : static_cast<int>(sizeof(T)), kUnits = 8 * static_cast<int>(sizeof(T)) / kUnit;
+    static __device__ __forceinline__ void copy(uint8_t* to, const T* row, int first, int step, int cols) {
+        const int threads = blockDim.x;
+        if (V == 8) {
+            if (first < cols) {
+#pragma unroll
+                for (int n = 0; n < kUnits; ++n)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(to + n * threads * kUnit)), "l"(row + first + n * (16 / sizeof(T))) : "memory");
+            }
+        } else if (sizeof(T) == 4) {
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+                if (first + n * step < cols)
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(ptx::smem_u32(to + n * threads * kUnit)), "l"(row + first + n * step) : "memory");
+        } else {   // two bytes are no asynchronous copy
+            T v[8];
+#pragma unroll
+            for (int n = 0; n < 8; ++n) v[n] = first + n * step < cols ? row[first + n * step] : rounded<T>(0.0f);
+#pragma unroll
+            for (int n = 0; n < 8; ++n) *reinterpret_cast<T*>(to + n * threads * kUnit) = v[n];
+        }
+    }
+    static __device__ __forceinline__ void get(Eight<T, V>& e, const uint8_t* from) {
+        const int threads = blockDim.x;
+        if (V == 8) {
+            uint4 w[kUnits];
+#pragma unroll
+            for (int n = 0; n < kUnits; ++n) w[n] = *reinterpret_cast<const uint4*>(from + n * threads * kUnit);
+            e = *reinterpret_cast<const Eight<T, V>*>(w);
+        } else {
+#pragma unroll
+            for (int n = 0; n < 8; ++n) e.g[n / V].v[n % V] = *reinterpret_cast<const T*>(from + n * threads * kUnit);
+        }
+    }
+    static __device__ __forceinline__ uint8_t* place(uint8_t* part) { return part + threadIdx.x * kUnit; }
+    static __device__ __forceinline__ void clear(uint8_t* to) {
+        const int threads = blockDim.x;
+#pragma unroll
+        for (int n = 0; n < kUnits; ++n) {
+            if (kUnit == 16) *reinterpret_cast<uint4*>(to + n * threads * kUnit) = make_uint4(0, 0, 0, 0);
+            else *reinterpret_cast<T*>(to + n * threads * kUnit) = rounded<T>(0.0f);
+        }
+    }
 };
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+constexpr int kMostWarps = 16;                  // of a block
+constexpr int kMostCols = kMostWarps * 32 * 8;  // columns that a block owns eight a thread
+
+// ------------------------------------------------------------------------------------------------------------ forward
+
+// Rows in shared memory, the one at work among them: three, or what 200 KB hold of rows of more than 8192 columns.
+template <typename TR, typename TA, int N> constexpr int fwd_depth() { return N < 4 ? 3 : sizeof(TR) + sizeof(TA) == 8 ? 1 : sizeof(TR) + sizeof(TA) == 6 ? 2 : 3; }
+// N: eights of columns of a thread, `threads` * 8 columns apart.
+template <typename TR, typename TA, int V, int N>
+__global__ void __launch_bounds__(kMostWarps * 32) norm_residual_fwd_kernel(NormResidualParams p) {
+    extern __shared__ __align__(16) uint8_t stages[];
+    __shared__ float part[2][2][kMostWarps];
+    constexpr int kDepth = fwd_depth<TR, TA, N>();
+    ptx::grid_dependency_wait();
+    const int threads = blockDim.x, warps = threads >> 5, lane = threadIdx.x & 31, me = threadIdx.x;
+    const int first = V == 8 ? me * 8 : me, step = V == 8 ? 0 : threads;
+    const bool block = p.y != nullptr, post = p.w_post != nullptr, pre = p.h != nullptr;
+    const uint32_t of_x = threads * 8 * sizeof(TR), of_y = threads * 8 * sizeof(TA), stage_bytes = N * (of_x + of_y);
+    auto cols_of = [&](int n) { return V == 8 ? p.cols - n * threads * 8 : min(p.cols - n * threads * 8, threads * 8); };   // of the n-th eight
+    const float of = 1.0f / static_cast<float>(p.cols);
+    const int64_t r0 = p.rows * blockIdx.x / gridDim.x, r1 = p.rows * (blockIdx.x + 1) / gridDim.x;
+
+    uint8_t* const mine_x = Staged<TR, V>::place(stages);
+    uint8_t* const mine_y = Staged<TA, V>::place(stages + N * of_x);
+    for (int s = 0; s < kDepth; ++s)
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            Staged<TR, V>::clear(mine_x + s * stage_bytes + n * of_x);
+            Staged<TA, V>::clear(mine_y + s * stage_bytes + n * of_y);
+        }
+    auto copy = [&](int64_t row, int stage) {
+        if (row < r1) {
+            const TR* x = static_cast<const TR*>(p.x) + row * p.ld_x;
+            const TA* y = static_cast<const TA*>(p.y) + row * p.ld_y;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                Staged<TR, V>::copy(mine_x + stage * stage_bytes + n * of_x, x + n * threads * 8, first, step, cols_of(n));
+                if (block) Staged<TA, V>::copy(mine_y + stage * stage_bytes + n * of_y, y + n * threads * 8, first, step, cols_of(n));
+            }
+        }
+        commit_copies();
+    };
+#pragma unroll
+    for (int i = 0; i + 1 < kDepth; ++i) copy(r0 + i, i);
+    int stage = 0;
+    // k = gate w_post, changed with the gate's row
+    float k[N][8], w_pre[N][8];
+    Eight<float, V> w;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        w.load(p.w_pre + n * threads * 8, first, step, cols_of(n), pre);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w_pre[n][i] = w.at(i);
+    }
+    auto load_k = [&](int64_t group) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            w.load(p.w_post + n * threads * 8, first, step, cols_of(n), post);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) k[n][i] = post ? w.at(i) : 1.0f;
+            if (p.gate != nullptr) {
+                w.load(p.gate + group * p.cols + n * threads * 8, first, step, cols_of(n), true);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) k[n][i] *= w.at(i);
+            }
+        }
+    };
+    // The sum over the block; two sets of places in turn, so that nobody writes one that is still read.
+    int turn = 0;
+    auto row_sum = [&](float s, int which) {
+        s = warp_sum(s);
+        if (warps == 1) return s;
+        if (lane == 0) part[turn][which][me >> 5] = s;
+        __syncthreads();
+        s = 0.0f;
+        for (int i = 0; i < warps; ++i) s += part[turn][which][i];
+        return s;
+    };
+    int64_t next_group = r0;   // first row of the next gate row
+    for (int64_t row = r0; row < r1; ++row) {
+        copy(row + kDepth - 1, stage == 0 ? kDepth - 1 : stage - 1);
+        if (row == next_group) {
+            const int64_t group = row / p.rows_per_gate;
+            load_k(group);
+            next_group = (group + 1) * p.rows_per_gate;
+        }
+        wait_copies<kDepth - 1>();
+        Eight<TR, V> x[N];
+        Eight<TA, V> y[N];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            Staged<TR, V>::get(x[n], mine_x + stage * stage_bytes + n * of_x);
+            Staged<TA, V>::get(y[n], mine_y + stage * stage_bytes + n * of_y);
+        }
+        if (++stage == kDepth) stage = 0;
+        float scale = p.scale, s = 0.0f;
+        if (post) {
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s = fmaf(y[n].at(i), y[n].at(i), s);
+            const float r = rsqrtf(fmaf(row_sum(s, 0), of, p.eps));
+            if (me == 0 && p.rstd_post != nullptr) p.rstd_post[row] = r;
+            scale *= r;
+            s = 0.0f;
+        }
+        float z[N][8];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                z[n][i] = block ? fmaf(scale * y[n].at(i), k[n][i], x[n].at(i)) : x[n].at(i);
+                s = fmaf(z[n][i], z[n][i], s);
+            }
+            x[n].put(z[n]);
+            if (block) x[n].store(static_cast<TR*>(p.out) + row * p.ld_out + n * threads * 8, first, step, cols_of(n));
+        }
+        if (pre) {
+            const float r = rsqrtf(fmaf(row_sum(s, 1), of, p.eps));
+            if (me == 0 && p.rstd_pre != nullptr) p.rstd_pre[row] = r;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) z[n][i] *= r * w_pre[n][i];
+                y[n].put(z[n]);
+                y[n].store(static_cast<TA*>(p.h) + row * p.ld_h + n * threads * 8, first, step, cols_of(n));
+            }
+        }
+        turn ^= 1;
+    }
+}
+
+// ----------------------------------------------------------------------------------------------------------- backward
+
+template <typename TR, typename TA> constexpr int bwd_depth() { return sizeof(TR) + sizeof(TA) == 8 ? 3 : 4; }
 
 // `units` pieces of equal groups of rows (rows of one gate); block (cluster) b takes units b, b + grid, ...
-template <typename TR, typename TA, int V, bool CLUSTER>
-__global__ void __launch_bounds__(kBwdWarps * 32, 1) norm_residual_bwd_kernel(NormResidualParams p, int units, int per_group) {
-    __shared__ float part[2][4 * kBwdWarps][3];   // of every warp of the cluster (up to four blocks)
+// WARPS: of a block at most; of up to eight three blocks share an SM.
+template <typename TR, typename TA, int V, bool CLUSTER, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, WARPS == 8 ? 3 : 1) norm_residual_bwd_kernel(NormResidualParams p, int units, int per_group) {
+    extern __shared__ __align__(16) uint8_t stages[];
+    __shared__ float4 part[2][4 * kMostWarps];   // of every warp of the cluster (up to four blocks)
+    constexpr int kDepth = bwd_depth<TR, TA>();
     ptx::grid_dependency_wait();
     const int threads = blockDim.x, warps = threads >> 5;
     const int ranks = CLUSTER ? p.cluster : 1;
@@ -178,114 +274,152 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 1) norm_residual_bwd_kernel(No
     const int me = blockIdx.x / ranks, blocks = gridDim.x / ranks;
     const int first = V == 8 ? (rank * threads + static_cast<int>(threadIdx.x)) * 8 : rank * threads * 8 + static_cast<int>(threadIdx.x);
     const int step = V == 8 ? 0 : threads;
-    const int cols = V == 8 ? p.cols : (p.cols < (rank + 1) * threads * 8 ? p.cols : (rank + 1) * threads * 8);
-    const bool pre = p.dh != nullptr, block = p.y != nullptr, post = p.w_post != nullptr;
+    const int cols = V == 8 ? p.cols : min(p.cols, (rank + 1) * threads * 8);
+    const bool pre = p.dh != nullptr, block = p.y != nullptr, post = p.w_post != nullptr, more = p.dout != nullptr;
+    const uint32_t of_r = threads * 8 * sizeof(TR), of_a = threads * 8 * sizeof(TA), stage_bytes = 2 * (of_r + of_a);
     const float of = 1.0f / static_cast<float>(p.cols);
     if (CLUSTER) ptx::cluster_sync_all();   // nobody writes into a block's shared memory before it runs
 
     Eight<float, V> weight;
-    float w_pre[8], e_w[8], acc_pre[8], acc_post[8];
+    float w_pre[8], acc_pre[8];
     weight.load(p.w_pre, first, step, cols, pre);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) { w_pre[i] = weight.at(i); acc_pre[i] = acc_post[i] = 0.0f; }
-    weight.load(p.w_post, first, step, cols, post);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e_w[i] = post ? weight.at(i) : 1.0f;
+    for (int i = 0; i < 8; ++i) { w_pre[i] = weight.at(i); acc_pre[i] = 0.0f; }
 
-    BwdRow<TR, TA, V> next;
-    auto load = [&](int64_t row) {
-        next.out.load(static_cast<const TR*>(p.out) + row * p.ld_out, first, step, cols, pre);
-        next.dout.load(static_cast<const TR*>(p.dout) + row * p.ld_dout, first, step, cols, p.dout != nullptr);
-        next.dh.load(static_cast<const TA*>(p.dh) + row * p.ld_dh, first, step, cols, pre);
-        next.y.load(static_cast<const TA*>(p.y) + row * p.ld_y, first, step, cols, block);
-        next.r_pre = pre ? p.rstd_pre[row] : 0.0f;
-        next.r_post = block && post ? p.rstd_post[row] : 1.0f;
-    };
+    uint8_t* const mine_r = Staged<TR, V>::place(stages);
+    uint8_t* const mine_a = Staged<TA, V>::place(stages + 2 * of_r);
+    for (int s = 0; s < kDepth; ++s)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            Staged<TR, V>::clear(mine_r + s * stage_bytes + n * of_r);
+            Staged<TA, V>::clear(mine_a + s * stage_bytes + n * of_a);
+        }
+
     int turn = 0;
     for (int u = me; u < units; u += blocks) {
         const int64_t group = u / per_group, part_of = u % per_group;
         const int64_t r0 = group * p.rows_per_gate + p.rows_per_gate * part_of / per_group;
         const int64_t r1 = group * p.rows_per_gate + p.rows_per_gate * (part_of + 1) / per_group;
-        float gate[8], acc_gate[8];
-        weight.load(p.gate + group * p.cols, first, step, cols, p.gate != nullptr);
+        auto copy = [&](int64_t row, int stage) {
+            if (row < r1) {
+                uint8_t* const at = mine_r + stage * stage_bytes;
+                uint8_t* const to = mine_a + stage * stage_bytes;
+                if (pre) {
+                    Staged<TR, V>::copy(at, static_cast<const TR*>(p.out) + row * p.ld_out, first, step, cols);
+                    Staged<TA, V>::copy(to, static_cast<const TA*>(p.dh) + row * p.ld_dh, first, step, cols);
+                }
+                if (more) Staged<TR, V>::copy(at + of_r, static_cast<const TR*>(p.dout) + row * p.ld_dout, first, step, cols);
+                if (block) Staged<TA, V>::copy(to + of_a, static_cast<const TA*>(p.y) + row * p.ld_y, first, step, cols);
+            }
+            commit_copies();
+        };
+        int stage = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) { gate[i] = p.gate != nullptr ? weight.at(i) : 1.0f; acc_gate[i] = 0.0f; }
-        if (r0 < r1) load(r0);
+        for (int i = 0; i + 1 < kDepth; ++i) copy(r0 + i, i);
+        // k = scale gate w_post
+        float k[8], sum_gc[8];
+        Eight<float, V> gate;
+        gate.load(p.gate + group * p.cols, first, step, cols, p.gate != nullptr);
+        weight.load(p.w_post, first, step, cols, post);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            k[i] = p.scale * (p.gate != nullptr ? gate.at(i) : 1.0f) * (post ? weight.at(i) : 1.0f);
+            sum_gc[i] = 0.0f;
+        }
         for (int64_t row = r0; row < r1; ++row) {
-            const BwdRow<TR, TA, V> now = next;
-            if (row + 1 < r1) load(row + 1);
+            copy(row + kDepth - 1, stage == 0 ? kDepth - 1 : stage - 1);
+            const float r_pre = pre ? p.rstd_pre[row] : 0.0f, r_post = block && post ? p.rstd_post[row] : 1.0f;
+            wait_copies<kDepth - 1>();
+            const uint8_t* const at = mine_r + stage * stage_bytes;
+            const uint8_t* const from = mine_a + stage * stage_bytes;
+            if (++stage == kDepth) stage = 0;
+            float out[8], y[8], q[8];   // q = dout + rstd_pre a
             float s_ab = 0.0f, s_eg = 0.0f, s_eb = 0.0f;
+            {
+                Eight<TR, V> o, d;
+                Eight<TA, V> h, v;
+                Staged<TR, V>::get(o, at);
+                Staged<TR, V>::get(d, at + of_r);
+                Staged<TA, V>::get(h, from);
+                Staged<TA, V>::get(v, from + of_a);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float a = now.dh.at(i) * w_pre[i], b = now.out.at(i) * now.r_pre;
-                s_ab = fmaf(a, b, s_ab);
-                const float ec = gate[i] * e_w[i] * now.y.at(i);
-                s_eg = fmaf(ec, fmaf(now.r_pre, a, now.dout.at(i)), s_eg);
-                s_eb = fmaf(ec, b, s_eb);
+                for (int i = 0; i < 8; ++i) {
+                    out[i] = o.at(i);
+                    y[i] = v.at(i);
+                    const float hr = h.at(i) * r_pre, ar = hr * w_pre[i];
+                    q[i] = d.at(i) + ar;
+                    acc_pre[i] = fmaf(hr, out[i], acc_pre[i]);
+                    s_ab = fmaf(ar, out[i], s_ab);   // the sum of a b
+                    const float ky = k[i] * y[i];    // e c without rstd_post
+                    s_eg = fmaf(ky, q[i], s_eg);
+                    s_eb = fmaf(ky, out[i], s_eb);   // and without rstd_pre
+                }
             }
             s_ab = warp_sum(s_ab);
-            s_eg = warp_sum(s_eg);
-            s_eb = warp_sum(s_eb);
+            if (block && post) {
+                s_eg = warp_sum(s_eg);
+                s_eb = warp_sum(s_eb);
+            }
             if (CLUSTER || warps > 1) {
                 // two turns of sums: whoever writes a third has seen everybody read the first
-                float (*mine)[3] = part[turn];
+                float4* const mine = part[turn];
                 turn ^= 1;
                 const int lane = threadIdx.x & 31, w = rank * warps + (threadIdx.x >> 5);
                 if (CLUSTER) {
                     if (lane < ranks) {
-                        const uint32_t at = ptx::mapa_shared(ptx::smem_u32(&mine[w][0]), static_cast<uint32_t>(lane));
-                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(s_ab) : "memory");
-                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at + 4), "f"(s_eg) : "memory");
-                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at + 8), "f"(s_eb) : "memory");
+                        const uint32_t to = ptx::mapa_shared(ptx::smem_u32(&mine[w]), static_cast<uint32_t>(lane));
+                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(s_ab) : "memory");
+                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4), "f"(s_eg) : "memory");
+                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 8), "f"(s_eb) : "memory");
                     }
                     __syncwarp();
                     ptx::cluster_sync_all();
                 } else {
-                    if (lane == 0) { mine[w][0] = s_ab; mine[w][1] = s_eg; mine[w][2] = s_eb; }
+                    if (lane == 0) mine[w] = make_float4(s_ab, s_eg, s_eb, 0.0f);
                     __syncthreads();
                 }
                 s_ab = s_eg = s_eb = 0.0f;
-                for (int i = 0; i < ranks * warps; ++i) { s_ab += mine[i][0]; s_eg += mine[i][1]; s_eb += mine[i][2]; }
+                for (int i = 0; i < ranks * warps; ++i) {
+                    const float4 v = mine[i];
+                    s_ab += v.x;
+                    s_eg += v.y;
+                    s_eb += v.z;
+                }
             }
-            const float m_ab = s_ab * of;
-            // mean(e g c), with the factors that a row shares (scale, rstd_post) outside
-            const float m_eg = p.scale * now.r_post * of * fmaf(-now.r_pre * m_ab, s_eb, s_eg);
+            // g = q - out rstd_pre^2 mean(a b);   dy = rstd_post (k g - y rstd_post^2 mean(k g y))
+            const float m_ab = s_ab * of * r_pre * r_pre;
+            const float m_eg = post ? r_post * r_post * r_post * of * fmaf(-m_ab, s_eb, s_eg) : 0.0f;
             Eight<TR, V> dx;
             Eight<TA, V> dy;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float dh = now.dh.at(i), b = now.out.at(i) * now.r_pre;
-                const float g = fmaf(now.r_pre, fmaf(-b, m_ab, dh * w_pre[i]), now.dout.at(i));
-                dx.put(i, g);
-                acc_pre[i] = fmaf(dh, b, acc_pre[i]);
-                const float c = now.y.at(i) * now.r_post, kg = p.scale * gate[i] * g;
-                acc_post[i] = fmaf(kg, c, acc_post[i]);
-                acc_gate[i] = fmaf(p.scale * g, c * e_w[i], acc_gate[i]);
-                dy.put(i, post ? now.r_post * fmaf(-c, m_eg, kg * e_w[i]) : kg);
+                q[i] = fmaf(-out[i], m_ab, q[i]);
+                const float gr = q[i] * r_post;
+                sum_gc[i] = fmaf(gr, y[i], sum_gc[i]);
+                y[i] = fmaf(-y[i], m_eg, k[i] * gr);
             }
+            dx.put(q);
+            dy.put(y);
             dx.store(static_cast<TR*>(p.dx) + row * p.ld_dx, first, step, cols);
             if (block) dy.store(static_cast<TA*>(p.dy) + row * p.ld_dy, first, step, cols);
         }
-        if (p.part_gate != nullptr) {
+        wait_copies<0>();   // the next unit's copies start anew
+        if (p.part_gc != nullptr) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) weight.put(i, acc_gate[i]);
-            weight.store(p.part_gate + static_cast<int64_t>(u) * p.cols, first, step, cols);
+            for (int i = 0; i < 8; ++i) weight.put(i, sum_gc[i]);
+            weight.store(p.part_gc + static_cast<int64_t>(u) * p.cols, first, step, cols);
         }
     }
     if (p.part_w != nullptr) {
-        float* to = p.part_w + static_cast<int64_t>(me) * 2 * p.cols;
 #pragma unroll
         for (int i = 0; i < 8; ++i) weight.put(i, acc_pre[i]);
-        weight.store(to, first, step, cols);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) weight.put(i, acc_post[i]);
-        weight.store(to + p.cols, first, step, cols);
+        weight.store(p.part_w + static_cast<int64_t>(me) * p.cols, first, step, cols);
     }
 }
 
 // Sums of the blocks' rows in a fixed order: blockIdx.y 0 -> dw_pre, 1 -> dw_post, 2 + g -> dgate of group g.
-constexpr int kSumCols = 32, kSumWays = 16;
-__global__ void __launch_bounds__(kSumCols * kSumWays) norm_residual_sums_kernel(NormResidualParams p, int blocks, int64_t groups, int per_group, float beta) {
+constexpr int kSumCols = 16, kSumWays = 32;
+__global__ void __launch_bounds__(kSumCols * kSumWays) norm_residual_sums_kernel(NormResidualParams p, int blocks, int units, int64_t groups, int per_group, float beta) {
     __shared__ float part[kSumWays][kSumCols];
     ptx::grid_dependency_wait();
     const int lane = threadIdx.x % kSumCols, way = threadIdx.x / kSumCols;
@@ -293,17 +427,25 @@ __global__ void __launch_bounds__(kSumCols * kSumWays) norm_residual_sums_kernel
     for (int64_t what = blockIdx.y; what < 2 + groups; what += gridDim.y) {
         float* to = what == 0 ? p.dw_pre : what == 1 ? p.dw_post : p.dgate;
         if (to == nullptr) continue;
-        const float* from = what < 2 ? p.part_w + what * p.cols : p.part_gate + (what - 2) * per_group * p.cols;
-        const int64_t pitch = what < 2 ? 2 * static_cast<int64_t>(p.cols) : p.cols;
-        const int n = what < 2 ? blocks : per_group;
+        const float* from = what == 0 ? p.part_w : p.part_gc + (what == 1 ? 0 : (what - 2) * per_group * p.cols);
+        const int n = what == 0 ? blocks : what == 1 ? units : per_group;
         float s = 0.0f;
-        if (col < p.cols)
-            for (int i = way; i < n; i += kSumWays) s += from[i * pitch + col];
+        if (col < p.cols) {
+            if (what == 1 && p.gate != nullptr) {
+#pragma unroll 4
+                for (int i = way; i < n; i += kSumWays) s = fmaf(p.gate[i / per_group * static_cast<int64_t>(p.cols) + col], from[i * static_cast<int64_t>(p.cols) + col], s);
+            } else {
+#pragma unroll 8
+                for (int i = way; i < n; i += kSumWays) s += from[i * static_cast<int64_t>(p.cols) + col];
+            }
+        }
         part[way][lane] = s;
         __syncthreads();
         if (way == 0 && col < p.cols) {
 #pragma unroll
             for (int i = 1; i < kSumWays; ++i) s += part[i][lane];
+            if (what > 0) s *= p.scale;
+            if (what > 1 && p.w_post != nullptr) s *= p.w_post[col];
             to += what < 2 ? col : (what - 2) * p.cols + col;
             *to = beta == 0.0f ? s : fmaf(beta, *to, s);
         }
@@ -313,16 +455,42 @@ __global__ void __launch_bounds__(kSumCols * kSumWays) norm_residual_sums_kernel
 
 // ------------------------------------------------------------------------------------------------------------- launches
 
-template <typename TR, typename TA, int V, int NV>
-cudaError_t fwd_rows(const NormResidualParams& p, cudaStream_t stream) {
-    const int warps = (p.cols + V * NV * 32 - 1) / (V * NV * 32);
-    const int64_t blocks = warps == 1 ? (p.rows + kFwdRows - 1) / kFwdRows : p.rows;
-    return launch_dependent(norm_residual_fwd_kernel<TR, TA, V, NV>, static_cast<unsigned>(blocks), 32u * (warps == 1 ? kFwdRows : warps), stream, p, warps);
+// Blocks that share an SM, by its threads, shared memory and registers (`regs` a thread).
+int blocks_per_sm(int warps, size_t smem, int regs) {
+    const int by_threads = 64 / warps, by_smem = static_cast<int>((200u << 10) / (smem + 2048)), by_regs = 65536 / (warps * 32 * regs);
+    int n = by_threads < by_smem ? by_threads : by_smem;
+    n = n < by_regs ? n : by_regs;
+    return n < 1 ? 1 : n > 16 ? 16 : n;
+}
+
+template <typename TR, typename TA, int V, int N>
+cudaError_t fwd_rows(const NormResidualParams& p, int sms, cudaStream_t stream) {
+    const int warps = (p.cols + N * 256 - 1) / (N * 256);
+    const size_t smem = static_cast<size_t>(fwd_depth<TR, TA, N>()) * N * warps * 256 * (sizeof(TR) + sizeof(TA));
+    auto kernel = norm_residual_fwd_kernel<TR, TA, V, N>;
+    if (smem > 40 * 1024) {   // with what a block has beside it, 48 KB is the limit
+        const cudaError_t set = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (set != cudaSuccess) return set;
+    }
+    const int64_t most = static_cast<int64_t>(sms) * blocks_per_sm(warps, smem, N == 1 ? 72 : 128);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(p.rows < most ? p.rows : most));
+    cfg.blockDim = dim3(32u * warps);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+    count_launch(1);
+    return e != cudaSuccess ? e : cudaGetLastError();
 }
 template <typename TR, typename TA>
-cudaError_t fwd_typed(const NormResidualParams& p, bool wide, cudaStream_t stream) {
-    if (wide) return p.cols <= 256 ? fwd_rows<TR, TA, 8, 1>(p, stream) : p.cols <= 1024 ? fwd_rows<TR, TA, 8, 2>(p, stream) : fwd_rows<TR, TA, 8, 4>(p, stream);
-    return p.cols <= 2048 ? fwd_rows<TR, TA, 1, 8>(p, stream) : fwd_rows<TR, TA, 1, 32>(p, stream);
+cudaError_t fwd_typed(const NormResidualParams& p, bool wide, int sms, cudaStream_t stream) {
+    if (wide) return p.cols <= kMostCols ? fwd_rows<TR, TA, 8, 1>(p, sms, stream) : p.cols <= 2 * kMostCols ? fwd_rows<TR, TA, 8, 2>(p, sms, stream) : fwd_rows<TR, TA, 8, 4>(p, sms, stream);
+    return p.cols <= kMostCols ? fwd_rows<TR, TA, 1, 1>(p, sms, stream) : p.cols <= 2 * kMostCols ? fwd_rows<TR, TA, 1, 2>(p, sms, stream) : fwd_rows<TR, TA, 1, 4>(p, sms, stream);
 }
 
 template <typename TR, typename TA>
@@ -336,11 +504,17 @@ cudaError_t bwd_typed(const NormResidualParams& p, const NormResidualPlan& pl, b
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(pl.blocks * pl.cluster));
     cfg.blockDim = dim3(32u * pl.warps);
+    cfg.dynamicSmemBytes = static_cast<size_t>(bwd_depth<TR, TA>()) * pl.warps * 512 * (sizeof(TR) + sizeof(TA));
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = pl.cluster > 1 ? 2 : 1;
-    auto kernel = pl.cluster > 1 ? (wide ? norm_residual_bwd_kernel<TR, TA, 8, true> : norm_residual_bwd_kernel<TR, TA, 1, true>)
-                                 : (wide ? norm_residual_bwd_kernel<TR, TA, 8, false> : norm_residual_bwd_kernel<TR, TA, 1, false>);
+    auto kernel = pl.cluster > 1 ? (wide ? norm_residual_bwd_kernel<TR, TA, 8, true, 16> : norm_residual_bwd_kernel<TR, TA, 1, true, 16>)
+                  : pl.warps > 8 ? (wide ? norm_residual_bwd_kernel<TR, TA, 8, false, 16> : norm_residual_bwd_kernel<TR, TA, 1, false, 16>)
+                                 : (wide ? norm_residual_bwd_kernel<TR, TA, 8, false, 8> : norm_residual_bwd_kernel<TR, TA, 1, false, 8>);
+    if (cfg.dynamicSmemBytes > 40 * 1024) {
+        const cudaError_t set = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(cfg.dynamicSmemBytes));
+        if (set != cudaSuccess) return set;
+    }
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p, pl.units, pl.per_group);
     count_launch(1);
     return e != cudaSuccess ? e : cudaGetLastError();
@@ -348,17 +522,17 @@ cudaError_t bwd_typed(const NormResidualParams& p, const NormResidualPlan& pl, b
 
 }  // namespace
 
-int norm_residual_max_cols() { return 4 * kBwdCols; }
+int norm_residual_max_cols() { return 4 * kMostCols; }
 
-NormResidualPlan norm_residual_plan(int64_t rows, int64_t cols, int64_t groups, bool want_w, bool want_gate, int sms) {
+NormResidualPlan norm_residual_plan(int64_t rows, int64_t cols, int64_t groups, int row_bytes, bool want_pre, bool want_gc, int sms) {
     NormResidualPlan pl{};
-    pl.cluster = static_cast<int>((cols + kBwdCols - 1) / kBwdCols);
+    pl.cluster = static_cast<int>((cols + kMostCols - 1) / kMostCols);
     pl.warps = static_cast<int>((cols + pl.cluster * 256 - 1) / (pl.cluster * 256));
     // Blocks that share an SM hide each other's row sums; each of them leaves a row of sums behind, so none takes less
-    // than eight rows while every SM has one.
-    int64_t most = static_cast<int64_t>(sms) * (pl.warps <= 8 ? (16 / pl.warps > 8 ? 8 : 16 / pl.warps) : 1) / pl.cluster;
+    // than two rows while every SM has one (1537 x 771 with eight: 52 us, with two NUMBER).
+    int64_t most = static_cast<int64_t>(sms) * blocks_per_sm(pl.warps, static_cast<size_t>(row_bytes == 16 ? 3 : 4) * pl.warps * 256 * row_bytes, pl.warps > 8 ? 128 : 80) / pl.cluster;
     if (most < 1) most = 1;
-    const int64_t few = (rows + 7) / 8 > sms ? (rows + 7) / 8 : sms;
+    const int64_t few = (rows + 1) / 2 > sms ? (rows + 1) / 2 : sms;
     if (most > few) most = few;
     if (most > rows) most = rows;
     const int64_t per_group_rows = rows / groups;
@@ -368,14 +542,14 @@ NormResidualPlan norm_residual_plan(int64_t rows, int64_t cols, int64_t groups, 
     pl.units = static_cast<int>(groups * per_group);
     pl.blocks = static_cast<int>(pl.units < most ? pl.units : most);
     if (pl.blocks < 1) pl.blocks = 1;
-    pl.floats_w = want_w ? 2 * cols * pl.blocks : 0;
-    pl.floats_gate = want_gate ? cols * pl.units : 0;
+    pl.floats_w = want_pre ? cols * pl.blocks : 0;
+    pl.floats_gc = want_gc ? cols * pl.units : 0;
     return pl;
 }
 
-cudaError_t launch_norm_residual_fwd(const NormResidualParams& p, int res_bf16, int act_bf16, bool wide, cudaStream_t stream) {
-    if (res_bf16) return fwd_typed<__nv_bfloat16, __nv_bfloat16>(p, wide, stream);
-    return act_bf16 ? fwd_typed<float, __nv_bfloat16>(p, wide, stream) : fwd_typed<float, float>(p, wide, stream);
+cudaError_t launch_norm_residual_fwd(const NormResidualParams& p, int res_bf16, int act_bf16, bool wide, int sms, cudaStream_t stream) {
+    if (res_bf16) return fwd_typed<__nv_bfloat16, __nv_bfloat16>(p, wide, sms, stream);
+    return act_bf16 ? fwd_typed<float, __nv_bfloat16>(p, wide, sms, stream) : fwd_typed<float, float>(p, wide, sms, stream);
 }
 
 cudaError_t launch_norm_residual_bwd(const NormResidualParams& p, const NormResidualPlan& pl, int res_bf16, int act_bf16, bool wide, float beta,
@@ -383,11 +557,11 @@ cudaError_t launch_norm_residual_bwd(const NormResidualParams& p, const NormResi
     cudaError_t e = res_bf16   ? bwd_typed<__nv_bfloat16, __nv_bfloat16>(p, pl, wide, stream)
                     : act_bf16 ? bwd_typed<float, __nv_bfloat16>(p, pl, wide, stream)
                                : bwd_typed<float, float>(p, pl, wide, stream);
-    if (e != cudaSuccess || (p.part_w == nullptr && p.part_gate == nullptr)) return e;
-    const int64_t groups = p.part_gate != nullptr ? pl.units / pl.per_group : 0;
+    if (e != cudaSuccess || (p.part_w == nullptr && p.part_gc == nullptr)) return e;
+    const int64_t groups = p.dgate != nullptr ? pl.units / pl.per_group : 0;
     const unsigned down = static_cast<unsigned>(2 + groups < 1024 ? 2 + groups : 1024);
     return launch_dependent(norm_residual_sums_kernel, dim3(static_cast<unsigned>((p.cols + kSumCols - 1) / kSumCols), down), kSumCols * kSumWays, stream,
-                            p, pl.blocks, groups, pl.per_group, beta);
+                            p, pl.blocks, pl.units, groups, pl.per_group, beta);
 }
 
 }  // namespace llmt_b200
