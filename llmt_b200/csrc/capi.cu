@@ -1810,8 +1810,8 @@ int llmt_b200_rope(const llmt_b200_rope_desc* d, void* stream) {
                     (long long)d->tokens, (long long)d->heads, (long long)d->head_dim, (long long)d->rot_dim);
     if (d->dtype != LLMT_B200_FP32 && d->dtype != LLMT_B200_BF16)
         return fail(LLMT_B200_ERR_UNSUPPORTED, "rope: no kernel for dtype code %d", d->dtype);
-    if (d->head_dim > 1024 || d->heads > 65536 || d->batch > 0x7fffffff || d->tokens > 0x7fffffff || d->batch * d->tokens > 0x3fffffff8ll)
-        return fail(LLMT_B200_ERR_UNSUPPORTED, "rope: head_dim above 1024, heads above 65536 or tokens above 2^34 - 8");
+    if (d->head_dim > 1024 || d->heads > 65536 || d->batch > 0x7fffffff || d->tokens > 0x7fffffff || d->batch * ((d->tokens + 7) / 8) > 0x7fffffff)
+        return fail(LLMT_B200_ERR_UNSUPPORTED, "rope: head_dim above 1024, heads above 65536 or more than 2^31 - 1 blocks of eight tokens");
     if (d->batch == 0 || d->tokens == 0 || d->heads == 0) return LLMT_B200_OK;
     if (d->x.data == nullptr || d->y.data == nullptr || (d->rot_dim > 0 && d->freqs == nullptr))
         return fail(LLMT_B200_ERR_INVALID, "rope: invalid tensor (null data)");
@@ -1830,11 +1830,11 @@ int llmt_b200_rope(const llmt_b200_rope_desc* d, void* stream) {
     p.x_batch = x.stride_batch; p.x_token = x.stride_token; p.x_head = x.stride_head;
     p.y_batch = y.stride_batch; p.y_token = y.stride_token; p.y_head = y.stride_head;
     p.freqs = d->freqs; p.positions = d->positions; p.offset = d->offset;
-    p.tokens = d->tokens; p.total = d->batch * d->tokens;
+    p.batch = d->batch; p.tokens = d->tokens;
     p.heads = static_cast<int32_t>(d->heads); p.head_dim = static_cast<int32_t>(d->head_dim); p.rot = static_cast<int32_t>(d->rot_dim);
     p.interleaved = d->interleaved != 0; p.inverse = d->inverse != 0; p.copy_rest = !same;
     p.scale = d->scale;
-    const cudaError_t e = launch_rope(p, d->dtype == LLMT_B200_BF16, static_cast<cudaStream_t>(stream));
+    const cudaError_t e = launch_rope(p, d->dtype == LLMT_B200_BF16, sm_count(), static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return fail(LLMT_B200_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
     return LLMT_B200_OK;
 }

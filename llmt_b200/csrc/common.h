@@ -230,10 +230,11 @@ struct RopeParams {
     int64_t x_batch, x_token, x_head, y_batch, y_token, y_head;
     const double* freqs;       // radians per token, [rot / 2]
     const int32_t* positions;  // [batch * tokens], or null: offset + the token's index
-    int64_t offset, tokens, total;   // tokens of a sequence, of all sequences
+    int64_t offset, batch, tokens;   // tokens of each sequence
     int32_t heads, head_dim, rot;
     int32_t interleaved, inverse, copy_rest;   // copy_rest: y is not x, the values behind the rotated ones move too
-    int32_t per_block;
+    int32_t per_block;          // tokens of a block
+    int64_t blocks_per_sequence;
     float scale;
 };
 
@@ -380,7 +381,7 @@ cudaError_t launch_ce_grad_rows(void* out, const float* lse, const float* mask, 
 cudaError_t launch_lse_from_stats(float* lse, const void* stats, int64_t rows, int parts, cudaStream_t stream);
 cudaError_t launch_rowdot(float* out, const void* x, const void* y, int64_t rows, int64_t cols, int64_t ldx,
                           int64_t ldy, int is_bf16, cudaStream_t stream);
-cudaError_t launch_rope(RopeParams p, int is_bf16, cudaStream_t stream);
+cudaError_t launch_rope(RopeParams p, int is_bf16, int sms, cudaStream_t stream);
 int norm_residual_max_cols(void);
 // row_bytes: of one column in the four tensors that the backward pass reads
 NormResidualPlan norm_residual_plan(int64_t rows, int64_t cols, int64_t groups, int row_bytes, bool want_pre, bool want_gc, int sms);

@@ -129,8 +129,8 @@ constexpr int kMostCols = kMostWarps * 32 * 8;  // columns that a block owns eig
 
 // ------------------------------------------------------------------------------------------------------------ forward
 
-// Rows in shared memory, the one at work among them: three, or what 200 KB hold of rows of more than 8192 columns.
-template <typename TR, typename TA, int N> constexpr int fwd_depth() { return N < 4 ? 3 : sizeof(TR) + sizeof(TA) == 8 ? 1 : sizeof(TR) + sizeof(TA) == 6 ? 2 : 3; }
+// Rows in shared memory, the one at work among them: two (three were no faster: 38 and 37 us at 8192 x 1600), or what 200 KB hold of rows of more than 8192 columns.
+template <typename TR, typename TA, int N> constexpr int fwd_depth() { return N < 4 ? 2 : sizeof(TR) + sizeof(TA) == 8 ? 1 : 2; }
 // N: eights of columns of a thread, `threads` * 8 columns apart.
 template <typename TR, typename TA, int V, int N>
 __global__ void __launch_bounds__(kMostWarps * 32) norm_residual_fwd_kernel(NormResidualParams p) {
@@ -529,7 +529,7 @@ NormResidualPlan norm_residual_plan(int64_t rows, int64_t cols, int64_t groups, 
     pl.cluster = static_cast<int>((cols + kMostCols - 1) / kMostCols);
     pl.warps = static_cast<int>((cols + pl.cluster * 256 - 1) / (pl.cluster * 256));
     // Blocks that share an SM hide each other's row sums; each of them leaves a row of sums behind, so none takes less
-    // than two rows while every SM has one (1537 x 771 with eight: 52 us, with two NUMBER).
+    // than two rows while every SM has one (1537 x 771 backward with sixteen rows or more each: 31 us, with two 19).
     int64_t most = static_cast<int64_t>(sms) * blocks_per_sm(pl.warps, static_cast<size_t>(row_bytes == 16 ? 3 : 4) * pl.warps * 256 * row_bytes, pl.warps > 8 ? 128 : 80) / pl.cluster;
     if (most < 1) most = 1;
     const int64_t few = (rows + 1) / 2 > sms ? (rows + 1) / 2 : sms;
