@@ -502,12 +502,13 @@ LLMT_B200_API uint64_t llmt_b200_norm_residual_workspace_bytes(const llmt_b200_n
  *   summed over the heads that share them, in a fixed order.
  *   head_dim is a multiple of 8, at most 128; bases are 16-byte aligned and strides multiples of 8
  *   elements, not 0 (an operand cannot be broadcast).  Results must not overlap one another or
- *   anything that is read.  scale is positive.
+ *   anything that is read.  scale is positive.  batch * heads * max(tokens_q, tokens_k) < 2^31.
  *   lse  fp32 [batch, heads, tokens_q]: written by _fwd (NULL: not wanted), read by _bwd.
  *
- * _bwd: dV = P^T dO,  dS = P (dP - D) with dP = dO v^T,  dQ = scale dS k,  dK = scale dS^T q, from out and lse
- * as _fwd left them.  D = rowsum(P dP) is taken as rowsum(dO out) for dQ; a row of dS adds up to nothing but
- * for the rounding of out, which is taken out of D again before dK is formed.  workspace: 16-byte aligned, llmt_b200_attention_window_workspace_bytes(desc) bytes.
+ * _bwd: dV = P^T dO,  dS = P (dP - D) with dP = dO v^T,  dQ = scale dS k,  dK = scale dS^T q, from out and
+ * lse as _fwd left them.  D = rowsum(P dP) is taken as rowsum(dO out) for dQ; a row of dS adds up to nothing
+ * but for the rounding of out, which is taken out of D again before dK is formed.  workspace: 16-byte
+ * aligned, llmt_b200_attention_window_workspace_bytes(desc) bytes.
  *
  * _decode: one new token per sequence (tokens_q = 1) over a cache of tokens_k places, of which
  * sequence b holds lengths[b] (device, int32; NULL: all; values beyond tokens_k count as tokens_k,

@@ -1,4 +1,6 @@
-// Causal attention with a sliding window and sinks, forward, backward and for one new token: a warp for each row.
+// Causal attention with a sliding window and sinks where there are no queries or no keys, a warp for each row: a forward pass
+// over no keys (zeros and -inf), its gradient, and the keys' gradients without queries (zeros).  No tensor map describes a
+// tensor without tokens; everything else is in the tiled kernels.
 #include "attention_rows.cuh"
 #include "ptx_sm100.cuh"
 

@@ -1824,6 +1824,9 @@ int llmt_b200_rope(const llmt_b200_rope_desc* d, void* stream) {
     if (!view_distinct(y, d->batch, d->tokens, d->heads, d->head_dim)) return fail(LLMT_B200_ERR_INVALID, "rope: y's elements overlap one another");
     const bool same = x.data == y.data && x.stride_batch == y.stride_batch && x.stride_token == y.stride_token && x.stride_head == y.stride_head;
     if (!same && overlaps(x.data, ex * es, y.data, ey * es)) return fail(LLMT_B200_ERR_INVALID, "rope: y must be x or not overlap it");
+    if ((d->rot_dim > 0 && overlaps(y.data, ey * es, d->freqs, d->rot_dim / 2 * 8)) ||
+        (d->positions != nullptr && overlaps(y.data, ey * es, d->positions, static_cast<size_t>(d->batch) * d->tokens * 4)))
+        return fail(LLMT_B200_ERR_INVALID, "rope: y overlaps freqs or positions");
     if (same && d->rot_dim == 0) return LLMT_B200_OK;
     RopeParams p{};
     p.x = x.data; p.y = y.data;
@@ -1873,6 +1876,14 @@ int norm_residual_row_bytes(const llmt_b200_norm_residual_desc* d) {
     return 2 * ((d->dtype_res == LLMT_B200_BF16 ? 2 : 4) + (d->dtype_act == LLMT_B200_BF16 ? 2 : 4));
 }
 
+// An fp32 array of a norm_residual call: weights, statistics, their gradients.
+struct FloatArray {
+    const char* name;
+    const float* data;
+    int64_t n;
+    bool written;
+};
+
 // A [rows, cols] tensor of a norm_residual call.
 struct RowTensor {
     const char* name;
@@ -1902,6 +1913,23 @@ int norm_residual_tensors(const llmt_b200_norm_residual_desc* d, const char* who
     return LLMT_B200_OK;
 }
 
+// That no array which is written overlaps another or a tensor, and no tensor which is written overlaps an array.
+int norm_residual_arrays(const llmt_b200_norm_residual_desc* d, const char* who, const FloatArray* f, int n, const RowTensor* t, int nt) {
+    for (int i = 0; i < n; ++i) {
+        if (f[i].data == nullptr) continue;
+        for (int j = 0; j < n; ++j)
+            if (i != j && f[i].written && f[j].data != nullptr && overlaps(f[i].data, 4 * f[i].n, f[j].data, 4 * f[j].n))
+                return fail(LLMT_B200_ERR_INVALID, "%s: %s overlaps %s", who, f[i].name, f[j].name);
+        for (int j = 0; j < nt && d->rows > 0; ++j) {
+            if (t[j].data == nullptr || !(f[i].written || t[j].written)) continue;
+            const size_t es = (t[j].act ? d->dtype_act : d->dtype_res) == LLMT_B200_BF16 ? 2 : 4;
+            if (overlaps(f[i].data, 4 * f[i].n, t[j].data, (static_cast<size_t>(d->rows - 1) * t[j].ld + d->cols) * es))
+                return fail(LLMT_B200_ERR_INVALID, "%s: %s overlaps %s", who, f[i].name, t[j].name);
+        }
+    }
+    return LLMT_B200_OK;
+}
+
 }  // namespace
 
 int llmt_b200_norm_residual_fwd(const llmt_b200_norm_residual_desc* d, void* stream) {
@@ -1916,6 +1944,11 @@ int llmt_b200_norm_residual_fwd(const llmt_b200_norm_residual_desc* d, void* str
                             {"out", d->y != nullptr ? d->out : nullptr, d->ld_out, false, true}, {"h", d->h, d->ld_h, true, true}};
     bool wide = d->cols % 8 == 0 && !misaligned(d->w_post, 16) && !misaligned(d->gate, 16) && !misaligned(d->w_pre, 16);
     st = norm_residual_tensors(d, who, t, 4, d->x, d->out, &wide);
+    if (st != LLMT_B200_OK) return st;
+    const FloatArray f[5] = {{"w_post", d->w_post, d->cols, false}, {"gate", d->gate, d->groups * d->cols, false}, {"w_pre", d->w_pre, d->cols, false},
+                             {"rstd_post", d->w_post != nullptr ? d->rstd_post : nullptr, d->rows, true},
+                             {"rstd_pre", d->w_pre != nullptr ? d->rstd_pre : nullptr, d->rows, true}};
+    st = norm_residual_arrays(d, who, f, 5, t, 4);
     if (st != LLMT_B200_OK) return st;
     const cudaError_t e = launch_norm_residual_fwd(p, d->dtype_res == LLMT_B200_BF16, d->dtype_act == LLMT_B200_BF16, wide, sm_count(), static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return fail(LLMT_B200_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
@@ -1953,24 +1986,16 @@ int llmt_b200_norm_residual_bwd(const llmt_b200_norm_residual_desc* d, void* str
         st = norm_residual_tensors(d, who, t, 6, d->dx, d->dout, &wide);
         if (st != LLMT_B200_OK) return st;
     }
-    // what is summed over the rows: written apart from everything that is read, and from one another
-    struct { const char* name; const float* data; int64_t n; } sums[3] = {{"dw_post", d->dw_post, d->cols}, {"dgate", d->dgate, d->groups * d->cols}, {"dw_pre", d->dw_pre, d->cols}};
-    struct { const char* name; const float* data; int64_t n; } read[5] = {{"w_post", d->w_post, d->cols}, {"gate", d->gate, d->groups * d->cols}, {"w_pre", d->w_pre, d->cols},
-                                                                          {"rstd_post", d->rstd_post, d->rows}, {"rstd_pre", d->rstd_pre, d->rows}};
-    for (int i = 0; i < 3; ++i) {
-        if (sums[i].data == nullptr) continue;
-        for (int j = 0; j < 5; ++j)
-            if (read[j].data != nullptr && overlaps(sums[i].data, 4 * sums[i].n, read[j].data, 4 * read[j].n))
-                return fail(LLMT_B200_ERR_INVALID, "%s: %s overlaps %s", who, sums[i].name, read[j].name);
-        for (int j = 0; j < i; ++j)
-            if (sums[j].data != nullptr && overlaps(sums[i].data, 4 * sums[i].n, sums[j].data, 4 * sums[j].n))
-                return fail(LLMT_B200_ERR_INVALID, "%s: %s overlaps %s", who, sums[i].name, sums[j].name);
-    }
+    const FloatArray f[8] = {{"dw_post", d->dw_post, d->cols, true}, {"dgate", d->dgate, d->groups * d->cols, true}, {"dw_pre", d->dw_pre, d->cols, true},
+                             {"w_post", d->w_post, d->cols, false}, {"gate", d->gate, d->groups * d->cols, false}, {"w_pre", d->w_pre, d->cols, false},
+                             {"rstd_post", d->rstd_post, d->rows, false}, {"rstd_pre", d->rstd_pre, d->rows, false}};
+    st = norm_residual_arrays(d, who, f, 8, t, 6);
+    if (st != LLMT_B200_OK) return st;
     const NormResidualPlan pl = norm_residual_plan(d->rows, d->cols, d->groups, norm_residual_row_bytes(d), d->dw_pre != nullptr, d->dw_post != nullptr || d->dgate != nullptr, sm_count());
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (d->rows == 0) {   // sums of nothing
-        for (const auto& g : sums) {
-            if (g.data == nullptr || d->beta == 1.0f) continue;
+        for (const FloatArray& g : f) {
+            if (!g.written || g.data == nullptr || d->beta == 1.0f) continue;
             if (d->beta != 0.0f) return fail(LLMT_B200_ERR_UNSUPPORTED, "%s: beta other than 0 and 1 with no rows", who);
             const cudaError_t e = launch_zero_f32(const_cast<float*>(g.data), g.n, s);
             if (e != cudaSuccess) return fail(LLMT_B200_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
@@ -1988,9 +2013,7 @@ int llmt_b200_norm_residual_bwd(const llmt_b200_norm_residual_desc* d, void* str
             if (x.data != nullptr && overlaps(d->workspace, need, x.data, (static_cast<size_t>(d->rows - 1) * x.ld + d->cols) * es))
                 return fail(LLMT_B200_ERR_INVALID, "%s: workspace overlaps %s", who, x.name);
         }
-        for (const auto& x : sums)
-            if (x.data != nullptr && overlaps(d->workspace, need, x.data, 4 * x.n)) return fail(LLMT_B200_ERR_INVALID, "%s: workspace overlaps %s", who, x.name);
-        for (const auto& x : read)
+        for (const FloatArray& x : f)
             if (x.data != nullptr && overlaps(d->workspace, need, x.data, 4 * x.n)) return fail(LLMT_B200_ERR_INVALID, "%s: workspace overlaps %s", who, x.name);
         p.part_w = pl.floats_w > 0 ? static_cast<float*>(d->workspace) : nullptr;
         p.part_gc = pl.floats_gc > 0 ? static_cast<float*>(d->workspace) + (pl.floats_w + 3) / 4 * 4 : nullptr;
@@ -2025,10 +2048,10 @@ int attention_params(const llmt_b200_attention_desc* d, const char* who, Attenti
     constexpr int64_t kMaxDim = 0x7fffffff - 1024;
     if (d->tokens_q > kMaxDim || d->tokens_k > kMaxDim || d->batch > kMaxDim || d->heads > 65536)
         return fail(LLMT_B200_ERR_UNSUPPORTED, "%s: dimension above 2^31 - 1025, or more than 65536 heads", who);
-    // a warp or more for each row of each head, counted in 32 bits
+    // a block for every row of every head in the worst case
     const int64_t rows = d->tokens_q > d->tokens_k ? d->tokens_q : d->tokens_k;
-    if (static_cast<__int128>(rows) * d->heads * d->batch > (int64_t{1} << 32))
-        return fail(LLMT_B200_ERR_UNSUPPORTED, "%s: more than 2^32 rows over all heads", who);
+    if (static_cast<__int128>(rows) * d->heads * d->batch > 0x7fffffff)
+        return fail(LLMT_B200_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 rows over all heads", who);
     if (!(d->scale > 0.0f) || !std::isfinite(d->scale)) return fail(LLMT_B200_ERR_INVALID, "%s: scale must be positive and finite", who);
     if (misaligned(d->lse, 4) || misaligned(d->lengths, 4)) return fail(LLMT_B200_ERR_INVALID, "%s: lse or lengths is not aligned to its element type", who);
     *p = AttentionParams{};
@@ -2218,8 +2241,11 @@ int llmt_b200_attention_window_decode(const llmt_b200_attention_desc* d, void* s
     const NamedView t[4] = {{"q", &d->q, false, false}, {"k", &d->k, true, false}, {"v", &d->v, true, false}, {"out", &d->out, false, true}};
     st = attention_views(d, who, t, 4);
     if (st == LLMT_B200_OK) st = attention_apart(d, who, "lse", d->lse, 4 * static_cast<size_t>(d->batch * d->heads), t, 4);
+    if (st == LLMT_B200_OK) st = attention_apart(d, who, "lengths", d->lengths, 4 * static_cast<size_t>(d->batch), t + 3, 1);
     if (st != LLMT_B200_OK) return st;
     if (p.batch == 0 || p.heads == 0) return LLMT_B200_OK;
+    if (d->lse != nullptr && d->lengths != nullptr && overlaps(d->lse, 4 * static_cast<size_t>(d->batch * d->heads), d->lengths, 4 * static_cast<size_t>(d->batch)))
+        return fail(LLMT_B200_ERR_INVALID, "%s: lse overlaps lengths", who);
     const uint64_t need = llmt_b200_attention_window_decode_workspace_bytes(d);
     if (need > 0) {
         if (d->workspace == nullptr || d->workspace_bytes < need)
