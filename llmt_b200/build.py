@@ -109,13 +109,15 @@ def build_native(force: bool = False) -> str:
 
 
 CPP_DIR = os.path.join(HERE, "cpp")
-CPP_SOURCES = ["runtime.cpp", "matmul.cpp", "layers.cpp", "attention.cpp", "peer_exchange.cpp", "cross_entropy.cpp"]
+CPP_SOURCES = ["runtime.cpp", "matmul.cpp", "layers.cpp", "attention.cpp", "peer_exchange.cpp", "cross_entropy.cpp", "rope.cpp",
+               "norm_residual.cpp"]
 HOST_LIB = os.path.join(LIB_DIR, "libllmt_b200_host.so")
 ROOT = os.path.dirname(HERE)
 CPP_TEST_SRC = os.path.join(ROOT, "tests", "cpp", "test_llmt_goldens.cpp")
 CPP_TEST_BIN = os.path.join(ROOT, "tests", "cpp", "_build", "test_llmt_goldens")
 CPP_TESTS = {"test_llmt_goldens": CPP_TEST_BIN,
-             "test_peer_exchange": os.path.join(ROOT, "tests", "cpp", "_build", "test_peer_exchange")}
+             "test_peer_exchange": os.path.join(ROOT, "tests", "cpp", "_build", "test_peer_exchange"),
+             "test_block_ops": os.path.join(ROOT, "tests", "cpp", "_build", "test_block_ops")}
 
 
 def build_cpp(force: bool = False) -> str:

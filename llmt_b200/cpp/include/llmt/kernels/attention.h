@@ -47,4 +47,30 @@ void softmax_fwd(const RunCtx& ctx, Tensor& y, const Tensor& x, MaskSpec mask) n
 void attention_fwd_packed(const RunCtx& ctx, Tensor& y, Tensor& scores, const Tensor& qkv, int64_t n_head,
                           MaskSpec mask) noexcept;
 
+// Causal attention of a packed projection without the [B, H, T, T] probabilities, bf16:
+//   qkv [B, T, (H + 2 Hkv) * hd]   per token Q | K | V; query head h reads key head h / (H / Hkv)
+//   y   [B, T, H * hd]             token rows, ready for the output projection
+//   lse [B, H, T] fp32             log-sum-exp of the scores, for the backward pass (forward: may be null)
+// Query i sees the last `window` keys up to its own (0: all of them) and the first `sinks`.  The backward pass writes all of
+// dqkv (the layout of qkv) from what the forward pass left; ctx.blas_workspace must hold
+// attention_window_workspace_bytes(...) bytes.
+struct WindowSpec {
+    int64_t window = 0;
+    int64_t sinks = 0;
+    float scale = 0.0f;  // 0: 1 / sqrt(hd)
+};
+void attention_window_fwd_packed(const RunCtx& ctx, Tensor& y, Tensor* lse, const Tensor& qkv, int64_t n_head, int64_t n_kv_head,
+                                 WindowSpec spec) noexcept;
+void attention_window_bwd_packed(const RunCtx& ctx, Tensor& dqkv, const Tensor& dy, const Tensor& qkv, const Tensor& y, const Tensor& lse,
+                                 int64_t n_head, int64_t n_kv_head, WindowSpec spec) noexcept;
+size_t attention_window_workspace_bytes(const Tensor& qkv, int64_t n_head, int64_t n_kv_head, WindowSpec spec) noexcept;
+
+// The same for one new token per sequence over a cache:
+//   q [B, W]: the token's row, whose first H * hd values are the query heads (a packed projection's row, W = (H + 2 Hkv) * hd,
+//   or the heads alone);  k, v [B, places, Hkv, hd];  lengths I32 [B]: the places that hold keys, the newest last (null: all)
+//   y [B, H * hd];  ctx.blas_workspace: attention_window_decode_workspace_bytes(...) bytes.
+void attention_window_decode(const RunCtx& ctx, Tensor& y, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor* lengths,
+                             int64_t n_head, WindowSpec spec) noexcept;
+size_t attention_window_decode_workspace_bytes(const Tensor& q, const Tensor& k, int64_t n_head, WindowSpec spec) noexcept;
+
 }  // namespace llmt::kernels

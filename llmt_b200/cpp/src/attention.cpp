@@ -207,4 +207,118 @@ void attention_bwd(const RunCtx& ctx, Tensor& dq, Tensor& dk, Tensor& dv, Tensor
     matmul(ctx, dk3, ds3, q3, true, false, scale, 0.0f);   // dK = a dS^T Q
 }
 
+namespace {
+
+llmt_b200_head_view packed_view(void* data, int64_t first, int64_t t, int64_t width, int64_t hd) noexcept {
+    llmt_b200_head_view v{};
+    v.data = static_cast<char*>(data) + first * 2;
+    v.stride_batch = t * width; v.stride_token = width; v.stride_head = hd;
+    return v;
+}
+
+// The shape of a packed windowed call; the caller puts the views.
+llmt_b200_attention_desc window_desc(const char* who, const Tensor& qkv, int64_t n_head, int64_t n_kv_head, WindowSpec spec) noexcept {
+    const int64_t parts = n_head + 2 * n_kv_head;
+    if (qkv.shape.rank != 3 || n_head <= 0 || n_kv_head <= 0 || qkv.shape[2] % parts != 0) detail::fatal(who, "qkv must be [B, T, (H + 2 Hkv)·hd]");
+    llmt_b200_attention_desc d{};
+    d.batch = qkv.shape[0]; d.tokens_q = d.tokens_k = qkv.shape[1];
+    d.heads = n_head; d.kv_heads = n_kv_head; d.head_dim = qkv.shape[2] / parts;
+    d.window = spec.window; d.sinks = spec.sinks;
+    d.scale = spec.scale != 0.0f ? spec.scale : 1.0f / std::sqrt(static_cast<float>(d.head_dim));
+    d.dtype = static_cast<int32_t>(qkv.dtype);
+    return d;
+}
+
+void put_packed(llmt_b200_attention_desc& d, const Tensor& qkv, const Tensor& y) noexcept {
+    const int64_t t = d.tokens_q, hd = d.head_dim, w = qkv.shape[2], a = d.heads * hd;
+    d.q = packed_view(qkv.data, 0, t, w, hd);
+    d.k = packed_view(qkv.data, a, t, w, hd);
+    d.v = packed_view(qkv.data, a + d.kv_heads * hd, t, w, hd);
+    d.out = packed_view(y.data, 0, t, a, hd);
+}
+
+void check_packed(const char* who, const llmt_b200_attention_desc& d, const Tensor& y, const Tensor* lse, DType dtype) noexcept {
+    if (!y.valid()) detail::fatal(who, "invalid tensor (null data)");
+    if (y.shape != Shape{d.batch, d.tokens_q, d.heads * d.head_dim}) detail::fatal(who, "y must be [B, T, H·hd]");
+    if (y.dtype != dtype) detail::fatal(who, "dtype mismatch");
+    if (lse != nullptr && (!lse->valid() || lse->dtype != DType::FP32 || lse->shape != Shape{d.batch, d.heads, d.tokens_q}))
+        detail::fatal(who, "lse must be fp32 [B, H, T]");
+}
+
+llmt_b200_attention_desc decode_desc(const char* who, const Tensor& q, const Tensor& k, int64_t n_head, WindowSpec spec) noexcept {
+    if (k.shape.rank != 4 || n_head <= 0) detail::fatal(who, "k and v must be [B, places, Hkv, hd]");
+    llmt_b200_attention_desc d{};
+    d.batch = k.shape[0]; d.tokens_q = 1; d.tokens_k = k.shape[1]; d.heads = n_head; d.kv_heads = k.shape[2]; d.head_dim = k.shape[3];
+    if (q.shape.rank != 2 || q.shape[0] != d.batch || q.shape[1] < n_head * d.head_dim) detail::fatal(who, "q must be [B, W] with the H·hd query values first");
+    d.window = spec.window; d.sinks = spec.sinks;
+    d.scale = spec.scale != 0.0f ? spec.scale : 1.0f / std::sqrt(static_cast<float>(d.head_dim));
+    d.dtype = static_cast<int32_t>(q.dtype);
+    return d;
+}
+
+}  // namespace
+
+void attention_window_fwd_packed(const RunCtx& ctx, Tensor& y, Tensor* lse, const Tensor& qkv, int64_t n_head, int64_t n_kv_head,
+                                 WindowSpec spec) noexcept {
+    const char* who = "attention_window_fwd_packed";
+    if (!qkv.valid()) detail::fatal(who, "invalid tensor (null data)");
+    llmt_b200_attention_desc d = window_desc(who, qkv, n_head, n_kv_head, spec);
+    check_packed(who, d, y, lse, qkv.dtype);
+    put_packed(d, qkv, y);
+    d.lse = lse != nullptr ? static_cast<float*>(lse->data) : nullptr;
+    if (llmt_b200_attention_window_fwd(&d, ctx.stream) != LLMT_B200_OK) detail::fatal(who, "%s", llmt_b200_last_error());
+}
+
+void attention_window_bwd_packed(const RunCtx& ctx, Tensor& dqkv, const Tensor& dy, const Tensor& qkv, const Tensor& y, const Tensor& lse,
+                                 int64_t n_head, int64_t n_kv_head, WindowSpec spec) noexcept {
+    const char* who = "attention_window_bwd_packed";
+    if (!qkv.valid() || !dqkv.valid()) detail::fatal(who, "invalid tensor (null data)");
+    llmt_b200_attention_desc d = window_desc(who, qkv, n_head, n_kv_head, spec);
+    check_packed(who, d, y, &lse, qkv.dtype);
+    check_packed(who, d, dy, nullptr, qkv.dtype);
+    if (dqkv.shape != qkv.shape || dqkv.dtype != qkv.dtype) detail::fatal(who, "dqkv must be laid out like qkv");
+    put_packed(d, qkv, y);
+    const int64_t t = d.tokens_q, hd = d.head_dim, w = qkv.shape[2], a = d.heads * hd;
+    d.dout = packed_view(dy.data, 0, t, a, hd);
+    d.dq = packed_view(dqkv.data, 0, t, w, hd);
+    d.dk = packed_view(dqkv.data, a, t, w, hd);
+    d.dv = packed_view(dqkv.data, a + d.kv_heads * hd, t, w, hd);
+    d.lse = static_cast<float*>(lse.data);
+    d.workspace = ctx.blas_workspace;
+    d.workspace_bytes = ctx.blas_workspace_bytes;
+    if (llmt_b200_attention_window_bwd(&d, ctx.stream) != LLMT_B200_OK) detail::fatal(who, "%s", llmt_b200_last_error());
+}
+
+size_t attention_window_workspace_bytes(const Tensor& qkv, int64_t n_head, int64_t n_kv_head, WindowSpec spec) noexcept {
+    const llmt_b200_attention_desc d = window_desc("attention_window_bwd_packed", qkv, n_head, n_kv_head, spec);
+    return static_cast<size_t>(llmt_b200_attention_window_workspace_bytes(&d));
+}
+
+void attention_window_decode(const RunCtx& ctx, Tensor& y, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor* lengths,
+                             int64_t n_head, WindowSpec spec) noexcept {
+    const char* who = "attention_window_decode";
+    for (const Tensor* t : std::initializer_list<const Tensor*>{&y, &q, &k, &v})
+        if (!t->valid()) detail::fatal(who, "invalid tensor (null data)");
+    llmt_b200_attention_desc d = decode_desc(who, q, k, n_head, spec);
+    if (v.shape != k.shape) detail::fatal(who, "k and v must be [B, places, Hkv, hd]");
+    if (y.shape != Shape{d.batch, n_head * d.head_dim}) detail::fatal(who, "y must be [B, H·hd]");
+    if (y.dtype != q.dtype || k.dtype != q.dtype || v.dtype != q.dtype) detail::fatal(who, "dtype mismatch");
+    d.q = packed_view(q.data, 0, 1, q.shape[1], d.head_dim);
+    d.out = packed_view(y.data, 0, 1, y.shape[1], d.head_dim);
+    d.k = packed_view(k.data, 0, d.tokens_k, d.kv_heads * d.head_dim, d.head_dim);
+    d.v = packed_view(v.data, 0, d.tokens_k, d.kv_heads * d.head_dim, d.head_dim);
+    if (lengths != nullptr) {
+        if (!lengths->valid() || lengths->dtype != DType::I32 || lengths->numel() != d.batch) detail::fatal(who, "lengths must be I32 [B]");
+        d.lengths = static_cast<const int32_t*>(lengths->data);
+    }
+    d.workspace = ctx.blas_workspace;
+    d.workspace_bytes = ctx.blas_workspace_bytes;
+    if (llmt_b200_attention_window_decode(&d, ctx.stream) != LLMT_B200_OK) detail::fatal(who, "%s", llmt_b200_last_error());
+}
+
+size_t attention_window_decode_workspace_bytes(const Tensor& q, const Tensor& k, int64_t n_head, WindowSpec spec) noexcept {
+    const llmt_b200_attention_desc d = decode_desc("attention_window_decode", q, k, n_head, spec);
+    return static_cast<size_t>(llmt_b200_attention_window_decode_workspace_bytes(&d));
+}
+
 }  // namespace llmt::kernels
