@@ -721,6 +721,7 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
     auto tile_of = [&](int it) { return it < sink_tiles ? it : low + it - sink_tiles; };
     roles.set_up(warp);
     const uint32_t tmem = uniform(roles.ctl->tmem);
+    grid_launch_dependents();   // the launch for dK and dV
     grid_dependency_wait();
     const int steps_d = (p.head_dim + 15) / 16;
     const uint32_t ring = tiles + 2 * kFixed;
@@ -879,6 +880,7 @@ attention_dkdv_kernel(const __grid_constant__ AttentionMaps maps, const __grid_c
     auto query_of = [&](int it) { return (q.first + (it0 + it) % q.count) * kCols; };
     roles.set_up(warp);
     const uint32_t tmem = uniform(roles.ctl->tmem);
+    if (plan.parts > 1 || plan.sink_parts > 1) grid_launch_dependents();   // the launch that adds the parts
     grid_dependency_wait();
     const int steps_d = (p.head_dim + 15) / 16;
     const uint32_t ring = tiles + 2 * kFixed;

@@ -40,7 +40,8 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
-// Eight columns of a thread: V = 8 neighbours, or (V = 1) eight that are the block's width apart.
+// Eight columns of a thread: V = 8 neighbours, or two groups of V = 4 neighbours or eight single ones (V = 1) that are the
+// block's width apart.
 template <typename T, int V> struct Eight {
     Vec<T, V> g[8 / V];
     __device__ __forceinline__ float at(int i) const { return to_float(g[i / V].v[i % V]); }
@@ -77,7 +78,7 @@ template <typename T, int V> struct Eight {
 // tensor's part of a stage, [16-byte piece or value][thread].  Places whose columns are not there are never copied to: the
 // kernels put zeros into all of them once.
 template <typename T, int V> struct Staged {
-    static constexpr int kUnit = V == 8 ? 16 : static_cast<int>(sizeof(T)), kUnits = 8 * static_cast<int>(sizeof(T)) / kUnit;
+    static constexpr int kUnit = V == 8 ? 16 : V * static_cast<int>(sizeof(T)), kUnits = 8 * static_cast<int>(sizeof(T)) / kUnit;
     static __device__ __forceinline__ void copy(uint8_t* to, const T* row, int first, int step, int cols) {
         const int threads = blockDim.x;
         if (V == 8) {
@@ -86,11 +87,16 @@ template <typename T, int V> struct Staged {
                 for (int n = 0; n < kUnits; ++n)
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(to + n * threads * kUnit)), "l"(row + first + n * (16 / sizeof(T))) : "memory");
             }
-        } else if (sizeof(T) == 4) {
+        } else if (kUnit == 16) {
 #pragma unroll
-            for (int n = 0; n < 8; ++n)
+            for (int n = 0; n < kUnits; ++n)
                 if (first + n * step < cols)
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(ptx::smem_u32(to + n * threads * kUnit)), "l"(row + first + n * step) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(to + n * threads * kUnit)), "l"(row + first + n * step) : "memory");
+        } else if (kUnit >= 4) {
+#pragma unroll
+            for (int n = 0; n < kUnits; ++n)
+                if (first + n * step < cols)
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(ptx::smem_u32(to + n * threads * kUnit)), "l"(row + first + n * step), "n"(kUnit < 4 ? 4 : kUnit) : "memory");
         } else {   // two bytes are no asynchronous copy
             T v[8];
 #pragma unroll
@@ -108,7 +114,7 @@ template <typename T, int V> struct Staged {
             e = *reinterpret_cast<const Eight<T, V>*>(w);
         } else {
 #pragma unroll
-            for (int n = 0; n < 8; ++n) e.g[n / V].v[n % V] = *reinterpret_cast<const T*>(from + n * threads * kUnit);
+            for (int n = 0; n < kUnits; ++n) e.g[n] = *reinterpret_cast<const Vec<T, V>*>(from + n * threads * kUnit);
         }
     }
     static __device__ __forceinline__ uint8_t* place(uint8_t* part) { return part + threadIdx.x * kUnit; }
@@ -117,12 +123,16 @@ template <typename T, int V> struct Staged {
 #pragma unroll
         for (int n = 0; n < kUnits; ++n) {
             if (kUnit == 16) *reinterpret_cast<uint4*>(to + n * threads * kUnit) = make_uint4(0, 0, 0, 0);
-            else *reinterpret_cast<T*>(to + n * threads * kUnit) = rounded<T>(0.0f);
+            else *reinterpret_cast<Vec<T, V>*>(to + n * threads * kUnit) = {};
         }
     }
 };
 __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Of neighbours that a thread owns where alignment allows it: 16 bytes of a residual stream's row, so that what a warp accesses
+// at once is contiguous (eight fp32 neighbours in two accesses: NUMBER us against NUMBER).
+template <typename TR> constexpr int kWide = 16 / sizeof(TR);
 
 constexpr int kMostWarps = 16;                  // of a block
 constexpr int kMostCols = kMostWarps * 32 * 8;  // columns that a block owns eight a thread
@@ -135,17 +145,19 @@ template <typename TR, typename TA, int N> constexpr int fwd_depth() { return N 
 template <typename TR, typename TA, int V, int N>
 __global__ void __launch_bounds__(kMostWarps * 32) norm_residual_fwd_kernel(NormResidualParams p) {
     extern __shared__ __align__(16) uint8_t stages[];
-    __shared__ float part[2][2][kMostWarps];
+    __shared__ float4 part[2][2][kMostWarps / 4];
     constexpr int kDepth = fwd_depth<TR, TA, N>();
     ptx::grid_dependency_wait();
     const int threads = blockDim.x, warps = threads >> 5, lane = threadIdx.x & 31, me = threadIdx.x;
-    const int first = V == 8 ? me * 8 : me, step = V == 8 ? 0 : threads;
+    const int first = me * V, step = threads * V;
     const bool block = p.y != nullptr, post = p.w_post != nullptr, pre = p.h != nullptr;
     const uint32_t of_x = threads * 8 * sizeof(TR), of_y = threads * 8 * sizeof(TA), stage_bytes = N * (of_x + of_y);
     auto cols_of = [&](int n) { return V == 8 ? p.cols - n * threads * 8 : min(p.cols - n * threads * 8, threads * 8); };   // of the n-th eight
     const float of = 1.0f / static_cast<float>(p.cols);
     const int64_t r0 = p.rows * blockIdx.x / gridDim.x, r1 = p.rows * (blockIdx.x + 1) / gridDim.x;
 
+    if (me < kMostWarps) part[me / 8][me / 4 % 2][me % 4] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);   // warps that are not there
+    __syncthreads();
     uint8_t* const mine_x = Staged<TR, V>::place(stages);
     uint8_t* const mine_y = Staged<TA, V>::place(stages + N * of_x);
     for (int s = 0; s < kDepth; ++s)
@@ -154,20 +166,25 @@ __global__ void __launch_bounds__(kMostWarps * 32) norm_residual_fwd_kernel(Norm
             Staged<TR, V>::clear(mine_x + s * stage_bytes + n * of_x);
             Staged<TA, V>::clear(mine_y + s * stage_bytes + n * of_y);
         }
-    auto copy = [&](int64_t row, int stage) {
-        if (row < r1) {
-            const TR* x = static_cast<const TR*>(p.x) + row * p.ld_x;
-            const TA* y = static_cast<const TA*>(p.y) + row * p.ld_y;
+    // the next row to copy, and the row at work
+    const TR* next_x = static_cast<const TR*>(p.x) + r0 * p.ld_x;
+    const TA* next_y = static_cast<const TA*>(p.y) + r0 * p.ld_y;
+    TR* to_out = static_cast<TR*>(p.out) + r0 * p.ld_out;
+    TA* to_h = static_cast<TA*>(p.h) + r0 * p.ld_h;
+    auto copy = [&](bool there, int stage) {
+        if (there) {
 #pragma unroll
             for (int n = 0; n < N; ++n) {
-                Staged<TR, V>::copy(mine_x + stage * stage_bytes + n * of_x, x + n * threads * 8, first, step, cols_of(n));
-                if (block) Staged<TA, V>::copy(mine_y + stage * stage_bytes + n * of_y, y + n * threads * 8, first, step, cols_of(n));
+                Staged<TR, V>::copy(mine_x + stage * stage_bytes + n * of_x, next_x + n * threads * 8, first, step, cols_of(n));
+                if (block) Staged<TA, V>::copy(mine_y + stage * stage_bytes + n * of_y, next_y + n * threads * 8, first, step, cols_of(n));
             }
+            next_x += p.ld_x;
+            next_y += p.ld_y;
         }
         commit_copies();
     };
 #pragma unroll
-    for (int i = 0; i + 1 < kDepth; ++i) copy(r0 + i, i);
+    for (int i = 0; i + 1 < kDepth; ++i) copy(r0 + i < r1, i);
     int stage = 0;
     // k = gate w_post, changed with the gate's row
     float k[N][8], w_pre[N][8];
@@ -196,15 +213,18 @@ __global__ void __launch_bounds__(kMostWarps * 32) norm_residual_fwd_kernel(Norm
     auto row_sum = [&](float s, int which) {
         s = warp_sum(s);
         if (warps == 1) return s;
-        if (lane == 0) part[turn][which][me >> 5] = s;
+        if (lane == 0) reinterpret_cast<float*>(part[turn][which])[me >> 5] = s;
         __syncthreads();
         s = 0.0f;
-        for (int i = 0; i < warps; ++i) s += part[turn][which][i];
+        for (int i = 0; i < warps; i += 4) {
+            const float4 v = part[turn][which][i / 4];
+            s += (v.x + v.y) + (v.z + v.w);
+        }
         return s;
     };
     int64_t next_group = r0;   // first row of the next gate row
-    for (int64_t row = r0; row < r1; ++row) {
-        copy(row + kDepth - 1, stage == 0 ? kDepth - 1 : stage - 1);
+    for (int64_t row = r0; row < r1; ++row, to_out += p.ld_out, to_h += p.ld_h) {
+        copy(row + kDepth - 1 < r1, stage == 0 ? kDepth - 1 : stage - 1);
         if (row == next_group) {
             const int64_t group = row / p.rows_per_gate;
             load_k(group);
@@ -239,7 +259,7 @@ __global__ void __launch_bounds__(kMostWarps * 32) norm_residual_fwd_kernel(Norm
                 s = fmaf(z[n][i], z[n][i], s);
             }
             x[n].put(z[n]);
-            if (block) x[n].store(static_cast<TR*>(p.out) + row * p.ld_out + n * threads * 8, first, step, cols_of(n));
+            if (block) x[n].store(to_out + n * threads * 8, first, step, cols_of(n));
         }
         if (pre) {
             const float r = rsqrtf(fmaf(row_sum(s, 1), of, p.eps));
@@ -249,7 +269,7 @@ __global__ void __launch_bounds__(kMostWarps * 32) norm_residual_fwd_kernel(Norm
 #pragma unroll
                 for (int i = 0; i < 8; ++i) z[n][i] *= r * w_pre[n][i];
                 y[n].put(z[n]);
-                y[n].store(static_cast<TA*>(p.h) + row * p.ld_h + n * threads * 8, first, step, cols_of(n));
+                y[n].store(to_h + n * threads * 8, first, step, cols_of(n));
             }
         }
         turn ^= 1;
@@ -267,13 +287,13 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 8 ? 3 : 1) norm_residual_
     extern __shared__ __align__(16) uint8_t stages[];
     __shared__ float4 part[2][4 * kMostWarps];   // of every warp of the cluster (up to four blocks)
     constexpr int kDepth = bwd_depth<TR, TA>();
+    if (p.part_w != nullptr || p.part_gc != nullptr) ptx::grid_launch_dependents();   // the launch that adds the sums
     ptx::grid_dependency_wait();
     const int threads = blockDim.x, warps = threads >> 5;
     const int ranks = CLUSTER ? p.cluster : 1;
     const int rank = CLUSTER ? static_cast<int>(ptx::cluster_ctarank()) : 0;
     const int me = blockIdx.x / ranks, blocks = gridDim.x / ranks;
-    const int first = V == 8 ? (rank * threads + static_cast<int>(threadIdx.x)) * 8 : rank * threads * 8 + static_cast<int>(threadIdx.x);
-    const int step = V == 8 ? 0 : threads;
+    const int first = rank * threads * 8 + static_cast<int>(threadIdx.x) * V, step = threads * V;
     const int cols = V == 8 ? p.cols : min(p.cols, (rank + 1) * threads * 8);
     const bool pre = p.dh != nullptr, block = p.y != nullptr, post = p.w_post != nullptr, more = p.dout != nullptr;
     const uint32_t of_r = threads * 8 * sizeof(TR), of_a = threads * 8 * sizeof(TA), stage_bytes = 2 * (of_r + of_a);
@@ -300,22 +320,33 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 8 ? 3 : 1) norm_residual_
         const int64_t group = u / per_group, part_of = u % per_group;
         const int64_t r0 = group * p.rows_per_gate + p.rows_per_gate * part_of / per_group;
         const int64_t r1 = group * p.rows_per_gate + p.rows_per_gate * (part_of + 1) / per_group;
-        auto copy = [&](int64_t row, int stage) {
-            if (row < r1) {
+        // the next row to copy, and the row at work
+        const TR* next_out = static_cast<const TR*>(p.out) + r0 * p.ld_out;
+        const TA* next_dh = static_cast<const TA*>(p.dh) + r0 * p.ld_dh;
+        const TR* next_dout = static_cast<const TR*>(p.dout) + r0 * p.ld_dout;
+        const TA* next_y = static_cast<const TA*>(p.y) + r0 * p.ld_y;
+        TR* to_dx = static_cast<TR*>(p.dx) + r0 * p.ld_dx;
+        TA* to_dy = static_cast<TA*>(p.dy) + r0 * p.ld_dy;
+        auto copy = [&](bool there, int stage) {
+            if (there) {
                 uint8_t* const at = mine_r + stage * stage_bytes;
                 uint8_t* const to = mine_a + stage * stage_bytes;
                 if (pre) {
-                    Staged<TR, V>::copy(at, static_cast<const TR*>(p.out) + row * p.ld_out, first, step, cols);
-                    Staged<TA, V>::copy(to, static_cast<const TA*>(p.dh) + row * p.ld_dh, first, step, cols);
+                    Staged<TR, V>::copy(at, next_out, first, step, cols);
+                    Staged<TA, V>::copy(to, next_dh, first, step, cols);
                 }
-                if (more) Staged<TR, V>::copy(at + of_r, static_cast<const TR*>(p.dout) + row * p.ld_dout, first, step, cols);
-                if (block) Staged<TA, V>::copy(to + of_a, static_cast<const TA*>(p.y) + row * p.ld_y, first, step, cols);
+                if (more) Staged<TR, V>::copy(at + of_r, next_dout, first, step, cols);
+                if (block) Staged<TA, V>::copy(to + of_a, next_y, first, step, cols);
+                next_out += p.ld_out;
+                next_dh += p.ld_dh;
+                next_dout += p.ld_dout;
+                next_y += p.ld_y;
             }
             commit_copies();
         };
         int stage = 0;
 #pragma unroll
-        for (int i = 0; i + 1 < kDepth; ++i) copy(r0 + i, i);
+        for (int i = 0; i + 1 < kDepth; ++i) copy(r0 + i < r1, i);
         // k = scale gate w_post
         float k[8], sum_gc[8];
         Eight<float, V> gate;
@@ -326,8 +357,8 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 8 ? 3 : 1) norm_residual_
             k[i] = p.scale * (p.gate != nullptr ? gate.at(i) : 1.0f) * (post ? weight.at(i) : 1.0f);
             sum_gc[i] = 0.0f;
         }
-        for (int64_t row = r0; row < r1; ++row) {
-            copy(row + kDepth - 1, stage == 0 ? kDepth - 1 : stage - 1);
+        for (int64_t row = r0; row < r1; ++row, to_dx += p.ld_dx, to_dy += p.ld_dy) {
+            copy(row + kDepth - 1 < r1, stage == 0 ? kDepth - 1 : stage - 1);
             const float r_pre = pre ? p.rstd_pre[row] : 0.0f, r_post = block && post ? p.rstd_post[row] : 1.0f;
             wait_copies<kDepth - 1>();
             const uint8_t* const at = mine_r + stage * stage_bytes;
@@ -400,8 +431,8 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 8 ? 3 : 1) norm_residual_
             }
             dx.put(q);
             dy.put(y);
-            dx.store(static_cast<TR*>(p.dx) + row * p.ld_dx, first, step, cols);
-            if (block) dy.store(static_cast<TA*>(p.dy) + row * p.ld_dy, first, step, cols);
+            dx.store(to_dx, first, step, cols);
+            if (block) dy.store(to_dy, first, step, cols);
         }
         wait_copies<0>();   // the next unit's copies start anew
         if (p.part_gc != nullptr) {
@@ -489,7 +520,7 @@ cudaError_t fwd_rows(const NormResidualParams& p, int sms, cudaStream_t stream) 
 }
 template <typename TR, typename TA>
 cudaError_t fwd_typed(const NormResidualParams& p, bool wide, int sms, cudaStream_t stream) {
-    if (wide) return p.cols <= kMostCols ? fwd_rows<TR, TA, 8, 1>(p, sms, stream) : p.cols <= 2 * kMostCols ? fwd_rows<TR, TA, 8, 2>(p, sms, stream) : fwd_rows<TR, TA, 8, 4>(p, sms, stream);
+    if (wide) return p.cols <= kMostCols ? fwd_rows<TR, TA, kWide<TR>, 1>(p, sms, stream) : p.cols <= 2 * kMostCols ? fwd_rows<TR, TA, kWide<TR>, 2>(p, sms, stream) : fwd_rows<TR, TA, kWide<TR>, 4>(p, sms, stream);
     return p.cols <= kMostCols ? fwd_rows<TR, TA, 1, 1>(p, sms, stream) : p.cols <= 2 * kMostCols ? fwd_rows<TR, TA, 1, 2>(p, sms, stream) : fwd_rows<TR, TA, 1, 4>(p, sms, stream);
 }
 
@@ -508,9 +539,9 @@ cudaError_t bwd_typed(const NormResidualParams& p, const NormResidualPlan& pl, b
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = pl.cluster > 1 ? 2 : 1;
-    auto kernel = pl.cluster > 1 ? (wide ? norm_residual_bwd_kernel<TR, TA, 8, true, 16> : norm_residual_bwd_kernel<TR, TA, 1, true, 16>)
-                  : pl.warps > 8 ? (wide ? norm_residual_bwd_kernel<TR, TA, 8, false, 16> : norm_residual_bwd_kernel<TR, TA, 1, false, 16>)
-                                 : (wide ? norm_residual_bwd_kernel<TR, TA, 8, false, 8> : norm_residual_bwd_kernel<TR, TA, 1, false, 8>);
+    auto kernel = pl.cluster > 1 ? (wide ? norm_residual_bwd_kernel<TR, TA, kWide<TR>, true, 16> : norm_residual_bwd_kernel<TR, TA, 1, true, 16>)
+                  : pl.warps > 8 ? (wide ? norm_residual_bwd_kernel<TR, TA, kWide<TR>, false, 16> : norm_residual_bwd_kernel<TR, TA, 1, false, 16>)
+                                 : (wide ? norm_residual_bwd_kernel<TR, TA, kWide<TR>, false, 8> : norm_residual_bwd_kernel<TR, TA, 1, false, 8>);
     if (cfg.dynamicSmemBytes > 40 * 1024) {
         const cudaError_t set = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(cfg.dynamicSmemBytes));
         if (set != cudaSuccess) return set;
