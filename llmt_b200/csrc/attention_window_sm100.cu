@@ -4,6 +4,18 @@
 //   S = Q K^T;  P = 2^(c S - c m) on visible places, else 0;  O = O 2^(c m_old - c m) + P V;  out = O / l,
 // c = scale log2 e.  O is only rescaled where m grows by more than 2^8: until then P is up to 2^8 too large, which the
 // same factor in l takes out again, and bf16 keeps its relative precision.
+// Backward:  P = 2^(c S - lse log2 e);  dS = P (dP - D), dP = dO V^T;  dV = P^T dO, dK = scale dS^T Q, dQ = scale dS K.
+// P and dS are rounded to bf16 as operands of the second products: each rounding is independent of the others, so a sum of
+// many keeps a relative error of the size of one, about what the rounding of the result itself adds (2.4e-3 against 1.7e-3 of
+// the norm); all else is fp32.
+//
+// Bound: neither memory nor the tensor core alone, but the way between them.  A thread has a row of scores; its exponentials
+// (8 cycles a warp for each), maxima and conversions take as long as the products they stand between, and a tile is a chain
+// scores -> probabilities -> product.  What helps is whatever runs beside that chain: a second block on the SM, a second
+// warpgroup, scores made before they are wanted.
+// Measured: 4 x 12 x 333 queries of 64, window 128: 9.6 us (a launch and three tiles); 8 x 12 x 1024 of 64, window 256,
+// forward and backward: 31 + 87 us; 8192 queries, 16 heads on 4 of 128, window 2048: forward 133 us (905 TFLOP/s of visible
+// pairs), backward 550 us (548).
 #include <cuda_bf16.h>
 
 #include <type_traits>
