@@ -505,6 +505,10 @@ LLMT_B200_API uint64_t llmt_b200_norm_residual_workspace_bytes(const llmt_b200_n
  *   anything that is read.  scale is positive.  batch * heads * max(tokens_q, tokens_k) < 2^31.
  *   lse  fp32 [batch, heads, tokens_q]: written by _fwd (NULL: not wanted), read by _bwd.
  *
+ * _fwd: with a workspace (16-byte aligned) of llmt_b200_attention_window_fwd_workspace_bytes(desc) bytes, 0
+ * for many calls, the keys of a few queries are shared out among the SMs in parts that are joined in a fixed
+ * order; with a smaller one or none they are not.
+ *
  * _bwd: dV = P^T dO,  dS = P (dP - D) with dP = dO v^T,  dQ = scale dS k,  dK = scale dS^T q, from out and
  * lse as _fwd left them.  D = rowsum(P dP) is taken as rowsum(dO out) for dQ; a row of dS adds up to nothing
  * but for the rounding of out, which is taken out of D again before dK is formed.  workspace: 16-byte
@@ -532,6 +536,7 @@ typedef struct llmt_b200_attention_desc {
 LLMT_B200_API int llmt_b200_attention_window_fwd(const llmt_b200_attention_desc* desc, void* stream);
 LLMT_B200_API int llmt_b200_attention_window_bwd(const llmt_b200_attention_desc* desc, void* stream);
 LLMT_B200_API int llmt_b200_attention_window_decode(const llmt_b200_attention_desc* desc, void* stream);
+LLMT_B200_API uint64_t llmt_b200_attention_window_fwd_workspace_bytes(const llmt_b200_attention_desc* desc);
 LLMT_B200_API uint64_t llmt_b200_attention_window_workspace_bytes(const llmt_b200_attention_desc* desc);
 LLMT_B200_API uint64_t llmt_b200_attention_window_decode_workspace_bytes(const llmt_b200_attention_desc* desc);
 

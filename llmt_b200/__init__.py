@@ -34,7 +34,7 @@ EXPORTS = [
     "llmt_b200_rowdot", "llmt_b200_cross_entropy_bwd", "llmt_b200_lm_head_ce_bwd",
     "llmt_b200_rope", "llmt_b200_rope_frequencies", "llmt_b200_norm_residual_fwd", "llmt_b200_norm_residual_bwd",
     "llmt_b200_norm_residual_workspace_bytes", "llmt_b200_attention_window_fwd", "llmt_b200_attention_window_bwd",
-    "llmt_b200_attention_window_decode", "llmt_b200_attention_window_workspace_bytes",
+    "llmt_b200_attention_window_decode", "llmt_b200_attention_window_fwd_workspace_bytes", "llmt_b200_attention_window_workspace_bytes",
     "llmt_b200_attention_window_decode_workspace_bytes",
 ]
 
@@ -208,7 +208,7 @@ def lib() -> ctypes.CDLL:
         for name in ("fwd", "bwd", "decode"):
             f = getattr(L, "llmt_b200_attention_window_" + name)
             f.argtypes, f.restype = [ctypes.POINTER(AttentionDesc), ctypes.c_void_p], ctypes.c_int
-        for name in ("workspace_bytes", "decode_workspace_bytes"):
+        for name in ("workspace_bytes", "fwd_workspace_bytes", "decode_workspace_bytes"):
             f = getattr(L, "llmt_b200_attention_window_" + name)
             f.argtypes, f.restype = [ctypes.POINTER(AttentionDesc)], ctypes.c_uint64
         L.llmt_b200_exchange_begin_step.argtypes = [ctypes.POINTER(CommDesc), ctypes.c_void_p]
@@ -750,14 +750,31 @@ def _put_lse(d: "AttentionDesc", who: str, lse, rows: int) -> None:
         d.lse = lse.data_ptr()
 
 
-def attention_window_fwd(out, lse, q, k, v, window: int = 0, sinks: int = 0, scale=None, stream=None) -> None:
+def attention_window_fwd(out, lse, q, k, v, window: int = 0, sinks: int = 0, scale=None, workspace=None, stream=None) -> None:
     """Causal attention of q [B, Tq, H, hd] over k, v [B, Tk, Hkv, hd] (any strides) into out, where a query at
     p = i + Tk - Tq sees keys j <= p that are among the last `window` (0: all) or the first `sinks`
-    (llmt_b200_attention_window_fwd).  lse: fp32 [B, H, Tq] for the backward pass, or None.  scale: 1 / sqrt(hd) if None."""
+    (llmt_b200_attention_window_fwd).  lse: fp32 [B, H, Tq] for the backward pass, or None.  scale: 1 / sqrt(hd) if None.
+    `workspace`: a uint8 tensor of attention_window_fwd_workspace_bytes (a smaller one is not used), or one is allocated
+    for the call where it helps."""
     who = "attention_window_fwd"
     d = _attention_desc(who, q, k, v, window, sinks, scale, dict(out=(out, q)))
     _put_lse(d, who, lse, d.batch * d.heads * d.tokens_q)
-    _on(_device_of(who, out, lse, q, k, v), stream, lambda s: lib().llmt_b200_attention_window_fwd(ctypes.byref(d), s))
+
+    def call(s):
+        ws = workspace
+        if ws is None:
+            need = lib().llmt_b200_attention_window_fwd_workspace_bytes(ctypes.byref(d))
+            ws = _scratch(need, q, stream) if need else None
+        if ws is not None:
+            d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
+        return lib().llmt_b200_attention_window_fwd(ctypes.byref(d), s)
+    _on(_device_of(who, out, lse, q, k, v, workspace), stream, call)
+
+
+def attention_window_fwd_workspace_bytes(q, k, window: int = 0, sinks: int = 0) -> int:
+    """Scratch of attention_window_fwd for tensors of these shapes on the current device."""
+    d = _attention_desc("attention_window_fwd_workspace_bytes", q, k, k, window, sinks, None, {})
+    return int(lib().llmt_b200_attention_window_fwd_workspace_bytes(ctypes.byref(d)))
 
 
 def attention_window_bwd(dq, dk, dv, dout, q, k, v, out, lse, window: int = 0, sinks: int = 0, scale=None, workspace=None, stream=None) -> None:

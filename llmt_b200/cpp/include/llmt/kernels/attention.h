@@ -53,7 +53,8 @@ void attention_fwd_packed(const RunCtx& ctx, Tensor& y, Tensor& scores, const Te
 //   lse [B, H, T] fp32             log-sum-exp of the scores, for the backward pass (forward: may be null)
 // Query i sees the last `window` keys up to its own (0: all of them) and the first `sinks`.  The backward pass writes all of
 // dqkv (the layout of qkv) from what the forward pass left; ctx.blas_workspace must hold
-// attention_window_workspace_bytes(...) bytes.
+// attention_window_workspace_bytes(...) bytes.  The forward pass uses it too, where it is large enough, to share the keys of a
+// few queries out among the SMs.
 struct WindowSpec {
     int64_t window = 0;
     int64_t sinks = 0;

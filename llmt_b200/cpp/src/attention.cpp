@@ -266,6 +266,8 @@ void attention_window_fwd_packed(const RunCtx& ctx, Tensor& y, Tensor* lse, cons
     check_packed(who, d, y, lse, qkv.dtype);
     put_packed(d, qkv, y);
     d.lse = lse != nullptr ? static_cast<float*>(lse->data) : nullptr;
+    d.workspace = ctx.blas_workspace;
+    d.workspace_bytes = ctx.blas_workspace_bytes;
     if (llmt_b200_attention_window_fwd(&d, ctx.stream) != LLMT_B200_OK) detail::fatal(who, "%s", llmt_b200_last_error());
 }
 

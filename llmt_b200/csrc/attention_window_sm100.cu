@@ -127,7 +127,10 @@ struct QueryBlock {
         high = p1 / kRows;
         sinks = min((min(p.sinks, first) + kRows - 1) / kRows, low);
     }
-    __device__ __forceinline__ int tiles() const { return any ? sinks + high - low + 1 : 0; }
+    // of the tiles [from, to)
+    __device__ __forceinline__ int count(int from, int to) const {
+        return any ? max(0, min(to, sinks) - from) + max(0, min(to, high + 1) - max(from, low)) : 0;
+    }
     __device__ __forceinline__ bool sees(int tile) const { return any && tile <= high && (tile >= low || tile < sinks); }
 };
 
@@ -186,6 +189,8 @@ __device__ __forceinline__ void copy_out(uint32_t* bad, int id, int threads, boo
 // head_dim <= 128: two warpgroups against the same keys: two heads that share a key head, or two neighbouring query blocks of
 // one head.  Scores and outputs fill tensor memory, the probabilities take their scores' place, and while one warpgroup takes
 // its exponentials the tensor core works for the other.
+// Where there are few query blocks, several blocks of threads share the keys of each, leave their part's output and log-sum-exp
+// in a workspace, and a second launch joins them.
 template <int WGS> struct FwdControl {
     static constexpr int kSlots = 4;   // tiles of K and V in flight
     uint64_t q_full[WGS], full[kSlots], empty[kSlots], s_full[WGS], s_taken[WGS], p_ready[WGS], o_done[WGS], o_full[WGS];
@@ -198,8 +203,8 @@ template <int HALVES, int WGS> constexpr size_t fwd_smem() { return 2048 + stati
 
 template <int HALVES, int WGS>
 __global__ void __launch_bounds__(128 * WGS + 64, 3 - WGS)
-attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_constant__ AttentionParams p, int pair_heads, int blocks_q, DeviceStatus* status,
-                     uint64_t wait_ns) {
+attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_constant__ AttentionParams p, int pair_heads, int blocks_q, int parts,
+                     DeviceStatus* status, uint64_t wait_ns) {
     using Control = FwdControl<WGS>;
     constexpr int kSlots = Control::kSlots, kLoadWarp = 4 * WGS, kProductWarp = 4 * WGS + 1, kHd = 64 * HALVES;
     constexpr bool kApart = HALVES == 1;   // the probabilities have a place of their own
@@ -214,7 +219,7 @@ attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_co
 
     // later queries see more keys: they go first
     const int units = p.batch * p.heads / (pair_heads ? 2 : 1);
-    const int unit = blockIdx.x % units, tile_q = blocks_q - 1 - static_cast<int>(blockIdx.x / units);
+    const int unit = blockIdx.x % units, item = static_cast<int>(blockIdx.x / units), part = item % parts, tile_q = blocks_q - 1 - item / parts;
     const int per_batch = units / p.batch, b = unit / per_batch, h0 = unit % per_batch * (pair_heads ? 2 : 1);
     const QueryBlock blk0(p, h0, tile_q * (pair_heads ? kRows : WGS * kRows));
     const QueryBlock blk1(p, pair_heads ? h0 + 1 : h0, WGS == 1 ? p.tq : pair_heads ? blk0.r0 : blk0.r0 + kRows);
@@ -226,6 +231,11 @@ attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_co
     const int sink_tiles = min(max(blk0.any ? blk0.sinks : 0, blk1.any ? blk1.sinks : 0), low);
     const int n_tiles = blk0.any || blk1.any ? sink_tiles + high - low + 1 : 0;
     auto tile_of = [&](int it) { return it < sink_tiles ? it : low + it - sink_tiles; };
+    // this block's part of them
+    const int first = static_cast<int>(static_cast<int64_t>(n_tiles) * part / parts), end = static_cast<int>(static_cast<int64_t>(n_tiles) * (part + 1) / parts);
+    auto tiles_of = [&](int w) {
+        return block(w).count(min(first, sink_tiles), min(end, sink_tiles)) + block(w).count(low + max(first - sink_tiles, 0), low + max(end - sink_tiles, 0));
+    };
 
     if (threadIdx.x == 0) {
         for (int w = 0; w < WGS; ++w) {
@@ -288,9 +298,9 @@ attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_co
             __syncwarp();
             if (++slot == kSlots) { slot = 0; phase ^= 1u; }
         };
-        for (int it = -1; it < n_tiles && ok; ++it) {
-            if (it + 1 < n_tiles) load(&maps.k, tile_of(it + 1));
-            if (ok && it >= 0) load(&maps.v, tile_of(it));
+        for (int it = first - 1; it < end && ok; ++it) {
+            if (it + 1 < end) load(&maps.k, tile_of(it + 1));
+            if (ok && it >= first) load(&maps.v, tile_of(it));
         }
     } else if (warp == kProductWarp) {
         // ---------------------------------------------------------------- products
@@ -299,6 +309,7 @@ attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_co
         int slot = 0;
         uint32_t phase = 0;
         int scores[2] = {0, 0}, values[2] = {0, 0};   // products made for either block
+        const int most[2] = {tiles_of(0), WGS == 1 ? 0 : tiles_of(1)};
         bool ok = true;
         for (int w = 0; w < WGS && ok; ++w)
             if (block(w).any) ok = bounded_wait_warp(smem_u32(&ctl->q_full[w]), 0, abort_flag, status, kDevWaitSmemFull, 100 + w, wait_ns);
@@ -328,14 +339,14 @@ attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_co
             tc_fence_after_thread_sync();
             if (elect_one()) {
                 product_ts<kRows / 16>(tmem_o(w), tmem_p(w), ring_v + v_slot * (kTile / 16), idesc_o, values[w] > 0);
-                umma_commit(smem_u32(values[w] + 1 < block(w).tiles() ? &ctl->o_done[w] : &ctl->o_full[w]));
+                umma_commit(smem_u32(values[w] + 1 < most[w] ? &ctl->o_done[w] : &ctl->o_full[w]));
             }
             __syncwarp();
             ++values[w];
         };
-        for (int it = -1; it < n_tiles && ok; ++it) {
+        for (int it = first - 1; it < end && ok; ++it) {
             int v_slot = -1, k_slot = -1;
-            if (it + 1 < n_tiles) k_slot = next();
+            if (it + 1 < end) k_slot = next();
             if (kApart) {   // scores first: their operands are there long before the probabilities
                 if (ok && k_slot >= 0) {
 #pragma unroll
@@ -344,7 +355,7 @@ attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_co
                     if (elect_one()) umma_commit(smem_u32(&ctl->empty[k_slot]));
                     __syncwarp();
                 }
-                if (ok && it >= 0) v_slot = next();
+                if (ok && it >= first) v_slot = next();
                 if (ok && v_slot >= 0) {
 #pragma unroll
                     for (int w = 0; w < WGS; ++w)
@@ -353,7 +364,7 @@ attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_co
                     __syncwarp();
                 }
             } else {
-                if (ok && it >= 0) v_slot = next();
+                if (ok && it >= first) v_slot = next();
 #pragma unroll
                 for (int w = 0; w < WGS; ++w) {
                     if (ok && v_slot >= 0 && block(w).sees(tile_of(it))) make_values(w, v_slot);
@@ -384,7 +395,7 @@ attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_co
             ok = bounded_wait_warp(smem_u32(&ctl->o_done[w]), static_cast<uint32_t>(done - 1) & 1u, abort_flag, status, kDevWaitTmemFull, 2 + w, wait_ns);
             tc_fence_after_thread_sync();
         };
-        for (int it = 0; it < n_tiles && ok; ++it) {
+        for (int it = first; it < end && ok; ++it) {
             const int j0 = tile_of(it) * kRows;
             if (!blk.sees(tile_of(it))) continue;
             ok = bounded_wait_warp(smem_u32(&ctl->s_full[w]), static_cast<uint32_t>(done) & 1u, abort_flag, status, kDevWaitTmemFull, w, wait_ns);
@@ -457,6 +468,9 @@ attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_co
             const float l = both(l2).x + both(l2).y;
             const float inv = l > 0.0f ? 1.0f / l : l;   // l NaN: so is the row
             bool bad = false;
+            const int64_t line = (static_cast<int64_t>(b) * p.heads + blk.head) * p.tq + i;
+            // of a block's part in the workspace: 16-byte pieces of rows, [piece][row], so that a warp's stores are contiguous
+            const int64_t place = ((static_cast<int64_t>(b) * p.heads + blk.head) * ((p.tq + kRows - 1) / kRows) + blk.r0 / kRows) * parts + part;
             for (int x = 0; x < 4 * HALVES; ++x) {
                 uint32_t o[16];
 #pragma unroll
@@ -471,18 +485,27 @@ attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_co
                     bad = bad || !(fabsf(f) < INFINITY);
                     o[y] = __float_as_uint(f);
                 }
-                put_row16(base + 1024 + w * kTile, row, x, o);
+                if (parts == 1) {
+                    put_row16(base + 1024 + w * kTile, row, x, o);
+                } else if (i < p.tq && x < steps_d) {
+                    uint4* const to_part = reinterpret_cast<uint4*>(p.partial) + (place * (kHd / 4) + x * 4) * kRows + row;
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) to_part[y * kRows] = make_uint4(o[4 * y], o[4 * y + 1], o[4 * y + 2], o[4 * y + 3]);
+                }
             }
-            if (i < p.tq && p.lse != nullptr)
-                p.lse[(static_cast<int64_t>(b) * p.heads + blk.head) * p.tq + i] = l == 0.0f ? -INFINITY : fmaf(m, p.scale, log2f(l) * (1.0f / kLog2e));
-            // A product with a hidden value that is not finite (0 * inf) has spoilt the row, or it sees such a value: it is
-            // formed again from the keys it sees.
-            copy_out(ctl->bad[w], 1 + w, 128, row == 0, quarter, true, __ballot_sync(0xffffffffu, bad && ok && i < p.tq), [&] {
-                for (int x = 0; x < HALVES; ++x) tma_store_4d(&maps.out, q_at + w * kTile + x * kHalfTile, x * 64, blk.r0, blk.head, b);
-            }, [&](int r) {
-                const int64_t at = blk.r0 + quarter * 32 + r;
-                attn::forward_row(p, b, blk.head, at, at + p.tk - p.tq);
-            });
+            if (parts > 1) {
+                if (i < p.tq) p.dvec[place * kRows + row] = l == 0.0f ? -INFINITY : fmaf(m, c, log2f(l));
+            } else {
+                if (i < p.tq && p.lse != nullptr) p.lse[line] = l == 0.0f ? -INFINITY : fmaf(m, p.scale, log2f(l) * (1.0f / kLog2e));
+                // A product with a hidden value that is not finite (0 * inf) has spoilt the row, or it sees such a value: it is
+                // formed again from the keys it sees.
+                copy_out(ctl->bad[w], 1 + w, 128, row == 0, quarter, true, __ballot_sync(0xffffffffu, bad && ok && i < p.tq), [&] {
+                    for (int x = 0; x < HALVES; ++x) tma_store_4d(&maps.out, q_at + w * kTile + x * kHalfTile, x * 64, blk.r0, blk.head, b);
+                }, [&](int r) {
+                    const int64_t at = blk.r0 + quarter * 32 + r;
+                    attn::forward_row(p, b, blk.head, at, at + p.tk - p.tq);
+                });
+            }
         }
     }
     // -------------------------------------------------------------------- teardown
@@ -492,6 +515,66 @@ attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_co
     if (warp == kProductWarp) {
         tc_fence_after_thread_sync();
         tmem_dealloc(tmem, kTmem);
+    }
+}
+
+// Joins the parts of 32 rows that were done in parts: out = sum of 2^(s_part - max) out_part over the sum of the
+// 2^(s_part - max), s_part = log2 sum exp of a part's scores.  A lane has a row, a warp PIECES of the row's 16-byte pieces; the
+// results cross shared memory, so that reads and writes are contiguous.
+constexpr int kJoinWarps = 8, kMostParts = 32;
+template <int PIECES>
+__global__ void __launch_bounds__(kJoinWarps * 32) attention_fwd_join_kernel(AttentionParams p, int parts) {
+    constexpr int kPieces = PIECES * kJoinWarps;
+    __shared__ uint2 tile[32][kPieces + 1];
+    __shared__ uint32_t bad[kJoinWarps];
+    grid_dependency_wait();
+    const int blocks_q = (p.tq + kRows - 1) / kRows, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t block = blockIdx.x / 4, bh = block / blocks_q, b = bh / p.heads, h = bh % p.heads;
+    const int in_block = static_cast<int>(blockIdx.x % 4) * 32 + lane;
+    const int64_t r0 = block % blocks_q * kRows + blockIdx.x % 4 * 32, i = r0 + lane;
+    if (r0 >= p.tq) return;
+    const float* const stat = p.dvec + block * parts * kRows + in_block;
+    const float4* const from = reinterpret_cast<const float4*>(p.partial) + (block * parts * kPieces + warp * PIECES) * kRows + in_block;
+    float top = -INFINITY, total = 0.0f, o[PIECES][4] = {};
+    if (i < p.tq) {
+        for (int part = 0; part < parts; ++part) top = fmaxf(top, stat[part * kRows]);
+#pragma unroll 2
+        for (int part = 0; part < parts; ++part) {
+            const float s = stat[part * kRows], w = s == -INFINITY ? 0.0f : exp2f(s - top);   // NaN in a part: in all
+            total += w;
+#pragma unroll
+            for (int n = 0; n < PIECES; ++n) {
+                if ((warp * PIECES + n) * 4 >= p.head_dim || w == 0.0f) continue;
+                const float4 v = from[(static_cast<int64_t>(part) * kPieces + n) * kRows];
+                o[n][0] = fmaf(w, v.x, o[n][0]); o[n][1] = fmaf(w, v.y, o[n][1]); o[n][2] = fmaf(w, v.z, o[n][2]); o[n][3] = fmaf(w, v.w, o[n][3]);
+            }
+        }
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    bool off = !(inv < INFINITY);
+#pragma unroll
+    for (int n = 0; n < PIECES; ++n) {
+#pragma unroll
+        for (float& x : o[n]) {
+            x *= inv;
+            off = off || !(fabsf(x) < INFINITY);
+        }
+        tile[lane][warp * PIECES + n] = make_uint2(pack_bf16(o[n][0], o[n][1]), pack_bf16(o[n][2], o[n][3]));
+    }
+    const uint32_t mine = __ballot_sync(0xffffffffu, off);
+    if (lane == 0) bad[warp] = mine;
+    if (warp == 0 && i < p.tq && p.lse != nullptr && !off)
+        p.lse[bh * p.tq + i] = total == 0.0f ? -INFINITY : (top + log2f(total)) * (1.0f / kLog2e);
+    __syncthreads();
+    uint32_t again = 0;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) again |= bad[w];
+    for (int r = warp; r < 32 && r0 + r < p.tq; r += kJoinWarps) {
+        if (again >> r & 1u) {   // as after one pass: from the keys that the row sees
+            attn::forward_row(p, b, h, r0 + r, r0 + r + p.tk - p.tq);
+        } else if (lane * 4 < p.head_dim) {
+            *reinterpret_cast<uint2*>(attn::row_to(p.out, b, r0 + r, h) + lane * 4) = tile[r][lane];
+        }
     }
 }
 
@@ -1161,17 +1244,72 @@ cudaError_t launch_attention_bwd_sm100(AttentionParams p, const CUtensorMap* m, 
     return e;
 }
 
-cudaError_t launch_attention_fwd_sm100(const AttentionParams& p, const CUtensorMap* m, DeviceStatus* status, uint64_t wait_ns, cudaStream_t stream) {
+// In how many parts the keys of a query block are done: more than one where the blocks alone leave SMs without work.
+namespace {
+int fwd_parts(const AttentionParams& p, int sms) {
+    const bool narrow = p.head_dim <= 64, pair_heads = !narrow && p.group % 2 == 0;
+    const int per = narrow || pair_heads ? kRows : 2 * kRows;
+    const int64_t blocks_q = (p.tq + per - 1) / per, units = static_cast<int64_t>(p.batch) * p.heads / (pair_heads ? 2 : 1), slots = static_cast<int64_t>(sms) * (narrow ? 2 : 1);
+    if (units * blocks_q >= 2 * slots) return 1;
+    int64_t total = 0, most = 0;   // tiles of all blocks, of the longest
+    for (int64_t q = 0; q < blocks_q; ++q) {
+        const int64_t p0 = q * per + p.tk - p.tq, p1 = (p.tq < (q + 1) * per ? p.tq : (q + 1) * per) - 1 + p.tk - p.tq;
+        if (p1 < 0) continue;
+        const int64_t begin = p0 - p.window + 1 > 0 ? p0 - p.window + 1 : 0, low = begin / kRows;
+        const int64_t kept = ((p.sinks < begin ? p.sinks : begin) + kRows - 1) / kRows;
+        const int64_t n = (kept < low ? kept : low) + p1 / kRows - low + 1;
+        total += n;
+        most = n > most ? n : most;
+    }
+    // Microseconds of a tile (where two blocks share an SM, and where they do not), of a block's beginning and end, and of the
+    // join: fitted to 1 .. 32 parts of seventeen shapes.  64 queries on 8192 keys, 16 heads on 4 of 128: 125 us whole, 22.6 in 16
+    // parts; 2 x 8192 of 128: 127 and 56 (4 parts); 4 x 4096 of 64: 49 and 37 (4); 12 x 1024 of 64: 16.4 and 20 (2: not taken).
+    const float alone = narrow ? 1.3f : 1.85f, shared = narrow ? 1.7f : 1.85f, per_block = 6.0f;
+    const int64_t blocks = units * blocks_q, row_blocks = static_cast<int64_t>(p.batch) * p.heads * ((p.tq + kRows - 1) / kRows);
+    float best = 0.0f;
+    int chosen = 1;
+    for (int parts : {1, 2, 3, 4, 6, 8, 12, 16, 24, kMostParts}) {
+        if (parts > 1 && parts * 2 > most) break;
+        const float longest = per_block + static_cast<float>((most + parts - 1) / parts) * (blocks * parts > sms ? shared : alone);
+        const float share = (static_cast<float>(total * units) * shared + static_cast<float>(blocks * parts) * per_block) / static_cast<float>(slots);
+        const float cost = (blocks * parts <= slots ? longest : (share > longest ? share : longest) + 0.25f * longest) +
+                           (parts > 1 ? 4.0f + static_cast<float>(row_blocks * parts) * (narrow ? 32768.0f : 65536.0f) / 3.5e6f : 0.0f);
+        if (parts == 1 || cost < best) {
+            best = cost;
+            chosen = parts;
+        }
+    }
+    return chosen;
+}
+}  // namespace
+
+size_t attention_fwd_sm100_workspace(const AttentionParams& p, int sms) {
+    if (p.tq == 0 || p.tk == 0 || p.batch == 0 || p.heads == 0) return 0;
+    const int parts = fwd_parts(p, sms);
+    return parts == 1 ? 0 : static_cast<size_t>(p.batch) * p.heads * ((p.tq + kRows - 1) / kRows) * kRows * parts * ((p.head_dim <= 64 ? 64 : 128) + 1) * sizeof(float);
+}
+
+cudaError_t launch_attention_fwd_sm100(AttentionParams p, const CUtensorMap* m, void* workspace, int sms, DeviceStatus* status, uint64_t wait_ns,
+                                       cudaStream_t stream) {
     AttentionMaps maps{};
     maps.q = m[0]; maps.k = m[1]; maps.v = m[2]; maps.out = m[3];
-    const int64_t heads = static_cast<int64_t>(p.batch) * p.heads;
-    if (p.head_dim <= 64) {
+    const bool narrow = p.head_dim <= 64;
+    const int parts = workspace != nullptr ? fwd_parts(p, sms) : 1;
+    const int64_t heads = static_cast<int64_t>(p.batch) * p.heads, row_blocks = heads * ((p.tq + kRows - 1) / kRows);
+    p.partial = static_cast<float*>(workspace);
+    p.dvec = parts > 1 ? p.partial + row_blocks * kRows * parts * (narrow ? 64 : 128) : nullptr;
+    cudaError_t e;
+    if (narrow) {
         const int blocks_q = (p.tq + kRows - 1) / kRows;
-        return launch_sm(attention_fwd_kernel<1, 1>, heads * blocks_q, 192, fwd_smem<1, 1>(), stream, maps, p, 0, blocks_q, status, wait_ns);
+        e = launch_sm(attention_fwd_kernel<1, 1>, heads * blocks_q * parts, 192, fwd_smem<1, 1>(), stream, maps, p, 0, blocks_q, parts, status, wait_ns);
+    } else {
+        const int pair_heads = p.group % 2 == 0, per = pair_heads ? kRows : 2 * kRows, blocks_q = (p.tq + per - 1) / per;
+        e = launch_sm(attention_fwd_kernel<2, 2>, heads / (pair_heads ? 2 : 1) * blocks_q * parts, 320, fwd_smem<2, 2>(), stream, maps, p, pair_heads, blocks_q,
+                      parts, status, wait_ns);
     }
-    const int pair_heads = p.group % 2 == 0, per = pair_heads ? kRows : 2 * kRows, blocks_q = (p.tq + per - 1) / per;
-    return launch_sm(attention_fwd_kernel<2, 2>, heads / (pair_heads ? 2 : 1) * blocks_q, 320, fwd_smem<2, 2>(), stream, maps, p, pair_heads, blocks_q, status,
-                     wait_ns);
+    if (e != cudaSuccess || parts == 1) return e;
+    return narrow ? launch_dependent(attention_fwd_join_kernel<2>, static_cast<unsigned>(row_blocks * 4), kJoinWarps * 32, stream, p, parts)
+                  : launch_dependent(attention_fwd_join_kernel<4>, static_cast<unsigned>(row_blocks * 4), kJoinWarps * 32, stream, p, parts);
 }
 
 }  // namespace llmt_b200

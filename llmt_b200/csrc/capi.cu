@@ -2148,6 +2148,12 @@ int head_map(CUtensorMap* map, const HeadView& v, const AttentionParams& p, bool
 
 }  // namespace
 
+uint64_t llmt_b200_attention_window_fwd_workspace_bytes(const llmt_b200_attention_desc* d) {
+    AttentionParams p;
+    if (attention_params(d, "attention_window_fwd", &p) != LLMT_B200_OK) return 0;
+    return (attention_fwd_sm100_workspace(p, sm_count()) + 15) / 16 * 16;
+}
+
 int llmt_b200_attention_window_fwd(const llmt_b200_attention_desc* d, void* stream) {
     const char* who = "attention_window_fwd";
     AttentionParams p;
@@ -2159,6 +2165,14 @@ int llmt_b200_attention_window_fwd(const llmt_b200_attention_desc* d, void* stre
     if (st == LLMT_B200_OK) st = attention_apart(d, who, "lse", d->lse, 4 * static_cast<size_t>(d->batch * d->heads * d->tokens_q), t, 4);
     if (st != LLMT_B200_OK) return st;
     if (p.batch == 0 || p.heads == 0 || p.tq == 0) return LLMT_B200_OK;
+    const uint64_t need = llmt_b200_attention_window_fwd_workspace_bytes(d);
+    if (need > 0 && d->workspace != nullptr && d->workspace_bytes >= need) {
+        if (misaligned(d->workspace, 16)) return fail(LLMT_B200_ERR_INVALID, "%s: workspace is not 16-byte aligned", who);
+        st = attention_apart(d, who, "workspace", d->workspace, need, t, 4);
+        if (st != LLMT_B200_OK) return st;
+        if (d->lse != nullptr && overlaps(d->workspace, need, d->lse, 4 * static_cast<size_t>(d->batch * d->heads * d->tokens_q)))
+            return fail(LLMT_B200_ERR_INVALID, "%s: workspace overlaps lse", who);
+    }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t e;
     if (p.tk == 0) {
@@ -2172,7 +2186,7 @@ int llmt_b200_attention_window_fwd(const llmt_b200_attention_desc* d, void* stre
         if (st != LLMT_B200_OK) return st;
         DeviceStatus* status = device_status_ptr();
         if (status == nullptr) return fail(LLMT_B200_ERR_CUDA, "cannot resolve the device status word");
-        e = launch_attention_fwd_sm100(p, maps, status, g_wait_limit_ns, s);
+        e = launch_attention_fwd_sm100(p, maps, need > 0 && d->workspace_bytes >= need ? d->workspace : nullptr, sm_count(), status, g_wait_limit_ns, s);
     }
     if (e != cudaSuccess) return fail(LLMT_B200_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
     return LLMT_B200_OK;

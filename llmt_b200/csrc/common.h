@@ -267,8 +267,8 @@ struct HeadView {
 struct AttentionParams {
     HeadView q, k, v, out, dout, dq, dk, dv;
     float* lse;                // [batch][heads][tq]
-    float* dvec;               // workspace: rowsum(dout * out), [batch][heads][tq]
-    float* partial;            // workspace: sums of dV and dK of key tiles that are done in parts
+    float* dvec;               // workspace: rowsum(dout * out), [batch][heads][tq]; forward: log2 sum exp of each part of a row
+    float* partial;            // workspace: sums of dV and dK of key tiles that are done in parts; forward: outputs of a row's parts
     const int32_t* lengths;    // one new token: keys of each sequence, or null (all)
     int32_t batch, heads, group, tq, tk, head_dim;   // group: query heads that share a key head
     int32_t window, sinks;     // 1 <= window <= max(tk, 1), 0 <= sinks <= tk
@@ -390,7 +390,9 @@ cudaError_t launch_norm_residual_bwd(const NormResidualParams& p, const NormResi
                                      cudaStream_t stream);
 cudaError_t launch_attention_window_fwd(const AttentionParams& p, cudaStream_t stream);
 // The tensor-core form; maps of q, k, v, out: boxes of 128 rows x 64 values, 128-byte swizzle.
-cudaError_t launch_attention_fwd_sm100(const AttentionParams& p, const CUtensorMap* maps, DeviceStatus* status, uint64_t wait_ns, cudaStream_t stream);
+cudaError_t launch_attention_fwd_sm100(AttentionParams p, const CUtensorMap* m, void* workspace, int sms, DeviceStatus* status, uint64_t wait_ns,
+                                       cudaStream_t stream);
+size_t attention_fwd_sm100_workspace(const AttentionParams& p, int sms);
 // The backward kernels; maps of q, dout, k, v, dq with boxes of 128, 128, 64, 64, 128 rows, then of q, dout, k, v, dk, dv with boxes
 // of 64, 64, 128, 128, 128, 128 rows.
 cudaError_t launch_attention_bwd_sm100(AttentionParams p, const CUtensorMap* maps, void* workspace, int sms, DeviceStatus* status, uint64_t wait_ns,

@@ -40,6 +40,7 @@ typedef struct {
     int (*attention_window_fwd)(const llmt_b200_attention_desc*, void*);
     int (*attention_window_bwd)(const llmt_b200_attention_desc*, void*);
     int (*attention_window_decode)(const llmt_b200_attention_desc*, void*);
+    uint64_t (*attention_window_fwd_workspace_bytes)(const llmt_b200_attention_desc*);
     uint64_t (*attention_window_workspace_bytes)(const llmt_b200_attention_desc*);
     uint64_t (*attention_window_decode_workspace_bytes)(const llmt_b200_attention_desc*);
 } Entry;
@@ -47,7 +48,8 @@ static const char* const kNames[] = {"gemm", "gemm_workspace_bytes_for", "gemm_g
                                      "gemm_softmax_fwd", "gemm_softmax_bwd", "rowdot", "head_split", "head_merge",
                                      "cross_entropy_fwd", "cross_entropy_bwd", "lm_head_ce_fwd", "lm_head_ce_bwd",
                                      "rope", "norm_residual_fwd", "norm_residual_bwd", "norm_residual_workspace_bytes", "attention_window_fwd",
-                                     "attention_window_bwd", "attention_window_decode", "attention_window_workspace_bytes",
+                                     "attention_window_bwd", "attention_window_decode", "attention_window_fwd_workspace_bytes",
+                                     "attention_window_workspace_bytes",
                                      "attention_window_decode_workspace_bytes"};
 #define N_ENTRIES ((Py_ssize_t)(sizeof(kNames) / sizeof(kNames[0])))
 _Static_assert(sizeof(Entry) == sizeof(kNames), "one pointer per name");
@@ -634,7 +636,7 @@ static int attention_of(llmt_b200_attention_desc* d, const Tensor* q, const Tens
 }
 
 FAST(attention_window_fwd) {
-    BEGIN(5, "out", "lse", "q", "k", "v", "window", "sinks", "scale", "stream");
+    BEGIN(5, "out", "lse", "q", "k", "v", "window", "sinks", "scale", "workspace", "stream");
     llmt_b200_attention_desc d;
     Tensor out, q, k, vv;
     int dev = -1;
@@ -643,11 +645,26 @@ FAST(attention_window_fwd) {
     NEED(as_heads(v[0], &out, &d.out, &dev) == 0 && as_heads(v[2], &q, &d.q, &dev) == 0 && as_heads(v[3], &k, &d.k, &dev) == 0 &&
          as_heads(v[4], &vv, &d.v, &dev) == 0);
     NEED(attention_of(&d, &q, &k, &vv, v[5], v[6], v[7]) == 0 && out.dtype == q.dtype && same_shape(&out, &q) &&
-         as_vector(v[1], LLMT_B200_FP32, d.batch * d.heads * d.tokens_q, &dev, &lse) == 0 && stream_of(v[8], dev, &s) == 0);
+         as_vector(v[1], LLMT_B200_FP32, d.batch * d.heads * d.tokens_q, &dev, &lse) == 0);
     d.lse = (float*)lse;
-    RUN(E.attention_window_fwd(&d, s));
+    PyObject* scratch = NULL;
+    if (is_there(v[8])) NEED(as_workspace(v[8], &dev, &d.workspace, &d.workspace_bytes) == 0);
+    NEED(stream_of(v[9], dev, &s) == 0);
+    if (!is_there(v[8])) {
+        d.workspace_bytes = E.attention_window_fwd_workspace_bytes(&d);
+        if (d.workspace_bytes > 0) {
+            scratch = scratch_for(d.workspace_bytes, v[2], v[9]);
+            if (scratch == NULL) return NULL;
+            if (as_ptr(scratch, &d.workspace) < 0) { Py_DECREF(scratch); SLOW(); }
+        }
+    }
+    int st;
+    Py_BEGIN_ALLOW_THREADS
+    st = E.attention_window_fwd(&d, s);
+    Py_END_ALLOW_THREADS
+    Py_XDECREF(scratch);
+    return finish(st);
 }
-
 FAST(attention_window_bwd) {
     BEGIN(9, "dq", "dk", "dv", "dout", "q", "k", "v", "out", "lse", "window", "sinks", "scale", "workspace", "stream");
     llmt_b200_attention_desc d;

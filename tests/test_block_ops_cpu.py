@@ -273,6 +273,16 @@ def test_attention_window_fwd_refuses(kw, status, needle):
     assert needle in L.last_error()
 
 
+def test_attention_window_fwd_refuses_a_workspace_on_a_tensor():
+    """64 queries on 8192 keys: done in parts, whose workspace is checked like any other (one that is too small is not used)."""
+    d = dict(batch=1, tokens_q=64, tokens_k=8192, q=view(1 * MB, 0, 256, 64), out=view(2 * MB, 0, 256, 64), k=view(100 * MB, 0, 128, 64), v=view(110 * MB, 0, 128, 64),
+             workspace_bytes=80 * MB)
+    lib = L.lib()
+    assert 0 < lib.llmt_b200_attention_window_fwd_workspace_bytes(ctypes.byref(attn_desc(**d))) <= 60 * MB
+    for at, needle in ((21 * MB + 8, "16-byte aligned"), (100 * MB, "workspace overlaps k"), (2 * MB + 64, "workspace overlaps out"), (20 * MB, "workspace overlaps lse")):
+        assert lib.llmt_b200_attention_window_fwd(ctypes.byref(attn_desc(**d, workspace=at)), None) == L.ERR_INVALID and needle in L.last_error()
+
+
 @pytest.mark.parametrize("kw,status,needle", [s for s in SHAPES if "out" not in s[0]] + [
     (dict(dout=view(3 * MB, 16 * 256, 256, 0)), L.ERR_INVALID, "dout is broadcast"),
     (dict(dq=view(1 * MB, 16 * 256, 256, 64)), L.ERR_INVALID, "dq overlaps q"),
@@ -340,7 +350,8 @@ def test_workspace_queries_answer_nothing_for_bad_descriptors():
     assert lib.llmt_b200_norm_residual_workspace_bytes(ctypes.byref(norm_desc(True, cols=0))) == 0
     assert lib.llmt_b200_attention_window_workspace_bytes(ctypes.byref(attn_desc(True, kv_heads=3))) == 0
     assert lib.llmt_b200_attention_window_decode_workspace_bytes(ctypes.byref(decode_desc(head_dim=12))) == 0
-    for f in ("norm_residual_workspace_bytes", "attention_window_workspace_bytes", "attention_window_decode_workspace_bytes"):
+    assert lib.llmt_b200_attention_window_fwd_workspace_bytes(ctypes.byref(attn_desc(head_dim=4))) == 0
+    for f in ("norm_residual_workspace_bytes", "attention_window_workspace_bytes", "attention_window_fwd_workspace_bytes", "attention_window_decode_workspace_bytes"):
         assert getattr(lib, "llmt_b200_" + f)(None) == 0
 
 
