@@ -494,7 +494,7 @@ attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_co
                 }
             }
             if (parts > 1) {
-                if (i < p.tq) p.dvec[place * kRows + row] = l == 0.0f ? -INFINITY : fmaf(m, c, log2f(l));
+                if (i < p.tq) p.part_stats[place * kRows + row] = l == 0.0f ? -INFINITY : fmaf(m, c, log2f(l));
             } else {
                 if (i < p.tq && p.lse != nullptr) p.lse[line] = l == 0.0f ? -INFINITY : fmaf(m, p.scale, log2f(l) * (1.0f / kLog2e));
                 // A product with a hidden value that is not finite (0 * inf) has spoilt the row, or it sees such a value: it is
@@ -518,30 +518,31 @@ attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_co
     }
 }
 
-// Joins the parts of 32 rows that were done in parts: out = sum of 2^(s_part - max) out_part over the sum of the
-// 2^(s_part - max), s_part = log2 sum exp of a part's scores.  A lane has a row, a warp PIECES of the row's 16-byte pieces; the
-// results cross shared memory, so that reads and writes are contiguous.
+// Joins the parts of 32 rows that were done in parts.  Forward: out = sum of 2^(s_part - max) out_part over the sum of the
+// 2^(s_part - max), s_part = log2 sum exp of a part's scores.  Backward: dQ and D are the parts' sums.  A lane has a row, a warp
+// PIECES of the row's 16-byte pieces; the results cross shared memory, so that reads and writes are contiguous.
 constexpr int kJoinWarps = 8, kMostParts = 32;
-template <int PIECES>
-__global__ void __launch_bounds__(kJoinWarps * 32) attention_fwd_join_kernel(AttentionParams p, int parts) {
+template <int PIECES, bool FORWARD>
+__global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(AttentionParams p, int parts) {
     constexpr int kPieces = PIECES * kJoinWarps;
     __shared__ uint2 tile[32][kPieces + 1];
     __shared__ uint32_t bad[kJoinWarps];
+    if (!FORWARD) grid_launch_dependents();   // the launch for dK and dV
     grid_dependency_wait();
     const int blocks_q = (p.tq + kRows - 1) / kRows, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t block = blockIdx.x / 4, bh = block / blocks_q, b = bh / p.heads, h = bh % p.heads;
     const int in_block = static_cast<int>(blockIdx.x % 4) * 32 + lane;
     const int64_t r0 = block % blocks_q * kRows + blockIdx.x % 4 * 32, i = r0 + lane;
     if (r0 >= p.tq) return;
-    const float* const stat = p.dvec + block * parts * kRows + in_block;
+    const float* const stat = p.part_stats + block * parts * kRows + in_block;
     const float4* const from = reinterpret_cast<const float4*>(p.partial) + (block * parts * kPieces + warp * PIECES) * kRows + in_block;
     float top = -INFINITY, total = 0.0f, o[PIECES][4] = {};
     if (i < p.tq) {
-        for (int part = 0; part < parts; ++part) top = fmaxf(top, stat[part * kRows]);
+        for (int part = 0; FORWARD && part < parts; ++part) top = fmaxf(top, stat[part * kRows]);
 #pragma unroll 2
         for (int part = 0; part < parts; ++part) {
-            const float s = stat[part * kRows], w = s == -INFINITY ? 0.0f : exp2f(s - top);   // NaN in a part: in all
-            total += w;
+            const float s = stat[part * kRows], w = !FORWARD ? 1.0f : s == -INFINITY ? 0.0f : exp2f(s - top);   // NaN in a part: in all
+            total += FORWARD ? w : s;
 #pragma unroll
             for (int n = 0; n < PIECES; ++n) {
                 if ((warp * PIECES + n) * 4 >= p.head_dim || w == 0.0f) continue;
@@ -550,8 +551,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_fwd_join_kernel(Att
             }
         }
     }
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    bool off = !(inv < INFINITY);
+    const float inv = !FORWARD ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
+    bool off = FORWARD && !(inv < INFINITY);
 #pragma unroll
     for (int n = 0; n < PIECES; ++n) {
 #pragma unroll
@@ -563,17 +564,21 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_fwd_join_kernel(Att
     }
     const uint32_t mine = __ballot_sync(0xffffffffu, off);
     if (lane == 0) bad[warp] = mine;
-    if (warp == 0 && i < p.tq && p.lse != nullptr && !off)
-        p.lse[bh * p.tq + i] = total == 0.0f ? -INFINITY : (top + log2f(total)) * (1.0f / kLog2e);
+    if (warp == 0 && i < p.tq) {
+        if (FORWARD && p.lse != nullptr && !off) p.lse[bh * p.tq + i] = total == 0.0f ? -INFINITY : (top + log2f(total)) * (1.0f / kLog2e);
+        if (!FORWARD)
+            p.dvec[bh * p.tq + i] = fabsf(total) < INFINITY ? total : attn::dot_rows(attn::row_of(p.dout, b, i, h), attn::row_of(p.out, b, i, h), p.head_dim);
+    }
     __syncthreads();
     uint32_t again = 0;
 #pragma unroll
     for (int w = 0; w < kJoinWarps; ++w) again |= bad[w];
     for (int r = warp; r < 32 && r0 + r < p.tq; r += kJoinWarps) {
         if (again >> r & 1u) {   // as after one pass: from the keys that the row sees
-            attn::forward_row(p, b, h, r0 + r, r0 + r + p.tk - p.tq);
+            if (FORWARD) attn::forward_row(p, b, h, r0 + r, r0 + r + p.tk - p.tq);
+            else attn::dq_row(p, b, h, r0 + r, attn::dot_rows(attn::row_of(p.dout, b, r0 + r, h), attn::row_of(p.out, b, r0 + r, h), p.head_dim));
         } else if (lane * 4 < p.head_dim) {
-            *reinterpret_cast<uint2*>(attn::row_to(p.out, b, r0 + r, h) + lane * 4) = tile[r][lane];
+            *reinterpret_cast<uint2*>(attn::row_to(FORWARD ? p.out : p.dq, b, r0 + r, h) + lane * 4) = tile[r][lane];
         }
     }
 }
@@ -792,11 +797,13 @@ __device__ __forceinline__ void row_products(const AttentionParams& p, int b, in
 // dQ of 128 queries: S = Q K^T and dP = dO V^T of 64 keys, dS = P (dP - D), dQ += dS K.
 // head_dim <= 64: one warpgroup a block and two blocks an SM, so that one works while the other begins or ends; dS has a place
 // of its own, and the next scores are made while the warpgroup works on the last ones.  (BUFFERS = 3 there: 8 x 12 x 1024,
-// window 256: dQ, dK, dV 100 us against 90; 2 x 16 x 4096: 368 against 344.)
+// window 256: dQ, dK, dV 100 us against 90; 2 x 16 x 4096: 368 against 344.)  Few query blocks are done in parts, as in the
+// forward pass.
 template <int HALVES, int BUFFERS> using DqRoles = BwdRoles<BUFFERS, BUFFERS * 2 * kCols + (BUFFERS == 1 ? kCols / 2 : 0) + 64 * HALVES>;
 template <int HALVES, int BUFFERS>
 __global__ void __launch_bounds__(128 * BUFFERS + 64, BUFFERS == 1 ? 2 : 1)
-attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_constant__ AttentionParams p, int blocks_q, DeviceStatus* status, uint64_t wait_ns) {
+attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_constant__ AttentionParams p, int blocks_q, int parts, DeviceStatus* status,
+                    uint64_t wait_ns) {
     extern __shared__ uint8_t raw[];
     uint8_t* const base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint8_t* const tiles_ptr = base + kBwdControl;
@@ -807,16 +814,19 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int units = p.batch * p.heads, unit = blockIdx.x % units;
     const int b = unit / p.heads, h = unit % p.heads, hk = h / p.group;
-    const int r0 = (blocks_q - 1 - static_cast<int>(blockIdx.x / units)) * kRows;
+    const int item = static_cast<int>(blockIdx.x / units), part = item % parts, r0 = (blocks_q - 1 - item / parts) * kRows;
     const int p0 = r0 + p.tk - p.tq, p1 = min(r0 + kRows, p.tq) - 1 + p.tk - p.tq;
     const int first = max(0, p0 - p.window + 1);
     const int low = first / kCols, sink_tiles = min((min(p.sinks, first) + kCols - 1) / kCols, low);
-    DqRoles<HALVES, BUFFERS> roles{reinterpret_cast<BwdControl*>(base), nullptr, status, wait_ns, p1 >= 0 ? sink_tiles + p1 / kCols - low + 1 : 0};
+    // this block's part of the tiles
+    const int n_tiles = p1 >= 0 ? sink_tiles + p1 / kCols - low + 1 : 0;
+    const int begin = static_cast<int>(static_cast<int64_t>(n_tiles) * part / parts), end = static_cast<int>(static_cast<int64_t>(n_tiles) * (part + 1) / parts);
+    DqRoles<HALVES, BUFFERS> roles{reinterpret_cast<BwdControl*>(base), nullptr, status, wait_ns, end - begin};
     roles.abort_flag = &roles.ctl->abort;
-    auto tile_of = [&](int it) { return it < sink_tiles ? it : low + it - sink_tiles; };
+    auto tile_of = [&](int it) { return begin + it < sink_tiles ? begin + it : low + begin + it - sink_tiles; };
     roles.set_up(warp);
     const uint32_t tmem = uniform(roles.ctl->tmem);
-    grid_launch_dependents();   // the launch for dK and dV
+    grid_launch_dependents();   // the launch that joins the parts, or the one for dK and dV
     grid_dependency_wait();
     const int steps_d = (p.head_dim + 15) / 16;
     const uint32_t ring = tiles + 2 * kFixed;
@@ -911,11 +921,13 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
         // A row of dS adds up to nothing but for what the rounding of `out` has put into D: dK's kernel gets D without it.
         roles.ctl->sums[w][row] = both(sum).x + both(sum).y;
         named_barrier_sync(1, roles.kSoftmax);
+        const int64_t place = (static_cast<int64_t>(unit) * blocks_q + r0 / kRows) * parts + part;   // of this part in the workspace, as in the forward pass
         if (w == 0 && i < p.tq) {
-            float more = d;
+            float more = part == 0 ? d : 0.0f;
 #pragma unroll
             for (int x = 0; x < kBuffers; ++x) more += roles.ctl->sums[x][row];
-            p.dvec[at] = fabsf(more) < INFINITY ? more : d;
+            if (parts > 1) p.part_stats[place * kRows + row] = more;
+            else p.dvec[at] = fabsf(more) < INFINITY ? more : d;
         }
         bool bad = false;
         for (int x = w; x < 4 * HALVES; x += kBuffers) {   // the warpgroups share the columns
@@ -932,12 +944,20 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
                 bad = bad || !(fabsf(f) < INFINITY);
                 o[y] = __float_as_uint(f);
             }
-            put_row16(tiles_ptr, row, x, o);
+            if (parts == 1) {
+                put_row16(tiles_ptr, row, x, o);
+            } else if (i < p.tq && x < steps_d) {
+                uint4* const to_part = reinterpret_cast<uint4*>(p.partial) + (place * (16 * HALVES) + x * 4) * kRows + row;
+#pragma unroll
+                for (int y = 0; y < 4; ++y) to_part[y * kRows] = make_uint4(o[4 * y], o[4 * y + 1], o[4 * y + 2], o[4 * y + 3]);
+            }
         }
-        // as in the forward kernel: a hidden key that is not finite has spoilt the row
-        copy_out(roles.ctl->bad, 1, roles.kSoftmax, threadIdx.x == 0, quarter, w == 0, __ballot_sync(0xffffffffu, bad && ok && i < p.tq), [&] {
-            for (int x = 0; x < HALVES; ++x) tma_store_4d(&maps.dq, tiles + x * kHalfTile, x * 64, r0, h, b);
-        }, [&](int r) { attn::dq_row(p, b, h, r0 + quarter * 32 + r, __shfl_sync(0xffffffffu, d, r)); });
+        if (parts == 1) {
+            // as in the forward kernel: a hidden key that is not finite has spoilt the row
+            copy_out(roles.ctl->bad, 1, roles.kSoftmax, threadIdx.x == 0, quarter, w == 0, __ballot_sync(0xffffffffu, bad && ok && i < p.tq), [&] {
+                for (int x = 0; x < HALVES; ++x) tma_store_4d(&maps.dq, tiles + x * kHalfTile, x * 64, r0, h, b);
+            }, [&](int r) { attn::dq_row(p, b, h, r0 + quarter * 32 + r, __shfl_sync(0xffffffffu, d, r)); });
+        }
     }
     roles.tear_down(warp, tmem);
 }
@@ -1211,8 +1231,72 @@ size_t dvec_bytes(const AttentionParams& p) { return (static_cast<size_t>(p.batc
 
 }  // namespace
 
+// In how many parts the keys of a query block are done: more than one where the blocks alone leave SMs without work.
+namespace {
+// Microseconds of a tile (where blocks share an SM's time, and where they do not), of a block's beginning and end.
+struct PartCosts {
+    float alone, shared, per_block;
+};
+int query_parts(const AttentionParams& p, int sms, int per, int64_t units, int blocks_per_sm, int cols, PartCosts cost_of) {
+    const int64_t blocks_q = (p.tq + per - 1) / per, blocks = units * blocks_q, slots = static_cast<int64_t>(sms) * blocks_per_sm;
+    if (blocks >= 2 * slots) return 1;
+    int64_t total = 0, most = 0;   // tiles of all blocks, of the longest
+    for (int64_t q = 0; q < blocks_q; ++q) {
+        const int64_t p0 = q * per + p.tk - p.tq, p1 = (p.tq < (q + 1) * per ? p.tq : (q + 1) * per) - 1 + p.tk - p.tq;
+        if (p1 < 0) continue;
+        const int64_t begin = p0 - p.window + 1 > 0 ? p0 - p.window + 1 : 0, low = begin / cols;
+        const int64_t kept = ((p.sinks < begin ? p.sinks : begin) + cols - 1) / cols;
+        const int64_t n = (kept < low ? kept : low) + p1 / cols - low + 1;
+        total += n;
+        most = n > most ? n : most;
+    }
+    const int64_t row_blocks = static_cast<int64_t>(p.batch) * p.heads * ((p.tq + kRows - 1) / kRows);
+    float best = 0.0f;
+    int chosen = 1;
+    for (int parts : {1, 2, 3, 4, 6, 8, 12, 16, 24, kMostParts}) {
+        if (parts > 1 && parts * 2 * kRows > most * cols) break;
+        const float longest = cost_of.per_block + static_cast<float>((most + parts - 1) / parts) * (blocks * parts > sms ? cost_of.shared : cost_of.alone);
+        const float share = (static_cast<float>(total * units) * cost_of.shared + static_cast<float>(blocks * parts) * cost_of.per_block) / static_cast<float>(slots);
+        const float cost = (blocks * parts <= slots ? longest : (share > longest ? share : longest) + 0.25f * longest) +
+                           (parts > 1 ? 4.0f + static_cast<float>(row_blocks * parts) * (p.head_dim <= 64 ? 32768.0f : 65536.0f) / 3.5e6f : 0.0f);   // the join
+        if (parts == 1 || cost < best) {
+            best = cost;
+            chosen = parts;
+        }
+    }
+    return chosen;
+}
+// Costs fitted to 1 .. 32 parts of seventeen shapes.  Forward: 64 queries on 8192 keys, 16 heads on 4 of 128: 125 us whole, 22 in 16
+// parts; 2 x 8192 of 128: 127 and 56 (4 parts); 4 x 4096 of 64: 49 and 37 (4); 12 x 1024 of 64: 16.4 and 20 (2: not taken).
+// Backward (with dK and dV): the first 124 and 46 (8 parts of dQ); 1 x 8192 of 64: 165 and 82 (8), of 128: 173 and 105 (4); 4 heads
+// on 1, 8192 of 128: 296 and 313 (2: not taken).
+int fwd_parts(const AttentionParams& p, int sms) {
+    const bool narrow = p.head_dim <= 64, pair_heads = !narrow && p.group % 2 == 0;
+    return query_parts(p, sms, narrow || pair_heads ? kRows : 2 * kRows, static_cast<int64_t>(p.batch) * p.heads / (pair_heads ? 2 : 1), narrow ? 2 : 1, kRows,
+                       narrow ? PartCosts{1.3f, 1.7f, 6.0f} : PartCosts{1.85f, 1.85f, 6.0f});
+}
+int dq_parts(const AttentionParams& p, int sms) {
+    const bool narrow = p.head_dim <= 64;
+    return query_parts(p, sms, kRows, static_cast<int64_t>(p.batch) * p.heads, narrow ? 2 : 1, kCols, narrow ? PartCosts{0.75f, 1.2f, 6.0f} : PartCosts{0.9f, 0.9f, 8.0f});
+}
+// What parts of query blocks take in a workspace: 16-byte pieces of fp32 rows, and a float a row.
+int64_t query_part_floats(const AttentionParams& p, int parts) {
+    return parts == 1 ? 0 : static_cast<int64_t>(p.batch) * p.heads * ((p.tq + kRows - 1) / kRows) * kRows * parts * ((p.head_dim <= 64 ? 64 : 128) + 1);
+}
+void put_query_parts(AttentionParams& p, int parts) {
+    p.part_stats = parts == 1 ? nullptr : p.partial + static_cast<int64_t>(p.batch) * p.heads * ((p.tq + kRows - 1) / kRows) * kRows * parts * (p.head_dim <= 64 ? 64 : 128);
+}
+template <bool FORWARD> cudaError_t launch_join(const AttentionParams& p, int parts, cudaStream_t stream) {
+    const unsigned blocks = static_cast<unsigned>(static_cast<int64_t>(p.batch) * p.heads * ((p.tq + kRows - 1) / kRows) * 4);
+    return p.head_dim <= 64 ? launch_dependent(attention_join_kernel<2, FORWARD>, blocks, kJoinWarps * 32, stream, p, parts)
+                            : launch_dependent(attention_join_kernel<4, FORWARD>, blocks, kJoinWarps * 32, stream, p, parts);
+}
+}  // namespace
+
 size_t attention_bwd_sm100_workspace(const AttentionParams& p, int sms) {
-    return dvec_bytes(p) + dkdv_partial_floats(p, dkdv_plan(p, sms)) * sizeof(float);
+    // the parts of dQ are joined before those of dK and dV come
+    const int64_t of_dq = p.tq > 0 && p.tk > 0 && p.batch > 0 && p.heads > 0 ? query_part_floats(p, dq_parts(p, sms)) : 0, of_dkdv = dkdv_partial_floats(p, dkdv_plan(p, sms));
+    return dvec_bytes(p) + (of_dq > of_dkdv ? of_dq : of_dkdv) * sizeof(float);
 }
 
 cudaError_t launch_attention_bwd_sm100(AttentionParams p, const CUtensorMap* m, void* workspace, int sms, DeviceStatus* status, uint64_t wait_ns,
@@ -1224,9 +1308,12 @@ cudaError_t launch_attention_bwd_sm100(AttentionParams p, const CUtensorMap* m, 
     maps.q = m[0]; maps.dout = m[1]; maps.k = m[2]; maps.v = m[3]; maps.dq = m[4];
     const int blocks_q = (p.tq + kRows - 1) / kRows;
     const bool narrow = p.head_dim <= 64;
-    int64_t blocks = static_cast<int64_t>(p.batch) * p.heads * blocks_q;
-    cudaError_t e = narrow ? launch_sm(attention_dq_kernel<1, 1>, blocks, DqRoles<1, 1>::kThreads, bwd_smem<1>(), stream, maps, p, blocks_q, status, wait_ns)
-                           : launch_sm(attention_dq_kernel<2, 3>, blocks, DqRoles<2, 3>::kThreads, bwd_smem<2>(), stream, maps, p, blocks_q, status, wait_ns);
+    const int parts = dq_parts(p, sms);
+    put_query_parts(p, parts);
+    int64_t blocks = static_cast<int64_t>(p.batch) * p.heads * blocks_q * parts;
+    cudaError_t e = narrow ? launch_sm(attention_dq_kernel<1, 1>, blocks, DqRoles<1, 1>::kThreads, bwd_smem<1>(), stream, maps, p, blocks_q, parts, status, wait_ns)
+                           : launch_sm(attention_dq_kernel<2, 3>, blocks, DqRoles<2, 3>::kThreads, bwd_smem<2>(), stream, maps, p, blocks_q, parts, status, wait_ns);
+    if (e == cudaSuccess && parts > 1) e = launch_join<false>(p, parts, stream);
     if (e != cudaSuccess) return e;
     maps.q = m[5]; maps.dout = m[6]; maps.k = m[7]; maps.v = m[8]; maps.dk = m[9]; maps.dv = m[10];
     const DkdvPlan pl = dkdv_plan(p, sms);
@@ -1244,49 +1331,9 @@ cudaError_t launch_attention_bwd_sm100(AttentionParams p, const CUtensorMap* m, 
     return e;
 }
 
-// In how many parts the keys of a query block are done: more than one where the blocks alone leave SMs without work.
-namespace {
-int fwd_parts(const AttentionParams& p, int sms) {
-    const bool narrow = p.head_dim <= 64, pair_heads = !narrow && p.group % 2 == 0;
-    const int per = narrow || pair_heads ? kRows : 2 * kRows;
-    const int64_t blocks_q = (p.tq + per - 1) / per, units = static_cast<int64_t>(p.batch) * p.heads / (pair_heads ? 2 : 1), slots = static_cast<int64_t>(sms) * (narrow ? 2 : 1);
-    if (units * blocks_q >= 2 * slots) return 1;
-    int64_t total = 0, most = 0;   // tiles of all blocks, of the longest
-    for (int64_t q = 0; q < blocks_q; ++q) {
-        const int64_t p0 = q * per + p.tk - p.tq, p1 = (p.tq < (q + 1) * per ? p.tq : (q + 1) * per) - 1 + p.tk - p.tq;
-        if (p1 < 0) continue;
-        const int64_t begin = p0 - p.window + 1 > 0 ? p0 - p.window + 1 : 0, low = begin / kRows;
-        const int64_t kept = ((p.sinks < begin ? p.sinks : begin) + kRows - 1) / kRows;
-        const int64_t n = (kept < low ? kept : low) + p1 / kRows - low + 1;
-        total += n;
-        most = n > most ? n : most;
-    }
-    // Microseconds of a tile (where two blocks share an SM, and where they do not), of a block's beginning and end, and of the
-    // join: fitted to 1 .. 32 parts of seventeen shapes.  64 queries on 8192 keys, 16 heads on 4 of 128: 125 us whole, 22.6 in 16
-    // parts; 2 x 8192 of 128: 127 and 56 (4 parts); 4 x 4096 of 64: 49 and 37 (4); 12 x 1024 of 64: 16.4 and 20 (2: not taken).
-    const float alone = narrow ? 1.3f : 1.85f, shared = narrow ? 1.7f : 1.85f, per_block = 6.0f;
-    const int64_t blocks = units * blocks_q, row_blocks = static_cast<int64_t>(p.batch) * p.heads * ((p.tq + kRows - 1) / kRows);
-    float best = 0.0f;
-    int chosen = 1;
-    for (int parts : {1, 2, 3, 4, 6, 8, 12, 16, 24, kMostParts}) {
-        if (parts > 1 && parts * 2 > most) break;
-        const float longest = per_block + static_cast<float>((most + parts - 1) / parts) * (blocks * parts > sms ? shared : alone);
-        const float share = (static_cast<float>(total * units) * shared + static_cast<float>(blocks * parts) * per_block) / static_cast<float>(slots);
-        const float cost = (blocks * parts <= slots ? longest : (share > longest ? share : longest) + 0.25f * longest) +
-                           (parts > 1 ? 4.0f + static_cast<float>(row_blocks * parts) * (narrow ? 32768.0f : 65536.0f) / 3.5e6f : 0.0f);
-        if (parts == 1 || cost < best) {
-            best = cost;
-            chosen = parts;
-        }
-    }
-    return chosen;
-}
-}  // namespace
-
 size_t attention_fwd_sm100_workspace(const AttentionParams& p, int sms) {
     if (p.tq == 0 || p.tk == 0 || p.batch == 0 || p.heads == 0) return 0;
-    const int parts = fwd_parts(p, sms);
-    return parts == 1 ? 0 : static_cast<size_t>(p.batch) * p.heads * ((p.tq + kRows - 1) / kRows) * kRows * parts * ((p.head_dim <= 64 ? 64 : 128) + 1) * sizeof(float);
+    return static_cast<size_t>(query_part_floats(p, fwd_parts(p, sms))) * sizeof(float);
 }
 
 cudaError_t launch_attention_fwd_sm100(AttentionParams p, const CUtensorMap* m, void* workspace, int sms, DeviceStatus* status, uint64_t wait_ns,
@@ -1295,9 +1342,9 @@ cudaError_t launch_attention_fwd_sm100(AttentionParams p, const CUtensorMap* m, 
     maps.q = m[0]; maps.k = m[1]; maps.v = m[2]; maps.out = m[3];
     const bool narrow = p.head_dim <= 64;
     const int parts = workspace != nullptr ? fwd_parts(p, sms) : 1;
-    const int64_t heads = static_cast<int64_t>(p.batch) * p.heads, row_blocks = heads * ((p.tq + kRows - 1) / kRows);
+    const int64_t heads = static_cast<int64_t>(p.batch) * p.heads;
     p.partial = static_cast<float*>(workspace);
-    p.dvec = parts > 1 ? p.partial + row_blocks * kRows * parts * (narrow ? 64 : 128) : nullptr;
+    put_query_parts(p, parts);
     cudaError_t e;
     if (narrow) {
         const int blocks_q = (p.tq + kRows - 1) / kRows;
@@ -1307,9 +1354,7 @@ cudaError_t launch_attention_fwd_sm100(AttentionParams p, const CUtensorMap* m, 
         e = launch_sm(attention_fwd_kernel<2, 2>, heads / (pair_heads ? 2 : 1) * blocks_q * parts, 320, fwd_smem<2, 2>(), stream, maps, p, pair_heads, blocks_q,
                       parts, status, wait_ns);
     }
-    if (e != cudaSuccess || parts == 1) return e;
-    return narrow ? launch_dependent(attention_fwd_join_kernel<2>, static_cast<unsigned>(row_blocks * 4), kJoinWarps * 32, stream, p, parts)
-                  : launch_dependent(attention_fwd_join_kernel<4>, static_cast<unsigned>(row_blocks * 4), kJoinWarps * 32, stream, p, parts);
+    return e != cudaSuccess || parts == 1 ? e : launch_join<true>(p, parts, stream);
 }
 
 }  // namespace llmt_b200

@@ -84,6 +84,30 @@ def test_hidden_places_reach_no_part(bad, hd):
     assert not bool(torch.isfinite(out[:, ~clean].float()).all(-1).any())
 
 
+@pytest.mark.parametrize("bad", [float("nan"), float("-inf"), torch.finfo(BF).max])
+@pytest.mark.parametrize("b,h,hkv,tq,tk,hd,window,sinks", [(1, 2, 1, 900, 4000, 128, 1500, 4), (1, 2, 2, 300, 2900, 64, 1200, 0), (1, 1, 1, 1300, 1200, 64, 0, 0)])
+def test_gradients_of_parts(b, h, hkv, tq, tk, hd, window, sinks, bad):
+    """dQ in parts (the workspace is larger than one whole pass wants), its share of D, and dK and dV after it, with keys that
+    no query sees and queries that see nothing holding anything."""
+    q, k, v, dout = _inputs(b, h, hkv, tq, tk, hd, seed=3)
+    seen = _visible(tq, tk, window, sinks)
+    hidden, idle = ~seen.any(0), ~seen.any(1)
+    assert bool(hidden.any()) or bool(idle.any())
+    ks, vs, qs, douts = k.clone(), v.clone(), q.clone(), dout.clone()
+    for clean, spoilt, rows in ((k, ks, hidden), (v, vs, hidden), (q, qs, idle), (dout, douts, idle)):
+        clean[:, rows], spoilt[:, rows] = 0, bad
+    out, lse = _results(q)
+    L.attention_window_fwd(out, lse, qs, ks, vs, window, sinks)
+    _check_forward(out, lse, q, k, v, window, sinks)
+    dq, dk, dv = (torch.full_like(x, float("nan")) for x in (q, k, v))
+    L.attention_window_bwd(dq, dk, dv, douts, qs, ks, vs, out, lse, window, sinks)
+    _check_backward(dq, dk, dv, dout, q, k, v, out, lse, window, sinks)
+    assert bool((dk[:, hidden] == 0).all()) and bool((dv[:, hidden] == 0).all()) and bool((dq[:, idle] == 0).all())
+    again = [torch.full_like(x, float("nan")) for x in (q, k, v)]
+    L.attention_window_bwd(*again, douts, qs, ks, vs, out, lse, window, sinks)
+    assert all(torch.equal(x, y) for x, y in zip(again, (dq, dk, dv)))
+
+
 def test_parts_in_a_graph_and_on_another_stream():
     q, k, v, _ = _inputs(1, 2, 1, 64, 8192, 128, seed=2)
     out, lse = _results(q)
