@@ -510,9 +510,9 @@ LLMT_B200_API uint64_t llmt_b200_norm_residual_workspace_bytes(const llmt_b200_n
  * order; with a smaller one or none they are not.
  *
  * _bwd: dV = P^T dO,  dS = P (dP - D) with dP = dO v^T,  dQ = scale dS k,  dK = scale dS^T q, from out and
- * lse as _fwd left them.  D = rowsum(P dP) is taken as rowsum(dO out) for dQ; a row of dS adds up to nothing
- * but for the rounding of out, which is taken out of D again before dK is formed.  workspace: 16-byte
- * aligned, llmt_b200_attention_window_workspace_bytes(desc) bytes.
+ * lse as _fwd left them.  D = rowsum(P dP) is taken as rowsum(dO out) for dQ where a query may see more than
+ * 128 keys, among which the rounding of out is lost beside that of dS; a row of dS adds up to nothing but for
+ * that rounding, which is taken out of D again before dK is formed.  workspace: 16-byte aligned, llmt_b200_attention_window_workspace_bytes(desc) bytes.
  *
  * _decode: one new token per sequence (tokens_q = 1) over a cache of tokens_k places, of which
  * sequence b holds lengths[b] (device, int32; NULL: all; values beyond tokens_k count as tokens_k,

@@ -735,8 +735,9 @@ template <int BUFFERS, int TMEM> struct BwdRoles {
         __syncwarp();
         if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&ctl->taken));
     }
-    // work(it): what warpgroup `w` does with a tile's scores once they are there; before(it) ahead of the wait.
-    template <typename Before, typename Work> __device__ __forceinline__ bool tiles(int w, Before before, Work work) const {
+    // work(it): what warpgroup `w` does with a tile's scores once they are there; before(it) ahead of the wait; last() when the
+    // warpgroup has no more tiles, before the products of all are waited for.
+    template <typename Before, typename Work, typename Last> __device__ __forceinline__ bool tiles(int w, Before before, Work work, Last last) const {
         uint32_t phase = 0;
         for (int it = w; it < n; it += BUFFERS) {
             before(it);
@@ -749,6 +750,7 @@ template <int BUFFERS, int TMEM> struct BwdRoles {
             if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&ctl->ready[w]));
             phase ^= 1u;
         }
+        last();
         if (n == 0) return true;
         const bool ok = bounded_wait_warp(smem_u32(&ctl->done), 0, abort_flag, status, kDevWaitTmemFull, 100, wait_ns);
         tc_fence_after_thread_sync();
@@ -795,6 +797,10 @@ __device__ __forceinline__ void row_products(const AttentionParams& p, int b, in
 }
 
 // dQ of 128 queries: S = Q K^T and dP = dO V^T of 64 keys, dS = P (dP - D), dQ += dS K.
+// D = rowsum(dO out) carries the rounding of out.  Over many keys that is lost beside the roundings of dS; over few it is not
+// (normal operands, error of dQ's norm against the result's own rounding of 1.7e-3: 4.4e-3 for 2 keys, 2.9e-3 for 8, 2.5e-3 for
+// 128, where an exact D gives 2.4e-3 for any number).  `exact`: the tiles are gone through twice, the first time for D as the
+// sum of P dP, with zeros for dS.
 // head_dim <= 64: one warpgroup a block and two blocks an SM, so that one works while the other begins or ends; dS has a place
 // of its own, and the next scores are made while the warpgroup works on the last ones.  (BUFFERS = 3 there: 8 x 12 x 1024,
 // window 256: dQ, dK, dV 100 us against 90; 2 x 16 x 4096: 368 against 344.)  Few query blocks are done in parts, as in the
@@ -802,8 +808,8 @@ __device__ __forceinline__ void row_products(const AttentionParams& p, int b, in
 template <int HALVES, int BUFFERS> using DqRoles = BwdRoles<BUFFERS, BUFFERS * 2 * kCols + (BUFFERS == 1 ? kCols / 2 : 0) + 64 * HALVES>;
 template <int HALVES, int BUFFERS>
 __global__ void __launch_bounds__(128 * BUFFERS + 64, BUFFERS == 1 ? 2 : 1)
-attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_constant__ AttentionParams p, int blocks_q, int parts, DeviceStatus* status,
-                    uint64_t wait_ns) {
+attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_constant__ AttentionParams p, int blocks_q, int parts, int exact,
+                    DeviceStatus* status, uint64_t wait_ns) {
     extern __shared__ uint8_t raw[];
     uint8_t* const base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint8_t* const tiles_ptr = base + kBwdControl;
@@ -821,9 +827,13 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
     // this block's part of the tiles
     const int n_tiles = p1 >= 0 ? sink_tiles + p1 / kCols - low + 1 : 0;
     const int begin = static_cast<int>(static_cast<int64_t>(n_tiles) * part / parts), end = static_cast<int>(static_cast<int64_t>(n_tiles) * (part + 1) / parts);
-    DqRoles<HALVES, BUFFERS> roles{reinterpret_cast<BwdControl*>(base), nullptr, status, wait_ns, end - begin};
+    const int once = end - begin;
+    DqRoles<HALVES, BUFFERS> roles{reinterpret_cast<BwdControl*>(base), nullptr, status, wait_ns, exact ? 2 * once : once};
     roles.abort_flag = &roles.ctl->abort;
-    auto tile_of = [&](int it) { return begin + it < sink_tiles ? begin + it : low + begin + it - sink_tiles; };
+    auto tile_of = [&](int it) {
+        const int n = begin + (it < once ? it : it - once);
+        return n < sink_tiles ? n : low + n - sink_tiles;
+    };
     roles.set_up(warp);
     const uint32_t tmem = uniform(roles.ctl->tmem);
     grid_launch_dependents();   // the launch that joins the parts, or the one for dK and dV
@@ -866,9 +876,12 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
         const float c = p.scale * kLog2e;
         const int64_t at = (static_cast<int64_t>(b) * p.heads + h) * p.tq + i;
-        row_products<HALVES, BUFFERS == 1 ? 4 : 8>(p, b, h, r0, roles.ctl->d, warp);
-        named_barrier_sync(1, roles.kSoftmax);
-        const float d = roles.ctl->d[row];
+        float d = 0.0f;
+        if (!exact) {
+            row_products<HALVES, BUFFERS == 1 ? 4 : 8>(p, b, h, r0, roles.ctl->d, warp);
+            named_barrier_sync(1, roles.kSoftmax);
+            d = roles.ctl->d[row];
+        }
         float lse2 = INFINITY;   // P = 0 for a query that is not there or sees nothing
         if (i < p.tq) {
             const float lse = p.lse[at];
@@ -876,8 +889,22 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
         }
         const int pw = r0 + quarter * 32 + p.tk - p.tq;   // position of the warp's first query
         uint64_t sum = 0;
-        const uint64_t c2 = two(c, c), less2 = two(-lse2, -lse2), lessd = two(-d, -d);
-        const bool ok = roles.tiles(w, [](int) {}, [&](int it) {
+        const uint64_t c2 = two(c, c), less2 = two(-lse2, -lse2);
+        uint64_t lessd = two(-d, -d);
+        bool first_time = exact != 0;   // D is still being summed
+        auto have_d = [&]() {
+            roles.ctl->sums[w][row] = both(sum).x + both(sum).y;
+            named_barrier_sync(1, roles.kSoftmax);
+#pragma unroll
+            for (int x = 0; x < kBuffers; ++x) d += roles.ctl->sums[x][row];
+            named_barrier_sync(1, roles.kSoftmax);   // they are written once more
+            lessd = two(-d, -d);
+            sum = 0;
+            first_time = false;
+        };
+        const bool ok = roles.tiles(w, [&](int it) {
+            if (first_time && it >= once) have_d();
+        }, [&](int it) {
 #pragma unroll
             for (int x = 0; x < 2; ++x) {   // 32 keys at a time
                 const uint32_t ts = tmem + w * 2 * kCols + x * 32 + lanes;
@@ -911,13 +938,16 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
 #pragma unroll
                     for (int y = 0; y < 16; ++y) {
                         sum = add2(sum, f[y]);
-                        s[y] = pack_bf16(both(f[y]).x, both(f[y]).y);
+                        s[y] = first_time ? 0 : pack_bf16(both(f[y]).x, both(f[y]).y);
                     }
                 }
                 if (kEarly && x == 0 && it > 0) roles.wait_second(it - 1);   // they have read the last dS (a wait that runs out ends the next one too)
                 tmem_st_32x16(kEarly ? tmem_ds + x * 16 + lanes : ts, s);
             }
+        }, [&] {
+            if (first_time) have_d();   // before the last products are waited for: they wait for the other warpgroups' tiles
         });
+        if (first_time) have_d();   // a wait has run out: the other warpgroups are not left at the barrier
         // A row of dS adds up to nothing but for what the rounding of `out` has put into D: dK's kernel gets D without it.
         roles.ctl->sums[w][row] = both(sum).x + both(sum).y;
         named_barrier_sync(1, roles.kSoftmax);
@@ -1095,7 +1125,7 @@ attention_dkdv_kernel(const __grid_constant__ AttentionMaps maps, const __grid_c
                 tmem_st_32x16(ts, s);
                 tmem_st_32x16(ts + kCols, dp);
             }
-        });
+        }, [] {});
         // the warpgroups share the 16-column pieces of dV and dK
         bool bad = false;
         for (int x = w; x < 8 * HALVES; x += kBuffers) {
@@ -1310,9 +1340,12 @@ cudaError_t launch_attention_bwd_sm100(AttentionParams p, const CUtensorMap* m, 
     const bool narrow = p.head_dim <= 64;
     const int parts = dq_parts(p, sms);
     put_query_parts(p, parts);
+    // A query sees 128 keys or fewer: six tiles, twice, are never done in parts.
+    const int64_t seen = static_cast<int64_t>(p.window) + p.sinks;
+    const int exact = parts == 1 && (seen < p.tk ? seen : p.tk) <= 128;
     int64_t blocks = static_cast<int64_t>(p.batch) * p.heads * blocks_q * parts;
-    cudaError_t e = narrow ? launch_sm(attention_dq_kernel<1, 1>, blocks, DqRoles<1, 1>::kThreads, bwd_smem<1>(), stream, maps, p, blocks_q, parts, status, wait_ns)
-                           : launch_sm(attention_dq_kernel<2, 3>, blocks, DqRoles<2, 3>::kThreads, bwd_smem<2>(), stream, maps, p, blocks_q, parts, status, wait_ns);
+    cudaError_t e = narrow ? launch_sm(attention_dq_kernel<1, 1>, blocks, DqRoles<1, 1>::kThreads, bwd_smem<1>(), stream, maps, p, blocks_q, parts, exact, status, wait_ns)
+                           : launch_sm(attention_dq_kernel<2, 3>, blocks, DqRoles<2, 3>::kThreads, bwd_smem<2>(), stream, maps, p, blocks_q, parts, exact, status, wait_ns);
     if (e == cudaSuccess && parts > 1) e = launch_join<false>(p, parts, stream);
     if (e != cudaSuccess) return e;
     maps.q = m[5]; maps.dout = m[6]; maps.k = m[7]; maps.v = m[8]; maps.dk = m[9]; maps.dv = m[10];

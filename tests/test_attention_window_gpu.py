@@ -56,7 +56,7 @@ def _check_forward(out, lse, q, k, v, window, sinks, scale=None):
 
 
 def _check_backward(dq, dk, dv, dout, q, k, v, out, lse, window, sinks, scale=None):
-    """Against the formulas on what the call read: out and lse as stored."""
+    """Against the formulas on what the call read: lse as stored, and out for queries that may see more than 128 keys."""
     b, tq, h, hd = q.shape
     hkv, tk = k.shape[2], k.shape[1]
     c = scale or hd ** -0.5
@@ -64,6 +64,8 @@ def _check_backward(dq, dk, dv, dout, q, k, v, out, lse, window, sinks, scale=No
     qd, kd, vd, od, dod = (_heads(x, h) for x in (q, k, v, out, dout))
     p = torch.where(seen, (qd @ kd.transpose(-1, -2) * c - lse.double()[..., None]).exp(), 0)
     dp, d = dod @ vd.transpose(-1, -2), (dod * od).sum(-1, keepdim=True)
+    if min(window + sinks if window > 0 else tk, tk) <= 128:
+        d = (p * dp).sum(-1, keepdim=True)
     ds = torch.where(seen, p * (dp - d), 0)
     # dK is formed with the row sums of P dP, which are D but for the rounding of out
     ds_k = torch.where(seen, p * (dp - (p * dp).sum(-1, keepdim=True)), 0)
