@@ -705,6 +705,7 @@ def norm_residual_bwd(dx, dy, dout, dh, out, y=None, w_post=None, gate=None, w_p
             need = lib().llmt_b200_norm_residual_workspace_bytes(ctypes.byref(d))
             ws = _scratch(need, dx, stream) if need else None
         if ws is not None:
+            _need(ws.is_contiguous(), f"{who}: workspace must be contiguous")
             d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
         return lib().llmt_b200_norm_residual_bwd(ctypes.byref(d), s)
     _on(device, stream, call)
@@ -766,6 +767,7 @@ def attention_window_fwd(out, lse, q, k, v, window: int = 0, sinks: int = 0, sca
             need = lib().llmt_b200_attention_window_fwd_workspace_bytes(ctypes.byref(d))
             ws = _scratch(need, q, stream) if need else None
         if ws is not None:
+            _need(ws.is_contiguous(), f"{who}: workspace must be contiguous")
             d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
         return lib().llmt_b200_attention_window_fwd(ctypes.byref(d), s)
     _on(_device_of(who, out, lse, q, k, v, workspace), stream, call)
@@ -791,6 +793,7 @@ def attention_window_bwd(dq, dk, dv, dout, q, k, v, out, lse, window: int = 0, s
             need = lib().llmt_b200_attention_window_workspace_bytes(ctypes.byref(d))
             ws = _scratch(need, q, stream) if need else None
         if ws is not None:
+            _need(ws.is_contiguous(), f"{who}: workspace must be contiguous")
             d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
         return lib().llmt_b200_attention_window_bwd(ctypes.byref(d), s)
     _on(_device_of(who, dq, dk, dv, dout, q, k, v, out, lse, workspace), stream, call)
@@ -821,6 +824,7 @@ def attention_window_decode(out, q, k, v, lengths=None, window: int = 0, sinks: 
             need = lib().llmt_b200_attention_window_decode_workspace_bytes(ctypes.byref(d))
             ws = _scratch(need, q, stream) if need else None
         if ws is not None:
+            _need(ws.is_contiguous(), f"{who}: workspace must be contiguous")
             d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
         return lib().llmt_b200_attention_window_decode(ctypes.byref(d), s)
     _on(_device_of(who, out, q, k, v, lengths, lse, workspace), stream, call)

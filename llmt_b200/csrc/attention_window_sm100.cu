@@ -201,10 +201,11 @@ template <int WGS> struct FwdControl {
 
 template <int HALVES, int WGS> constexpr size_t fwd_smem() { return 2048 + static_cast<size_t>(WGS + FwdControl<WGS>::kSlots) * HALVES * kHalfTile; }
 
-template <int HALVES, int WGS>
+template <int HALVES, int WGS, bool PARTS>
 __global__ void __launch_bounds__(128 * WGS + 64, 3 - WGS)
-attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_constant__ AttentionParams p, int pair_heads, int blocks_q, int parts,
+attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_constant__ AttentionParams p, int pair_heads, int blocks_q, int n_parts,
                      DeviceStatus* status, uint64_t wait_ns) {
+    const int parts = PARTS ? n_parts : 1;   // (known to be one: 133 us instead of 136 for 8192 queries, window 2048, head_dim 128)
     using Control = FwdControl<WGS>;
     constexpr int kSlots = Control::kSlots, kLoadWarp = 4 * WGS, kProductWarp = 4 * WGS + 1, kHd = 64 * HALVES;
     constexpr bool kApart = HALVES == 1;   // the probabilities have a place of their own
@@ -263,6 +264,7 @@ attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_co
     __syncthreads();
     tc_fence_after_thread_sync();
     const uint32_t tmem = uniform(ctl->tmem);
+    if (parts > 1) grid_launch_dependents();   // the launch that joins them
     grid_dependency_wait();
 
     const uint32_t q_at = tiles, ring = tiles + WGS * kTile;
@@ -800,16 +802,19 @@ __device__ __forceinline__ void row_products(const AttentionParams& p, int b, in
 // D = rowsum(dO out) carries the rounding of out.  Over many keys that is lost beside the roundings of dS; over few it is not
 // (normal operands, error of dQ's norm against the result's own rounding of 1.7e-3: 4.4e-3 for 2 keys, 2.9e-3 for 8, 2.5e-3 for
 // 128, where an exact D gives 2.4e-3 for any number).  `exact`: the tiles are gone through twice, the first time for D as the
-// sum of P dP, with zeros for dS.
+// sum of P dP, with zeros for dS.  (Three kinds of the kernel, since the ordinary one gains 3 % from not having the others.)
 // head_dim <= 64: one warpgroup a block and two blocks an SM, so that one works while the other begins or ends; dS has a place
 // of its own, and the next scores are made while the warpgroup works on the last ones.  (BUFFERS = 3 there: 8 x 12 x 1024,
 // window 256: dQ, dK, dV 100 us against 90; 2 x 16 x 4096: 368 against 344.)  Few query blocks are done in parts, as in the
 // forward pass.
 template <int HALVES, int BUFFERS> using DqRoles = BwdRoles<BUFFERS, BUFFERS * 2 * kCols + (BUFFERS == 1 ? kCols / 2 : 0) + 64 * HALVES>;
-template <int HALVES, int BUFFERS>
+enum class Dq { kWhole, kParts, kExact };
+template <int HALVES, int BUFFERS, Dq KIND>
 __global__ void __launch_bounds__(128 * BUFFERS + 64, BUFFERS == 1 ? 2 : 1)
-attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_constant__ AttentionParams p, int blocks_q, int parts, int exact,
-                    DeviceStatus* status, uint64_t wait_ns) {
+attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_constant__ AttentionParams p, int blocks_q, int n_parts, DeviceStatus* status,
+                    uint64_t wait_ns) {
+    const int parts = KIND == Dq::kParts ? n_parts : 1;
+    constexpr bool exact = KIND == Dq::kExact;
     extern __shared__ uint8_t raw[];
     uint8_t* const base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint8_t* const tiles_ptr = base + kBwdControl;
@@ -891,7 +896,7 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
         uint64_t sum = 0;
         const uint64_t c2 = two(c, c), less2 = two(-lse2, -lse2);
         uint64_t lessd = two(-d, -d);
-        bool first_time = exact != 0;   // D is still being summed
+        bool first_time = exact;   // D is still being summed
         auto have_d = [&]() {
             roles.ctl->sums[w][row] = both(sum).x + both(sum).y;
             named_barrier_sync(1, roles.kSoftmax);
@@ -1342,10 +1347,13 @@ cudaError_t launch_attention_bwd_sm100(AttentionParams p, const CUtensorMap* m, 
     put_query_parts(p, parts);
     // A query sees 128 keys or fewer: six tiles, twice, are never done in parts.
     const int64_t seen = static_cast<int64_t>(p.window) + p.sinks;
-    const int exact = parts == 1 && (seen < p.tk ? seen : p.tk) <= 128;
+    const bool exact = (seen < p.tk ? seen : p.tk) <= 128;
     int64_t blocks = static_cast<int64_t>(p.batch) * p.heads * blocks_q * parts;
-    cudaError_t e = narrow ? launch_sm(attention_dq_kernel<1, 1>, blocks, DqRoles<1, 1>::kThreads, bwd_smem<1>(), stream, maps, p, blocks_q, parts, exact, status, wait_ns)
-                           : launch_sm(attention_dq_kernel<2, 3>, blocks, DqRoles<2, 3>::kThreads, bwd_smem<2>(), stream, maps, p, blocks_q, parts, exact, status, wait_ns);
+    auto dq = [&](auto kernel, int threads, size_t smem) { return launch_sm(kernel, blocks, threads, smem, stream, maps, p, blocks_q, parts, status, wait_ns); };
+    cudaError_t e = narrow ? dq(parts > 1 ? attention_dq_kernel<1, 1, Dq::kParts> : exact ? attention_dq_kernel<1, 1, Dq::kExact> : attention_dq_kernel<1, 1, Dq::kWhole>,
+                                DqRoles<1, 1>::kThreads, bwd_smem<1>())
+                           : dq(parts > 1 ? attention_dq_kernel<2, 3, Dq::kParts> : exact ? attention_dq_kernel<2, 3, Dq::kExact> : attention_dq_kernel<2, 3, Dq::kWhole>,
+                                DqRoles<2, 3>::kThreads, bwd_smem<2>());
     if (e == cudaSuccess && parts > 1) e = launch_join<false>(p, parts, stream);
     if (e != cudaSuccess) return e;
     maps.q = m[5]; maps.dout = m[6]; maps.k = m[7]; maps.v = m[8]; maps.dk = m[9]; maps.dv = m[10];
@@ -1381,10 +1389,10 @@ cudaError_t launch_attention_fwd_sm100(AttentionParams p, const CUtensorMap* m, 
     cudaError_t e;
     if (narrow) {
         const int blocks_q = (p.tq + kRows - 1) / kRows;
-        e = launch_sm(attention_fwd_kernel<1, 1>, heads * blocks_q * parts, 192, fwd_smem<1, 1>(), stream, maps, p, 0, blocks_q, parts, status, wait_ns);
+        e = launch_sm(parts > 1 ? attention_fwd_kernel<1, 1, true> : attention_fwd_kernel<1, 1, false>, heads * blocks_q * parts, 192, fwd_smem<1, 1>(), stream, maps, p, 0, blocks_q, parts, status, wait_ns);
     } else {
         const int pair_heads = p.group % 2 == 0, per = pair_heads ? kRows : 2 * kRows, blocks_q = (p.tq + per - 1) / per;
-        e = launch_sm(attention_fwd_kernel<2, 2>, heads / (pair_heads ? 2 : 1) * blocks_q * parts, 320, fwd_smem<2, 2>(), stream, maps, p, pair_heads, blocks_q,
+        e = launch_sm(parts > 1 ? attention_fwd_kernel<2, 2, true> : attention_fwd_kernel<2, 2, false>, heads / (pair_heads ? 2 : 1) * blocks_q * parts, 320, fwd_smem<2, 2>(), stream, maps, p, pair_heads, blocks_q,
                       parts, status, wait_ns);
     }
     return e != cudaSuccess || parts == 1 ? e : launch_join<true>(p, parts, stream);

@@ -477,12 +477,15 @@ static int as_vector(PyObject* o, int dtype, int64_t n, int* device, void** out)
     return 0;
 }
 static int as_workspace(PyObject* o, int* device, void** at, uint64_t* bytes) {
+    Tensor t;
     PyObject* nb = PyObject_GetAttr(o, s_nbytes);
     if (nb == NULL) { PyErr_Clear(); return -1; }
     *bytes = PyLong_AsUnsignedLongLong(nb);
     Py_DECREF(nb);
     if (PyErr_Occurred()) { PyErr_Clear(); return -1; }
-    return as_ptr(o, at) < 0 || on_device(o, device) < 0 ? -1 : 0;
+    if (as_tensor(o, &t) < 0 || !is_contiguous(&t) || on_device(o, device) < 0) return -1;
+    *at = t.ptr;
+    return 0;
 }
 // Scratch for one call; NULL with an exception set if torch has none.
 static PyObject* scratch_for(uint64_t need, PyObject* like, PyObject* stream) {

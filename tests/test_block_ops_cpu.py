@@ -361,6 +361,9 @@ def t(*shape, dtype=torch.bfloat16):
     return torch.zeros(*shape, dtype=dtype)
 
 
+python = inspect.unwrap
+
+
 def refused(call, needle):
     with pytest.raises(L.LlmtB200Error) as e:
         call()
@@ -412,3 +415,14 @@ def test_python_refuses_shapes_and_types():
     refused(lambda: L.attention_window_decode(t(2, 4, 64), q, k, k), "[batch, heads, head_dim]")
     refused(lambda: L.attention_window_decode(t(2, 4, 64), t(2, 4, 64), k, k, lengths=torch.zeros(2, dtype=torch.int64)), "lengths")
     refused(lambda: L.attention_window_decode(t(2, 4, 64), t(2, 4, 64), k, k, lengths=torch.zeros(3, dtype=torch.int32)), "lengths")
+    flat = torch.zeros(1, dtype=torch.uint8).expand(1 << 20)   # a megabyte in name only
+    gpu = lambda: pytest.MonkeyPatch.context()
+    with gpu() as m:
+        m.setattr(L, "_device_of", lambda *a: None)
+        m.setattr(L, "_on", lambda device, stream, call: call(None))
+        wf = t(64, dtype=f32)
+        for call in (lambda: python(L.attention_window_fwd)(q, None, q, k, k, workspace=flat),
+                     lambda: python(L.attention_window_bwd)(q, k, k, q, q, k, k, q, t(2, 4, 4, dtype=f32), workspace=flat),
+                     lambda: python(L.attention_window_decode)(t(2, 4, 64), t(2, 4, 64), k, k, workspace=flat),
+                     lambda: python(L.norm_residual_bwd)(t(4, 64), None, None, t(4, 64), t(4, 64), w_pre=wf, rstd_pre=t(4, dtype=f32), dw_pre=wf, workspace=flat)):
+            refused(call, "workspace must be contiguous")
