@@ -882,5 +882,8 @@ if os.path.exists(os.path.join(_HERE, "_native" + importlib.machinery.EXTENSION_
     for _f in (_group_run, gemm, gemm_desc, zero_grads, softmax_fwd, softmax_bwd, gemm_softmax_fwd, gemm_softmax_bwd, rowdot,
                head_split, head_merge, cross_entropy_fwd, cross_entropy_bwd, lm_head_ce_fwd, lm_head_ce_bwd, rope, norm_residual_fwd,
                norm_residual_bwd, attention_window_fwd, attention_window_bwd, attention_window_decode):
-        globals()[_f.__name__] = _native.fast(_f)
+        try:
+            globals()[_f.__name__] = _native.fast(_f)
+        except ValueError:   # built before there was such a function: the Python one, until the next build
+            pass
     del _f

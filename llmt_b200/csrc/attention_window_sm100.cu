@@ -14,8 +14,8 @@
 // scores -> probabilities -> product.  What helps is whatever runs beside that chain: a second block on the SM, a second
 // warpgroup, scores made before they are wanted.
 // Measured: 4 x 12 x 333 queries of 64, window 128: 9.6 us (a launch and three tiles); 8 x 12 x 1024 of 64, window 256,
-// forward and backward: 31 + 87 us; 8192 queries, 16 heads on 4 of 128, window 2048: forward 133 us (905 TFLOP/s of visible
-// pairs), backward 550 us (548).
+// forward and backward: 31 + 86 us; 8192 queries, 16 heads on 4 of 128, window 2048: forward 131 us (921 TFLOP/s of visible
+// pairs), backward 520 us (580).
 #include <cuda_bf16.h>
 
 #include <type_traits>
@@ -205,7 +205,7 @@ template <int HALVES, int WGS, bool PARTS>
 __global__ void __launch_bounds__(128 * WGS + 64, 3 - WGS)
 attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_constant__ AttentionParams p, int pair_heads, int blocks_q, int n_parts,
                      DeviceStatus* status, uint64_t wait_ns) {
-    const int parts = PARTS ? n_parts : 1;   // (known to be one: 133 us instead of 136 for 8192 queries, window 2048, head_dim 128)
+    const int parts = PARTS ? n_parts : 1;   // (known to be one: 131 us instead of 136 for 8192 queries, window 2048, head_dim 128)
     using Control = FwdControl<WGS>;
     constexpr int kSlots = Control::kSlots, kLoadWarp = 4 * WGS, kProductWarp = 4 * WGS + 1, kHd = 64 * HALVES;
     constexpr bool kApart = HALVES == 1;   // the probabilities have a place of their own

@@ -6,6 +6,7 @@ import math
 import os
 import shutil
 import subprocess
+import sys
 
 import pytest
 import torch
@@ -54,6 +55,18 @@ def test_native_functions_keep_their_python_face(name):
     assert (f.__name__, f.__module__, f.__doc__) == (name, "llmt_b200", python.__doc__)
     with pytest.raises(TypeError):
         f(no_such_argument=1)
+
+
+def test_an_extension_from_before_these_functions_is_no_obstacle():
+    """Importing (which building does first) over an extension that does not know a function leaves that function in Python."""
+    code = ("import sys, types\n"
+            "def fast(f):\n"
+            "    if f.__name__ in %r: raise ValueError(f)\n"
+            "    return f\n"
+            "sys.modules['llmt_b200._native'] = types.SimpleNamespace(setup=lambda *a: None, fast=fast, NAMES=())\n"
+            "import llmt_b200 as L, inspect\n"
+            "assert inspect.isfunction(L.rope) and inspect.isfunction(L.attention_window_decode)\n" % NATIVE)
+    subprocess.check_call([sys.executable, "-c", code], cwd=ROOT)
 
 
 # ------------------------------------------------------------------------------------------------- rotary frequencies
