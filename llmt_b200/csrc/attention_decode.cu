@@ -10,7 +10,7 @@
 // sequence has several chunks, a second launch joins those.  Chunks have one length for all sequences, so a long one of a
 // ragged batch is many blocks (shares of every sequence, in clusters that join through distributed shared memory: 4 sequences
 // of 8 to 65536 places, 32 heads on 8 of 128, 177 us against 147).
-// Measured: those 4 sequences 155 us with both launches, 721 MB at 4.7 TB/s; 32 sequences of up to 1024 places, 12 heads of 64,
+// Measured: those 4 sequences 153 us with both launches, 721 MB at 4.7 TB/s; 32 sequences of up to 1024 places, 12 heads of 64,
 // window 256: 8.5 us for 25 MB, a launch and one chunk's latency.
 #include "attention_rows.cuh"
 #include "ptx_sm100.cuh"
@@ -261,18 +261,21 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 2) attention_decode_kernel(
     }
 }
 
-// Joins the chunks of one head's sequence.  Four groups of threads, a value of the output per thread, share the chunks; each
-// thread has eight of its chunks' values under way (one after the other, 148 chunks took 40 us).
-constexpr int kJoinGroups = 4, kJoinCols = 128, kJoinThreads = kJoinGroups * kJoinCols;
+// Joins the chunks of one head's sequence.  A thread has four neighbouring values of every 16th chunk (head_dim 128; of every
+// 32nd for 64), eight of them under way: with one after the other 148 chunks took 40 us, with a value and every fourth chunk a
+// thread one sequence of 65536 places (4 heads on 1, 256 chunks) 27 us with both launches, so 15.
+constexpr int kJoinThreads = 512;
 __global__ void __launch_bounds__(kJoinThreads) attention_decode_join_kernel(AttentionParams p, DecodePlan plan, int pitch) {
-    __shared__ float weight[kJoinThreads], red[32], part[kJoinGroups][kJoinCols];
+    __shared__ float weight[kJoinThreads], red[32];
+    __shared__ float4 part[kJoinThreads];
     ptx::grid_dependency_wait();
-    const int b = blockIdx.x / p.heads, h = blockIdx.x % p.heads, col = threadIdx.x % kJoinCols, group = threadIdx.x / kJoinCols;
+    const int b = blockIdx.x / p.heads, h = blockIdx.x % p.heads;
+    const int fours = pitch / 4, groups = kJoinThreads / fours, group = threadIdx.x / fours;
     const attn::Keys keys(p, last_place(p, b));
     const int64_t steps = (keys.count + 15) / 16;
     const int chunks = steps > plan.steps ? static_cast<int>((steps + plan.steps - 1) / plan.steps) : 1;
     const float2* ml = plan.ml + static_cast<int64_t>(blockIdx.x) * plan.chunks;
-    const float* o = plan.o + static_cast<int64_t>(blockIdx.x) * plan.chunks * pitch + col;
+    const float4* o = reinterpret_cast<const float4*>(plan.o) + static_cast<int64_t>(blockIdx.x) * plan.chunks * fours + threadIdx.x % fours;
     auto block = [&](float v, bool max) {   // of all threads, in one order
         v = max ? attn::warp_max(v) : attn::warp_add(v);
         __syncthreads();
@@ -282,7 +285,8 @@ __global__ void __launch_bounds__(kJoinThreads) attention_decode_join_kernel(Att
         for (int i = 1; i < kJoinThreads / 32; ++i) r = max ? fmaxf(r, red[i]) : r + red[i];
         return r;
     };
-    float top = -INFINITY, total = 0.0f, sum = 0.0f;
+    float top = -INFINITY, total = 0.0f;
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int x = threadIdx.x; x < chunks; x += kJoinThreads) top = fmaxf(top, ml[x].x);
     top = block(top, true);
     const float c = p.scale * kLog2e, from = top == -INFINITY ? 0.0f : top * c;
@@ -297,18 +301,20 @@ __global__ void __launch_bounds__(kJoinThreads) attention_decode_join_kernel(Att
         __syncthreads();
         weight[threadIdx.x] = w;
         __syncthreads();
-        if (col < pitch) {
 #pragma unroll 8
-            for (int x = group; x < n; x += kJoinGroups) sum = fmaf(weight[x], o[static_cast<int64_t>(x0 + x) * pitch], sum);
+        for (int x = group; x < n; x += groups) {
+            const float4 v = o[static_cast<int64_t>(x0 + x) * fours];
+            const float w = weight[x];
+            sum.x = fmaf(w, v.x, sum.x); sum.y = fmaf(w, v.y, sum.y); sum.z = fmaf(w, v.z, sum.z); sum.w = fmaf(w, v.w, sum.w);
         }
     }
+    part[threadIdx.x] = sum;
     total = block(total, false);
-    part[group][col] = sum;
-    __syncthreads();
-    if (group != 0) return;
-#pragma unroll
-    for (int i = 1; i < kJoinGroups; ++i) sum += part[i][col];
-    finish(p, b, h, col, top, sum, total);
+    const int col = threadIdx.x;
+    if (col >= p.head_dim) return;
+    float s = 0.0f;
+    for (int i = 0; i < groups; ++i) s += reinterpret_cast<const float*>(part)[i * pitch + col];
+    finish(p, b, h, col, top, s, total);
 }
 
 template <int CHUNKS, int ROWS>
