@@ -1893,8 +1893,8 @@ struct RowTensor {
 };
 
 // Pitches and alignment of the tensors that are there (null ones are skipped), and that no written one overlaps another,
-// but for the pair that may be one tensor (`a` and `b`, same pitch).  `wide`: every row starts on a multiple of 8 elements.
-int norm_residual_tensors(const llmt_b200_norm_residual_desc* d, const char* who, const RowTensor* t, int n, const void* a, const void* b, bool* wide) {
+// but for the pair that may be one tensor (t[a] and t[b], same pitch).  `wide`: every row starts on a multiple of 8 elements.
+int norm_residual_tensors(const llmt_b200_norm_residual_desc* d, const char* who, const RowTensor* t, int n, int a, int b, bool* wide) {
     auto size = [&](const RowTensor& r) { return static_cast<size_t>((r.act ? d->dtype_act : d->dtype_res) == LLMT_B200_BF16 ? 2 : 4); };
     auto bytes = [&](const RowTensor& r) { return (static_cast<size_t>(d->rows - 1) * r.ld + d->cols) * size(r); };
     for (int i = 0; i < n; ++i) {
@@ -1907,7 +1907,7 @@ int norm_residual_tensors(const llmt_b200_norm_residual_desc* d, const char* who
     for (int i = 0; i < n; ++i)
         for (int j = 0; j < n; ++j) {
             if (i == j || !t[i].written || t[i].data == nullptr || t[j].data == nullptr) continue;
-            if (((t[i].data == a && t[j].data == b) || (t[i].data == b && t[j].data == a)) && a == b && t[i].ld == t[j].ld && size(t[i]) == size(t[j])) continue;
+            if (((i == a && j == b) || (i == b && j == a)) && t[i].data == t[j].data && (d->rows <= 1 || t[i].ld == t[j].ld)) continue;
             if (overlaps(t[i].data, bytes(t[i]), t[j].data, bytes(t[j]))) return fail(LLMT_B200_ERR_INVALID, "%s: %s overlaps %s", who, t[i].name, t[j].name);
         }
     return LLMT_B200_OK;
@@ -1943,7 +1943,7 @@ int llmt_b200_norm_residual_fwd(const llmt_b200_norm_residual_desc* d, void* str
     const RowTensor t[4] = {{"x", d->x, d->ld_x, false, false}, {"y", d->y, d->ld_y, true, false},
                             {"out", d->y != nullptr ? d->out : nullptr, d->ld_out, false, true}, {"h", d->h, d->ld_h, true, true}};
     bool wide = d->cols % 8 == 0 && !misaligned(d->w_post, 16) && !misaligned(d->gate, 16) && !misaligned(d->w_pre, 16);
-    st = norm_residual_tensors(d, who, t, 4, d->x, d->out, &wide);
+    st = norm_residual_tensors(d, who, t, 4, 0, 2, &wide);   // out may be x
     if (st != LLMT_B200_OK) return st;
     const FloatArray f[5] = {{"w_post", d->w_post, d->cols, false}, {"gate", d->gate, d->groups * d->cols, false}, {"w_pre", d->w_pre, d->cols, false},
                              {"rstd_post", d->w_post != nullptr ? d->rstd_post : nullptr, d->rows, true},
@@ -1983,7 +1983,7 @@ int llmt_b200_norm_residual_bwd(const llmt_b200_norm_residual_desc* d, void* str
                             {"dx", d->dx, d->ld_dx, false, true}, {"dy", d->y != nullptr ? d->dy : nullptr, d->ld_dy, true, true}};
     bool wide = d->cols % 8 == 0 && !misaligned(d->w_post, 16) && !misaligned(d->gate, 16) && !misaligned(d->w_pre, 16);
     if (d->rows > 0) {
-        st = norm_residual_tensors(d, who, t, 6, d->dx, d->dout, &wide);
+        st = norm_residual_tensors(d, who, t, 6, 2, 4, &wide);   // dx may be dout
         if (st != LLMT_B200_OK) return st;
     }
     const FloatArray f[8] = {{"dw_post", d->dw_post, d->cols, true}, {"dgate", d->dgate, d->groups * d->cols, true}, {"dw_pre", d->dw_pre, d->cols, true},

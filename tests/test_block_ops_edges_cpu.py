@@ -1,0 +1,37 @@
+"""Rotary positions, norms around a block and windowed attention: calls at the edge of what the header allows, as far as no GPU
+is needed (an accepted call ends at the missing workspace or at the launch)."""
+import ctypes
+
+import pytest
+
+import llmt_b200 as L
+from tests.test_block_ops_cpu import MB, norm_desc
+
+BF = dict(dtype_res=L.BF16, dtype_act=L.BF16)
+
+
+@pytest.mark.parametrize("kw,needle", [
+    (dict(out=1 * MB, h=1 * MB), "overlaps h"),   # out may be x, h is a result of its own
+    (dict(out=1 * MB, y=1 * MB), "out overlaps y"),
+    (dict(out=1 * MB, ld_out=128), "out overlaps x"),
+])
+def test_norm_residual_fwd_in_place_shares_nothing_else(kw, needle):
+    assert L.lib().llmt_b200_norm_residual_fwd(ctypes.byref(norm_desc(**BF, **kw)), None) == L.ERR_INVALID
+    assert needle in L.last_error()
+
+
+@pytest.mark.parametrize("kw,needle", [
+    (dict(dx=5 * MB, dy=5 * MB), "overlaps"),     # dx may be dout (at 5 MB), dy is a result of its own
+    (dict(dx=5 * MB, dh=5 * MB), "dx overlaps dh"),
+    (dict(dx=5 * MB, out=5 * MB), "dx overlaps out"),
+])
+def test_norm_residual_bwd_in_place_shares_nothing_else(kw, needle):
+    assert L.lib().llmt_b200_norm_residual_bwd(ctypes.byref(norm_desc(True, **BF, **kw)), None) == L.ERR_INVALID
+    assert needle in L.last_error()
+
+
+def test_norm_residual_in_place_is_accepted():
+    lib = L.lib()
+    # one row has no pitch; the backward call ends at the workspace that it is not given
+    for kw in (dict(dx=5 * MB), dict(dx=5 * MB, rows=1, groups=1, ld_dx=1024)):
+        assert lib.llmt_b200_norm_residual_bwd(ctypes.byref(norm_desc(True, **BF, workspace=None, **kw)), None) == L.ERR_WORKSPACE
