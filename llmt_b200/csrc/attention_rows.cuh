@@ -129,7 +129,7 @@ static __device__ __noinline__ void dkdv_row(const AttentionParams& p, int64_t b
     const int64_t first = j - off > 0 ? j - off : 0;
     const int64_t last = j < p.sinks || j + p.window >= p.tk ? p.tq : j + p.window - off;   // one past the last query
     Four dk, dv;
-    for (int64_t h = hk * p.group; h < (hk + 1) * p.group; ++h)
+    for (int64_t h = hk * p.group; h < (hk + 1) * p.group && h < p.heads; ++h)
         for (int64_t i0 = first; i0 < last; i0 += 32) {
             const int64_t i = i0 + lane;
             float e = 0.0f, ds = 0.0f;

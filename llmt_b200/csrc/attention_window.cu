@@ -1,6 +1,6 @@
 // Causal attention with a sliding window and sinks where there are no queries or no keys, a warp for each row: a forward pass
-// over no keys (zeros and -inf), its gradient, and the keys' gradients without queries (zeros).  No tensor map describes a
-// tensor without tokens; everything else is in the tiled kernels.
+// over no keys (zeros and -inf), its gradient, and the keys' gradients without queries or query heads (zeros).  No tensor map
+// describes a tensor without elements; everything else is in the tiled kernels.
 #include "attention_rows.cuh"
 #include "ptx_sm100.cuh"
 
@@ -30,7 +30,7 @@ __global__ void __launch_bounds__(kRowThreads) attention_dq_rows_kernel(Attentio
 __global__ void __launch_bounds__(kRowThreads) attention_dkdv_rows_kernel(AttentionParams p) {
     ptx::grid_dependency_wait();
     const int64_t row = (static_cast<int64_t>(blockIdx.x) * kRowThreads + threadIdx.x) >> 5;
-    const int64_t hkv = p.heads / p.group;
+    const int64_t hkv = p.kv_heads;
     if (row >= static_cast<int64_t>(p.batch) * hkv * p.tk) return;
     const int64_t j = row % p.tk, bh = row / p.tk;
     attn::dkdv_row(p, bh / hkv, bh % hkv, j);
@@ -45,11 +45,11 @@ cudaError_t launch_attention_window_fwd(const AttentionParams& p, cudaStream_t s
 }
 cudaError_t launch_attention_window_bwd(AttentionParams p, void* workspace, cudaStream_t stream) {
     p.dvec = static_cast<float*>(workspace);
-    if (p.tq > 0) {
+    if (p.tq > 0 && p.heads > 0) {
         const cudaError_t e = launch_dependent(attention_dq_rows_kernel, row_blocks(static_cast<int64_t>(p.batch) * p.heads * p.tq), kRowThreads, stream, p);
         if (e != cudaSuccess || p.tk == 0) return e;
     }
-    return launch_dependent(attention_dkdv_rows_kernel, row_blocks(static_cast<int64_t>(p.batch) * (p.heads / p.group) * p.tk), kRowThreads, stream, p);
+    return launch_dependent(attention_dkdv_rows_kernel, row_blocks(static_cast<int64_t>(p.batch) * p.kv_heads * p.tk), kRowThreads, stream, p);
 }
 
 }  // namespace llmt_b200

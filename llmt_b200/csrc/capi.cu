@@ -2046,11 +2046,11 @@ int attention_params(const llmt_b200_attention_desc* d, const char* who, Attenti
     if (d->head_dim > 128 || d->head_dim % 8 != 0)
         return fail(LLMT_B200_ERR_UNSUPPORTED, "%s: head_dim %lld is not a multiple of 8 up to 128", who, (long long)d->head_dim);
     constexpr int64_t kMaxDim = 0x7fffffff - 1024;
-    if (d->tokens_q > kMaxDim || d->tokens_k > kMaxDim || d->batch > kMaxDim || d->heads > 65536)
+    if (d->tokens_q > kMaxDim || d->tokens_k > kMaxDim || d->batch > kMaxDim || d->heads > 65536 || d->kv_heads > 65536)
         return fail(LLMT_B200_ERR_UNSUPPORTED, "%s: dimension above 2^31 - 1025, or more than 65536 heads", who);
     // a block for every row of every head in the worst case
     const int64_t rows = d->tokens_q > d->tokens_k ? d->tokens_q : d->tokens_k;
-    if (static_cast<__int128>(rows) * d->heads * d->batch > 0x7fffffff)
+    if (static_cast<__int128>(rows) * (d->heads > 0 ? d->heads : d->kv_heads) * d->batch > 0x7fffffff)
         return fail(LLMT_B200_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 rows over all heads", who);
     if (!(d->scale > 0.0f) || !std::isfinite(d->scale)) return fail(LLMT_B200_ERR_INVALID, "%s: scale must be positive and finite", who);
     if (misaligned(d->lse, 4) || misaligned(d->lengths, 4)) return fail(LLMT_B200_ERR_INVALID, "%s: lse or lengths is not aligned to its element type", who);
@@ -2071,6 +2071,7 @@ int attention_params(const llmt_b200_attention_desc* d, const char* who, Attenti
     p->lengths = d->lengths;
     p->batch = static_cast<int32_t>(d->batch);
     p->heads = static_cast<int32_t>(d->heads);
+    p->kv_heads = static_cast<int32_t>(d->kv_heads);
     p->group = d->heads > 0 ? static_cast<int32_t>(d->heads / d->kv_heads) : 1;
     p->tq = static_cast<int32_t>(d->tokens_q);
     p->tk = static_cast<int32_t>(d->tokens_k);
@@ -2208,8 +2209,8 @@ int llmt_b200_attention_window_bwd(const llmt_b200_attention_desc* d, void* stre
                             {"dout", &d->dout, false, false}, {"dq", &d->dq, false, true}, {"dk", &d->dk, true, true}, {"dv", &d->dv, true, true}};
     st = attention_views(d, who, t, 8);
     if (st != LLMT_B200_OK) return st;
-    if (p.batch == 0 || p.heads == 0 || (p.tq == 0 && p.tk == 0)) return LLMT_B200_OK;
-    if (p.tq > 0 && d->lse == nullptr) return fail(LLMT_B200_ERR_INVALID, "%s: invalid tensor lse (null data)", who);
+    if (p.batch == 0 || ((p.heads == 0 || p.tq == 0) && (p.kv_heads == 0 || p.tk == 0))) return LLMT_B200_OK;   // no gradient has an element
+    if (p.heads > 0 && p.tq > 0 && d->lse == nullptr) return fail(LLMT_B200_ERR_INVALID, "%s: invalid tensor lse (null data)", who);
     st = attention_apart(d, who, "lse", d->lse, 4 * static_cast<size_t>(d->batch * d->heads * d->tokens_q), t + 5, 3);
     if (st != LLMT_B200_OK) return st;
     const uint64_t need = llmt_b200_attention_window_workspace_bytes(d);
@@ -2223,7 +2224,7 @@ int llmt_b200_attention_window_bwd(const llmt_b200_attention_desc* d, void* stre
         return fail(LLMT_B200_ERR_INVALID, "%s: workspace overlaps lse", who);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t e;
-    if (p.tq == 0 || p.tk == 0) {
+    if (p.heads == 0 || p.tq == 0 || p.tk == 0) {
         e = launch_attention_window_bwd(p, d->workspace, s);
     } else {
         const struct { const HeadView* v; bool keys; int rows; } views[11] = {{&p.q, false, 128}, {&p.dout, false, 128}, {&p.k, true, 64}, {&p.v, true, 64},

@@ -271,7 +271,7 @@ struct AttentionParams {
     float* partial;            // workspace: sums of dV and dK of key tiles that are done in parts; of queries that are done in parts
     float* part_stats;         // workspace: a float for each row of each part (forward: log2 sum exp; dQ: its share of D)
     const int32_t* lengths;    // one new token: keys of each sequence, or null (all)
-    int32_t batch, heads, group, tq, tk, head_dim;   // group: query heads that share a key head
+    int32_t batch, heads, kv_heads, group, tq, tk, head_dim;   // group: query heads that share a key head (1 where there are none)
     int32_t window, sinks;     // 1 <= window <= max(tk, 1), 0 <= sinks <= tk
     float scale;
 };

@@ -3,9 +3,10 @@ is needed (an accepted call ends at the missing workspace or at the launch)."""
 import ctypes
 
 import pytest
+import torch
 
 import llmt_b200 as L
-from tests.test_block_ops_cpu import MB, norm_desc
+from tests.test_block_ops_cpu import MB, attn_desc, norm_desc
 
 BF = dict(dtype_res=L.BF16, dtype_act=L.BF16)
 
@@ -35,3 +36,14 @@ def test_norm_residual_in_place_is_accepted():
     # one row has no pitch; the backward call ends at the workspace that it is not given
     for kw in (dict(dx=5 * MB), dict(dx=5 * MB, rows=1, groups=1, ld_dx=1024)):
         assert lib.llmt_b200_norm_residual_bwd(ctypes.byref(norm_desc(True, **BF, workspace=None, **kw)), None) == L.ERR_WORKSPACE
+
+
+def test_attention_without_query_heads_has_key_gradients():
+    """dk and dv have elements and are to be zeroed: the call goes on to its launch, which fails here."""
+    if torch.cuda.is_available():
+        pytest.skip("the addresses are not real")
+    before = L.launch_count()
+    assert L.lib().llmt_b200_attention_window_bwd(ctypes.byref(attn_desc(True, heads=0, lse=None)), None) != L.OK and L.launch_count() > before
+    for kw in (dict(heads=0, kv_heads=0), dict(heads=0, tokens_k=0), dict(heads=0, batch=0)):
+        before = L.launch_count()
+        assert L.lib().llmt_b200_attention_window_bwd(ctypes.byref(attn_desc(True, lse=None, **kw)), None) == L.OK and L.launch_count() == before
