@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 8 ? 3 : 1) norm_residual_
             const uint8_t* const at = mine_r + stage * stage_bytes;
             const uint8_t* const from = mine_a + stage * stage_bytes;
             if (++stage == kDepth) stage = 0;
-            float out[8], y[8], q[8];   // q = dout + rstd_pre a
+            float b[8], c[8], q[8];   // q = dout + rstd_pre a
             float s_ab = 0.0f, s_eg = 0.0f, s_eb = 0.0f;
             {
                 Eight<TR, V> o, d;
@@ -381,15 +381,15 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 8 ? 3 : 1) norm_residual_
                 Staged<TA, V>::get(v, from + of_a);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    out[i] = o.at(i);
-                    y[i] = v.at(i);
-                    const float hr = h.at(i) * r_pre, ar = hr * w_pre[i];
-                    q[i] = d.at(i) + ar;
-                    acc_pre[i] = fmaf(hr, out[i], acc_pre[i]);
-                    s_ab = fmaf(ar, out[i], s_ab);   // the sum of a b
-                    const float ky = k[i] * y[i];    // e c without rstd_post
-                    s_eg = fmaf(ky, q[i], s_eg);
-                    s_eb = fmaf(ky, out[i], s_eb);   // and without rstd_pre
+                    // b and c are of ordinary size whatever the rows' is; products of rstd alone may leave the range
+                    b[i] = o.at(i) * r_pre;
+                    c[i] = v.at(i) * r_post;
+                    const float a = h.at(i) * w_pre[i], ec = k[i] * c[i];
+                    q[i] = fmaf(r_pre, a, d.at(i));
+                    acc_pre[i] = fmaf(h.at(i), b[i], acc_pre[i]);
+                    s_ab = fmaf(a, b[i], s_ab);
+                    s_eg = fmaf(ec, q[i], s_eg);
+                    s_eb = fmaf(ec, b[i], s_eb);
                 }
             }
             s_ab = warp_sum(s_ab);
@@ -423,20 +423,19 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 8 ? 3 : 1) norm_residual_
                     s_eb += v.z;
                 }
             }
-            // g = q - out rstd_pre^2 mean(a b);   dy = rstd_post (k g - y rstd_post^2 mean(k g y))
-            const float m_ab = s_ab * of * r_pre * r_pre;
-            const float m_eg = post ? r_post * r_post * r_post * of * fmaf(-m_ab, s_eb, s_eg) : 0.0f;
+            // g = q - b rstd_pre mean(a b);   dy = rstd_post (e g - c mean(e g c))
+            const float m_ab = s_ab * of * r_pre;
+            const float m_eg = post ? of * fmaf(-m_ab, s_eb, s_eg) : 0.0f;
             Eight<TR, V> dx;
             Eight<TA, V> dy;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                q[i] = fmaf(-out[i], m_ab, q[i]);
-                const float gr = q[i] * r_post;
-                sum_gc[i] = fmaf(gr, y[i], sum_gc[i]);
-                y[i] = fmaf(-y[i], m_eg, k[i] * gr);
+                q[i] = fmaf(-b[i], m_ab, q[i]);
+                sum_gc[i] = fmaf(q[i], c[i], sum_gc[i]);
+                c[i] = r_post * fmaf(-c[i], m_eg, k[i] * q[i]);
             }
             dx.put(q);
-            dy.put(y);
+            dy.put(c);
             dx.store(to_dx, first, step, cols);
             if (block) dy.store(to_dy, first, step, cols);
         }

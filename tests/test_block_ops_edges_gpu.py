@@ -4,6 +4,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import llmt_b200 as L
+from tests.test_norm_residual_gpu import _close
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -17,3 +18,27 @@ def test_attention_without_query_heads_zeroes_the_key_gradients():
     L.attention_window_fwd(q.clone(), lse, q, k, v)
     L.attention_window_bwd(q.clone(), dk, dv, q.clone(), q, k, v, q.clone(), lse)
     assert bool((dk == 0).all()) and bool((dv == 0).all())
+
+
+@pytest.mark.parametrize("cols", [64, 61])
+def test_norm_gradients_of_rows_of_any_size(cols):
+    """Rows so small or large that a power of their rstd leaves fp32's range, while every result is inside it."""
+    g = torch.Generator(device=DEV).manual_seed(cols)
+    n = lambda *s: torch.randn(*s, device=DEV, generator=g)
+    out_size = torch.tensor([0, 0, 0, -62, 58, -30, 0, 20], device=DEV)[:, None]
+    y_size = torch.tensor([0, -46, 52, 0, 0, 30, -60, -20], device=DEV)[:, None]
+    rows = out_size.shape[0]
+    out, y = n(rows, cols) * 2.0 ** out_size, n(rows, cols) * 2.0 ** y_size
+    dout, dh, w_post, w_pre = n(rows, cols), 16 * n(rows, cols), 1 + 0.1 * n(cols), 1 + 0.1 * n(cols)
+    rs, rp = (z.double().square().mean(-1).rsqrt().float() for z in (out, y))
+    dx, dy, dw_post, dw_pre = torch.empty_like(out), torch.empty_like(y), torch.empty(cols, device=DEV), torch.empty(cols, device=DEV)
+    L.norm_residual_bwd(dx, dy, dout, dh, out, y, w_post=w_post, w_pre=w_pre, rstd_post=rp, rstd_pre=rs, dw_post=dw_post, dw_pre=dw_pre)
+    r, a, k, c = rs.double()[:, None], dh.double() * w_pre.double(), w_post.double(), y.double() * rp.double()[:, None]
+    b, mean = out.double() * r, lambda t: t.mean(-1, keepdim=True)
+    gx, size = dout.double() + r * (a - b * mean(a * b)), dout.double().abs() + r * (a.abs() + b.abs() * mean((a * b).abs()))
+    # the roundings are counted as in tests/test_norm_residual_gpu.py: products and the sums of a row's terms
+    _close(dx, gx, 64, size, "dx")
+    q = rp.double()[:, None]
+    _close(dy, q * (k * gx - c * mean(k * gx * c)), 160, q * (k.abs() * size + c.abs() * mean(k.abs() * size * c.abs())), "dy")
+    _close(dw_pre, (dh.double() * b).sum(0), 100, (dh.double() * b).abs().sum(0), "dw_pre")
+    _close(dw_post, (gx * c).sum(0), 200, (size * c.abs()).sum(0), "dw_post")
