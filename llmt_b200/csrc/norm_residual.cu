@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 8 ? 3 : 1) norm_residual_
             for (int i = 0; i < 8; ++i) {
                 q[i] = fmaf(-b[i], m_ab, q[i]);
                 sum_gc[i] = fmaf(q[i], c[i], sum_gc[i]);
-                c[i] = r_post * fmaf(-c[i], m_eg, k[i] * q[i]);
+                c[i] = post ? r_post * fmaf(-c[i], m_eg, k[i] * q[i]) : k[i] * q[i];   // without a norm y has no part in it, whatever it holds
             }
             dx.put(q);
             dy.put(c);

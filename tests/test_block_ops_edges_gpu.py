@@ -42,3 +42,17 @@ def test_norm_gradients_of_rows_of_any_size(cols):
     _close(dy, q * (k * gx - c * mean(k * gx * c)), 160, q * (k.abs() * size + c.abs() * mean(k.abs() * size * c.abs())), "dy")
     _close(dw_pre, (dh.double() * b).sum(0), 100, (dh.double() * b).abs().sum(0), "dw_pre")
     _close(dw_post, (gx * c).sum(0), 200, (size * c.abs()).sum(0), "dw_post")
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_norm_gradient_of_a_block_without_a_norm_does_not_depend_on_it(bad):
+    rows, cols = 5, 40
+    g = torch.Generator(device=DEV).manual_seed(1)
+    dout, y, gate = (torch.randn(rows, cols, device=DEV, generator=g) for _ in range(3))
+    dx, dy, dgate, want = (torch.empty_like(y) for _ in range(4))
+    L.norm_residual_bwd(dx, want, dout, None, None, y, gate=gate, dgate=dgate, scale=0.5)
+    y[2, 7] = bad
+    L.norm_residual_bwd(dx, dy, dout, None, None, y, gate=gate, dgate=dgate, scale=0.5)
+    assert torch.equal(dx, dout) and torch.equal(dy, want)
+    there = torch.isfinite(dgate)   # the gate's gradient is g y
+    assert not bool(there[2, 7]) and int(there.sum()) == rows * cols - 1
