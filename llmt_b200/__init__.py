@@ -876,14 +876,21 @@ def _bind_native() -> None:
                  torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice, torch.float32, torch.bfloat16, torch.int32, torch.float64, GemmDesc)
 
 
+# The entry points that the extension binds, in its order.  One that was built from other sources knows others (and takes
+# other arguments to bind them): all functions are then the Python ones, until the next build.
+_NATIVE_ENTRIES = (
+    "gemm", "gemm_workspace_bytes_for", "gemm_grouped", "zero_grads", "softmax_fwd", "softmax_bwd", "gemm_softmax_fwd", "gemm_softmax_bwd",
+    "rowdot", "head_split", "head_merge", "cross_entropy_fwd", "cross_entropy_bwd", "lm_head_ce_fwd", "lm_head_ce_bwd", "rope",
+    "norm_residual_fwd", "norm_residual_bwd", "norm_residual_workspace_bytes", "attention_window_fwd", "attention_window_bwd",
+    "attention_window_decode", "attention_window_fwd_workspace_bytes", "attention_window_workspace_bytes",
+    "attention_window_decode_workspace_bytes")
+
 if os.path.exists(os.path.join(_HERE, "_native" + importlib.machinery.EXTENSION_SUFFIXES[0])):   # built for this interpreter
     from . import _native
-    _native.setup(_bind_native, _check, _scratch)
-    for _f in (_group_run, gemm, gemm_desc, zero_grads, softmax_fwd, softmax_bwd, gemm_softmax_fwd, gemm_softmax_bwd, rowdot,
-               head_split, head_merge, cross_entropy_fwd, cross_entropy_bwd, lm_head_ce_fwd, lm_head_ce_bwd, rope, norm_residual_fwd,
-               norm_residual_bwd, attention_window_fwd, attention_window_bwd, attention_window_decode):
-        try:
+    if tuple(_native.NAMES) == _NATIVE_ENTRIES:
+        _native.setup(_bind_native, _check, _scratch)
+        for _f in (_group_run, gemm, gemm_desc, zero_grads, softmax_fwd, softmax_bwd, gemm_softmax_fwd, gemm_softmax_bwd, rowdot,
+                   head_split, head_merge, cross_entropy_fwd, cross_entropy_bwd, lm_head_ce_fwd, lm_head_ce_bwd, rope, norm_residual_fwd,
+                   norm_residual_bwd, attention_window_fwd, attention_window_bwd, attention_window_decode):
             globals()[_f.__name__] = _native.fast(_f)
-        except ValueError:   # built before there was such a function: the Python one, until the next build
-            pass
-    del _f
+        del _f

@@ -1,12 +1,15 @@
 """Rotary positions, norms around a block and windowed attention: calls at the edge of what the header allows, as far as no GPU
 is needed (an accepted call ends at the missing workspace or at the launch)."""
 import ctypes
+import inspect
+import subprocess
+import sys
 
 import pytest
 import torch
 
 import llmt_b200 as L
-from tests.test_block_ops_cpu import MB, attn_desc, norm_desc
+from tests.test_block_ops_cpu import MB, ROOT, attn_desc, norm_desc
 
 BF = dict(dtype_res=L.BF16, dtype_act=L.BF16)
 
@@ -47,3 +50,28 @@ def test_attention_without_query_heads_has_key_gradients():
     for kw in (dict(heads=0, kv_heads=0), dict(heads=0, tokens_k=0), dict(heads=0, batch=0)):
         before = L.launch_count()
         assert L.lib().llmt_b200_attention_window_bwd(ctypes.byref(attn_desc(True, lse=None, **kw)), None) == L.OK and L.launch_count() == before
+
+
+def test_an_extension_of_other_sources_leaves_every_function_in_python():
+    """One that lacks the block's functions: the functions that it has are not taken from it either, since it binds other
+    arguments.  (The call is over nothing, and reaches torch's stream at most.)"""
+    code = ("import sys, types, inspect\n"
+            "def setup(binder, *rest): fake.binder = binder\n"
+            "def bind(entries, raw_stream, get_device, float32, bfloat16, int32, desc): pass\n"
+            "def fast(f):\n"
+            "    if f.__name__ not in fake.NAMES: raise ValueError(f)\n"
+            "    def call(*a, **k): fake.binder()\n"
+            "    return call\n"
+            "fake = types.SimpleNamespace(setup=setup, bind=bind, fast=fast, NAMES=('gemm', 'softmax_fwd', 'rowdot'))\n"
+            "sys.modules['llmt_b200._native'] = fake\n"
+            "import torch, llmt_b200 as L\n"
+            "assert all(inspect.isfunction(getattr(L, n)) and getattr(L, n).__name__ == n for n in ('gemm', 'softmax_fwd', 'rowdot', 'rope'))\n"
+            "try: L.gemm(torch.empty(0, 8), torch.empty(0, 4), torch.empty(4, 8))\n"
+            "except TypeError: raise\n"
+            "except Exception: pass\n")
+    subprocess.check_call([sys.executable, "-c", code], cwd=ROOT)
+
+
+def test_the_extension_of_these_sources_is_in_place():
+    from llmt_b200 import _native
+    assert tuple(_native.NAMES) == L._NATIVE_ENTRIES and not inspect.isfunction(L.gemm)
