@@ -345,6 +345,60 @@ bool overlaps(const void* p, size_t pb, const void* q, size_t qb) {
     return a < b + qb && b < a + pb;
 }
 
+// Runs of `width` bytes, n[0] * n[1] * n[2] of them, s[] bytes apart (not negative).
+struct Runs {
+    uintptr_t at;
+    int64_t n[3], s[3], width;
+};
+
+// Whether two sets of runs share a byte.  That is so if one of the distances  b.at - a.at + sum of j t - sum of i s  is within
+// (-b.width, a.width); the indexes of equal strides are taken as their difference, and the strides from the longest down, each
+// with the indexes that the shorter ones' reach leaves.  For strides that nest these are two or three each; a search that
+// grows beyond kMostSteps is given up as a shared byte.
+bool runs_meet(const Runs& a, const Runs& b) {
+    constexpr int kMostSteps = 4096;
+    struct Term { int64_t s, lo, hi; } term[6];
+    int terms = 0;
+    auto put = [&](int64_t s, int64_t lo, int64_t hi) {
+        if (s == 0 || lo == hi) return;
+        int i = 0;
+        while (i < terms && term[i].s > s) ++i;
+        if (i < terms && term[i].s == s) {
+            term[i].lo += lo;
+            term[i].hi += hi;
+            return;
+        }
+        for (int k = terms++; k > i; --k) term[k] = term[k - 1];
+        term[i] = {s, lo, hi};
+    };
+    for (int i = 0; i < 3; ++i) {
+        if (a.n[i] < 1 || b.n[i] < 1) return false;
+        put(a.s[i], 1 - a.n[i], 0);
+        put(b.s[i], 0, b.n[i] - 1);
+    }
+    if (a.width < 1 || b.width < 1) return false;
+    using Wide = __int128;
+    Wide least[7], most[7];   // what the terms from i on can add
+    least[terms] = most[terms] = 0;
+    for (int i = terms - 1; i >= 0; --i) {
+        least[i] = least[i + 1] + Wide{term[i].lo} * term[i].s;
+        most[i] = most[i + 1] + Wide{term[i].hi} * term[i].s;
+    }
+    int steps = 0;
+    auto search = [&](auto&& self, int i, Wide gap) -> bool {
+        if (i == terms) return gap > -b.width && gap < a.width;
+        // k s has to be above `low` and below `high`
+        const Wide s = term[i].s, low = -b.width - gap - most[i + 1], high = a.width - gap - least[i + 1];
+        Wide first = low / s + (low % s >= 0 ? 1 : 0), last = high / s - (high % s <= 0 ? 1 : 0);
+        if (first < term[i].lo) first = term[i].lo;
+        if (last > term[i].hi) last = term[i].hi;
+        for (Wide k = first; k <= last; ++k)
+            if (++steps > kMostSteps || self(self, i + 1, gap + k * s)) return true;
+        return false;
+    };
+    return search(search, 0, static_cast<Wide>(b.at) - static_cast<Wide>(a.at));
+}
+
 struct Checked {
     int64_t a_rows, a_cols, b_rows, b_cols;
     size_t a_bytes, b_bytes, c_bytes;  // extent of each operand in memory (0 for an empty problem)
@@ -1781,6 +1835,10 @@ llmt_b200_head_view without_idle_strides(llmt_b200_head_view v, int64_t batch, i
     return v;
 }
 
+Runs runs_of(const llmt_b200_head_view& v, int64_t batch, int64_t tokens, int64_t heads, int64_t hd, int64_t es) {
+    return {reinterpret_cast<uintptr_t>(v.data), {batch, tokens, heads}, {v.stride_batch * es, v.stride_token * es, v.stride_head * es}, hd * es};
+}
+
 bool misaligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
 
 }  // namespace
@@ -2104,23 +2162,9 @@ int attention_views(const llmt_b200_attention_desc* d, const char* who, const Na
             return fail(LLMT_B200_ERR_INVALID, "%s: the elements of %s overlap one another", who, t[i].name);
         bytes[i] = 2 * extent;
     }
-    // Two views may lie in each other's rows (dq, dk and dv of a packed projection): they are apart if one base is behind the
-    // other by less than the smallest common stride leaves room for.
-    auto apart = [&](int a, int b) {
-        if (bytes[a] == 0 || bytes[b] == 0 || !overlaps(view[a].data, bytes[a], view[b].data, bytes[b])) return true;
-        if (reinterpret_cast<uintptr_t>(view[a].data) > reinterpret_cast<uintptr_t>(view[b].data)) { const int c = a; a = b; b = c; }
-        const int64_t gap = static_cast<int64_t>(reinterpret_cast<uintptr_t>(view[b].data) - reinterpret_cast<uintptr_t>(view[a].data)) / 2;
-        auto heads = [&](int i) { return t[i].keys ? d->kv_heads : d->heads; };
-        auto tokens = [&](int i) { return t[i].keys ? d->tokens_k : d->tokens_q; };
-        // token rows of one pitch, both within the first view's row
-        const int64_t wa = (heads(a) - 1) * view[a].stride_head + d->head_dim, wb = (heads(b) - 1) * view[b].stride_head + d->head_dim;
-        const int64_t pitch = tokens(a) > 1 ? view[a].stride_token : tokens(b) > 1 ? view[b].stride_token : d->batch > 1 ? view[a].stride_batch : 0;
-        if ((tokens(a) > 1 && view[a].stride_token != pitch) || (tokens(b) > 1 && view[b].stride_token != pitch)) return false;
-        if (d->batch > 1 && (view[a].stride_batch != view[b].stride_batch || pitch <= 0 || view[a].stride_batch % pitch != 0 ||
-                             (tokens(a) - 1) * pitch + pitch > view[a].stride_batch || (tokens(b) - 1) * pitch + pitch > view[a].stride_batch))
-            return false;
-        return pitch > 0 && wa <= gap && gap + wb <= pitch;
-    };
+    // Two views may lie between each other's runs (dq, dk and dv of a packed projection).
+    auto runs = [&](int i) { return runs_of(view[i], d->batch, t[i].keys ? d->tokens_k : d->tokens_q, t[i].keys ? d->kv_heads : d->heads, d->head_dim, 2); };
+    auto apart = [&](int a, int b) { return bytes[a] == 0 || bytes[b] == 0 || !overlaps(view[a].data, bytes[a], view[b].data, bytes[b]) || !runs_meet(runs(a), runs(b)); };
     for (int i = 0; i < n; ++i)
         for (int j = 0; j < n; ++j)
             if (i != j && t[i].written && !apart(i, j)) return fail(LLMT_B200_ERR_INVALID, "%s: %s overlaps %s", who, t[i].name, t[j].name);

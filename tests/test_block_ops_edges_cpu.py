@@ -2,6 +2,8 @@
 is needed (an accepted call ends at the missing workspace or at the launch)."""
 import ctypes
 import inspect
+import itertools
+import random
 import subprocess
 import sys
 
@@ -9,7 +11,7 @@ import pytest
 import torch
 
 import llmt_b200 as L
-from tests.test_block_ops_cpu import MB, ROOT, attn_desc, norm_desc
+from tests.test_block_ops_cpu import MB, ROOT, attn_desc, norm_desc, view
 
 BF = dict(dtype_res=L.BF16, dtype_act=L.BF16)
 
@@ -75,3 +77,60 @@ def test_an_extension_of_other_sources_leaves_every_function_in_python():
 def test_the_extension_of_these_sources_is_in_place():
     from llmt_b200 import _native
     assert tuple(_native.NAMES) == L._NATIVE_ENTRIES and not inspect.isfunction(L.gemm)
+
+
+def _bytes_of(base, shape, strides, hd, size):
+    runs = [base + size * sum(i * s for i, s in zip(at, strides)) for at in itertools.product(*map(range, shape))]
+    return {r + k for r in runs for k in range(0, hd * size, size)}   # element by element: all are aligned to their size
+
+
+def _nested(rng, extents, unit, pad):
+    """Strides of dimensions in a random order of nesting, each with up to `pad` units between."""
+    order, strides, at = rng.sample(range(3), 3), [0, 0, 0], unit
+    for i in order:
+        strides[i] = at
+        at = at * extents[i] + unit * rng.choice((0, 0, 1, pad))
+    return strides, at
+
+
+def test_gradients_may_lie_between_each_others_rows():
+    """dq, dk and dv as views of one buffer are refused where they share an element, and only there.  (An accepted call ends at
+    the workspace that it is not given.)"""
+    rng, lib, base, seen = random.Random(5), L.lib(), 50 * MB, {True: 0, False: 0}
+    for _ in range(1500):
+        b, hkv, hd = rng.randint(1, 3), rng.randint(1, 2), 8
+        h, tq, tk = hkv * rng.randint(1, 2), rng.randint(1, 4), rng.randint(1, 4)
+        shapes = dict(dq=(b, tq, h), dk=(b, tk, hkv), dv=(b, tk, hkv))
+        common, span = _nested(rng, (b, max(tq, tk), h + 2 * hkv), hd, 3)
+        at, parts = {}, {}
+        for n, first in (("dq", 0), ("dk", h), ("dv", h + hkv)):
+            if rng.random() < 0.7:   # of the common buffer, mostly in its own place there
+                strides, off = common, common[2] * first if rng.random() < 0.8 else 8 * rng.randint(0, span // 8)
+            else:
+                strides, off = _nested(rng, shapes[n], hd, 3)[0], 8 * rng.randint(0, span // 8)
+            at[n], parts[n] = view(base + 2 * off, *strides), _bytes_of(base + 2 * off, shapes[n], strides, hd, 2)
+        meet = any(parts[x] & parts[y] for x, y in (("dq", "dk"), ("dq", "dv"), ("dk", "dv")))
+        d = attn_desc(True, batch=b, heads=h, kv_heads=hkv, tokens_q=tq, tokens_k=tk, head_dim=hd, workspace=None, **at)
+        status = lib.llmt_b200_attention_window_bwd(ctypes.byref(d), None)
+        assert status == (L.ERR_INVALID if meet else L.ERR_WORKSPACE), (b, h, hkv, tq, tk, meet, L.last_error())
+        assert not meet or "overlaps" in L.last_error()
+        seen[meet] += 1
+    assert min(seen.values()) > 200
+
+
+@pytest.mark.parametrize("batch", [1, 2, 64])
+@pytest.mark.parametrize("order", ["bhtd", "bthd", "hbtd", "thbd"])
+def test_packed_gradients_of_any_order_are_accepted(batch, order):
+    h, hkv, t, hd = 8, 2, 4096, 64
+    n, at, strides = dict(b=batch, t=t, h=h + 2 * hkv), hd, {}
+    for dim in reversed(order[:3]):
+        strides[dim] = at
+        at *= n[dim]
+    where = lambda first: view(50 * MB + 2 * first * strides["h"], strides["b"], strides["t"], strides["h"])
+    d = attn_desc(True, batch=batch, heads=h, kv_heads=hkv, tokens_q=t, tokens_k=t, workspace=None, dq=where(0), dk=where(h), dv=where(h + hkv))
+    for i, name in enumerate(["q", "out", "dout", "k", "v"]):
+        setattr(d, name, view((4096 + 1024 * i) * MB, t * h * hd, h * hd, hd))
+    d.lse = 16384 * MB
+    assert L.lib().llmt_b200_attention_window_bwd(ctypes.byref(d), None) == L.ERR_WORKSPACE, L.last_error()
+    d.dv = where(h + hkv - 1)   # dk's last head
+    assert L.lib().llmt_b200_attention_window_bwd(ctypes.byref(d), None) == L.ERR_INVALID and "dk overlaps dv" in L.last_error()

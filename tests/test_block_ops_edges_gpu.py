@@ -4,6 +4,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import llmt_b200 as L
+from tests.test_attention_window_gpu import _make
 from tests.test_norm_residual_gpu import _close
 
 pytestmark = pytest.mark.gpu
@@ -56,3 +57,21 @@ def test_norm_gradient_of_a_block_without_a_norm_does_not_depend_on_it(bad):
     assert torch.equal(dx, dout) and torch.equal(dy, want)
     there = torch.isfinite(dgate)   # the gate's gradient is g y
     assert not bool(there[2, 7]) and int(there.sum()) == rows * cols - 1
+
+
+@pytest.mark.parametrize("order", ["bhtd", "bthd", "thbd"])
+def test_gradients_packed_in_any_order(order):
+    """dq, dk and dv as views of one buffer, whatever the order of its dimensions."""
+    b, h, hkv, t, hd, window, sinks = 2, 4, 2, 130, 64, 50, 3
+    q, k, v, dout = _make(b, h, hkv, t, t, hd)
+    out, lse = torch.empty_like(q), torch.empty(b, h, t, device=DEV)
+    L.attention_window_fwd(out, lse, q, k, v, window, sinks)
+    want = [torch.empty_like(x) for x in (q, k, v)]
+    L.attention_window_bwd(*want, dout, q, k, v, out, lse, window, sinks)
+    n = dict(b=b, t=t, h=h + 2 * hkv + 1, d=hd)
+    buffer = torch.full([n[x] for x in order], 5.0, device=DEV, dtype=BF)
+    grads = buffer.permute(*(order.index(x) for x in "bthd"))
+    parts = grads[:, :, :h], grads[:, :, h:h + hkv], grads[:, :, h + hkv:h + 2 * hkv]
+    L.attention_window_bwd(*parts, dout, q, k, v, out, lse, window, sinks)
+    assert all(torch.equal(x, y) for x, y in zip(parts, want))
+    assert bool((grads[:, :, h + 2 * hkv:] == 5.0).all()), "what lies beside the gradients stays"
