@@ -1881,7 +1881,9 @@ int llmt_b200_rope(const llmt_b200_rope_desc* d, void* stream) {
     if (ex < 0 || ey < 0) return fail(LLMT_B200_ERR_INVALID, "rope: negative or overlong strides");
     if (!view_distinct(y, d->batch, d->tokens, d->heads, d->head_dim)) return fail(LLMT_B200_ERR_INVALID, "rope: y's elements overlap one another");
     const bool same = x.data == y.data && x.stride_batch == y.stride_batch && x.stride_token == y.stride_token && x.stride_head == y.stride_head;
-    if (!same && overlaps(x.data, ex * es, y.data, ey * es)) return fail(LLMT_B200_ERR_INVALID, "rope: y must be x or not overlap it");
+    if (!same && overlaps(x.data, ex * es, y.data, ey * es) &&
+        runs_meet(runs_of(x, d->batch, d->tokens, d->heads, d->head_dim, es), runs_of(y, d->batch, d->tokens, d->heads, d->head_dim, es)))
+        return fail(LLMT_B200_ERR_INVALID, "rope: y must be x or not overlap it");
     if ((d->rot_dim > 0 && overlaps(y.data, ey * es, d->freqs, d->rot_dim / 2 * 8)) ||
         (d->positions != nullptr && overlaps(y.data, ey * es, d->positions, static_cast<size_t>(d->batch) * d->tokens * 4)))
         return fail(LLMT_B200_ERR_INVALID, "rope: y overlaps freqs or positions");

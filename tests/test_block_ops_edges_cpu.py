@@ -11,7 +11,7 @@ import pytest
 import torch
 
 import llmt_b200 as L
-from tests.test_block_ops_cpu import MB, ROOT, attn_desc, norm_desc, view
+from tests.test_block_ops_cpu import MB, ROOT, attn_desc, norm_desc, rope_desc, view
 
 BF = dict(dtype_res=L.BF16, dtype_act=L.BF16)
 
@@ -134,3 +134,31 @@ def test_packed_gradients_of_any_order_are_accepted(batch, order):
     assert L.lib().llmt_b200_attention_window_bwd(ctypes.byref(d), None) == L.ERR_WORKSPACE, L.last_error()
     d.dv = where(h + hkv - 1)   # dk's last head
     assert L.lib().llmt_b200_attention_window_bwd(ctypes.byref(d), None) == L.ERR_INVALID and "dk overlaps dv" in L.last_error()
+
+
+def test_rope_may_write_between_the_rows_that_it_reads():
+    """x and y in one buffer are refused where they share an element, and only there (the frequencies lie on y, which ends the call
+    before it begins)."""
+    rng, lib, base, seen = random.Random(6), L.lib(), 50 * MB, {True: 0, False: 0}
+    for _ in range(800):
+        shape, hd = [rng.randint(1, 3), rng.randint(1, 4), rng.randint(1, 3)], rng.choice((2, 4, 6))
+        (xs, span), (ys, _) = (_nested(rng, (shape[0], shape[1], 2 * shape[2]), hd, 3) for _ in range(2))
+        off = rng.randint(0, span)
+        if rng.random() < 0.5:   # y: the heads behind x's
+            ys, off = xs, xs[2] * shape[2]
+        if rng.random() < 0.2:
+            xs = [0] + xs[1:]    # one sequence read for all
+        x, y = _bytes_of(base, shape, xs, hd, 4), _bytes_of(base + 4 * off, shape, ys, hd, 4)
+        same = off == 0 and all(n == 1 or a == b for n, a, b in zip(shape, xs, ys))
+        d = rope_desc(batch=shape[0], tokens=shape[1], heads=shape[2], head_dim=hd, rot_dim=0 if same else 2, dtype=L.FP32, x=view(base, *xs),
+                      y=view(base + 4 * off, *ys), freqs=base + 4 * off // 8 * 8)
+        status = lib.llmt_b200_rope(ctypes.byref(d), None)
+        if same:
+            assert status == L.OK
+            continue
+        meet = bool(x & y)
+        # where x and y are apart the frequencies are what is refused: they lie on y
+        assert status == L.ERR_INVALID and ("y must be x" in L.last_error()) == meet, (shape, hd, xs, ys, off)
+        assert meet or "freqs" in L.last_error()
+        seen[meet] += 1
+    assert min(seen.values()) > 100

@@ -75,3 +75,14 @@ def test_gradients_packed_in_any_order(order):
     L.attention_window_bwd(*parts, dout, q, k, v, out, lse, window, sinks)
     assert all(torch.equal(x, y) for x, y in zip(parts, want))
     assert bool((grads[:, :, h + 2 * hkv:] == 5.0).all()), "what lies beside the gradients stays"
+
+
+def test_rope_between_the_rows_that_it_reads():
+    """The turned heads beside the plain ones in one token row."""
+    g = torch.Generator(device=DEV).manual_seed(4)
+    rows = torch.randn(2, 9, 6, 32, device=DEV, generator=g).to(BF)
+    freqs = L.rope_frequencies(32, device=DEV)
+    want, before = torch.empty(2, 9, 3, 32, device=DEV, dtype=BF), rows.clone()
+    L.rope(want, rows[:, :, :3], freqs, offset=5)
+    L.rope(rows[:, :, 3:], rows[:, :, :3], freqs, offset=5)
+    assert torch.equal(rows[:, :, 3:], want) and torch.equal(rows[:, :, :3], before[:, :, :3])
