@@ -1957,6 +1957,10 @@ struct RowTensor {
 int norm_residual_tensors(const llmt_b200_norm_residual_desc* d, const char* who, const RowTensor* t, int n, int a, int b, bool* wide) {
     auto size = [&](const RowTensor& r) { return static_cast<size_t>((r.act ? d->dtype_act : d->dtype_res) == LLMT_B200_BF16 ? 2 : 4); };
     auto bytes = [&](const RowTensor& r) { return (static_cast<size_t>(d->rows - 1) * r.ld + d->cols) * size(r); };
+    auto runs = [&](const RowTensor& r) {
+        const int64_t es = static_cast<int64_t>(size(r));
+        return Runs{reinterpret_cast<uintptr_t>(r.data), {d->rows, 1, 1}, {r.ld * es, 0, 0}, d->cols * es};
+    };
     for (int i = 0; i < n; ++i) {
         if (t[i].data == nullptr) continue;
         if (d->rows > 1 && (t[i].ld < 0 || t[i].ld > (int64_t{1} << 28) || (t[i].written && t[i].ld < d->cols)))
@@ -1968,7 +1972,8 @@ int norm_residual_tensors(const llmt_b200_norm_residual_desc* d, const char* who
         for (int j = 0; j < n; ++j) {
             if (i == j || !t[i].written || t[i].data == nullptr || t[j].data == nullptr) continue;
             if (((i == a && j == b) || (i == b && j == a)) && t[i].data == t[j].data && (d->rows <= 1 || t[i].ld == t[j].ld)) continue;
-            if (overlaps(t[i].data, bytes(t[i]), t[j].data, bytes(t[j]))) return fail(LLMT_B200_ERR_INVALID, "%s: %s overlaps %s", who, t[i].name, t[j].name);
+            if (overlaps(t[i].data, bytes(t[i]), t[j].data, bytes(t[j])) && runs_meet(runs(t[i]), runs(t[j])))
+                return fail(LLMT_B200_ERR_INVALID, "%s: %s overlaps %s", who, t[i].name, t[j].name);
         }
     return LLMT_B200_OK;
 }

@@ -162,3 +162,20 @@ def test_rope_may_write_between_the_rows_that_it_reads():
         assert meet or "freqs" in L.last_error()
         seen[meet] += 1
     assert min(seen.values()) > 100
+
+
+def test_norm_residual_may_write_between_the_rows_that_it_reads():
+    """dx among the rows of the other tensors is refused where they share an element, and only there."""
+    rng, lib, base, seen = random.Random(7), L.lib(), 50 * MB, {True: 0, False: 0}
+    for _ in range(600):
+        rows, cols, pitch = rng.randint(1, 6), rng.randint(1, 5), rng.randint(5, 12)
+        other, off = (pitch, rng.randint(0, 2 * pitch)) if rng.random() < 0.6 else (rng.randint(5, 12), rng.randint(0, 40))
+        meet = bool(_bytes_of(base, (rows, 1, 1), (pitch, 0, 0), cols, 4) & _bytes_of(base + 4 * off, (rows, 1, 1), (other, 0, 0), cols, 4))
+        name = rng.choice(["out", "dout"])
+        if name == "dout" and off == 0 and (rows == 1 or pitch == other):
+            continue   # in place
+        kw = {"dx": base, "ld_dx": pitch, name: base + 4 * off, "ld_" + name: other}
+        status = lib.llmt_b200_norm_residual_bwd(ctypes.byref(norm_desc(True, rows=rows, cols=cols, groups=1, workspace=None, **kw)), None)
+        assert status == (L.ERR_INVALID if meet else L.ERR_WORKSPACE), (rows, cols, pitch, other, off, L.last_error())
+        seen[meet] += 1
+    assert min(seen.values()) > 100

@@ -86,3 +86,16 @@ def test_rope_between_the_rows_that_it_reads():
     L.rope(want, rows[:, :, :3], freqs, offset=5)
     L.rope(rows[:, :, 3:], rows[:, :, :3], freqs, offset=5)
     assert torch.equal(rows[:, :, 3:], want) and torch.equal(rows[:, :, :3], before[:, :, :3])
+
+
+def test_norm_rows_beside_one_another():
+    """The residual stream, its sum with the block and the normed rows as columns of one buffer."""
+    rows, c = 13, 24
+    g = torch.Generator(device=DEV).manual_seed(5)
+    buffer = torch.randn(rows, 4 * c, device=DEV, generator=g)
+    x, y, out, h = (buffer[:, i * c:(i + 1) * c] for i in range(4))
+    w = torch.ones(c, device=DEV)
+    want, before = (torch.empty(rows, c, device=DEV), torch.empty(rows, c, device=DEV)), buffer.clone()
+    L.norm_residual_fwd(*want, x.contiguous(), y.contiguous(), w_pre=w)
+    L.norm_residual_fwd(out, h, x, y, w_pre=w)
+    assert torch.equal(out, want[0]) and torch.equal(h, want[1]) and torch.equal(buffer[:, :2 * c], before[:, :2 * c])
