@@ -14,26 +14,25 @@ __global__ void __launch_bounds__(kRowThreads) attention_fwd_rows_kernel(Attenti
     const int64_t row = (static_cast<int64_t>(blockIdx.x) * kRowThreads + threadIdx.x) >> 5;
     if (row >= static_cast<int64_t>(p.batch) * p.heads * p.tq) return;
     const int64_t i = row % p.tq, bh = row / p.tq;
-    attn::forward_row(p, bh / p.heads, bh % p.heads, i, i + p.tk - p.tq);
+    attn::Four().store(attn::row_to(p.out, bh / p.heads, i, bh % p.heads), 0.0f, p.head_dim);
+    if ((threadIdx.x & 31) == 0 && p.lse != nullptr) p.lse[row] = -INFINITY;
 }
 
 __global__ void __launch_bounds__(kRowThreads) attention_dq_rows_kernel(AttentionParams p) {
     ptx::grid_dependency_wait();
     const int64_t row = (static_cast<int64_t>(blockIdx.x) * kRowThreads + threadIdx.x) >> 5;
     if (row >= static_cast<int64_t>(p.batch) * p.heads * p.tq) return;
-    const int64_t i = row % p.tq, bh = row / p.tq, b = bh / p.heads, h = bh % p.heads;
-    const float d = attn::dot_rows(attn::row_of(p.dout, b, i, h), attn::row_of(p.out, b, i, h), p.head_dim);
-    if ((threadIdx.x & 31) == 0) p.dvec[row] = d;
-    attn::dq_row(p, b, h, i, d);
+    const int64_t i = row % p.tq, bh = row / p.tq;
+    attn::Four().store(attn::row_to(p.dq, bh / p.heads, i, bh % p.heads), 0.0f, p.head_dim);
 }
 
 __global__ void __launch_bounds__(kRowThreads) attention_dkdv_rows_kernel(AttentionParams p) {
     ptx::grid_dependency_wait();
     const int64_t row = (static_cast<int64_t>(blockIdx.x) * kRowThreads + threadIdx.x) >> 5;
-    const int64_t hkv = p.kv_heads;
-    if (row >= static_cast<int64_t>(p.batch) * hkv * p.tk) return;
+    if (row >= static_cast<int64_t>(p.batch) * p.kv_heads * p.tk) return;
     const int64_t j = row % p.tk, bh = row / p.tk;
-    attn::dkdv_row(p, bh / hkv, bh % hkv, j);
+    attn::Four().store(attn::row_to(p.dk, bh / p.kv_heads, j, bh % p.kv_heads), 0.0f, p.head_dim);
+    attn::Four().store(attn::row_to(p.dv, bh / p.kv_heads, j, bh % p.kv_heads), 0.0f, p.head_dim);
 }
 
 unsigned row_blocks(int64_t rows) { return static_cast<unsigned>((rows * 32 + kRowThreads - 1) / kRowThreads); }
@@ -43,8 +42,7 @@ unsigned row_blocks(int64_t rows) { return static_cast<unsigned>((rows * 32 + kR
 cudaError_t launch_attention_window_fwd(const AttentionParams& p, cudaStream_t stream) {
     return launch_dependent(attention_fwd_rows_kernel, row_blocks(static_cast<int64_t>(p.batch) * p.heads * p.tq), kRowThreads, stream, p);
 }
-cudaError_t launch_attention_window_bwd(AttentionParams p, void* workspace, cudaStream_t stream) {
-    p.dvec = static_cast<float*>(workspace);
+cudaError_t launch_attention_window_bwd(const AttentionParams& p, cudaStream_t stream) {
     if (p.tq > 0 && p.heads > 0) {
         const cudaError_t e = launch_dependent(attention_dq_rows_kernel, row_blocks(static_cast<int64_t>(p.batch) * p.heads * p.tq), kRowThreads, stream, p);
         if (e != cudaSuccess || p.tk == 0) return e;

@@ -160,10 +160,10 @@ __device__ __forceinline__ void put_row16(uint8_t* tile, int row, int x, const u
 }
 
 // The end of a copy-out by `threads` threads that meet at barrier `id`: `mine` rows of this warp's 32 hold values that are
-// not finite.  store() issues the copies (by the thread that `first` names); the rows are formed again by again(row in the
-// quarter) once the copies are complete, by the warps that `mend` names.
+// not finite and may owe them to a hidden place.  store() issues the copies (by the thread that `first` names); the rows go to
+// again(row) once the copies are complete, in turn to the warps.
 template <typename Store, typename Again>
-__device__ __forceinline__ void copy_out(uint32_t* bad, int id, int threads, bool first, int quarter, bool mend, uint32_t mine, Store store, Again again) {
+__device__ __forceinline__ void copy_out(uint32_t* bad, int id, int threads, bool first, int quarter, uint32_t mine, Store store, Again again) {
     if ((threadIdx.x & 31) == 0 && mine != 0) atomicOr(&bad[quarter], mine);
     fence_proxy_async_smem();
     named_barrier_sync(id, threads);
@@ -176,7 +176,11 @@ __device__ __forceinline__ void copy_out(uint32_t* bad, int id, int threads, boo
     }
     if (!any) return;
     named_barrier_sync(id, threads);
-    for (uint32_t m = mend ? bad[quarter] : 0; m != 0; m &= m - 1) again(__ffs(m) - 1);
+    const int warps = threads / 32, me = static_cast<int>(threadIdx.x >> 5) % warps;
+    int n = 0;
+    for (int x = 0; x < 4; ++x)
+        for (uint32_t m = bad[x]; m != 0; m &= m - 1, ++n)
+            if (n % warps == me) again(x * 32 + __ffs(m) - 1);
 }
 
 // ------------------------------------------------------------------------------------------------------------ forward
@@ -499,12 +503,12 @@ attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_co
                 if (i < p.tq) p.part_stats[place * kRows + row] = l == 0.0f ? -INFINITY : fmaf(m, c, log2f(l));
             } else {
                 if (i < p.tq && p.lse != nullptr) p.lse[line] = l == 0.0f ? -INFINITY : fmaf(m, p.scale, log2f(l) * (1.0f / kLog2e));
-                // A product with a hidden value that is not finite (0 * inf) has spoilt the row, or it sees such a value: it is
-                // formed again from the keys it sees.
-                copy_out(ctl->bad[w], 1 + w, 128, row == 0, quarter, true, __ballot_sync(0xffffffffu, bad && ok && i < p.tq), [&] {
+                // A product with a hidden value that is not finite (0 * inf) may have spoilt columns of the row.  A sum that is NaN
+                // is of visible scores only: so is the whole row then.
+                copy_out(ctl->bad[w], 1 + w, 128, row == 0, quarter, __ballot_sync(0xffffffffu, bad && l == l && ok && i < p.tq), [&] {
                     for (int x = 0; x < HALVES; ++x) tma_store_4d(&maps.out, q_at + w * kTile + x * kHalfTile, x * 64, blk.r0, blk.head, b);
                 }, [&](int r) {
-                    const int64_t at = blk.r0 + quarter * 32 + r;
+                    const int64_t at = blk.r0 + r;
                     attn::forward_row(p, b, blk.head, at, at + p.tk - p.tq);
                 });
             }
@@ -524,8 +528,9 @@ attention_fwd_kernel(const __grid_constant__ AttentionMaps maps, const __grid_co
 // 2^(s_part - max), s_part = log2 sum exp of a part's scores.  Backward: dQ and D are the parts' sums.  A lane has a row, a warp
 // PIECES of the row's 16-byte pieces; the results cross shared memory, so that reads and writes are contiguous.
 constexpr int kJoinWarps = 8, kMostParts = 32;
+// (Blocks an SM: as many as the join alone would have; rows that are formed again may not cost it registers.)
 template <int PIECES, bool FORWARD>
-__global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(AttentionParams p, int parts) {
+__global__ void __launch_bounds__(kJoinWarps * 32, FORWARD ? 3 : 2) attention_join_kernel(const __grid_constant__ AttentionParams p, int parts) {
     constexpr int kPieces = PIECES * kJoinWarps;
     __shared__ uint2 tile[32][kPieces + 1];
     __shared__ uint32_t bad[kJoinWarps];
@@ -554,20 +559,22 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(Attenti
         }
     }
     const float inv = !FORWARD ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
-    bool off = FORWARD && !(inv < INFINITY);
+    // a sum that is NaN is of visible places only (or a D without any): so is the whole row
+    const bool known = total != total && i + p.tk - p.tq >= 0;
+    bool off = false;
 #pragma unroll
     for (int n = 0; n < PIECES; ++n) {
 #pragma unroll
         for (float& x : o[n]) {
             x *= inv;
-            off = off || !(fabsf(x) < INFINITY);
+            off = off || (!known && !(fabsf(x) < INFINITY));
         }
         tile[lane][warp * PIECES + n] = make_uint2(pack_bf16(o[n][0], o[n][1]), pack_bf16(o[n][2], o[n][3]));
     }
     const uint32_t mine = __ballot_sync(0xffffffffu, off);
     if (lane == 0) bad[warp] = mine;
     if (warp == 0 && i < p.tq) {
-        if (FORWARD && p.lse != nullptr && !off) p.lse[bh * p.tq + i] = total == 0.0f ? -INFINITY : (top + log2f(total)) * (1.0f / kLog2e);
+        if (FORWARD && p.lse != nullptr) p.lse[bh * p.tq + i] = total == 0.0f ? -INFINITY : (top + log2f(total)) * (1.0f / kLog2e);
         if (!FORWARD)
             p.dvec[bh * p.tq + i] = fabsf(total) < INFINITY ? total : attn::dot_rows(attn::row_of(p.dout, b, i, h), attn::row_of(p.out, b, i, h), p.head_dim);
     }
@@ -575,13 +582,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(Attenti
     uint32_t again = 0;
 #pragma unroll
     for (int w = 0; w < kJoinWarps; ++w) again |= bad[w];
-    for (int r = warp; r < 32 && r0 + r < p.tq; r += kJoinWarps) {
-        if (again >> r & 1u) {   // as after one pass: from the keys that the row sees
-            if (FORWARD) attn::forward_row(p, b, h, r0 + r, r0 + r + p.tk - p.tq);
-            else attn::dq_row(p, b, h, r0 + r, attn::dot_rows(attn::row_of(p.dout, b, r0 + r, h), attn::row_of(p.out, b, r0 + r, h), p.head_dim));
-        } else if (lane * 4 < p.head_dim) {
-            *reinterpret_cast<uint2*>(attn::row_to(FORWARD ? p.out : p.dq, b, r0 + r, h) + lane * 4) = tile[r][lane];
-        }
+    for (int r = warp; r < 32 && r0 + r < p.tq; r += kJoinWarps)
+        if (lane * 4 < p.head_dim) *reinterpret_cast<uint2*>(attn::row_to(FORWARD ? p.out : p.dq, b, r0 + r, h) + lane * 4) = tile[r][lane];
+    for (int r = warp; again != 0 && r < 32 && r0 + r < p.tq; r += kJoinWarps) {   // as after one pass
+        if (!(again >> r & 1u)) continue;
+        if (FORWARD) attn::forward_row(p, b, h, r0 + r, r0 + r + p.tk - p.tq);
+        else attn::dq_row(p, b, h, r0 + r, attn::dot_rows(attn::row_of(p.dout, b, r0 + r, h), attn::row_of(p.out, b, r0 + r, h), p.head_dim));
     }
 }
 
@@ -955,12 +961,14 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
         if (first_time) have_d();   // a wait has run out: the other warpgroups are not left at the barrier
         // A row of dS adds up to nothing but for what the rounding of `out` has put into D: dK's kernel gets D without it.
         roles.ctl->sums[w][row] = both(sum).x + both(sum).y;
+        if (exact && w == 0) roles.ctl->d[row] = d;   // for a row that is formed again
         named_barrier_sync(1, roles.kSoftmax);
+        float of_row = 0.0f;
+#pragma unroll
+        for (int x = 0; x < kBuffers; ++x) of_row += roles.ctl->sums[x][row];
         const int64_t place = (static_cast<int64_t>(unit) * blocks_q + r0 / kRows) * parts + part;   // of this part in the workspace, as in the forward pass
         if (w == 0 && i < p.tq) {
-            float more = part == 0 ? d : 0.0f;
-#pragma unroll
-            for (int x = 0; x < kBuffers; ++x) more += roles.ctl->sums[x][row];
+            const float more = (part == 0 ? d : 0.0f) + of_row;
             if (parts > 1) p.part_stats[place * kRows + row] = more;
             else p.dvec[at] = fabsf(more) < INFINITY ? more : d;
         }
@@ -988,10 +996,10 @@ attention_dq_kernel(const __grid_constant__ AttentionMaps maps, const __grid_con
             }
         }
         if (parts == 1) {
-            // as in the forward kernel: a hidden key that is not finite has spoilt the row
-            copy_out(roles.ctl->bad, 1, roles.kSoftmax, threadIdx.x == 0, quarter, w == 0, __ballot_sync(0xffffffffu, bad && ok && i < p.tq), [&] {
+            // as in the forward kernel: a hidden key that is not finite may have spoilt the row, unless its dS is NaN
+            copy_out(roles.ctl->bad, 1, roles.kSoftmax, threadIdx.x == 0, quarter, __ballot_sync(0xffffffffu, bad && of_row == of_row && ok && i < p.tq), [&] {
                 for (int x = 0; x < HALVES; ++x) tma_store_4d(&maps.dq, tiles + x * kHalfTile, x * 64, r0, h, b);
-            }, [&](int r) { attn::dq_row(p, b, h, r0 + quarter * 32 + r, __shfl_sync(0xffffffffu, d, r)); });
+            }, [&](int r) { attn::dq_row(p, b, h, r0 + r, roles.ctl->d[r]); });
         }
     }
     roles.tear_down(warp, tmem);
@@ -1158,19 +1166,19 @@ attention_dkdv_kernel(const __grid_constant__ AttentionMaps maps, const __grid_c
             }
         }
         if (parts == 1)
-            copy_out(roles.ctl->bad, 1, roles.kSoftmax, threadIdx.x == 0, quarter, w == 0, __ballot_sync(0xffffffffu, bad && ok && j < p.tk), [&] {
+            copy_out(roles.ctl->bad, 1, roles.kSoftmax, threadIdx.x == 0, quarter, __ballot_sync(0xffffffffu, bad && ok && j < p.tk), [&] {
                 for (int x = 0; x < HALVES; ++x) {
                     tma_store_4d(&maps.dv, tiles + x * kHalfTile, x * 64, j0, hk, b);
                     tma_store_4d(&maps.dk, tiles + kFixed + x * kHalfTile, x * 64, j0, hk, b);
                 }
-            }, [&](int r) { attn::dkdv_row(p, b, hk, j0 + quarter * 32 + r); });
+            }, [&](int r) { attn::dkdv_row(p, b, hk, j0 + r); });
     }
     roles.tear_down(warp, tmem);
 }
 
 // Adds the parts of the tiles that were done in parts, a row of dV and dK per warp.
 constexpr int kSumThreads = 256;
-__global__ void __launch_bounds__(kSumThreads) attention_dkdv_sum_kernel(AttentionParams p, DkdvPlan plan, int kept, int pitch) {
+__global__ void __launch_bounds__(kSumThreads, 2) attention_dkdv_sum_kernel(const __grid_constant__ AttentionParams p, DkdvPlan plan, int kept, int pitch) {
     grid_dependency_wait();
     const int64_t at = (static_cast<int64_t>(blockIdx.x) * kSumThreads + threadIdx.x) >> 5;
     const int units = p.batch * (p.heads / p.group), n_tiles = kept ? plan.sink_tiles : plan.tiles - plan.sink_tiles, parts = kept ? plan.sink_parts : plan.parts;

@@ -2276,7 +2276,7 @@ int llmt_b200_attention_window_bwd(const llmt_b200_attention_desc* d, void* stre
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t e;
     if (p.heads == 0 || p.tq == 0 || p.tk == 0) {
-        e = launch_attention_window_bwd(p, d->workspace, s);
+        e = launch_attention_window_bwd(p, s);
     } else {
         const struct { const HeadView* v; bool keys; int rows; } views[11] = {{&p.q, false, 128}, {&p.dout, false, 128}, {&p.k, true, 64}, {&p.v, true, 64},
                                                                               {&p.dq, false, 128}, {&p.q, false, 64}, {&p.dout, false, 64}, {&p.k, true, 128},

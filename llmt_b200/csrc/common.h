@@ -399,7 +399,7 @@ size_t attention_fwd_sm100_workspace(const AttentionParams& p, int sms);
 cudaError_t launch_attention_bwd_sm100(AttentionParams p, const CUtensorMap* maps, void* workspace, int sms, DeviceStatus* status, uint64_t wait_ns,
                                        cudaStream_t stream);
 size_t attention_bwd_sm100_workspace(const AttentionParams& p, int sms);
-cudaError_t launch_attention_window_bwd(AttentionParams p, void* workspace, cudaStream_t stream);
+cudaError_t launch_attention_window_bwd(const AttentionParams& p, cudaStream_t stream);
 cudaError_t launch_attention_window_decode(const AttentionParams& p, int sms, void* workspace, cudaStream_t stream);
 size_t attention_decode_workspace(const AttentionParams& p, int sms);
 DeviceStatus* device_status_ptr(void);

@@ -1,10 +1,12 @@
 """Rotary positions, norms around a block and windowed attention at the edge of what their header allows."""
+import math
+
 import pytest
 
 torch = pytest.importorskip("torch")
 
 import llmt_b200 as L
-from tests.test_attention_window_gpu import _make
+from tests.test_attention_window_gpu import P, _heads, _make, _visible
 from tests.test_norm_residual_gpu import _close
 
 pytestmark = pytest.mark.gpu
@@ -99,3 +101,113 @@ def test_norm_rows_beside_one_another():
     L.norm_residual_fwd(*want, x.contiguous(), y.contiguous(), w_pre=w)
     L.norm_residual_fwd(out, h, x, y, w_pre=w)
     assert torch.equal(out, want[0]) and torch.equal(h, want[1]) and torch.equal(buffer[:, :2 * c], before[:, :2 * c])
+
+
+def _summed(seen, f, x):
+    """Sum over the second-last dimension of x of f[..., i, j] x[..., j, :], visible pairs only (0 * inf of the others apart)."""
+    return torch.where(seen[..., None], f[..., None] * x[..., None, :, :], 0).sum(-2)
+
+
+def _same_kind(got, want, bound, what):
+    """NaN and infinity where the definition has them, the others within the bound (nothing is asked where that has no size)."""
+    assert bool((torch.isnan(got) == torch.isnan(want)).all()), f"{what}: NaN at {int((torch.isnan(got) != torch.isnan(want)).sum())} other places"
+    inf = torch.isinf(want)
+    assert bool((torch.isinf(got) == inf).all()) and bool((got[inf] == want[inf]).all()), f"{what}: infinities"
+    off, finite = (got - want).abs(), torch.isfinite(want) & torch.isfinite(bound)
+    assert bool((off[finite] <= bound[finite]).all()), f"{what}: {float((off[finite] / bound[finite]).max()):.2f} of the bound"
+
+
+SPOILT = [(n, how, bad) for n in ("q", "k", "v", "dout") for how in ("column", "one", "some") for bad in (math.nan, math.inf, -math.inf)]
+
+
+@pytest.mark.parametrize("b,h,hkv,tq,tk,hd,window,sinks", [
+    (1, 2, 1, 200, 200, 64, 30, 2),       # a short window: D summed exactly
+    (1, 2, 2, 260, 260, 128, 0, 0),
+    (1, 2, 1, 40, 1300, 64, 700, 3),      # in parts
+    (1, 4, 2, 150, 100, 72, 0, 0)])       # queries that see nothing
+def test_values_that_are_not_finite_reach_what_the_definition_says(b, h, hkv, tq, tk, hd, window, sinks):
+    """A weight, a token or some values that are NaN or infinite, and hidden places that hold infinities beside them."""
+    g = torch.Generator(device=DEV).manual_seed(9)
+    seen, c = _visible(tq, tk, window, sinks), hd ** -0.5
+    for name, how, bad in SPOILT:
+        q, k, v, dout = _make(b, h, hkv, tq, tk, hd)
+        x = dict(q=q, k=k, v=v, dout=dout)[name]
+        if how == "column":
+            x[..., 5] = bad
+        elif how == "one":
+            x[0, x.shape[1] * 2 // 3, 0, 3] = bad
+        else:
+            at = torch.randint(0, x.numel(), (3,), device=DEV, generator=g)
+            x.view(-1)[at] = torch.tensor([bad, -bad, bad], device=DEV, dtype=BF)
+        hidden = ~seen.any(0)
+        k[:, hidden], v[:, hidden] = math.inf, -math.inf
+        out, lse = torch.empty_like(q), torch.empty(b, h, tq, device=DEV)
+        L.attention_window_fwd(out, lse, q, k, v, window, sinks)
+        qd, kd, vd, dod = (_heads(y, h) for y in (q, k, v, dout))
+        s = torch.where(seen, qd @ kd.transpose(-1, -2) * c, -math.inf)
+        m = s.amax(-1, keepdim=True)
+        e = (s - torch.where(m == -math.inf, 0, m)).exp()
+        total = e.sum(-1, keepdim=True)
+        p = e / torch.where(total == 0, 1, total)
+        what = f"{name} {how} {bad}"
+        want = _summed(seen, p, vd)
+        _same_kind(out.double().transpose(1, 2), want, want.abs() * 2.0 ** -8 + _summed(seen, p, vd.abs()) * P + 1e-30, what + ": out")
+        want_lse = torch.where(total == 0, -math.inf, m + total.log())[..., 0]
+        _same_kind(lse.double(), want_lse, torch.full_like(want_lse, 2.0 ** -10 + 16 * 2.0 ** -22), what + ": lse")
+
+        dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+        L.attention_window_bwd(dq, dk, dv, dout, q, k, v, out, lse, window, sinks)
+        assert L.device_status() == (0, 0)
+        ld, od = lse.double()[..., None], _heads(out, h)
+        p = torch.where(seen, torch.where(ld == -math.inf, 0, (qd @ kd.transpose(-1, -2) * c - ld).exp()), 0)
+        dp, by_rows = dod @ vd.transpose(-1, -2), torch.where(seen, p * (dod @ vd.transpose(-1, -2)), 0).sum(-1, keepdim=True)
+        d = by_rows if min(window + sinks if window > 0 else tk, tk) <= 128 else (dod * od).sum(-1, keepdim=True)
+        d_k = torch.where(torch.isfinite(by_rows), by_rows, d)
+        ds, ds_k = (torch.where(seen, p * (dp - y), 0) for y in (d, d_k))
+        off = P * torch.maximum(ds.abs(), ds_k.abs()) + p * hd * 2.0 ** -23 * (dod.abs() @ vd.abs().transpose(-1, -2) + (dod * od).abs().sum(-1, keepdim=True))
+
+        def group(y):
+            return y.reshape(b, hkv, h // hkv, tk, hd).sum(2).transpose(1, 2)
+        t = seen.T
+        for n, got, want, bound in (("dq", dq, _summed(seen, c * ds, kd).transpose(1, 2), _summed(seen, c * off, kd.abs()).transpose(1, 2)),
+                                    ("dk", dk, group(_summed(t, c * ds_k.transpose(-1, -2), qd)), group(_summed(t, c * off.transpose(-1, -2), qd.abs()))),
+                                    ("dv", dv, group(_summed(t, p.transpose(-1, -2), dod)), group(_summed(t, P * p.transpose(-1, -2), dod.abs())))):
+            _same_kind(got.double(), want, want.abs() * 2.0 ** -8 + bound * (1 + 2.0 ** -3) + 1e-30, f"{what}: {n}")
+
+
+def _time(call):
+    """The least time of a few calls, in microseconds."""
+    call()
+    best = math.inf
+    for _ in range(5):
+        a, e = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        call()
+        e.record()
+        e.synchronize()
+        best = min(best, 1e3 * a.elapsed_time(e))
+    return best
+
+
+@pytest.mark.parametrize("b,h,hkv,t,hd,window,sinks", [(1, 4, 2, 2048, 128, 0, 0), (2, 4, 4, 1024, 64, 256, 4)])
+def test_a_step_whose_values_are_nan_takes_no_longer_than_a_few_others(b, h, hkv, t, hd, window, sinks):
+    """Sixty times as long and more it took when every row that is NaN was summed again.  A token that is NaN still spoils the rows
+    that share a tile with it and do not see it, 128 a head and pass at most: a warp has 32 of them in turn, and goes to memory
+    for 32 places four times for their sums and for 16 places once to look at them, a microsecond each time at most."""
+    def step(**spoil):
+        x = dict(zip(("q", "k", "v", "dout"), _make(b, h, hkv, t, t, hd)))
+        for name, where in spoil.items():
+            x[name][where] = math.nan
+        out, lse = torch.empty_like(x["q"]), torch.empty(b, h, t, device=DEV)
+        dq, dk, dv = (torch.empty_like(x[n]) for n in "qkv")
+
+        def call():
+            L.attention_window_fwd(out, lse, x["q"], x["k"], x["v"], window, sinks)
+            L.attention_window_bwd(dq, dk, dv, x["dout"], x["q"], x["k"], x["v"], out, lse, window, sinks)
+        return _time(call)
+    clean, column, token = step(), (Ellipsis, 5), (0, t // 2)
+    for spoil in (dict(q=..., k=..., v=..., dout=...), dict(q=column), dict(k=column), dict(v=column), dict(dout=column), dict(q=token, k=token, v=token)):
+        spoilt = step(**spoil)
+        places = min(t, window + sinks) if window else t
+        rows = 3 * 32 * (4 * places / 32 + places / 16) if token in spoil.values() else 0
+        assert spoilt <= 10 * clean + rows, (spoil, clean, spoilt)
