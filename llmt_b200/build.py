@@ -117,7 +117,8 @@ CPP_TEST_SRC = os.path.join(ROOT, "tests", "cpp", "test_llmt_goldens.cpp")
 CPP_TEST_BIN = os.path.join(ROOT, "tests", "cpp", "_build", "test_llmt_goldens")
 CPP_TESTS = {"test_llmt_goldens": CPP_TEST_BIN,
              "test_peer_exchange": os.path.join(ROOT, "tests", "cpp", "_build", "test_peer_exchange"),
-             "test_block_ops": os.path.join(ROOT, "tests", "cpp", "_build", "test_block_ops")}
+             "test_block_ops": os.path.join(ROOT, "tests", "cpp", "_build", "test_block_ops"),
+             "test_block_ops_host": os.path.join(ROOT, "tests", "cpp", "_build", "test_block_ops_host")}
 
 
 def build_cpp(force: bool = False) -> str:

@@ -53,8 +53,9 @@ void attention_fwd_packed(const RunCtx& ctx, Tensor& y, Tensor& scores, const Te
 //   lse [B, H, T] fp32             log-sum-exp of the scores, for the backward pass (forward: may be null)
 // Query i sees the last `window` keys up to its own (0: all of them) and the first `sinks`.  The backward pass writes all of
 // dqkv (the layout of qkv) from what the forward pass left; ctx.blas_workspace must hold
-// attention_window_workspace_bytes(...) bytes.  The forward pass uses it too, where it is large enough, to share the keys of a
-// few queries out among the SMs.
+// attention_window_workspace_bytes(...) bytes, which is enough for either direction.  The forward pass alone asks for
+// attention_window_fwd_workspace_bytes(...) (0 for many shapes), to share the keys of a few queries out among the SMs; with less
+// it does without.
 struct WindowSpec {
     int64_t window = 0;
     int64_t sinks = 0;
@@ -65,6 +66,7 @@ void attention_window_fwd_packed(const RunCtx& ctx, Tensor& y, Tensor* lse, cons
 void attention_window_bwd_packed(const RunCtx& ctx, Tensor& dqkv, const Tensor& dy, const Tensor& qkv, const Tensor& y, const Tensor& lse,
                                  int64_t n_head, int64_t n_kv_head, WindowSpec spec) noexcept;
 size_t attention_window_workspace_bytes(const Tensor& qkv, int64_t n_head, int64_t n_kv_head, WindowSpec spec) noexcept;
+size_t attention_window_fwd_workspace_bytes(const Tensor& qkv, int64_t n_head, int64_t n_kv_head, WindowSpec spec) noexcept;
 
 // The same for one new token per sequence over a cache:
 //   q [B, W]: the token's row, whose first H * hd values are the query heads (a packed projection's row, W = (H + 2 Hkv) * hd,

@@ -293,7 +293,13 @@ void attention_window_bwd_packed(const RunCtx& ctx, Tensor& dqkv, const Tensor& 
 
 size_t attention_window_workspace_bytes(const Tensor& qkv, int64_t n_head, int64_t n_kv_head, WindowSpec spec) noexcept {
     const llmt_b200_attention_desc d = window_desc("attention_window_bwd_packed", qkv, n_head, n_kv_head, spec);
-    return static_cast<size_t>(llmt_b200_attention_window_workspace_bytes(&d));
+    const uint64_t fwd = llmt_b200_attention_window_fwd_workspace_bytes(&d), bwd = llmt_b200_attention_window_workspace_bytes(&d);
+    return static_cast<size_t>(fwd > bwd ? fwd : bwd);
+}
+
+size_t attention_window_fwd_workspace_bytes(const Tensor& qkv, int64_t n_head, int64_t n_kv_head, WindowSpec spec) noexcept {
+    const llmt_b200_attention_desc d = window_desc("attention_window_fwd_packed", qkv, n_head, n_kv_head, spec);
+    return static_cast<size_t>(llmt_b200_attention_window_fwd_workspace_bytes(&d));
 }
 
 void attention_window_decode(const RunCtx& ctx, Tensor& y, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor* lengths,
