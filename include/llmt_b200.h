@@ -502,7 +502,8 @@ LLMT_B200_API uint64_t llmt_b200_norm_residual_workspace_bytes(const llmt_b200_n
  *   summed over the heads that share them, in a fixed order.
  *   head_dim is a multiple of 8, at most 128; bases are 16-byte aligned and strides multiples of 8
  *   elements, not 0 (an operand cannot be broadcast).  Results must not overlap one another or
- *   anything that is read.  scale is positive.  batch * heads * max(tokens_q, tokens_k) < 2^31.
+ *   anything that is read.  scale is positive.  batch * heads * max(tokens_q, tokens_k) < 2^31 (_decode: batch * heads, and
+ *   fewer than 2^31 - 1024 places).
  *   lse  fp32 [batch, heads, tokens_q]: written by _fwd (NULL: not wanted), read by _bwd.
  *
  * _fwd: with a workspace (16-byte aligned) of llmt_b200_attention_window_fwd_workspace_bytes(desc) bytes, 0

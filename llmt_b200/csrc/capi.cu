@@ -2100,8 +2100,9 @@ struct NamedView {
     bool keys, written;   // tokens_k and kv_heads; a result
 };
 
-// The checks that the attention calls share; fills in everything but the gradients.
-int attention_params(const llmt_b200_attention_desc* d, const char* who, AttentionParams* p) {
+// The checks that the attention calls share; fills in everything but the gradients.  `decode`: one token a sequence, whose
+// blocks are counted by heads, not by places of the cache.
+int attention_params(const llmt_b200_attention_desc* d, const char* who, AttentionParams* p, bool decode = false) {
     if (d == nullptr) return fail(LLMT_B200_ERR_INVALID, "%s: null descriptor", who);
     if (d->batch < 0 || d->heads < 0 || d->tokens_q < 0 || d->tokens_k < 0 || d->kv_heads < 0 || d->head_dim < 1 || d->sinks < 0)
         return fail(LLMT_B200_ERR_INVALID, "%s: negative dimension", who);
@@ -2114,7 +2115,7 @@ int attention_params(const llmt_b200_attention_desc* d, const char* who, Attenti
     if (d->tokens_q > kMaxDim || d->tokens_k > kMaxDim || d->batch > kMaxDim || d->heads > 65536 || d->kv_heads > 65536)
         return fail(LLMT_B200_ERR_UNSUPPORTED, "%s: dimension above 2^31 - 1025, or more than 65536 heads", who);
     // a block for every row of every head in the worst case
-    const int64_t rows = d->tokens_q > d->tokens_k ? d->tokens_q : d->tokens_k;
+    const int64_t rows = decode ? 1 : d->tokens_q > d->tokens_k ? d->tokens_q : d->tokens_k;
     if (static_cast<__int128>(rows) * (d->heads > 0 ? d->heads : d->kv_heads) * d->batch > 0x7fffffff)
         return fail(LLMT_B200_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 rows over all heads", who);
     if (!(d->scale > 0.0f) || !std::isfinite(d->scale)) return fail(LLMT_B200_ERR_INVALID, "%s: scale must be positive and finite", who);
@@ -2294,14 +2295,14 @@ int llmt_b200_attention_window_bwd(const llmt_b200_attention_desc* d, void* stre
 
 uint64_t llmt_b200_attention_window_decode_workspace_bytes(const llmt_b200_attention_desc* d) {
     AttentionParams p;
-    if (attention_params(d, "attention_window_decode", &p) != LLMT_B200_OK) return 0;
+    if (attention_params(d, "attention_window_decode", &p, true) != LLMT_B200_OK) return 0;
     return (attention_decode_workspace(p, sm_count()) + 15) / 16 * 16;
 }
 
 int llmt_b200_attention_window_decode(const llmt_b200_attention_desc* d, void* stream) {
     const char* who = "attention_window_decode";
     AttentionParams p;
-    int st = attention_params(d, who, &p);
+    int st = attention_params(d, who, &p, true);
     if (st != LLMT_B200_OK) return st;
     if (d->tokens_q != 1) return fail(LLMT_B200_ERR_INVALID, "%s: tokens_q must be 1 (%lld)", who, (long long)d->tokens_q);
     const NamedView t[4] = {{"q", &d->q, false, false}, {"k", &d->k, true, false}, {"v", &d->v, true, false}, {"out", &d->out, false, true}};

@@ -11,7 +11,7 @@ import pytest
 import torch
 
 import llmt_b200 as L
-from tests.test_block_ops_cpu import MB, ROOT, attn_desc, norm_desc, rope_desc, view
+from tests.test_block_ops_cpu import MB, ROOT, attn_desc, decode_desc, norm_desc, rope_desc, view
 
 BF = dict(dtype_res=L.BF16, dtype_act=L.BF16)
 
@@ -179,3 +179,23 @@ def test_norm_residual_may_write_between_the_rows_that_it_reads():
         assert status == (L.ERR_INVALID if meet else L.ERR_WORKSPACE), (rows, cols, pitch, other, off, L.last_error())
         seen[meet] += 1
     assert min(seen.values()) > 100
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(batch=128, heads=128, kv_heads=8, tokens_k=131072, head_dim=128), L.ERR_WORKSPACE),   # 2^31 rows, 69 GB of keys and values
+    (dict(batch=1 << 20, heads=1, kv_heads=1, tokens_k=4096), L.ERR_WORKSPACE),
+    (dict(batch=1 << 20, heads=2048, kv_heads=1, tokens_k=16), L.ERR_UNSUPPORTED),              # 2^31 heads
+    (dict(tokens_k=(1 << 31) - 1), L.ERR_UNSUPPORTED)])
+def test_decode_counts_heads_not_places(kw, status):
+    """A missing workspace is what ends the calls that are accepted; those that need none are given one that lies on q."""
+    d = decode_desc(lse=None, lengths=None, workspace=None, workspace_bytes=0, **kw)
+    hd, h, hkv, places = d.head_dim, d.heads, d.kv_heads, d.tokens_k
+    at = 1 << 44
+    for name, n, strides in (("q", h, (h * hd, 0, hd)), ("out", h, (h * hd, 0, hd)), ("k", hkv, (places * hkv * hd, hkv * hd, hd)),
+                             ("v", hkv, (places * hkv * hd, hkv * hd, hd))):
+        setattr(d, name, view(at, *strides))
+        at += 1 << 42
+    need = L.lib().llmt_b200_attention_window_decode_workspace_bytes(ctypes.byref(d))
+    if status == L.ERR_WORKSPACE and need == 0:
+        d.lse, status = d.q.data, L.ERR_INVALID
+    assert L.lib().llmt_b200_attention_window_decode(ctypes.byref(d), None) == status, L.last_error()

@@ -6,7 +6,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import llmt_b200 as L
-from tests.test_attention_window_gpu import P, _heads, _make, _visible
+from tests.test_attention_window_gpu import P, _check_forward, _heads, _make, _visible
 from tests.test_norm_residual_gpu import _close
 
 pytestmark = pytest.mark.gpu
@@ -211,3 +211,24 @@ def test_a_step_whose_values_are_nan_takes_no_longer_than_a_few_others(b, h, hkv
         places = min(t, window + sinks) if window else t
         rows = 3 * 32 * (4 * places / 32 + places / 16) if token in spoil.values() else 0
         assert spoilt <= 10 * clean + rows, (spoil, clean, spoilt)
+
+
+def test_decode_of_more_rows_than_an_index_counts():
+    """256 sequences x 64 heads on 1 x 131072 places: 2^31 rows of all heads, 1 GB of keys and values; most places are empty."""
+    b, h, places, hd = 256, 64, 131072, 8
+    g = torch.Generator(device=DEV).manual_seed(8)
+    q = torch.randn(b, h, hd, device=DEV, generator=g).to(BF)
+    k, v = (torch.empty(b, places, 1, hd, device=DEV, dtype=BF) for _ in "kv")
+    held = 70
+    lengths = torch.randint(1, held + 1, (b,), device=DEV, generator=g, dtype=torch.int32)
+    lengths[-1] = places
+    k[:, :held], v[:, :held] = (torch.randn(b, held, 1, hd, device=DEV, generator=g).to(BF) for _ in "kv")
+    k[-1], v[-1] = (torch.randn(places, 1, hd, device=DEV, generator=g).to(BF) for _ in "kv")
+    out = torch.full_like(q, 7.0)
+    L.attention_window_decode(out, q, k, v, lengths)
+    for i in (0, 1, 100, b - 2, b - 1):
+        n = int(lengths[i])
+        lse = torch.empty(1, h, 1, device=DEV)
+        one = torch.empty(1, h, hd, device=DEV, dtype=BF)
+        L.attention_window_decode(one, q[i:i + 1], k[i:i + 1], v[i:i + 1], lengths[i:i + 1], lse=lse.view(1, h))
+        _check_forward(out[i][None, None], lse, q[i][None, None], k[i:i + 1, :n], v[i:i + 1, :n], 0, 0)
