@@ -104,10 +104,13 @@ static int read_tuple(PyObject* t, int64_t* out, int most) {   // steals t
     Py_DECREF(t);
     return n;
 }
-static int as_tensor(PyObject* o, Tensor* t) {
+static int as_layout(PyObject* o, Tensor* t) {   // of any type
     if (as_ptr(o, &t->ptr) < 0) return -1;
     t->nd = read_tuple(PyObject_GetAttr(o, s_shape), t->shape, 4);
-    if (t->nd < 0 || read_tuple(PyObject_CallMethodNoArgs(o, s_stride), t->stride, 4) != t->nd) return -1;
+    return t->nd < 0 || read_tuple(PyObject_CallMethodNoArgs(o, s_stride), t->stride, 4) != t->nd ? -1 : 0;
+}
+static int as_tensor(PyObject* o, Tensor* t) {
+    if (as_layout(o, t) < 0) return -1;
     PyObject* d = PyObject_GetAttr(o, s_dtype);
     if (d == NULL) { PyErr_Clear(); return -1; }
     t->dtype = d == g_float32 ? LLMT_B200_FP32 : d == g_bfloat16 ? LLMT_B200_BF16 : d == g_int32 ? 2 : d == g_float64 ? 3 : -1;
@@ -483,7 +486,7 @@ static int as_workspace(PyObject* o, int* device, void** at, uint64_t* bytes) {
     *bytes = PyLong_AsUnsignedLongLong(nb);
     Py_DECREF(nb);
     if (PyErr_Occurred()) { PyErr_Clear(); return -1; }
-    if (as_tensor(o, &t) < 0 || !is_contiguous(&t) || on_device(o, device) < 0) return -1;
+    if (as_layout(o, &t) < 0 || !is_contiguous(&t) || on_device(o, device) < 0) return -1;   // bytes, as a rule
     *at = t.ptr;
     return 0;
 }

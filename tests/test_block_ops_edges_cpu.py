@@ -199,3 +199,50 @@ def test_decode_counts_heads_not_places(kw, status):
     if status == L.ERR_WORKSPACE and need == 0:
         d.lse, status = d.q.data, L.ERR_INVALID
     assert L.lib().llmt_b200_attention_window_decode(ctypes.byref(d), None) == status, L.last_error()
+
+
+class _Tensor:
+    """What the native functions look at of a tensor."""
+    def __init__(self, at, dtype, *shape, stride=None):
+        t = torch.empty(shape, dtype=dtype, device="meta")
+        self.at, self.dtype, self.shape, self.nbytes, self.strides = at, dtype, t.shape, t.numel() * t.element_size(), stride or t.stride()
+
+    def data_ptr(self):
+        return self.at
+
+    def stride(self):
+        return self.strides
+
+    def get_device(self):
+        return 0
+
+
+@pytest.mark.parametrize("name", ["norm_residual_bwd", "attention_window_fwd", "attention_window_bwd", "attention_window_decode"])
+def test_a_workspace_of_bytes_stays_on_the_native_path(name):
+    """The native function with what torch would tell it of a GPU, and addresses that the library refuses: its own message comes
+    back, and the Python function is not asked."""
+    code = ("import sys, ctypes, pytest, torch, llmt_b200 as L\n"
+            "from llmt_b200 import _native\n"
+            "from tests.test_block_ops_edges_cpu import MB, _Tensor as T\n"
+            "name = sys.argv[1]\n"
+            "asked = []\n"
+            "exec(f'def {name}(*a, **k): asked.append(1)')\n"
+            "bind = lambda: _native.bind(tuple(ctypes.cast(getattr(L.lib(), 'llmt_b200_' + n), ctypes.c_void_p).value for n in _native.NAMES),\n"
+            "                            lambda d: 0, lambda: 0, torch.float32, torch.bfloat16, torch.int32, torch.float64, L.GemmDesc)\n"
+            "_native.setup(bind, L._check, L._scratch)\n"
+            "native = _native.fast(locals()[name])\n"
+            "bf, f32 = torch.bfloat16, torch.float32\n"
+            "q, k = (lambda i: T(i * MB, bf, 1, 64, 2, 64)), (lambda i: T(i * MB, bf, 1, 8192, 1, 64))\n"
+            "token, lse = (lambda i: T(i * MB, bf, 2, 64, 64)), T(20 * MB, f32, 1, 2, 64)\n"
+            "cache = lambda i: T(i * MB, bf, 2, 65536, 1, 64)\n"
+            "row, w = (lambda i: T(i * MB, f32, 64, 64)), (lambda i: T(i * MB, f32, 64))\n"
+            "calls = dict(norm_residual_bwd=lambda **ws: native(row(1), None, None, row(2), row(3), w_pre=w(4), rstd_pre=w(5), dw_pre=w(6), **ws),\n"
+            "             attention_window_fwd=lambda **ws: native(q(1), lse, q(2), k(3), k(6), **ws),\n"
+            "             attention_window_bwd=lambda **ws: native(q(1), k(3), k(6), q(2), q(9), k(10), k(13), q(16), lse, **ws),\n"
+            "             attention_window_decode=lambda **ws: native(token(1), token(2), cache(100), cache(200), **ws))\n"
+            "with pytest.raises(L.LlmtB200Error, match='16-byte aligned'):\n"
+            "    calls[name](workspace=T(300 * MB + 8, torch.uint8, 64 * MB))\n"
+            "assert not asked\n"
+            "calls[name](workspace=T(300 * MB, torch.uint8, 64 * MB, stride=(0,)))\n"
+            "assert asked, 'one that is not contiguous is'\n")
+    subprocess.check_call([sys.executable, "-c", code, name], cwd=ROOT)
