@@ -665,7 +665,7 @@ def _norm_residual_desc(who: str, like, tensors: dict, w_post, gate, w_pre, rstd
     d.groups = 1
     if gate is not None:
         _need(gate.dtype == torch.float32 and gate.is_contiguous() and gate.dim() in (1, 2) and gate.shape[-1] == d.cols, f"{who}: gate must be contiguous fp32 [groups, {d.cols}]")
-        d.gate, d.groups = gate.data_ptr(), gate.numel() // d.cols
+        d.gate, d.groups = gate.data_ptr(), gate.shape[0] if gate.dim() == 2 else 1
     d.scale, d.eps = float(scale), float(eps)
     return d
 

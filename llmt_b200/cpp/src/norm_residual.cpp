@@ -30,7 +30,7 @@ llmt_b200_norm_residual_desc describe(const char* who, const Tensor& res, const 
         if (!n.gate->valid() || n.gate->dtype != DType::FP32 || n.gate->shape[n.gate->shape.rank - 1] != d.cols || n.gate->shape.rank > 2)
             detail::fatal(who, "gate must be fp32 [C] or [groups, C]");
         d.gate = static_cast<const float*>(n.gate->data);
-        d.groups = n.gate->numel() / d.cols;
+        d.groups = n.gate->shape.rank == 2 ? n.gate->shape[0] : 1;
     }
     d.dtype_res = static_cast<int32_t>(res.dtype);
     d.dtype_act = static_cast<int32_t>(act != nullptr ? act->dtype : res.dtype);

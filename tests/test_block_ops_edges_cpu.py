@@ -246,3 +246,11 @@ def test_a_workspace_of_bytes_stays_on_the_native_path(name):
             "calls[name](workspace=T(300 * MB, torch.uint8, 64 * MB, stride=(0,)))\n"
             "assert asked, 'one that is not contiguous is'\n")
     subprocess.check_call([sys.executable, "-c", code, name], cwd=ROOT)
+
+
+def test_python_refuses_rows_without_columns():
+    x, w = torch.zeros(4, 0), torch.zeros(0)
+    for call in (lambda: L.norm_residual_fwd(x, x, x, x, gate=torch.zeros(1, 0), w_pre=w),
+                 lambda: L.norm_residual_bwd(x, x, x, x, x, x, gate=torch.zeros(1, 0), dgate=torch.zeros(1, 0), w_pre=w)):
+        with pytest.raises(L.LlmtB200Error):
+            call()

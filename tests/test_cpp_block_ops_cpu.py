@@ -1,6 +1,7 @@
 """What the block operators of llmt's C++ interface answer without a GPU."""
 import ctypes
 import os
+import signal
 import subprocess
 
 import pytest
@@ -24,3 +25,8 @@ def test_attention_workspace_is_enough_for_either_direction(b, t, h, hkv, hd, wi
     fwd, bwd = (int(getattr(L.lib(), f"llmt_b200_attention_window_{n}workspace_bytes")(ctypes.byref(d))) for n in ("fwd_", ""))
     r = run("workspace", b, t, h, hkv, hd, window, sinks)
     assert r.returncode == 0 and [int(x) for x in r.stdout.split()] == [max(fwd, bwd), fwd]
+
+
+def test_rows_without_columns_are_refused_with_a_message():
+    r = run("norm", 4, 0)
+    assert r.returncode == -signal.SIGABRT and "[llmt] norm_residual_fwd" in r.stderr and "bad shape" in r.stderr
