@@ -1932,8 +1932,14 @@ int norm_residual_params(const llmt_b200_norm_residual_desc* d, const char* who,
     return LLMT_B200_OK;
 }
 
-int norm_residual_row_bytes(const llmt_b200_norm_residual_desc* d) {
-    return 2 * ((d->dtype_res == LLMT_B200_BF16 ? 2 : 4) + (d->dtype_act == LLMT_B200_BF16 ? 2 : 4));
+// The plan of a call and the workspace that it takes.  A call forms it once: the budget of SMs is the process's and may change.
+NormResidualPlan norm_residual_plan_of(const llmt_b200_norm_residual_desc* d) {
+    const int row_bytes = 2 * ((d->dtype_res == LLMT_B200_BF16 ? 2 : 4) + (d->dtype_act == LLMT_B200_BF16 ? 2 : 4));
+    return norm_residual_plan(d->rows, d->cols, d->groups, row_bytes, d->dw_pre != nullptr, d->dw_post != nullptr || d->dgate != nullptr, sm_count());
+}
+uint64_t norm_residual_need(const NormResidualPlan& pl) {
+    if (pl.floats_w + pl.floats_gc == 0) return 0;
+    return static_cast<uint64_t>(pl.floats_w + pl.floats_gc + 8) / 4 * 16;   // both parts start on 16 bytes
 }
 
 // An fp32 array of a norm_residual call: weights, statistics, their gradients.
@@ -2023,9 +2029,7 @@ int llmt_b200_norm_residual_fwd(const llmt_b200_norm_residual_desc* d, void* str
 uint64_t llmt_b200_norm_residual_workspace_bytes(const llmt_b200_norm_residual_desc* d) {
     NormResidualParams p;
     if (norm_residual_params(d, "norm_residual_bwd", &p) != LLMT_B200_OK || d->rows == 0) return 0;
-    const NormResidualPlan pl = norm_residual_plan(d->rows, d->cols, d->groups, norm_residual_row_bytes(d), d->dw_pre != nullptr, d->dw_post != nullptr || d->dgate != nullptr, sm_count());
-    if (pl.floats_w + pl.floats_gc == 0) return 0;
-    return static_cast<uint64_t>(pl.floats_w + pl.floats_gc + 8) / 4 * 16;   // both parts start on 16 bytes
+    return norm_residual_need(norm_residual_plan_of(d));
 }
 
 int llmt_b200_norm_residual_bwd(const llmt_b200_norm_residual_desc* d, void* stream) {
@@ -2056,7 +2060,7 @@ int llmt_b200_norm_residual_bwd(const llmt_b200_norm_residual_desc* d, void* str
                              {"rstd_post", d->rstd_post, d->rows, false}, {"rstd_pre", d->rstd_pre, d->rows, false}};
     st = norm_residual_arrays(d, who, f, 8, t, 6);
     if (st != LLMT_B200_OK) return st;
-    const NormResidualPlan pl = norm_residual_plan(d->rows, d->cols, d->groups, norm_residual_row_bytes(d), d->dw_pre != nullptr, d->dw_post != nullptr || d->dgate != nullptr, sm_count());
+    const NormResidualPlan pl = norm_residual_plan_of(d);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (d->rows == 0) {   // sums of nothing
         for (const FloatArray& g : f) {
@@ -2067,7 +2071,7 @@ int llmt_b200_norm_residual_bwd(const llmt_b200_norm_residual_desc* d, void* str
         }
         return LLMT_B200_OK;
     }
-    const uint64_t need = llmt_b200_norm_residual_workspace_bytes(d);
+    const uint64_t need = norm_residual_need(pl);
     if (need > 0) {
         if (d->workspace == nullptr || d->workspace_bytes < need)
             return fail(LLMT_B200_ERR_WORKSPACE, "%s: workspace of %llu bytes needed, %llu given", who, (unsigned long long)need,
@@ -2191,6 +2195,8 @@ int attention_apart(const llmt_b200_attention_desc* d, const char* who, const ch
     return LLMT_B200_OK;
 }
 
+uint64_t whole_pieces(size_t bytes) { return (bytes + 15) / 16 * 16; }
+
 // Tensor map of a head view: boxes of 64 values x box_rows tokens of one head, 128-byte swizzle.
 int head_map(CUtensorMap* map, const HeadView& v, const AttentionParams& p, bool keys, int box_rows) {
     const int64_t tokens = keys ? p.tk : p.tq, heads = keys ? p.heads / p.group : p.heads;
@@ -2204,7 +2210,7 @@ int head_map(CUtensorMap* map, const HeadView& v, const AttentionParams& p, bool
 uint64_t llmt_b200_attention_window_fwd_workspace_bytes(const llmt_b200_attention_desc* d) {
     AttentionParams p;
     if (attention_params(d, "attention_window_fwd", &p) != LLMT_B200_OK) return 0;
-    return (attention_fwd_sm100_workspace(p, sm_count()) + 15) / 16 * 16;
+    return whole_pieces(attention_fwd_sm100_workspace(p, sm_count()));
 }
 
 int llmt_b200_attention_window_fwd(const llmt_b200_attention_desc* d, void* stream) {
@@ -2218,7 +2224,8 @@ int llmt_b200_attention_window_fwd(const llmt_b200_attention_desc* d, void* stre
     if (st == LLMT_B200_OK) st = attention_apart(d, who, "lse", d->lse, 4 * static_cast<size_t>(d->batch * d->heads * d->tokens_q), t, 4);
     if (st != LLMT_B200_OK) return st;
     if (p.batch == 0 || p.heads == 0 || p.tq == 0) return LLMT_B200_OK;
-    const uint64_t need = llmt_b200_attention_window_fwd_workspace_bytes(d);
+    const int sms = sm_count();   // once: the budget is the process's and may change, and the workspace is of this plan
+    const uint64_t need = whole_pieces(attention_fwd_sm100_workspace(p, sms));
     if (need > 0 && d->workspace != nullptr && d->workspace_bytes >= need) {
         if (misaligned(d->workspace, 16)) return fail(LLMT_B200_ERR_INVALID, "%s: workspace is not 16-byte aligned", who);
         st = attention_apart(d, who, "workspace", d->workspace, need, t, 4);
@@ -2239,7 +2246,7 @@ int llmt_b200_attention_window_fwd(const llmt_b200_attention_desc* d, void* stre
         if (st != LLMT_B200_OK) return st;
         DeviceStatus* status = device_status_ptr();
         if (status == nullptr) return fail(LLMT_B200_ERR_CUDA, "cannot resolve the device status word");
-        e = launch_attention_fwd_sm100(p, maps, need > 0 && d->workspace_bytes >= need ? d->workspace : nullptr, sm_count(), status, g_wait_limit_ns, s);
+        e = launch_attention_fwd_sm100(p, maps, need > 0 && d->workspace_bytes >= need ? d->workspace : nullptr, sms, status, g_wait_limit_ns, s);
     }
     if (e != cudaSuccess) return fail(LLMT_B200_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
     return LLMT_B200_OK;
@@ -2265,7 +2272,8 @@ int llmt_b200_attention_window_bwd(const llmt_b200_attention_desc* d, void* stre
     if (p.heads > 0 && p.tq > 0 && d->lse == nullptr) return fail(LLMT_B200_ERR_INVALID, "%s: invalid tensor lse (null data)", who);
     st = attention_apart(d, who, "lse", d->lse, 4 * static_cast<size_t>(d->batch * d->heads * d->tokens_q), t + 5, 3);
     if (st != LLMT_B200_OK) return st;
-    const uint64_t need = llmt_b200_attention_window_workspace_bytes(d);
+    const int sms = sm_count();
+    const uint64_t need = attention_bwd_sm100_workspace(p, sms);
     if (need > 0 && (d->workspace == nullptr || d->workspace_bytes < need))
         return fail(LLMT_B200_ERR_WORKSPACE, "%s: workspace of %llu bytes needed, %llu given", who, (unsigned long long)need,
                     (unsigned long long)(d->workspace == nullptr ? 0 : d->workspace_bytes));
@@ -2287,7 +2295,7 @@ int llmt_b200_attention_window_bwd(const llmt_b200_attention_desc* d, void* stre
         if (st != LLMT_B200_OK) return st;
         DeviceStatus* status = device_status_ptr();
         if (status == nullptr) return fail(LLMT_B200_ERR_CUDA, "cannot resolve the device status word");
-        e = launch_attention_bwd_sm100(p, maps, d->workspace, sm_count(), status, g_wait_limit_ns, s);
+        e = launch_attention_bwd_sm100(p, maps, d->workspace, sms, status, g_wait_limit_ns, s);
     }
     if (e != cudaSuccess) return fail(LLMT_B200_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
     return LLMT_B200_OK;
@@ -2296,7 +2304,7 @@ int llmt_b200_attention_window_bwd(const llmt_b200_attention_desc* d, void* stre
 uint64_t llmt_b200_attention_window_decode_workspace_bytes(const llmt_b200_attention_desc* d) {
     AttentionParams p;
     if (attention_params(d, "attention_window_decode", &p, true) != LLMT_B200_OK) return 0;
-    return (attention_decode_workspace(p, sm_count()) + 15) / 16 * 16;
+    return whole_pieces(attention_decode_workspace(p, sm_count()));
 }
 
 int llmt_b200_attention_window_decode(const llmt_b200_attention_desc* d, void* stream) {
@@ -2313,7 +2321,8 @@ int llmt_b200_attention_window_decode(const llmt_b200_attention_desc* d, void* s
     if (p.batch == 0 || p.heads == 0) return LLMT_B200_OK;
     if (d->lse != nullptr && d->lengths != nullptr && overlaps(d->lse, 4 * static_cast<size_t>(d->batch * d->heads), d->lengths, 4 * static_cast<size_t>(d->batch)))
         return fail(LLMT_B200_ERR_INVALID, "%s: lse overlaps lengths", who);
-    const uint64_t need = llmt_b200_attention_window_decode_workspace_bytes(d);
+    const int sms = sm_count();
+    const uint64_t need = whole_pieces(attention_decode_workspace(p, sms));
     if (need > 0) {
         if (d->workspace == nullptr || d->workspace_bytes < need)
             return fail(LLMT_B200_ERR_WORKSPACE, "%s: workspace of %llu bytes needed, %llu given", who, (unsigned long long)need,
@@ -2325,7 +2334,7 @@ int llmt_b200_attention_window_decode(const llmt_b200_attention_desc* d, void* s
             (d->lengths != nullptr && overlaps(d->workspace, need, d->lengths, 4 * static_cast<size_t>(d->batch))))
             return fail(LLMT_B200_ERR_INVALID, "%s: workspace overlaps lse or lengths", who);
     }
-    const cudaError_t e = launch_attention_window_decode(p, sm_count(), d->workspace, static_cast<cudaStream_t>(stream));
+    const cudaError_t e = launch_attention_window_decode(p, sms, d->workspace, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return fail(LLMT_B200_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
     return LLMT_B200_OK;
 }

@@ -3,7 +3,9 @@ is needed (an accepted call ends at the missing workspace or at the launch)."""
 import ctypes
 import inspect
 import itertools
+import os
 import random
+import re
 import subprocess
 import sys
 
@@ -254,3 +256,13 @@ def test_python_refuses_rows_without_columns():
                  lambda: L.norm_residual_bwd(x, x, x, x, x, x, gate=torch.zeros(1, 0), dgate=torch.zeros(1, 0), w_pre=w)):
         with pytest.raises(L.LlmtB200Error):
             call()
+
+
+@pytest.mark.parametrize("name", ["norm_residual_bwd", "attention_window_fwd", "attention_window_bwd", "attention_window_decode"])
+def test_a_call_reads_the_budget_of_sms_once(name):
+    """The workspace that is asked for and the plan that is run are of one reading: the budget is the process's, and calls for
+    another device may be under way while it is set."""
+    source = open(os.path.join(ROOT, "llmt_b200", "csrc", "capi.cu")).read()
+    body = source[source.index(f"int llmt_b200_{name}(const"):]
+    body = re.sub(r"//[^\n]*", "", body[:body.index("\n}\n")])
+    assert len(re.findall(r"\bsm_count\(\)|\bnorm_residual_plan_of\(|_workspace_bytes\(d\)", body)) == 1
