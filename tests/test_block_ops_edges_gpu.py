@@ -124,7 +124,9 @@ SPOILT = [(n, how, bad) for n in ("q", "k", "v", "dout") for how in ("column", "
     (1, 2, 1, 200, 200, 64, 30, 2),       # a short window: D summed exactly
     (1, 2, 2, 260, 260, 128, 0, 0),
     (1, 2, 1, 40, 1300, 64, 700, 3),      # in parts
-    (1, 4, 2, 150, 100, 72, 0, 0)])       # queries that see nothing
+    (1, 4, 2, 150, 100, 72, 0, 0),        # queries that see nothing
+    (1, 4, 1, 700, 700, 64, 0, 0),        # dK and dV in parts
+    (1, 2, 1, 600, 600, 128, 100, 130)])  # sinks of two tiles
 def test_values_that_are_not_finite_reach_what_the_definition_says(b, h, hkv, tq, tk, hd, window, sinks):
     """A weight, a token or some values that are NaN or infinite, and hidden places that hold infinities beside them."""
     g = torch.Generator(device=DEV).manual_seed(9)
