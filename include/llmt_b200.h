@@ -422,7 +422,8 @@ typedef struct llmt_b200_head_view {
  * Values behind rot_dim are copied.  y may be x (same base and strides), else the two must not
  * overlap; y's elements must be distinct.
  *   freqs      device, fp64 [rot_dim / 2], radians per token; llmt_b200_rope_frequencies fills a host
- *              array with them.  Angles are reduced in 64-bit fixed point, exact at any position.
+ *              array with them.  An angle is a product in 64-bit fixed point, from which whole turns go
+ *              exactly: off by 2^-52 of itself (the conversion of freqs to turns) before its sine is taken.
  *   positions  device, int32 [batch, tokens] contiguous, or NULL: offset + t.
  *   dtype      fp32 or bf16; arithmetic in fp32.  head_dim <= 1024, rot_dim even.
  * One call may do q and k of a packed projection together (heads = H + Hkv).  Nothing is done for
@@ -462,7 +463,7 @@ LLMT_B200_API int llmt_b200_rope_frequencies(double* freqs, int64_t rot_dim, dou
  *
  * llmt_b200_norm_residual_bwd: with g = dout + (gradient of h through N(.; w_pre)),
  *   dx = g,  dy = the gradient of y,  dw_pre, dw_post [cols], dgate [groups, cols] summed over the rows they
- *   serve, in fp32 and in a fixed order:  d = beta * d + sum.
+ *   serve, in fp32 and in a fixed order:  d = beta * d + sum  (without rows beta must be 0 or 1).
  * Reads out (as stored), y and the statistics of the forward call.  dout NULL: no gradient but the one
  * through h.  dh NULL: h was not made.  dw_post, dgate, dw_pre NULL: not wanted.  dx may be dout.
  * For y NULL `out` is the forward call's x, and dy is not written.  workspace: 16-byte aligned,
@@ -511,9 +512,11 @@ LLMT_B200_API uint64_t llmt_b200_norm_residual_workspace_bytes(const llmt_b200_n
  * order; with a smaller one or none they are not.
  *
  * _bwd: dV = P^T dO,  dS = P (dP - D) with dP = dO v^T,  dQ = scale dS k,  dK = scale dS^T q, from out and
- * lse as _fwd left them.  D = rowsum(P dP) is taken as rowsum(dO out) for dQ where a query may see more than
- * 128 keys, among which the rounding of out is lost beside that of dS; a row of dS adds up to nothing but for
- * that rounding, which is taken out of D again before dK is formed.  workspace: 16-byte aligned, llmt_b200_attention_window_workspace_bytes(desc) bytes.
+ * lse as _fwd left them.  Where no query can see more than 128 keys (window + sinks, tokens_k), D is
+ * rowsum(P dP); in all other calls dQ takes it as rowsum(dO out).  Over many keys the rounding of out is lost there beside
+ * that of dS; the first queries of such a call see few keys and carry it (error of dQ's norm 4.4e-3 for rows of 2 keys, 2.9e-3
+ * of 8, 2.5e-3 of 128).  A row of dS adds up to nothing but for that rounding, which is taken out of D again before dK is
+ * formed.  workspace: 16-byte aligned, llmt_b200_attention_window_workspace_bytes(desc) bytes.
  *
  * _decode: one new token per sequence (tokens_q = 1) over a cache of tokens_k places, of which
  * sequence b holds lengths[b] (device, int32; NULL: all; values beyond tokens_k count as tokens_k,

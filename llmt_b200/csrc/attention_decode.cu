@@ -11,7 +11,7 @@
 // ragged batch is many blocks (shares of every sequence, in clusters that join through distributed shared memory: 4 sequences
 // of 8 to 65536 places, 32 heads on 8 of 128, 177 us against 147).
 // Measured: those 4 sequences 153 us with both launches, 721 MB at 4.7 TB/s; 32 sequences of up to 1024 places, 12 heads of 64,
-// window 256: 8.5 us for 25 MB, a launch and one chunk's latency.
+// window 256: 8.7 us for 25 MB, a launch and one chunk's latency.
 #include "attention_rows.cuh"
 #include "ptx_sm100.cuh"
 

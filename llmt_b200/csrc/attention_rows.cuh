@@ -1,4 +1,5 @@
-// Causal attention with a sliding window and sinks, one row by one warp with plain loads and FMAs.
+// Causal attention with a sliding window and sinks, one row by one warp with plain loads and FMAs: for rows that came out of the
+// tiles with values that are not finite.
 //
 // A query at position p = i + tk - tq sees key j when j <= p and (j > p - window or j < sinks).  The functions here touch
 // visible pairs only, so nothing that a hidden key or query holds reaches a result.

@@ -807,8 +807,9 @@ __device__ __forceinline__ void row_products(const AttentionParams& p, int b, in
 // dQ of 128 queries: S = Q K^T and dP = dO V^T of 64 keys, dS = P (dP - D), dQ += dS K.
 // D = rowsum(dO out) carries the rounding of out.  Over many keys that is lost beside the roundings of dS; over few it is not
 // (normal operands, error of dQ's norm against the result's own rounding of 1.7e-3: 4.4e-3 for 2 keys, 2.9e-3 for 8, 2.5e-3 for
-// 128, where an exact D gives 2.4e-3 for any number).  `exact`: the tiles are gone through twice, the first time for D as the
-// sum of P dP, with zeros for dS.  (Three kinds of the kernel, since the ordinary one gains 3 % from not having the others.)
+// 128, where an exact D gives 2.4e-3 for any number).  `exact`, for calls in which no query sees more than 128 keys: the tiles are
+// gone through twice, the first time for D as the sum of P dP, with zeros for dS.  The first queries of other calls, which see
+// few keys too, keep the rounded D, as the public header says.  (Three kinds of the kernel, since the ordinary one gains 3 % from not having the others.)
 // head_dim <= 64: one warpgroup a block and two blocks an SM, so that one works while the other begins or ends; dS has a place
 // of its own, and the next scores are made while the warpgroup works on the last ones.  (BUFFERS = 3 there: 8 x 12 x 1024,
 // window 256: dQ, dK, dV 100 us against 90; 2 x 16 x 4096: 368 against 344.)  Few query blocks are done in parts, as in the

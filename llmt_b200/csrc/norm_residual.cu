@@ -16,7 +16,7 @@
 // its own pieces of the rows to come into shared memory (cp.async, two or three rows ahead): what is under way takes no
 // registers, and nobody else reads it, so nothing has to be waited for but the row sums.
 // Measured at 8192 x 1600: forward (fp32 stream, bf16 block, both norms and the gate) 28.9 us, 157 MB at 5.4 TB/s; backward
-// (bf16, a gate a sequence, all three weight gradients) 43.6 us, 157 MB with the sums' way through memory at 3.6 TB/s: its
+// (bf16, a gate a sequence, all three weight gradients) 43.8 us, 157 MB with the sums' way through memory at 3.6 TB/s: its
 // 420 instructions a row and warp keep the schedulers busy 60 % of the time, the row sums' exchange takes most of the rest (with
 // 64 registers and four blocks an SM, which spill: 63 us; sums of three values in 6 exchanges for 15 and statistics loaded a row
 // ahead: the same).  8 rows of 768: 6.9 us, launch and two row sums.
